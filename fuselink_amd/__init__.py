@@ -5,4 +5,4 @@ The compute lives in ``lib/libnccl-net-fuselink.so`` (hand-written HIP); this pa
 host mirror used by the tests, the smoke check and the benchmark.  Submodules import torch lazily
 so that ``import fuselink_amd`` stays cheap."""
 
-__all__ = ["build", "core", "plugin"]
+__all__ = ["build", "core", "kv", "plugin"]

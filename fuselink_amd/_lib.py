@@ -61,6 +61,48 @@ class Windows(C.Structure):
                 ("pad", C.c_uint32)]
 
 
+class KvCache(C.Structure):
+    _fields_ = [("d_pages", C.c_void_p), ("page_stride", C.c_uint64), ("n_pages", C.c_uint32), ("tokens", C.c_uint32),
+                ("heads", C.c_uint32), ("dim", C.c_uint32)]
+
+
+class KvSeqs(C.Structure):
+    _fields_ = [("d_starts", C.c_void_p), ("d_lens", C.c_void_p), ("d_table", C.c_void_p), ("table_stride", C.c_uint64),
+                ("table_width", C.c_uint32), ("n_seqs", C.c_uint32), ("n_tokens", C.c_uint32), ("pad", C.c_uint32)]
+
+
+class KvStoreParams(C.Structure):
+    _fields_ = [("cache", KvCache), ("seqs", KvSeqs), ("d_k", C.c_void_p), ("d_v", C.c_void_p), ("k_token_stride", C.c_uint64),
+                ("k_head_stride", C.c_uint64), ("v_token_stride", C.c_uint64), ("v_head_stride", C.c_uint64), ("type", C.c_uint32),
+                ("pad", C.c_uint32), ("d_status", C.c_void_p)]
+
+
+class KvAttendParams(C.Structure):
+    _fields_ = [("cache", KvCache), ("seqs", KvSeqs), ("d_q", C.c_void_p), ("d_out", C.c_void_p), ("q_token_stride", C.c_uint64),
+                ("q_head_stride", C.c_uint64), ("out_token_stride", C.c_uint64), ("out_head_stride", C.c_uint64), ("d_lse", C.c_void_p),
+                ("type", C.c_uint32), ("q_heads", C.c_uint32), ("scale", C.c_float), ("causal", C.c_uint32), ("d_selected", C.c_void_p),
+                ("d_weights_in", C.c_void_p), ("d_weights", C.c_void_p), ("weights_in_seq_stride", C.c_uint64),
+                ("weights_in_head_stride", C.c_uint64), ("weights_seq_stride", C.c_uint64), ("weights_head_stride", C.c_uint64),
+                ("n_selected", C.c_uint32), ("weights_width", C.c_uint32), ("d_workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+                ("d_status", C.c_void_p)]
+
+
+class KvSelectParams(C.Structure):
+    _fields_ = [("cache", KvCache), ("seqs", KvSeqs), ("d_q", C.c_void_p), ("q_token_stride", C.c_uint64), ("q_head_stride", C.c_uint64),
+                ("type", C.c_uint32), ("q_heads", C.c_uint32), ("count", C.c_uint32), ("first", C.c_uint32), ("last", C.c_uint32),
+                ("causal", C.c_uint32), ("d_out", C.c_void_p), ("d_workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+                ("d_status", C.c_void_p)]
+
+
+class KvEvictParams(C.Structure):
+    _fields_ = [("cache", KvCache), ("to", KvCache), ("seqs", KvSeqs), ("d_to_table", C.c_void_p), ("to_table_stride", C.c_uint64),
+                ("d_weights", C.c_void_p), ("weights_seq_stride", C.c_uint64), ("weights_head_stride", C.c_uint64),
+                ("d_new_weights", C.c_void_p), ("new_weights_seq_stride", C.c_uint64), ("new_weights_head_stride", C.c_uint64),
+                ("d_kept", C.c_void_p), ("d_new_lens", C.c_void_p), ("to_table_width", C.c_uint32), ("weights_width", C.c_uint32),
+                ("new_weights_width", C.c_uint32), ("budget", C.c_uint32), ("first", C.c_uint32), ("recent", C.c_uint32),
+                ("d_status", C.c_void_p)]
+
+
 # name -> (restype, argtypes); every symbol declared in include/fuselink_hip.h
 SIGNATURES = {
     "flh_init": (C.c_int, [C.c_int]),
@@ -133,6 +175,13 @@ SIGNATURES = {
     "flh_region_refs": (C.c_int, [C.c_void_p]),
     "flh_region_windows": (C.c_int, [C.c_void_p, C.POINTER(Windows)]),
     "flh_region_translate": (C.c_void_p, [C.c_void_p, C.c_uint32, C.c_void_p]),
+    "flh_kv_page_bytes": (C.c_uint64, [C.c_uint32, C.c_uint32, C.c_uint32]),
+    "flh_kv_store": (C.c_int, [C.POINTER(KvStoreParams), C.c_void_p]),
+    "flh_kv_attend_workspace_bytes": (C.c_int64, [C.POINTER(KvAttendParams)]),
+    "flh_kv_attend": (C.c_int, [C.POINTER(KvAttendParams), C.c_void_p]),
+    "flh_kv_select_workspace_bytes": (C.c_uint64, [C.c_uint32, C.c_uint32, C.c_uint32]),
+    "flh_kv_select": (C.c_int, [C.POINTER(KvSelectParams), C.c_void_p]),
+    "flh_kv_evict": (C.c_int, [C.POINTER(KvEvictParams), C.c_void_p]),
     "flh_tune": (C.c_int, [C.c_char_p, C.c_int64]),
     "flh_prof_begin": (C.c_int, [C.c_int]),
     "flh_prof_end": (C.c_int, [C.POINTER(C.c_double), C.POINTER(C.c_int), C.c_int]),

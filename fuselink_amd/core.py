@@ -38,7 +38,8 @@ def tune(key: str, value: int) -> None:
     check(_lib.load().flh_tune(key.encode(), int(value)))
 
 
-PROF_KERNELS = {1: "schedule", 2: "stripe", 3: "reassemble", 4: "gather", 5: "scatter", 6: "copy", 7: "stage_deliver"}
+PROF_KERNELS = {1: "schedule", 2: "stripe", 3: "reassemble", 4: "gather", 5: "scatter", 6: "copy", 7: "stage_deliver",
+                8: "kv_store", 9: "kv_attend", 10: "kv_select", 11: "kv_evict"}
 
 
 def prof_begin(capacity: int) -> None:

@@ -1,0 +1,1436 @@
+// fl_kv.hip -- operators on KV pages held in 8 bits: storing keys and values into page records (flh_kv_store),
+// attention over them (flh_kv_attend), the choice of pages by their key bounds (flh_kv_select) and the repacking of
+// the tokens that attention has dwelt on (flh_kv_evict).  The records are bytes to the page movers of fl_copy.hip.
+#include <hip/hip_runtime.h>
+
+#include <cstring>
+
+#include "fl_device.h"
+#include "fl_internal.h"
+#include "fl_launch.h"
+#include "fuselink_hip.h"
+
+namespace {
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef int i4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+
+constexpr float kInf = __builtin_inff();
+constexpr float kNan = __builtin_nanf("");
+
+// ------------------------------------------------------------------------------------------------
+// records and sequences
+// ------------------------------------------------------------------------------------------------
+struct Cache {
+  uint8_t* pages;
+  uint64_t stride;
+  uint32_t n_pages, T, H, D;
+  uint64_t side, low, high, scales;   // byte offsets inside a record: V codes, bounds, scales
+};
+
+// Token counts come from device memory, so every use of them is clamped to what the host could check.
+struct Seqs {
+  const int32_t* starts;   // may be null: per tokens each
+  const int32_t* lens;
+  const int32_t* table;
+  uint64_t table_stride;
+  uint32_t width, n_seqs, n_tokens, per;
+  int32_t* status;
+};
+
+__device__ __forceinline__ void report(int32_t* status) { *status = FLH_E_RANGE; }
+
+__device__ __forceinline__ void seq_tokens(const Seqs& s, uint32_t b, uint32_t& first, uint32_t& n) {
+  if (!s.starts) { first = b * s.per; n = s.per; return; }
+  const int32_t lo = s.starts[b], hi = s.starts[b + 1];
+  if (lo < 0 || hi < lo || (uint32_t)hi > s.n_tokens) { report(s.status); first = 0; n = 0; return; }
+  first = (uint32_t)lo;
+  n = (uint32_t)(hi - lo);
+}
+
+// tokens that sequence b holds, at most what its row of the page table can name
+__device__ __forceinline__ uint32_t seq_len(const Seqs& s, uint32_t T, uint32_t b) {
+  const int32_t len = s.lens[b];
+  const uint64_t most = (uint64_t)s.width * T;
+  if (len < 0 || (uint64_t)len > most) { report(s.status); return len < 0 ? 0u : (uint32_t)most; }
+  return (uint32_t)len;
+}
+
+// Item x of the sequences' items laid end to end: which sequence, and which of its items.  A wavefront looks at 64
+// sequences at a time.  False if there are fewer items.
+template <class Count>
+__device__ __forceinline__ bool find_seq(uint32_t n_seqs, uint32_t x, Count count, uint32_t& b, uint32_t& local) {
+  const int lane = threadIdx.x & 63;
+  for (uint32_t base = 0; base < n_seqs; base += 64) {
+    const uint32_t c = base + lane < n_seqs ? count(base + lane) : 0;
+    const uint32_t incl = wave_incl_sum_u32(c, lane);
+    const uint32_t total = bcast_lane_u32(incl, 63);
+    if (x < total) {
+      const int l = __builtin_ctzll(__ballot(incl > x));
+      b = base + (uint32_t)l;
+      local = x - (bcast_lane_u32(incl, l) - bcast_lane_u32(c, l));
+      return true;
+    }
+    x -= total;
+  }
+  return false;
+}
+
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+
+// ------------------------------------------------------------------------------------------------
+// e4m3 codes under a power-of-two scale
+// ------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127
+
+// Smallest 2^e >= amax / 448 with e >= -126, 0 for amax = 0: 448 = 1.75 * 2^8, so the mantissa decides between two exponents.
+__device__ __forceinline__ float block_scale(float amax) {
+  if (!(amax > 0.f)) return 0.f;
+  const uint32_t u = __float_as_uint(amax);
+  const int x = (int)(u >> 23) - 127;
+  int e = (u & 0x7fffffu) <= 0x600000u ? x - 8 : x - 7;
+  if (e < -126 || u < 0x800000u) e = -126;
+  return pow2f(e);
+}
+__device__ __forceinline__ float inverse(float s) {   // of a power of two, exact; 0 for 0
+  return s > 0.f ? __uint_as_float((254u << 23) - __float_as_uint(s)) : 0.f;
+}
+__device__ __forceinline__ void unpack4(uint32_t w, float* x) {
+  x[0] = __builtin_amdgcn_cvt_f32_fp8((int)w, 0);
+  x[1] = __builtin_amdgcn_cvt_f32_fp8((int)w, 1);
+  x[2] = __builtin_amdgcn_cvt_f32_fp8((int)w, 2);
+  x[3] = __builtin_amdgcn_cvt_f32_fp8((int)w, 3);
+}
+__device__ __forceinline__ uint32_t pack4(const float* x) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
+}
+
+// ------------------------------------------------------------------------------------------------
+// blocks of tokens into records: new tokens behind those that a page holds (store), or chosen tokens of other
+// records (evict)
+// ------------------------------------------------------------------------------------------------
+struct PackArgs {
+  Cache c;
+  Seqs s;
+  // store
+  const void* src[2];
+  uint64_t token_stride[2], head_stride[2];   // in elements
+  uint32_t vec;                               // 16-byte loads are aligned
+  // evict
+  Cache from;
+  const int32_t* to_table;
+  uint64_t to_stride;
+  const int32_t* kept;
+  uint64_t kept_stride;
+  uint32_t budget, per_seq;
+};
+
+template <class E>
+__device__ __forceinline__ void load8(const E* p, bool vec, float* x);
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, bool vec, float* x) {
+  if (vec) {
+    const f4 a = *reinterpret_cast<const f4*>(p), b = *reinterpret_cast<const f4*>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[4 + i] = b[i]; }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = p[i];
+  }
+}
+template <>
+__device__ __forceinline__ void load8<_Float16>(const _Float16* p, bool vec, float* x) {
+  if (vec) {
+    const h8 a = *reinterpret_cast<const h8*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)p[i];
+  }
+}
+template <>
+__device__ __forceinline__ void load8<__bf16>(const __bf16* p, bool vec, float* x) {
+  if (vec) {
+    const u32x4 a = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(a[i] << 16); x[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u); }
+  } else {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float((uint32_t)q[i] << 16);
+  }
+}
+
+// One wavefront packs one side (K or V) of one head of one page.  A lane holds 8 neighbouring channels of every
+// RP-th token (RP = 64 / (D / 8) tokens at a time), so both the codes' rows and the channels' bounds come out of
+// registers.  The largest magnitude of the new tokens fixes the scale, then the same rows become codes.  Up to
+// kRows rows per lane stay in registers between the two; longer blocks are read twice (the second time from cache).
+// In evict the rows are codes of other records under their own scales.
+constexpr int kRows = 8;
+
+template <class E, bool EVICT, bool ONE>
+__global__ __launch_bounds__(256) void fl_kv_pack(const PackArgs a) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t unit = blockIdx.y * 4 + uniform(threadIdx.x >> 6);
+  const Cache& c = a.c;
+  if (unit >= 2 * c.H) return;
+  const uint32_t h = unit >> 1, side = unit & 1, T = c.T, D = c.D;
+  uint32_t b, j, first = 0, n, held;
+  int32_t page;
+  if constexpr (EVICT) {
+    b = blockIdx.x / a.per_seq;
+    j = blockIdx.x - b * a.per_seq;
+    n = seq_len(a.s, a.from.T, b);
+    if (n > a.budget) n = a.budget;
+    held = 0;
+    if (j * T >= n) return;
+    page = a.to_table[b * a.to_stride + j];
+  } else {
+    const auto items = [&](uint32_t q) {
+      uint32_t f, m;
+      seq_tokens(a.s, q, f, m);
+      const uint32_t l = seq_len(a.s, T, q);
+      return m ? (l + m + T - 1) / T - l / T : 0;
+    };
+    if (!find_seq(a.s.n_seqs, blockIdx.x, items, b, j)) return;
+    b = uniform(b);
+    seq_tokens(a.s, b, first, n);
+    held = seq_len(a.s, T, b);
+    j += held / T;
+    if (j >= a.s.width) { if (lane == 0) report(a.s.status); return; }
+    page = a.s.table[b * a.s.table_stride + j];
+  }
+  if (page < 0 || (uint32_t)page >= c.n_pages) { if (lane == 0) report(a.s.status); return; }
+  const uint32_t at = j * T;                                   // position of the page's first slot
+  const uint32_t old = held > at ? held - at : 0;              // slots that hold a token already
+  const uint64_t end64 = (uint64_t)held + n - at;
+  const uint32_t fill = end64 < T ? (uint32_t)end64 : T;       // slots that hold one afterwards
+  uint8_t* rec = c.pages + (uint64_t)page * c.stride;
+  uint8_t* codes = rec + side * c.side + (uint64_t)h * T * D;
+  float* scale_at = reinterpret_cast<float*>(rec + c.scales) + 2 * h + side;
+
+  const uint32_t CG = D >> 3, RP = 64 / CG, grp = (uint32_t)lane / CG, cg = (uint32_t)lane - grp * CG;
+  const bool on = grp < RP;
+  const uint32_t passes = (T + RP - 1) / RP;
+  const float s_old = !EVICT && old ? *scale_at : 0.f;
+
+  float x[kRows][8];
+  const auto load = [&](uint32_t p0) {   // rows (p0 + i) * RP + grp: new tokens' values (evict: all of them), 0 elsewhere
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const uint32_t r = (p0 + i) * RP + grp;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
+      if (!on || r >= fill || r < old) continue;
+      if constexpr (EVICT) {
+        const int32_t pos = a.kept[b * a.kept_stride * c.H + (uint64_t)h * a.kept_stride + at + r];
+        const uint32_t slot = (uint32_t)pos / a.from.T;
+        const int32_t pg = pos >= 0 && slot < a.s.width ? a.s.table[b * a.s.table_stride + slot] : -1;
+        if (pg < 0 || (uint32_t)pg >= a.from.n_pages) { report(a.s.status); continue; }
+        const uint8_t* f = a.from.pages + (uint64_t)pg * a.from.stride;
+        const float s = reinterpret_cast<const float*>(f + a.from.scales)[2 * h + side];
+        const u2 w = *reinterpret_cast<const u2*>(f + side * a.from.side + ((uint64_t)h * a.from.T + ((uint32_t)pos - slot * a.from.T)) * D + cg * 8);
+        unpack4(w[0], x[i]);
+        unpack4(w[1], x[i] + 4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[i][e] *= s;
+      } else {
+        const E* p = reinterpret_cast<const E*>(a.src[side]) + (uint64_t)(first + at + r - held) * a.token_stride[side] + h * a.head_stride[side] + cg * 8;
+        load8<E>(p, a.vec, x[i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[i][e] = __builtin_isfinite(x[i][e]) ? x[i][e] : kNan;
+      }
+    }
+  };
+
+  float amax = 0.f;
+  for (uint32_t p0 = 0; p0 < passes; p0 += kRows) {
+    load(p0);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[i][e]));   // fmaxf passes over NaN
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+  const float s = fmaxf(s_old, block_scale(amax)), inv = inverse(s);
+  const bool grown = old && s != s_old;
+  const float ratio = s_old * inv;
+
+  float lo[8], hi[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) { lo[e] = kInf; hi[e] = -kInf; }
+  for (uint32_t p0 = 0; p0 < passes; p0 += kRows) {
+    if (!ONE) load(p0);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const uint32_t r = (p0 + i) * RP + grp;
+      if (!on || r >= T) continue;
+      u2* row = reinterpret_cast<u2*>(codes + (uint64_t)r * D + cg * 8);
+      float y[8];
+      if (r < old) {
+        if (side == 1 && !grown) continue;
+        const u2 w = *row;
+        unpack4(w[0], y);
+        unpack4(w[1], y + 4);
+        if (grown) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] *= ratio;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = x[i][e] * inv;
+      }
+      if (r < fill) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { lo[e] = fminf(lo[e], y[e]); hi[e] = fmaxf(hi[e], y[e]); }
+      }
+      if (r < old ? grown : (r < fill || !old)) {   // slots behind the tokens of a page that this call opens are zero
+        u2 w;
+        w[0] = pack4(y);
+        w[1] = pack4(y + 4);
+        *row = w;
+      }
+    }
+  }
+  if (lane == 0) *scale_at = s;
+  if (side == 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float l = lo[e], u = hi[e];
+      for (uint32_t k = 1; k < RP; ++k) {
+        l = fminf(l, __shfl(lo[e], cg + k * CG));
+        u = fmaxf(u, __shfl(hi[e], cg + k * CG));
+      }
+      lo[e] = l;
+      hi[e] = u;
+    }
+    if (lane < (int)CG) {   // rounding is monotonic: the smallest value's code is the smallest code
+      uint32_t wl[2] = {0, 0}, wh[2] = {0, 0};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool any = lo[e] <= hi[e];
+        const uint32_t two = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(any ? lo[e] : 0.f, any ? hi[e] : 0.f, 0, false);
+        const int li = (int)floorf(__builtin_amdgcn_cvt_f32_fp8((int)two, 0) * 0.25f), hi_i = (int)ceilf(__builtin_amdgcn_cvt_f32_fp8((int)two, 1) * 0.25f);
+        wl[e >> 2] |= (uint32_t)(li & 0xff) << (8 * (e & 3));
+        wh[e >> 2] |= (uint32_t)(hi_i & 0xff) << (8 * (e & 3));
+      }
+      u2 w;
+      w[0] = wl[0]; w[1] = wl[1];
+      *reinterpret_cast<u2*>(rec + c.low + (uint64_t)h * D + cg * 8) = w;
+      w[0] = wh[0]; w[1] = wh[1];
+      *reinterpret_cast<u2*>(rec + c.high + (uint64_t)h * D + cg * 8) = w;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// attention
+// ------------------------------------------------------------------------------------------------
+struct AttendArgs {
+  Cache c;
+  Seqs s;
+  const void* q;
+  void* out;
+  float* lse;                 // natural logarithm, for the caller (may be null)
+  float* lse2;                // [n_tokens][H G] base 2, for the weights (may be null)
+  uint64_t q_token, q_head, o_token, o_head;
+  uint32_t G, tiles_x, splits;
+  float scale2;               // scale * log2(e)
+  uint32_t causal, q_vec, o_vec;
+  const int32_t* sel;         // [n_tokens][H][count] pages of every query token, or null
+  uint32_t count;
+  float* part_o;              // [splits][n_tokens * H * G][D]
+  float* part_l;              // [splits][n_tokens * H * G]
+  const float* w_in;          // [n_seqs][H][w_stride]
+  float* w_out;
+  uint64_t wi_seq, wi_head, wo_seq, wo_head;
+  uint32_t w_width;
+};
+
+template <class E> struct Frag;
+template <> struct Frag<_Float16> {
+  typedef h8 v8;
+  template <bool HI> static __device__ __forceinline__ h2 pk(uint32_t w) { return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HI); }
+  static __device__ __forceinline__ f4 mfma(v8 a, v8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Frag<__bf16> {
+  typedef b8 v8;
+  template <bool HI> static __device__ __forceinline__ b2 pk(uint32_t w) { return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HI); }
+  static __device__ __forceinline__ f4 mfma(v8 a, v8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+// 8 codes as 8 numbers of the query's type: e4m3 fits both exactly
+template <class E>
+__device__ __forceinline__ typename Frag<E>::v8 codes8(uint32_t w0, uint32_t w1) {
+  typename Frag<E>::v8 r;
+  const auto a = Frag<E>::template pk<false>(w0), b = Frag<E>::template pk<true>(w0), c = Frag<E>::template pk<false>(w1), d = Frag<E>::template pk<true>(w1);
+  r[0] = a[0]; r[1] = a[1]; r[2] = b[0]; r[3] = b[1]; r[4] = c[0]; r[5] = c[1]; r[6] = d[0]; r[7] = d[1];
+  return r;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// the four lanes that share a column of a 16 x 16 result: l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float column_max(float v) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float column_sum(float v) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <class E>
+__device__ __forceinline__ typename Frag<E>::v8 load_q8(const E* p, bool ok, bool vec) {
+  typename Frag<E>::v8 r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = (E)0.f;
+  if (ok) {
+    if (vec) {
+      r = *reinterpret_cast<const typename Frag<E>::v8*>(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] = p[i];
+    }
+  }
+  return r;
+}
+
+// Softmax and both products in one pass over the keys.  S^T = K Q^T and O^T = V^T P^T on 16 x 16 x 32 matrix
+// instructions: a lane's column is one query row in both, so the row's maximum, sum and rescaling need no data from
+// other rows, and S^T leaves the first product in the very lanes and order in which the second one wants P^T if the
+// 32 keys of a step are numbered (two tiles of 16) x (four lane groups) x 4 -- an order that sums do not see.  K and V
+// come as rows of codes straight into registers; V's bytes are interleaved token against token on the way to pairs.
+// P is rounded to 16-bit floats with 11 bits of mantissa at 2^14 times its value relative to the row's maximum so
+// far, normal down to 2^-28 of it; V's codes are multiplied there by their block's scale over a reference that moves
+// only when the scales leave 2^+-6 of it.  Sums, maxima and the accumulators are 32 bits wide.
+template <class E, int DP, int NQ, int KVW, bool SEL>
+__global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
+  constexpr int KK = DP / 32, KW = DP / 16, VJ = DP / 16, VW = DP / 64;
+  constexpr uint32_t TR = 16 * NQ * (4 / KVW);
+  typedef typename Frag<E>::v8 v8;
+  __shared__ float sm_o[KVW > 1 ? KVW * 16 * NQ * (DP + 4) : 1];
+  __shared__ float sm_m[KVW > 1 ? KVW * 16 * NQ : 1], sm_l[KVW > 1 ? KVW * 16 * NQ : 1];
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const uint32_t wave = uniform(threadIdx.x >> 6), H = a.c.H, G = a.G, T = a.c.T, D = a.c.D;
+  const uint32_t h = blockIdx.x % H, rest = blockIdx.x / H, split = rest / a.tiles_x, x = rest - split * a.tiles_x;
+
+  uint32_t b, tile, first, n, len, r0, rows, tok0 = 0;
+  if constexpr (SEL) {
+    const uint32_t per = (G + TR - 1) / TR, t = x / per;
+    const auto items = [&](uint32_t q) { uint32_t f, m; seq_tokens(a.s, q, f, m); return m; };
+    if (!find_seq(a.s.n_seqs, t, items, b, tok0)) return;
+    b = uniform(b); tok0 = uniform(tok0);
+    tile = x - t * per;
+  } else {
+    const auto items = [&](uint32_t q) { uint32_t f, m; seq_tokens(a.s, q, f, m); return (m * G + TR - 1) / TR; };
+    if (!find_seq(a.s.n_seqs, x, items, b, tile)) return;
+    b = uniform(b); tile = uniform(tile);
+  }
+  seq_tokens(a.s, b, first, n);
+  first = uniform(first); n = uniform(n);
+  len = uniform(seq_len(a.s, T, b));
+  // rows of this workgroup: (query token, head of the group), tokens first
+  if constexpr (SEL) { r0 = tok0 * G + tile * TR; rows = (tok0 + 1) * G; } else { r0 = tile * TR; rows = n * G; }
+  const uint32_t wr0 = r0 + (KVW == 1 ? wave * 16 * NQ : 0);
+  const auto limit = [&](uint32_t r) -> uint32_t {   // keys that row r sees
+    if (r >= rows) return 0;
+    if (!a.causal) return len;
+    const int64_t l = (int64_t)len - n + r / G + 1;
+    return l > 0 ? (uint32_t)l : 0;
+  };
+  const uint32_t last_row = wr0 + 16 * NQ - 1 < rows ? wr0 + 16 * NQ - 1 : rows - 1;
+  const uint32_t l_min = uniform(wr0 < rows ? limit(wr0) : 0), l_max = uniform(wr0 < rows ? limit(last_row) : 0);
+
+  v8 qf[NQ][KK];
+  uint32_t lim[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const uint32_t r = wr0 + q * 16 + c;
+    lim[q] = limit(r);
+    const uint32_t i = r / G;
+    const E* p = reinterpret_cast<const E*>(a.q) + (uint64_t)(first + i) * a.q_token + (uint64_t)(h * G + (r - i * G)) * a.q_head;
+#pragma unroll
+    for (int k = 0; k < KK; ++k) {
+      const uint32_t d = g * (DP / 4) + k * 8;
+      qf[q][k] = load_q8<E>(p + d, r < rows && d < D, a.q_vec);
+    }
+  }
+
+  f4 o[NQ][VJ];
+  float m[NQ], l[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    m[q] = -kInf;
+    l[q] = 0.f;
+#pragma unroll
+    for (int j = 0; j < VJ; ++j) o[q][j] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  float vref = 0.f;
+
+  // The keys of this split, in steps of 32.  The host knows how many splits there are, the device how long the sequence
+  // is: every split takes an equal share of it in whole rounds of the workgroup's wavefronts.
+  const uint32_t space = SEL ? a.count * T : l_max, share = KVW * 32 * ((space + a.splits * KVW * 32 - 1) / (a.splits * KVW * 32));
+  const uint64_t k0_64 = (uint64_t)split * share;
+  const uint32_t k0 = k0_64 < space ? (uint32_t)k0_64 : space, k1 = share < space - k0 ? k0 + share : space;
+  const int32_t* table = a.s.table + b * a.s.table_stride;
+  const int32_t* sel = SEL ? a.sel + ((uint64_t)(first + tok0) * H + h) * a.count : nullptr;
+  for (uint32_t k = k0 + (KVW > 1 ? wave * 32 : 0); k < k1; k += 32 * KVW) {
+    uint32_t pos[2];
+    const uint8_t* rec[2];
+    uint32_t slot[2];
+    bool ok[2];
+    float ks[2], vs[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint32_t v = k + 16 * t, j = v / T, off = v - j * T;
+      uint32_t at = j;
+      ok[t] = v < space;
+      if (SEL) {
+        const int32_t sj = ok[t] ? sel[j] : -1;
+        ok[t] = sj >= 0 && (uint32_t)sj < a.s.width;
+        at = ok[t] ? (uint32_t)sj : 0;
+      }
+      pos[t] = at * T + off;
+      ok[t] = ok[t] && pos[t] < l_max;
+      const int32_t pg = ok[t] ? table[at] : 0;
+      if (pg < 0 || (uint32_t)pg >= a.c.n_pages) { ok[t] = false; if (lane == 0) report(a.s.status); }
+      rec[t] = a.c.pages + (ok[t] ? (uint64_t)pg * a.c.stride : 0);
+      slot[t] = off;
+      const float* sc = reinterpret_cast<const float*>(rec[t] + a.c.scales) + 2 * h;
+      ks[t] = sc[0];
+      vs[t] = sc[1];
+    }
+    if (!ok[0] && !ok[1]) continue;
+    uint32_t kw[2][KW], vw[8][VW];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint8_t* base = rec[t] + (uint64_t)(h * T + slot[t]) * D;
+      const uint32_t d = g * (DP / 4);
+#pragma unroll
+      for (int i = 0; i < KW / 4; ++i) {
+        u32x4 w = {0, 0, 0, 0};
+        if (d + 16 * i < D) w = *reinterpret_cast<const u32x4*>(base + c * D + d + 16 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) kw[t][4 * i + e] = w[e];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* p = base + a.c.side + (4 * g + i) * D + c * VJ;
+        const bool in = (uint32_t)(c * VJ) < D;
+#pragma unroll
+        for (int e = 0; e < VW; ++e) vw[4 * t + i][e] = in ? reinterpret_cast<const uint32_t*>(p)[e] : 0;
+      }
+    }
+    const bool masked = !ok[0] || !ok[1] || pos[0] + 16 > l_min || pos[1] + 16 > l_min;
+
+    f4 s[NQ][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) s[q][t] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        const v8 kf = codes8<E>(kw[t][2 * kk], kw[t][2 * kk + 1]);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) s[q][t] = Frag<E>::mfma(kf, qf[q][kk], s[q][t]);
+      }
+    }
+
+    if (masked) {
+      // A row that does not see a key must not see its value either, and 0 * NaN is NaN: values nobody sees become
+      // zero, and a NaN that some rows see goes into their sums by hand.
+      uint32_t seen_nan = 0;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t p = pos[t] + 4 * g + i;
+          const bool keep = ok[t] && p < l_max;
+#pragma unroll
+          for (int e = 0; e < VW; ++e) {
+            uint32_t w = keep ? vw[4 * t + i][e] : 0;
+            const uint32_t mag = w & 0x7f7f7f7fu;
+            const uint32_t nan = (mag + 0x01010101u) & 0x80808080u;   // bytes whose magnitude is 0x7f
+            seen_nan |= nan;
+            w &= ~((nan >> 7) * 0xffu);
+            vw[4 * t + i][e] = w;
+          }
+        }
+      if (__ballot(seen_nan != 0)) {
+        for (int t = 0; t < 2; ++t) {
+          if (!ok[t]) continue;
+          const uint8_t* base = rec[t] + a.c.side + (uint64_t)(h * T + slot[t]) * D;
+          for (uint32_t kx = 0; kx < 16 && pos[t] + kx < l_max; ++kx)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int j = 0; j < VJ; ++j) {
+                const uint32_t d = (4 * g + i) * VJ + j;
+                if (d < D && (base[kx * D + d] & 0x7f) == 0x7f) {
+#pragma unroll
+                  for (int q = 0; q < NQ; ++q)
+                    if (pos[t] + kx < lim[q]) o[q][j][i] = kNan;
+                }
+              }
+        }
+      }
+    }
+
+    const float vmax = fmaxf(vs[0], vs[1]);
+    if (vmax > 0.f && !(vmax <= vref * 64.f && vmax * 64.f >= vref)) {
+      const float f = vref > 0.f ? vref / vmax : 0.f;
+      if (vref > 0.f) {
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int j = 0; j < VJ; ++j) o[q][j] *= f;
+      }
+      vref = vmax;
+    }
+    const float inv_ref = inverse(vref);
+
+    h8 pf[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      float xs[8], mx = -kInf;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v = s[q][t][i] * (ks[t] * a.scale2);
+          if (masked && !(ok[t] && pos[t] + 4 * g + i < lim[q])) v = -kInf;
+          xs[4 * t + i] = v;
+          mx = fmaxf(mx, v);
+        }
+      mx = column_max(mx);
+      const float mn = fmaxf(m[q], mx), ref = mn == -kInf ? 0.f : mn - 14.f;
+      const float alpha = exp2_fast(m[q] - (mn == -kInf ? 0.f : mn));
+      m[q] = mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float p = exp2_fast(xs[i] - ref);
+        sum += p;
+        pf[q][i] = (_Float16)p;
+      }
+      l[q] = l[q] * alpha + sum;
+      if (__ballot(alpha != 1.f)) {
+#pragma unroll
+        for (int j = 0; j < VJ; ++j) o[q][j] *= alpha;
+      }
+    }
+
+    h8 vf[VJ];
+    const float f0 = vs[0] * inv_ref, f1 = vs[1] * inv_ref;
+#pragma unroll
+    for (int pr = 0; pr < 4; ++pr) {
+      const float f = pr < 2 ? f0 : f1;
+#pragma unroll
+      for (int e = 0; e < VW; ++e) {
+        const uint32_t lo = __builtin_amdgcn_perm(vw[2 * pr + 1][e], vw[2 * pr][e], 0x05010400u), hi = __builtin_amdgcn_perm(vw[2 * pr + 1][e], vw[2 * pr][e], 0x07030602u);
+        const h2 x0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, f, false), x1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, f, true);
+        const h2 x2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, f, false), x3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, f, true);
+        vf[4 * e][2 * pr] = x0[0]; vf[4 * e][2 * pr + 1] = x0[1];
+        vf[4 * e + 1][2 * pr] = x1[0]; vf[4 * e + 1][2 * pr + 1] = x1[1];
+        vf[4 * e + 2][2 * pr] = x2[0]; vf[4 * e + 2][2 * pr + 1] = x2[1];
+        vf[4 * e + 3][2 * pr] = x3[0]; vf[4 * e + 3][2 * pr + 1] = x3[1];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < VJ; ++j)
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) o[q][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[j], pf[q], o[q][j], 0, 0, 0);
+  }
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) l[q] = column_sum(l[q]);
+
+  // a row's result: dims [d, d + 4 VJ) of lane group g, in order i, j
+  const uint64_t row_out = (uint64_t)a.s.n_tokens * H * G;
+  const auto emit = [&](uint32_t r, float mm, float ll, const float* v, uint32_t d, uint32_t cnt, bool head) {
+    const uint32_t i = r / G;
+    const uint64_t tok = first + i, hq = h * G + (r - i * G);
+    const float lg = ll > 0.f ? mm + __builtin_amdgcn_logf(ll) - 14.f : (ll == 0.f ? -kInf : kNan);
+    if (a.splits > 1) {
+      const uint64_t at = split * row_out + tok * H * G + hq;
+      if (head) a.part_l[at] = lg;
+      for (uint32_t e = 0; e < cnt; ++e)
+        if (d + e < D) a.part_o[at * D + d + e] = v[e];
+    } else {
+      if (head) {
+        if (a.lse) a.lse[tok * H * G + hq] = lg * 0.6931471805599453f;
+        if (a.lse2) a.lse2[tok * H * G + hq] = lg;
+      }
+      E* p = reinterpret_cast<E*>(a.out) + tok * a.o_token + hq * a.o_head;
+      for (uint32_t e = 0; e < cnt; ++e)
+        if (d + e < D) p[d + e] = (E)v[e];
+    }
+  };
+
+  if constexpr (KVW == 1) {
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const uint32_t r = wr0 + q * 16 + c;
+      const float f = l[q] == 0.f ? 0.f : vref / l[q];
+      float v[4 * VJ];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < VJ; ++j) v[i * VJ + j] = o[q][j][i] * f;
+      if (r < rows) emit(r, m[q], l[q], v, g * 4 * VJ, 4 * VJ, g == 0);
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const int w = (int)wave * 16 * NQ + q * 16 + c;
+      if (g == 0) { sm_m[w] = m[q]; sm_l[w] = l[q]; }
+      float* p = sm_o + w * (DP + 4) + g * 4 * VJ;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < VJ; ++j) p[i * VJ + j] = o[q][j][i] * vref;
+    }
+    __syncthreads();
+    for (uint32_t u = threadIdx.x; u < 16 * NQ * (DP / 8); u += 256) {
+      const uint32_t rr = u / (DP / 8), d = (u - rr * (DP / 8)) * 8, r = r0 + rr;
+      if (r >= rows || d >= D) continue;
+      float mm = -kInf, ll = 0.f, v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 0.f;
+      for (int w = 0; w < KVW; ++w) mm = fmaxf(mm, sm_m[w * 16 * NQ + rr]);
+      for (int w = 0; w < KVW; ++w) {
+        const float f = mm == -kInf ? 1.f : exp2_fast(sm_m[w * 16 * NQ + rr] - mm);
+        ll += sm_l[w * 16 * NQ + rr] * f;
+        const float* p = sm_o + (w * 16 * NQ + rr) * (DP + 4) + d;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += p[e] * f;
+      }
+      const float f = ll == 0.f ? 0.f : 1.f / ll;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= f;
+      emit(r, mm, ll, v, d, 8, d == 0);
+    }
+  }
+}
+
+// The splits' results of every row, weighted by what their shares of the keys add up to.  Same rows per workgroup as
+// in fl_kv_attend: rows of no sequence are not touched.
+template <class E, bool SEL>
+__global__ __launch_bounds__(256) void fl_kv_join(const AttendArgs a, uint32_t TR) {
+  const uint32_t H = a.c.H, G = a.G, D = a.c.D, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t h = blockIdx.x % H, x = blockIdx.x / H;
+  uint32_t b, tile, first, n, r0, rows, tok0 = 0;
+  if constexpr (SEL) {
+    const uint32_t per = (G + TR - 1) / TR, t = x / per;
+    const auto items = [&](uint32_t q) { uint32_t f, m; seq_tokens(a.s, q, f, m); return m; };
+    if (!find_seq(a.s.n_seqs, t, items, b, tok0)) return;
+    tile = x - t * per;
+  } else {
+    const auto items = [&](uint32_t q) { uint32_t f, m; seq_tokens(a.s, q, f, m); return (m * G + TR - 1) / TR; };
+    if (!find_seq(a.s.n_seqs, x, items, b, tile)) return;
+  }
+  seq_tokens(a.s, b, first, n);
+  if constexpr (SEL) { r0 = tok0 * G + tile * TR; rows = (tok0 + 1) * G; } else { r0 = tile * TR; rows = n * G; }
+  const uint64_t row_out = (uint64_t)a.s.n_tokens * H * G;
+  for (uint32_t r = r0 + wave; r < r0 + TR && r < rows; r += 4) {
+    const uint32_t i = r / G;
+    const uint64_t tok = first + i, hq = h * G + (r - i * G), at = tok * H * G + hq;
+    float top = -kInf, bad = 0.f;
+    for (uint32_t s = lane; s < a.splits; s += 64) {
+      const float v = a.part_l[s * row_out + at];
+      top = fmaxf(top, v);
+      bad += v != v ? 1.f : 0.f;
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) { top = fmaxf(top, __shfl_xor(top, o)); bad += __shfl_xor(bad, o); }
+    float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    if (top != -kInf || bad > 0.f) {
+      for (uint32_t s = 0; s < a.splits; ++s) {
+        const float v = a.part_l[s * row_out + at];
+        if (v == -kInf) continue;
+        const float w = exp2_fast(v - (top == -kInf ? 0.f : top));
+        sum += w;
+        const float* p = a.part_o + (s * row_out + at) * D;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (lane + 64 * e < D) acc[e] += p[lane + 64 * e] * w;
+      }
+    }
+    const float f = sum == 0.f ? 0.f : 1.f / sum, lg = sum == 0.f ? -kInf : top + __builtin_amdgcn_logf(sum);
+    if (lane == 0) {
+      if (a.lse) a.lse[at] = lg * 0.6931471805599453f;
+      if (a.lse2) a.lse2[at] = lg;
+    }
+    E* p = reinterpret_cast<E*>(a.out) + tok * a.o_token + hq * a.o_head;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (lane + 64 * e < D) p[lane + 64 * e] = (E)(acc[e] * f);
+  }
+}
+
+// What every key of a sequence was worth to the call's queries: the probabilities exp2(s - lse) summed over the rows of
+// its key-value head, on top of w_in.  One wavefront owns 64 keys and walks over all rows, so the sums need no atomics.
+template <class E, int DP>
+__global__ __launch_bounds__(256) void fl_kv_weights(const AttendArgs a) {
+  constexpr int KK = DP / 32, KW = DP / 16;
+  typedef typename Frag<E>::v8 v8;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const uint32_t wave = uniform(threadIdx.x >> 6), H = a.c.H, G = a.G, T = a.c.T, D = a.c.D, h = blockIdx.y, b = blockIdx.z;
+  const uint32_t k0 = (blockIdx.x * 4 + wave) * 64;
+  uint32_t first, n;
+  seq_tokens(a.s, b, first, n);
+  first = uniform(first); n = uniform(n);
+  const uint32_t len = uniform(seq_len(a.s, T, b)), rows = n * G;
+  const float* w_in = a.w_in ? a.w_in + b * a.wi_seq + h * a.wi_head : nullptr;
+  float* w_out = a.w_out + b * a.wo_seq + h * a.wo_head;
+  if (len > a.w_width && lane == 0) report(a.s.status);
+  const int32_t* table = a.s.table + b * a.s.table_stride;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const uint32_t v = k0 + 16 * t, j = v / T, off = v - j * T;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    if (v < len && rows) {
+      const int32_t pg = table[j];
+      if (pg < 0 || (uint32_t)pg >= a.c.n_pages) {
+        if (lane == 0) report(a.s.status);
+      } else {
+        const uint8_t* rec = a.c.pages + (uint64_t)pg * a.c.stride;
+        const float kc = reinterpret_cast<const float*>(rec + a.c.scales)[2 * h] * a.scale2;
+        const uint8_t* base = rec + (uint64_t)(h * T + off + c) * D;
+        const uint32_t d0 = g * (DP / 4);
+        v8 kf[KK];
+#pragma unroll
+        for (int i = 0; i < KW / 4; ++i) {
+          u32x4 w = {0, 0, 0, 0};
+          if (d0 + 16 * i < D) w = *reinterpret_cast<const u32x4*>(base + d0 + 16 * i);
+          kf[2 * i] = codes8<E>(w[0], w[1]);
+          kf[2 * i + 1] = codes8<E>(w[2], w[3]);
+        }
+        for (uint32_t r0 = 0; r0 < rows; r0 += 16) {
+          const uint32_t r = r0 + c, i = r / G;
+          const bool in = r < rows;
+          const uint64_t tok = first + i, hq = h * G + (r - i * G);
+          const E* p = reinterpret_cast<const E*>(a.q) + tok * a.q_token + hq * a.q_head;
+          f4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < KK; ++k) s = Frag<E>::mfma(kf[k], load_q8<E>(p + d0 + k * 8, in && d0 + k * 8 < D, a.q_vec), s);
+          int64_t lim = !in ? 0 : a.causal ? (int64_t)len - n + i + 1 : len;
+          const float lg = in ? a.lse2[tok * H * G + hq] : 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if ((int64_t)(v + 4 * g + e) < lim) acc[e] += exp2_fast(s[e] * kc - lg);
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+#pragma unroll
+      for (int o = 8; o; o >>= 1) acc[e] += __shfl_xor(acc[e], o);
+      const uint32_t p = v + 4 * g + e;
+      if (c == 0 && p < a.w_width && (p < len || w_in != w_out)) w_out[p] = (w_in ? w_in[p] : 0.f) + (p < len ? acc[e] : 0.f);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// the choice of pages, and of tokens
+// ------------------------------------------------------------------------------------------------
+struct SelectArgs {
+  Cache c;
+  Seqs s;
+  const void* q;
+  uint64_t q_token, q_head;
+  uint32_t G, causal, q_vec, first, last, count;
+  float* scores;              // [n_tokens][H][width]
+  int32_t* out;               // [n_tokens][H][count]
+};
+
+__device__ __forceinline__ uint32_t token_limit(const SelectArgs& a, uint32_t len, uint32_t n, uint32_t i) {
+  if (!a.causal) return len;
+  const int64_t l = (int64_t)len - n + i + 1;
+  return l > 0 ? (uint32_t)l : 0;
+}
+
+// score(page) = max over the group's heads of ks * qs * sum_d q8_d (q8_d > 0 ? high_d : low_d): an estimate of the
+// largest product that a key of the page can have with the query, in whole numbers (8-bit queries against the page's
+// 8-bit bounds), so equal scores are equal and the choice does not depend on the order of a sum.  The sum splits into
+// max(q8, 0) . high + min(q8, 0) . low, two runs of 16 x 16 x 64 integer matrix instructions whose operands are the
+// bytes of the record as they lie.
+template <class E, int DP>
+__global__ __launch_bounds__(256) void fl_kv_score(const SelectArgs a) {
+  constexpr int KK = DP / 64;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const uint32_t wave = uniform(threadIdx.x >> 6), H = a.c.H, G = a.G, T = a.c.T, D = a.c.D, h = blockIdx.y;
+  uint32_t b, i, first, n;
+  const auto items = [&](uint32_t q) { uint32_t f, m; seq_tokens(a.s, q, f, m); return m; };
+  if (!find_seq(a.s.n_seqs, blockIdx.z, items, b, i)) return;
+  b = uniform(b);
+  seq_tokens(a.s, b, first, n);
+  const uint32_t lim = token_limit(a, seq_len(a.s, T, b), n, i), pages = (lim + T - 1) / T;
+  const uint32_t p0 = (blockIdx.x * 4 + wave) * 64;
+  if (p0 >= pages) return;
+  const uint64_t tok = first + i;
+  float best[4][4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) best[t][e] = -kInf;
+  const int32_t* table = a.s.table + b * a.s.table_stride;
+  const uint8_t* rec[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const uint32_t p = p0 + 16 * t + c;
+    const int32_t pg = p < pages ? table[p] : 0;
+    const bool ok = pg >= 0 && (uint32_t)pg < a.c.n_pages;
+    if (!ok) report(a.s.status);
+    rec[t] = ok ? a.c.pages + (uint64_t)pg * a.c.stride : nullptr;
+  }
+  for (uint32_t h0 = 0; h0 < G; h0 += 16) {
+    const bool in = h0 + c < G;
+    const E* q = reinterpret_cast<const E*>(a.q) + tok * a.q_token + (uint64_t)(h * G + h0 + c) * a.q_head;
+    float x[KK][16], amax = 0.f;
+#pragma unroll
+    for (int k = 0; k < KK; ++k)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t d = k * 64 + g * 16 + u * 8;
+        const typename Frag<E>::v8 w = load_q8<E>(q + d, in && d < D, a.q_vec);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float v = (float)w[e];
+          if (!__builtin_isfinite(v)) v = 0.f;
+          x[k][8 * u + e] = v;
+          amax = fmaxf(amax, fabsf(v));
+        }
+      }
+    amax = column_max(amax);
+    float step = 0.f;   // smallest 2^e >= amax / 127, 127 = 1.984375 * 2^6
+    if (amax > 0.f) {
+      const uint32_t u = __float_as_uint(amax);
+      int e = (int)(u >> 23) - 127 - ((u & 0x7fffffu) <= 0x7e0000u ? 6 : 5);
+      if (e < -126 || u < 0x800000u) e = -126;
+      step = pow2f(e);
+    }
+    const float inv = inverse(step);
+    i4 up[KK], dn[KK];
+#pragma unroll
+    for (int k = 0; k < KK; ++k)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t pu = 0, pd = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int v = (int)rintf(x[k][4 * w + e] * inv);
+          pu |= (uint32_t)(v > 0 ? v : 0) << (8 * e);
+          pd |= (uint32_t)((v < 0 ? v : 0) & 0xff) << (8 * e);
+        }
+        up[k][w] = (int)pu;
+        dn[k][w] = (int)pd;
+      }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if (p0 + 16 * t >= pages) break;
+      i4 sum = {0, 0, 0, 0};
+#pragma unroll
+      for (int k = 0; k < KK; ++k) {
+        const uint32_t d = k * 64 + g * 16;
+        i4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+        if (rec[t] && d < D) {
+          lo = *reinterpret_cast<const i4*>(rec[t] + a.c.low + (uint64_t)h * D + d);
+          hi = *reinterpret_cast<const i4*>(rec[t] + a.c.high + (uint64_t)h * D + d);
+        }
+        sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(hi, up[k], sum, 0, 0, 0);
+        sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(lo, dn[k], sum, 0, 0, 0);
+      }
+      // row 4 g + e: a page; column c: a head
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (in) best[t][e] = fmaxf(best[t][e], (float)sum[e] * step);
+    }
+  }
+  float* out = a.scores + (tok * H + h) * a.s.width;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float v = best[t][e];
+#pragma unroll
+      for (int o = 8; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+      const uint32_t p = p0 + 16 * t + 4 * g + e;
+      if (c == 0 && p < pages) {
+        const int32_t pg = table[p];
+        const bool ok = pg >= 0 && (uint32_t)pg < a.c.n_pages;
+        out[p] = ok ? v * reinterpret_cast<const float*>(a.c.pages + (uint64_t)pg * a.c.stride + a.c.scales)[2 * h] : -kInf;
+      }
+    }
+}
+
+// Numbers in their order as unsigned integers; NaN before all of them, what has to stay behind.
+__device__ __forceinline__ uint32_t order_key(float f) {
+  if (f != f) return 0;
+  uint32_t u = __float_as_uint(f);
+  if (u == 0x80000000u) u = 0;
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+struct Pick { uint32_t key, need; };
+
+// The k-th largest of n keys (k < n), by its bytes from the top: key, and how many of its equals belong to the k.
+// One workgroup of 1024.
+template <class Key>
+__device__ Pick kth_largest(uint32_t n, uint32_t k, Key key, uint32_t* hist, uint32_t* word) {
+  uint32_t prefix = 0, mask = 0;
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    if (threadIdx.x < 256) hist[threadIdx.x] = 0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += 1024) {
+      const uint32_t u = key(i);
+      if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift) & 255], 1u);
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {   // lane l looks at bins 255 - 4 l ... 252 - 4 l
+      const uint32_t l = threadIdx.x;
+      uint32_t cnt[4], sum = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { cnt[e] = hist[255 - 4 * l - e]; sum += cnt[e]; }
+      const uint32_t incl = wave_incl_sum_u32(sum, (int)l);
+      uint32_t before = incl - sum;
+      if (before < k && k <= incl) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (before < k && k <= before + cnt[e]) { word[0] = 255 - 4 * l - e; word[1] = k - before; }
+          before += cnt[e];
+        }
+      }
+    }
+    __syncthreads();
+    prefix |= word[0] << shift;
+    mask |= 255u << shift;
+    k = word[1];
+    __syncthreads();
+  }
+  return {prefix, k};
+}
+
+// Indices of the keys above the pick and of the first `need` equal to it, in ascending order.
+template <class Key, class Put>
+__device__ void put_picked(uint32_t n, Pick pick, Key key, Put put, uint32_t* sums) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t above = 0, equal = 0;   // in all rounds so far
+  for (uint32_t base = 0; base < n; base += 1024) {
+    const uint32_t i = base + threadIdx.x;
+    const uint32_t u = i < n ? key(i) : 0;
+    const bool gt = i < n && u > pick.key, eq = i < n && u == pick.key;
+    const uint64_t bg = __ballot(gt), be = __ballot(eq), below = (1ull << lane) - 1;
+    if (lane == 0) { sums[wave] = (uint32_t)__popcll(bg); sums[16 + wave] = (uint32_t)__popcll(be); }
+    __syncthreads();
+    uint32_t g0 = above, e0 = equal;
+    for (uint32_t w = 0; w < 16; ++w) {
+      if (w < wave) { g0 += sums[w]; e0 += sums[16 + w]; }
+      above += sums[w];
+      equal += sums[16 + w];
+    }
+    g0 += (uint32_t)__popcll(bg & below);
+    e0 += (uint32_t)__popcll(be & below);
+    if (gt || (eq && e0 < pick.need)) put(g0 + (e0 < pick.need ? e0 : pick.need), i);
+    __syncthreads();
+  }
+}
+
+__global__ __launch_bounds__(1024) void fl_kv_pick_pages(const SelectArgs a) {
+  __shared__ uint32_t hist[256], word[2], sums[32];
+  const uint32_t h = blockIdx.x % a.c.H, t = blockIdx.x / a.c.H;
+  uint32_t b, i, first, n;
+  const auto items = [&](uint32_t q) { uint32_t f, m; seq_tokens(a.s, q, f, m); return m; };
+  if (!find_seq(a.s.n_seqs, t, items, b, i)) return;
+  seq_tokens(a.s, b, first, n);
+  const uint32_t lim = token_limit(a, seq_len(a.s, a.c.T, b), n, i), pages = (lim + a.c.T - 1) / a.c.T;
+  const uint64_t row = (uint64_t)(first + i) * a.c.H + h;
+  const float* score = a.scores + row * a.s.width;
+  int32_t* out = a.out + row * a.count;
+  for (uint32_t k = (pages < a.count ? pages : a.count) + threadIdx.x; k < a.count; k += 1024) out[k] = -1;
+  if (pages <= a.count) {
+    for (uint32_t k = threadIdx.x; k < pages; k += 1024) out[k] = (int32_t)k;
+    return;
+  }
+  const auto key = [&](uint32_t p) { return p < a.first || p + a.last >= pages ? 0xffffffffu : order_key(score[p]); };
+  const Pick pick = kth_largest(pages, a.count, key, hist, word);
+  put_picked(pages, pick, key, [&](uint32_t at, uint32_t p) { out[at] = (int32_t)p; }, sums);
+}
+
+struct KeepArgs {
+  Seqs s;
+  uint32_t T, H, budget, first, recent, w_width, nw_width;
+  const float* w;
+  uint64_t w_seq, w_head, nw_seq, nw_head, kept_stride;
+  float* nw;
+  int32_t* kept;
+  int32_t* new_lens;
+};
+
+__global__ __launch_bounds__(1024) void fl_kv_keep(const KeepArgs a) {
+  __shared__ uint32_t hist[256], word[2], sums[32];
+  const uint32_t h = blockIdx.x % a.H, b = blockIdx.x / a.H;
+  uint32_t len = seq_len(a.s, a.T, b);
+  if (len > a.w_width) { if (threadIdx.x == 0) report(a.s.status); len = a.w_width; }
+  const float* w = a.w + b * a.w_seq + h * a.w_head;
+  float* nw = a.nw + b * a.nw_seq + h * a.nw_head;
+  int32_t* kept = a.kept + ((uint64_t)b * a.H + h) * a.kept_stride;
+  const uint32_t m = len < a.budget ? len : a.budget;
+  if (h == 0 && threadIdx.x == 0) a.new_lens[b] = (int32_t)m;
+  for (uint32_t k = m + threadIdx.x; k < a.budget; k += 1024) kept[k] = -1;
+  for (uint32_t k = m + threadIdx.x; k < a.nw_width; k += 1024) nw[k] = 0.f;
+  if (len <= a.budget) {
+    for (uint32_t k = threadIdx.x; k < len; k += 1024) { kept[k] = (int32_t)k; nw[k] = w[k]; }
+    return;
+  }
+  const auto key = [&](uint32_t p) { return p < a.first || p + a.recent >= len ? 0xffffffffu : order_key(w[p]); };
+  const Pick pick = kth_largest(len, m, key, hist, word);
+  put_picked(len, pick, key, [&](uint32_t at, uint32_t p) { kept[at] = (int32_t)p; nw[at] = w[p]; }, sums);
+}
+
+// ------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------
+bool aligned(const void* p, uint64_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+int check_cache(const flh_kv_cache* k, Cache* c, const char* what) {
+  if (!k->d_pages || !aligned(k->d_pages, 16)) return fl_set_error(FLH_E_ARG, "%s: the pool must be a 16-byte aligned device pointer", what);
+  if (k->tokens == 0 || k->tokens % 16 || k->tokens > 256) return fl_set_error(FLH_E_ARG, "%s: %u tokens a page (a multiple of 16, up to 256)", what, k->tokens);
+  if (k->dim == 0 || k->dim % 16 || k->dim > 256) return fl_set_error(FLH_E_ARG, "%s: head dim %u (a multiple of 16, up to 256)", what, k->dim);
+  if (k->heads == 0 || k->heads > 1024) return fl_set_error(FLH_E_ARG, "%s: %u heads (1..1024)", what, k->heads);
+  if (k->n_pages == 0 || k->n_pages > 0x7fffffffu) return fl_set_error(FLH_E_ARG, "%s: %u pages", what, k->n_pages);
+  const uint64_t need = flh_kv_page_bytes(k->tokens, k->heads, k->dim);
+  if (k->page_stride < need || k->page_stride % 16)
+    return fl_set_error(FLH_E_ARG, "%s: page stride %llu (a multiple of 16, at least %llu)", what, (unsigned long long)k->page_stride, (unsigned long long)need);
+  c->pages = (uint8_t*)k->d_pages;
+  c->stride = k->page_stride;
+  c->n_pages = k->n_pages;
+  c->T = k->tokens;
+  c->H = k->heads;
+  c->D = k->dim;
+  c->side = (uint64_t)c->H * c->T * c->D;
+  c->low = 2 * c->side;
+  c->high = c->low + (uint64_t)c->H * c->D;
+  c->scales = c->high + (uint64_t)c->H * c->D;
+  return FLH_OK;
+}
+
+int check_seqs(const flh_kv_seqs* k, Seqs* s, int32_t* d_status, const char* what) {
+  if (!k->d_lens || !k->d_table || !d_status) return fl_set_error(FLH_E_ARG, "%s: lens, page table and status are required", what);
+  if (k->n_seqs == 0 || k->n_seqs > 65535) return fl_set_error(FLH_E_ARG, "%s: %u sequences (1..65535)", what, k->n_seqs);
+  if (k->table_width == 0 || k->table_stride < k->table_width || k->table_width > (0x7fffffffu >> 8))
+    return fl_set_error(FLH_E_ARG, "%s: page table of %u columns, stride %llu", what, k->table_width, (unsigned long long)k->table_stride);
+  if (k->n_tokens > (1u << 24)) return fl_set_error(FLH_E_ARG, "%s: %u tokens in one call (up to 2^24)", what, k->n_tokens);
+  if (!k->d_starts && k->n_tokens % k->n_seqs) return fl_set_error(FLH_E_ARG, "%s: %u tokens do not divide into %u sequences; give starts", what, k->n_tokens, k->n_seqs);
+  s->starts = k->d_starts;
+  s->lens = k->d_lens;
+  s->table = k->d_table;
+  s->table_stride = k->table_stride;
+  s->width = k->table_width;
+  s->n_seqs = k->n_seqs;
+  s->n_tokens = k->n_tokens;
+  s->per = k->d_starts ? 0 : k->n_tokens / k->n_seqs;
+  s->status = d_status;
+  return FLH_OK;
+}
+
+int finish(const char* what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? FLH_OK : fl_set_error(FLH_E_HIP, "%s: %s", what, hipGetErrorString(e));
+}
+
+constexpr uint64_t kMaxGroups = (1ull << 24) - 1;   // of 256 threads: a launch counts its threads in 32 bits
+
+struct Plan {
+  int dp, nq, kvw;
+  uint32_t tr, tiles_x, splits;
+  uint64_t rows, part_o, part_l, lse2, bytes;
+};
+
+// How a call of flh_kv_attend is cut up; sizes only, so that the workspace can be asked for beforehand.
+int make_plan(const flh_kv_attend_params* p, Plan* pl) {
+  const uint32_t H = p->cache.heads, D = p->cache.dim, G = H ? p->q_heads / H : 0, n = p->seqs.n_tokens, B = p->seqs.n_seqs;
+  if (G == 0 || p->q_heads % H) return fl_set_error(FLH_E_ARG, "flh_kv_attend: %u query heads over %u key-value heads", p->q_heads, H);
+  if ((uint64_t)n * p->q_heads > 0x7fffffffull) return fl_set_error(FLH_E_ARG, "flh_kv_attend: %u tokens of %u heads", n, p->q_heads);
+  pl->dp = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+  const bool sel = p->d_selected != nullptr;
+  const uint64_t rows = sel ? G : ((uint64_t)n * G + B - 1) / B;   // of a sequence, on average
+  pl->kvw = rows <= 32 || sel ? 4 : 1;
+  pl->nq = pl->kvw == 4 ? (rows <= 16 || pl->dp == 256 ? 1 : 2) : (pl->dp == 256 ? 2 : 4);
+  pl->tr = 16 * pl->nq * (4 / pl->kvw);
+  uint64_t tiles, est;
+  if (sel) tiles = est = (uint64_t)n * ((G + pl->tr - 1) / pl->tr);
+  else if (!p->seqs.d_starts) tiles = est = (uint64_t)B * (((uint64_t)(n / B) * G + pl->tr - 1) / pl->tr);
+  else {
+    tiles = (uint64_t)n * G / pl->tr + B;
+    est = (uint64_t)n * G / pl->tr > B ? (uint64_t)n * G / pl->tr : B;
+  }
+  const uint64_t space = sel ? (uint64_t)p->n_selected * p->cache.tokens : (uint64_t)p->seqs.table_width * p->cache.tokens;
+  const uint64_t want = est * H ? (1024 + est * H - 1) / (est * H) : 1, most = (space + 127) / 128;
+  pl->splits = (uint32_t)(want < most ? want : most);
+  if (pl->kvw == 1 || pl->splits < 1) pl->splits = 1;
+  if (tiles * H * pl->splits > kMaxGroups) return fl_set_error(FLH_E_ARG, "flh_kv_attend: too much for one launch");
+  pl->tiles_x = (uint32_t)tiles;
+  pl->rows = (uint64_t)n * p->q_heads;
+  uint64_t at = 0;
+  pl->part_o = at;
+  if (pl->splits > 1) at += pl->splits * pl->rows * D * 4;
+  pl->part_l = at;
+  if (pl->splits > 1) at += pl->splits * pl->rows * 4;
+  pl->lse2 = at;
+  if (p->d_weights) at += pl->rows * 4;
+  pl->bytes = at;
+  return FLH_OK;
+}
+
+template <class E, int DP, int NQ, int KVW>
+void launch_attend(const AttendArgs& a, hipStream_t st) {
+  const dim3 grid(a.tiles_x * a.c.H * a.splits);
+  if (a.tiles_x == 0) return;
+  if constexpr (KVW == 4) {
+    if (a.sel) { FL_LAUNCH((fl_kv_attend<E, DP, NQ, KVW, true>), grid, dim3(256), 0, st, a); return; }
+  }
+  FL_LAUNCH((fl_kv_attend<E, DP, NQ, KVW, false>), grid, dim3(256), 0, st, a);
+}
+
+template <class E>
+void run_attend(const AttendArgs& a, const Plan& pl, hipStream_t st) {
+  if (pl.dp == 64) {
+    if (pl.kvw == 1) launch_attend<E, 64, 4, 1>(a, st);
+    else if (pl.nq == 1) launch_attend<E, 64, 1, 4>(a, st);
+    else launch_attend<E, 64, 2, 4>(a, st);
+  } else if (pl.dp == 128) {
+    if (pl.kvw == 1) launch_attend<E, 128, 4, 1>(a, st);
+    else if (pl.nq == 1) launch_attend<E, 128, 1, 4>(a, st);
+    else launch_attend<E, 128, 2, 4>(a, st);
+  } else {
+    if (pl.kvw == 1) launch_attend<E, 256, 2, 1>(a, st);
+    else launch_attend<E, 256, 1, 4>(a, st);
+  }
+  if (pl.splits > 1 && a.tiles_x) {
+    if (a.sel) FL_LAUNCH((fl_kv_join<E, true>), dim3(a.tiles_x * a.c.H), dim3(256), 0, st, a, pl.tr);
+    else FL_LAUNCH((fl_kv_join<E, false>), dim3(a.tiles_x * a.c.H), dim3(256), 0, st, a, pl.tr);
+  }
+  if (a.w_out) {
+    const uint64_t span = (uint64_t)a.s.width * a.c.T > a.w_width ? (uint64_t)a.s.width * a.c.T : a.w_width;
+    const dim3 grid((uint32_t)((span + 255) / 256), a.c.H, a.s.n_seqs);
+    if (pl.dp == 64) FL_LAUNCH((fl_kv_weights<E, 64>), grid, dim3(256), 0, st, a);
+    else if (pl.dp == 128) FL_LAUNCH((fl_kv_weights<E, 128>), grid, dim3(256), 0, st, a);
+    else FL_LAUNCH((fl_kv_weights<E, 256>), grid, dim3(256), 0, st, a);
+  }
+}
+
+template <class E, bool EVICT>
+void launch_pack(const PackArgs& a, uint32_t items, hipStream_t st) {
+  const uint32_t rp = 64 / (a.c.D / 8);
+  const dim3 grid(items, (2 * a.c.H + 3) / 4);
+  if ((a.c.T + rp - 1) / rp <= (uint32_t)kRows) FL_LAUNCH((fl_kv_pack<E, EVICT, true>), grid, dim3(256), 0, st, a);
+  else FL_LAUNCH((fl_kv_pack<E, EVICT, false>), grid, dim3(256), 0, st, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t flh_kv_page_bytes(uint32_t tokens, uint32_t heads, uint32_t dim) {
+  return (2ull * heads * tokens * dim + 2ull * heads * dim + 8ull * heads + 127) / 128 * 128;
+}
+
+int flh_kv_store(const flh_kv_store_params* p, void* stream) {
+  if (!p) return fl_set_error(FLH_E_ARG, "flh_kv_store: null parameters");
+  PackArgs a;
+  memset(&a, 0, sizeof(a));
+  int rc = check_cache(&p->cache, &a.c, "flh_kv_store");
+  if (!rc) rc = check_seqs(&p->seqs, &a.s, p->d_status, "flh_kv_store");
+  if (rc) return rc;
+  if (p->type > FLH_KV_FP32) return fl_set_error(FLH_E_ARG, "flh_kv_store: type %u", p->type);
+  const uint32_t esz = p->type == FLH_KV_FP32 ? 4 : 2;
+  if (p->seqs.n_tokens && (!p->d_k || !p->d_v || !aligned(p->d_k, esz) || !aligned(p->d_v, esz))) return fl_set_error(FLH_E_ARG, "flh_kv_store: keys and values are required");
+  if (p->seqs.n_tokens == 0) return FLH_OK;
+  if ((rc = fl_need_init())) return rc;
+  a.src[0] = p->d_k;
+  a.src[1] = p->d_v;
+  a.token_stride[0] = p->k_token_stride;
+  a.token_stride[1] = p->v_token_stride;
+  a.head_stride[0] = p->k_head_stride;
+  a.head_stride[1] = p->v_head_stride;
+  const uint64_t unit = 16 / esz, strides = p->k_token_stride | p->v_token_stride | p->k_head_stride | p->v_head_stride;
+  a.vec = aligned(p->d_k, 16) && aligned(p->d_v, 16) && strides % unit == 0;
+  // a sequence's new tokens touch at most n / T + 2 pages
+  const uint32_t items = a.s.n_tokens / a.c.T + 2 * a.s.n_seqs;
+  fl_prof().kid = 8;
+  const hipStream_t st = (hipStream_t)stream;
+  if (p->type == FLH_KV_BF16) launch_pack<__bf16, false>(a, items, st);
+  else if (p->type == FLH_KV_FP16) launch_pack<_Float16, false>(a, items, st);
+  else launch_pack<float, false>(a, items, st);
+  return finish("flh_kv_store");
+}
+
+int64_t flh_kv_attend_workspace_bytes(const flh_kv_attend_params* p) {
+  Plan pl;
+  if (!p) return fl_set_error(FLH_E_ARG, "flh_kv_attend_workspace_bytes: null parameters");
+  if (!p->seqs.n_seqs || !p->cache.tokens) return fl_set_error(FLH_E_ARG, "flh_kv_attend_workspace_bytes: no sequences or no page size");
+  const int rc = make_plan(p, &pl);
+  return rc ? rc : (int64_t)pl.bytes;
+}
+
+int flh_kv_attend(const flh_kv_attend_params* p, void* stream) {
+  if (!p) return fl_set_error(FLH_E_ARG, "flh_kv_attend: null parameters");
+  AttendArgs a;
+  memset(&a, 0, sizeof(a));
+  int rc = check_cache(&p->cache, &a.c, "flh_kv_attend");
+  if (!rc) rc = check_seqs(&p->seqs, &a.s, p->d_status, "flh_kv_attend");
+  if (rc) return rc;
+  if (p->type != FLH_KV_BF16 && p->type != FLH_KV_FP16) return fl_set_error(FLH_E_ARG, "flh_kv_attend: type %u (bf16 or fp16)", p->type);
+  if (p->seqs.n_tokens && (!p->d_q || !p->d_out || !aligned(p->d_q, 2) || !aligned(p->d_out, 2))) return fl_set_error(FLH_E_ARG, "flh_kv_attend: queries and output are required");
+  if (p->d_selected && (p->n_selected == 0 || p->n_selected > p->seqs.table_width))
+    return fl_set_error(FLH_E_ARG, "flh_kv_attend: %u selected pages of a table of %u", p->n_selected, p->seqs.table_width);
+  if (p->d_selected && p->d_weights) return fl_set_error(FLH_E_ARG, "flh_kv_attend: weights are kept over all pages, not over selected ones");
+  if (!p->d_weights && p->d_weights_in) return fl_set_error(FLH_E_ARG, "flh_kv_attend: weights to start from, but none to write");
+  if (p->d_weights && p->weights_width == 0) return fl_set_error(FLH_E_ARG, "flh_kv_attend: weights of no positions");
+  Plan pl;
+  if ((rc = make_plan(p, &pl))) return rc;
+  if (pl.bytes && (!p->d_workspace || !aligned(p->d_workspace, 16) || p->workspace_bytes < pl.bytes))
+    return fl_set_error(FLH_E_ARG, "flh_kv_attend: a workspace of %llu bytes is needed", (unsigned long long)pl.bytes);
+  if (p->seqs.n_tokens == 0 && !p->d_weights) return FLH_OK;
+  if ((rc = fl_need_init())) return rc;
+  a.q = p->d_q;
+  a.out = p->d_out;
+  a.lse = p->d_lse;
+  a.q_token = p->q_token_stride;
+  a.q_head = p->q_head_stride;
+  a.o_token = p->out_token_stride;
+  a.o_head = p->out_head_stride;
+  a.G = p->q_heads / p->cache.heads;
+  a.tiles_x = pl.tiles_x;
+  a.splits = pl.splits;
+  a.scale2 = p->scale * 1.4426950408889634f;
+  a.causal = p->causal != 0;
+  a.q_vec = aligned(p->d_q, 16) && (p->q_token_stride | p->q_head_stride) % 8 == 0;
+  a.o_vec = aligned(p->d_out, 16) && (p->out_token_stride | p->out_head_stride) % 8 == 0;
+  a.sel = p->d_selected;
+  a.count = p->n_selected;
+  uint8_t* ws = (uint8_t*)p->d_workspace;
+  a.part_o = (float*)(ws + pl.part_o);
+  a.part_l = (float*)(ws + pl.part_l);
+  a.lse2 = p->d_weights ? (float*)(ws + pl.lse2) : nullptr;
+  a.w_in = p->d_weights_in;
+  a.w_out = p->d_weights;
+  a.wi_seq = p->weights_in_seq_stride;
+  a.wi_head = p->weights_in_head_stride;
+  a.wo_seq = p->weights_seq_stride;
+  a.wo_head = p->weights_head_stride;
+  a.w_width = p->weights_width;
+  fl_prof().kid = 9;
+  const hipStream_t st = (hipStream_t)stream;
+  if (p->seqs.n_tokens == 0) a.tiles_x = 0;
+  if (p->type == FLH_KV_BF16) run_attend<__bf16>(a, pl, st);
+  else run_attend<_Float16>(a, pl, st);
+  return finish("flh_kv_attend");
+}
+
+uint64_t flh_kv_select_workspace_bytes(uint32_t n_tokens, uint32_t heads, uint32_t table_width) { return 4ull * n_tokens * heads * table_width; }
+
+int flh_kv_select(const flh_kv_select_params* p, void* stream) {
+  if (!p) return fl_set_error(FLH_E_ARG, "flh_kv_select: null parameters");
+  SelectArgs a;
+  memset(&a, 0, sizeof(a));
+  int rc = check_cache(&p->cache, &a.c, "flh_kv_select");
+  if (!rc) rc = check_seqs(&p->seqs, &a.s, p->d_status, "flh_kv_select");
+  if (rc) return rc;
+  if (p->type != FLH_KV_BF16 && p->type != FLH_KV_FP16) return fl_set_error(FLH_E_ARG, "flh_kv_select: type %u (bf16 or fp16)", p->type);
+  if (p->q_heads == 0 || p->q_heads % p->cache.heads) return fl_set_error(FLH_E_ARG, "flh_kv_select: %u query heads over %u key-value heads", p->q_heads, p->cache.heads);
+  if (p->count == 0 || (uint64_t)p->first + p->last > p->count) return fl_set_error(FLH_E_ARG, "flh_kv_select: %u pages with %u first and %u last ones", p->count, p->first, p->last);
+  if (p->seqs.n_tokens > 65535 || (uint64_t)p->seqs.n_tokens * p->cache.heads > kMaxGroups / 4)
+    return fl_set_error(FLH_E_ARG, "flh_kv_select: %u tokens of %u heads in one call (up to 65535, and 2^22 - 1 rows)", p->seqs.n_tokens, p->cache.heads);
+  if (p->seqs.n_tokens == 0) return FLH_OK;
+  if (!p->d_q || !p->d_out || !aligned(p->d_q, 2)) return fl_set_error(FLH_E_ARG, "flh_kv_select: queries and output are required");
+  const uint64_t need = flh_kv_select_workspace_bytes(p->seqs.n_tokens, p->cache.heads, p->seqs.table_width);
+  if (!p->d_workspace || !aligned(p->d_workspace, 16) || p->workspace_bytes < need)
+    return fl_set_error(FLH_E_ARG, "flh_kv_select: a workspace of %llu bytes is needed", (unsigned long long)need);
+  if ((rc = fl_need_init())) return rc;
+  a.q = p->d_q;
+  a.q_token = p->q_token_stride;
+  a.q_head = p->q_head_stride;
+  a.G = p->q_heads / p->cache.heads;
+  a.causal = p->causal != 0;
+  a.q_vec = aligned(p->d_q, 16) && (p->q_token_stride | p->q_head_stride) % 8 == 0;
+  a.first = p->first;
+  a.last = p->last;
+  a.count = p->count;
+  a.scores = (float*)p->d_workspace;
+  a.out = p->d_out;
+  fl_prof().kid = 10;
+  const hipStream_t st = (hipStream_t)stream;
+  const dim3 grid((a.s.width + 255) / 256, a.c.H, a.s.n_tokens);
+  const bool bf = p->type == FLH_KV_BF16;
+  if (a.c.D <= 64) { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 64>), grid, dim3(256), 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 64>), grid, dim3(256), 0, st, a); }
+  else if (a.c.D <= 128) { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 128>), grid, dim3(256), 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 128>), grid, dim3(256), 0, st, a); }
+  else { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 256>), grid, dim3(256), 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 256>), grid, dim3(256), 0, st, a); }
+  FL_LAUNCH(fl_kv_pick_pages, dim3(a.s.n_tokens * a.c.H), dim3(1024), 0, st, a);
+  return finish("flh_kv_select");
+}
+
+int flh_kv_evict(const flh_kv_evict_params* p, void* stream) {
+  if (!p) return fl_set_error(FLH_E_ARG, "flh_kv_evict: null parameters");
+  PackArgs a;
+  memset(&a, 0, sizeof(a));
+  int rc = check_cache(&p->cache, &a.from, "flh_kv_evict: from");
+  if (!rc) rc = check_cache(&p->to, &a.c, "flh_kv_evict: to");
+  if (!rc) rc = check_seqs(&p->seqs, &a.s, p->d_status, "flh_kv_evict");
+  if (rc) return rc;
+  if (a.c.H != a.from.H || a.c.D != a.from.D) return fl_set_error(FLH_E_ARG, "flh_kv_evict: the caches differ in heads or head dim");
+  if (!p->d_weights || !p->d_to_table || !p->d_kept || !p->d_new_weights || !p->d_new_lens) return fl_set_error(FLH_E_ARG, "flh_kv_evict: weights, tables and outputs are required");
+  if (p->budget == 0 || p->budget > (1u << 30) || (uint64_t)p->first + p->recent > p->budget)
+    return fl_set_error(FLH_E_ARG, "flh_kv_evict: a budget of %u with %u first and %u recent tokens", p->budget, p->first, p->recent);
+  const uint32_t per = (p->budget + a.c.T - 1) / a.c.T;
+  if (p->to_table_width < per || p->to_table_stride < p->to_table_width)
+    return fl_set_error(FLH_E_ARG, "flh_kv_evict: %u tokens need %u pages, the new table has %u", p->budget, per, p->to_table_width);
+  if (p->weights_width == 0 || p->new_weights_width < p->budget) return fl_set_error(FLH_E_ARG, "flh_kv_evict: weights of %u positions, new ones of %u", p->weights_width, p->new_weights_width);
+  if ((uint64_t)per * a.s.n_seqs > kMaxGroups || (uint64_t)a.s.n_seqs * a.c.H > kMaxGroups / 4) return fl_set_error(FLH_E_ARG, "flh_kv_evict: too much for one launch");
+  if ((rc = fl_need_init())) return rc;
+  KeepArgs k;
+  memset(&k, 0, sizeof(k));
+  k.s = a.s;
+  k.T = a.from.T;
+  k.H = a.c.H;
+  k.budget = p->budget;
+  k.first = p->first;
+  k.recent = p->recent;
+  k.w_width = p->weights_width;
+  k.nw_width = p->new_weights_width;
+  k.w = p->d_weights;
+  k.w_seq = p->weights_seq_stride;
+  k.w_head = p->weights_head_stride;
+  k.nw = p->d_new_weights;
+  k.nw_seq = p->new_weights_seq_stride;
+  k.nw_head = p->new_weights_head_stride;
+  k.kept = p->d_kept;
+  k.kept_stride = p->budget;
+  k.new_lens = p->d_new_lens;
+  a.to_table = p->d_to_table;
+  a.to_stride = p->to_table_stride;
+  a.kept = p->d_kept;
+  a.kept_stride = p->budget;
+  a.budget = p->budget;
+  a.per_seq = per;
+  fl_prof().kid = 11;
+  const hipStream_t st = (hipStream_t)stream;
+  FL_LAUNCH(fl_kv_keep, dim3(a.s.n_seqs * a.c.H), dim3(1024), 0, st, k);
+  launch_pack<__bf16, true>(a, per * a.s.n_seqs, st);
+  return finish("flh_kv_evict");
+}
+
+}  // extern "C"

@@ -173,7 +173,7 @@ int flh_tune(const char* key, int64_t value);
  * own start/stop HIP events that bracket the kernel alone; the launches stay asynchronous.
  * flh_prof_end waits for them and returns how many were recorded, filling up to `max` durations
  * (microseconds) and the entry point that launched each: 1 schedule, 2 stripe, 3 reassemble,
- * 4 gather, 5 scatter, 6 copy, 7 stage + deliver.  Launches beyond `capacity` are not timed. */
+ * 4 gather, 5 scatter, 6 copy, 7 stage + deliver, 8 KV store, 9 KV attend, 10 KV select, 11 KV evict.  Launches beyond `capacity` are not timed. */
 int flh_prof_begin(int capacity);
 int flh_prof_end(double* us_out, int* kernel_out, int max);
 
@@ -487,6 +487,154 @@ int flh_region_release(flh_region* r);            /* returns remaining refs (>= 
 int flh_region_refs(const flh_region* r);
 int flh_region_windows(const flh_region* r, flh_windows* out);
 void* flh_region_translate(const flh_region* r, uint32_t lane, const void* data);
+
+/* ---- KV pages held in 8 bits -------------------------------------------------------------------------------------
+ * A key-value cache whose pages the page movers carry (flh_gather_pages / flh_scatter_pages see only bytes), held at
+ * half the size, and the operators that fill it, read it and thin it.  No counterpart in the reference, whose
+ * prefill -> decode experiment sends 16-bit caches [blocks][layers][heads][block][dim] (experiments/serving/model.hh:198-201,
+ * 280-309) and leaves the rest to its inference library.
+ *
+ * A page record holds `tokens` tokens of `heads` key-value heads of `dim` dimensions, everything that its reader needs:
+ *   K codes  e4m3  [heads][tokens][dim]   at 0
+ *   V codes  e4m3  [heads][tokens][dim]   behind them
+ *   low      int8  [heads][dim]           floor(smallest K code / 4) over the tokens held
+ *   high     int8  [heads][dim]           ceil(largest K code / 4)
+ *   scales   f32   [heads][2]             of K and of V
+ * rounded up to a multiple of 128 bytes (flh_kv_page_bytes).  A value is code * scale.  A scale is the smallest power of two s >= 2^-126 with
+ * |value| <= 448 s for all finite values of the block when they were stored (0 if all are 0): e4m3 codes lose nothing by
+ * a power of two, the code is the value's rounding to nearest even, and rescaling rounds only what falls below the
+ * smallest normal code.  What is not finite is stored as NaN.  `tokens` and `dim` are multiples of 16 up to 256;
+ * pages lie page_stride >= flh_kv_page_bytes bytes apart (a multiple of 16: several layers may share a page).
+ *
+ * Sequences: d_table (rows table_stride apart, table_width columns in use) names the pages of each, d_lens how many
+ * tokens it holds, d_starts (n_seqs + 1 ascending, or NULL for n_tokens / n_seqs each) which of the call's n_tokens tokens are its
+ * own; tokens before the first and behind the last start are left alone.  These live on the device, so what is wrong
+ * with them is found there: FLH_E_RANGE is stored to *d_status for a page number outside the pool (the page is not
+ * written; its keys are not seen), a length the table cannot hold (cut off), or starts that leave the call's tokens or
+ * descend (the sequence is skipped).  Nothing is read or written out of bounds.  All entry points only launch: they
+ * neither allocate nor wait and can be captured into a graph. */
+#define FLH_KV_BF16 0u
+#define FLH_KV_FP16 1u
+#define FLH_KV_FP32 2u
+
+typedef struct flh_kv_cache {
+  void*    d_pages;          /* the first record, 16-byte aligned */
+  uint64_t page_stride;
+  uint32_t n_pages;
+  uint32_t tokens;
+  uint32_t heads;
+  uint32_t dim;
+} flh_kv_cache;
+
+typedef struct flh_kv_seqs {
+  const int32_t* d_starts;
+  const int32_t* d_lens;
+  const int32_t* d_table;
+  uint64_t table_stride;
+  uint32_t table_width;
+  uint32_t n_seqs;           /* 1..65535 */
+  uint32_t n_tokens;         /* up to 2^24 */
+  uint32_t pad;
+} flh_kv_seqs;
+
+uint64_t flh_kv_page_bytes(uint32_t tokens, uint32_t heads, uint32_t dim);
+
+/* Appends the call's keys and values [n_tokens][heads][dim] (strides in elements, channels contiguous) to their
+ * sequences, which hold d_lens tokens before it.  A page that holds tokens already keeps its scale unless the new ones
+ * need a larger one; its codes are then rounded once more.  The slots behind the last token are zero in a page that the
+ * call opens.  A page may be written by one sequence of a call only. */
+typedef struct flh_kv_store_params {
+  flh_kv_cache cache;
+  flh_kv_seqs  seqs;
+  const void*  d_k;
+  const void*  d_v;
+  uint64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  uint32_t type;             /* FLH_KV_* of d_k and d_v */
+  uint32_t pad;
+  int32_t* d_status;
+} flh_kv_store_params;
+int flh_kv_store(const flh_kv_store_params* p, void* stream);
+
+/* Attention of queries [n_tokens][q_heads][dim] (bf16 or fp16; query head h reads key-value head h / (q_heads / heads))
+ * over the d_lens tokens of their sequences:  out = sum_j p_j v_j, p = softmax over the keys j a query sees of
+ * scale * q . k_j.  causal: the call's n tokens of a sequence are the last n of its d_lens, and token i sees the keys before and
+ * at its own position; else all see all.  A query that sees no key gets zeros and a log-sum of -inf.  d_lse (optional):
+ * natural logarithm of each row's sum, [n_tokens][q_heads].
+ * d_selected (optional): [n_tokens][heads][n_selected] indices into the sequence's row of the table, each at most once, -1
+ * for none; only these pages are read (flh_kv_select writes it).
+ * d_weights (optional; not with d_selected): [n_seqs][heads][weights_width], = d_weights_in (the same memory, other memory, or
+ * NULL for 0) plus, for each key, the probabilities that all the call's queries of its head gave it.
+ * P is rounded to 11 bits of mantissa for the second product; sums, maxima and accumulators hold 32 bits. */
+typedef struct flh_kv_attend_params {
+  flh_kv_cache cache;
+  flh_kv_seqs  seqs;
+  const void*  d_q;
+  void*        d_out;
+  uint64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  float*   d_lse;
+  uint32_t type;
+  uint32_t q_heads;
+  float    scale;
+  uint32_t causal;
+  const int32_t* d_selected;
+  const float*   d_weights_in;
+  float*         d_weights;
+  uint64_t weights_in_seq_stride, weights_in_head_stride, weights_seq_stride, weights_head_stride;
+  uint32_t n_selected;
+  uint32_t weights_width;
+  void*    d_workspace;      /* flh_kv_attend_workspace_bytes bytes, 16-byte aligned; its contents need not survive the call */
+  uint64_t workspace_bytes;
+  int32_t* d_status;
+} flh_kv_attend_params;
+int64_t flh_kv_attend_workspace_bytes(const flh_kv_attend_params* p);   /* depends on sizes only; negative: FLH_E_* */
+int flh_kv_attend(const flh_kv_attend_params* p, void* stream);
+
+/* For every query token and key-value head the `count` pages whose keys may weigh most, ascending, -1 behind them when the
+ * sequence has fewer: [n_tokens][heads][count].  score(page) = max over the head's query heads of
+ * sum_d q8_d (q8_d > 0 ? high_d : low_d) * step * K scale, with q8 = round(q / step) and step the smallest power of two with
+ * |q| <= 127 step (what is not finite counts as 0).  The first `first` and last `last` pages that the query sees are always
+ * among them; of equal scores the lower index is taken.  Only what causal lets a query see is counted as a page. */
+typedef struct flh_kv_select_params {
+  flh_kv_cache cache;
+  flh_kv_seqs  seqs;
+  const void*  d_q;
+  uint64_t q_token_stride, q_head_stride;
+  uint32_t type;
+  uint32_t q_heads;
+  uint32_t count, first, last;
+  uint32_t causal;
+  int32_t* d_out;
+  void*    d_workspace;      /* flh_kv_select_workspace_bytes bytes, 16-byte aligned */
+  uint64_t workspace_bytes;
+  int32_t* d_status;
+} flh_kv_select_params;
+uint64_t flh_kv_select_workspace_bytes(uint32_t n_tokens, uint32_t heads, uint32_t table_width);
+int flh_kv_select(const flh_kv_select_params* p, void* stream);
+
+/* Cuts every sequence back to `budget` tokens a head (those that hold no more are copied whole): the `first` first, the `recent`
+ * last and, between them, those of the largest weights (NaN the least; of equal weights the earlier token), in their
+ * order.  The tokens kept are packed into the pages that d_to_table names, under scales and bounds of their own;
+ * `to` may be the same pool, but the new pages must not be among those the call reads.  d_kept [n_seqs][heads][budget] receives
+ * the positions (-1 behind them), d_new_weights the weights kept and zeros up to new_weights_width, d_new_lens the new
+ * lengths.  seqs.d_starts and n_tokens are not used. */
+typedef struct flh_kv_evict_params {
+  flh_kv_cache cache;
+  flh_kv_cache to;
+  flh_kv_seqs  seqs;
+  const int32_t* d_to_table;
+  uint64_t to_table_stride;
+  const float* d_weights;
+  uint64_t weights_seq_stride, weights_head_stride;
+  float*   d_new_weights;
+  uint64_t new_weights_seq_stride, new_weights_head_stride;
+  int32_t* d_kept;
+  int32_t* d_new_lens;
+  uint32_t to_table_width;
+  uint32_t weights_width, new_weights_width;
+  uint32_t budget, first, recent;
+  int32_t* d_status;
+} flh_kv_evict_params;
+int flh_kv_evict(const flh_kv_evict_params* p, void* stream);
 
 #ifdef __cplusplus
 }
