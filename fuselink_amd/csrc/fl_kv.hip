@@ -343,7 +343,9 @@ struct AttendArgs {
   float* lse2;                // [n_tokens][H G] base 2, for the weights (may be null)
   uint64_t q_token, q_head, o_token, o_head;
   uint32_t G, tiles_x, splits;
-  float scale2;               // scale * log2(e)
+  uint32_t per_page, per_page_inv;   // tiles of 16 tokens to a page; 2^32 over it, rounded up: exact for the 2^27 tiles there can be
+  float scale2;               // |scale| * log2(e); the queries carry the sign
+  uint32_t flip;              // sign bits of two 16-bit numbers, or 0
   uint32_t causal, q_vec, o_vec;
   const int32_t* sel;         // [n_tokens][H][count] pages of every query token, or null
   uint32_t count;
@@ -407,6 +409,13 @@ __device__ __forceinline__ typename Frag<E>::v8 load_q8(const E* p, bool ok, boo
   return r;
 }
 
+template <class E>
+__device__ __forceinline__ typename Frag<E>::v8 flipped(typename Frag<E>::v8 x, uint32_t flip) {
+  u32x4 w = __builtin_bit_cast(u32x4, x);
+  w ^= flip;
+  return __builtin_bit_cast(typename Frag<E>::v8, w);
+}
+
 // Softmax and both products in one pass over the keys.  S^T = K Q^T and O^T = V^T P^T on 16 x 16 x 32 matrix
 // instructions: a lane's column is one query row in both, so the row's maximum, sum and rescaling need no data from
 // other rows, and S^T leaves the first product in the very lanes and order in which the second one wants P^T if the
@@ -464,7 +473,7 @@ __global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
 #pragma unroll
     for (int k = 0; k < KK; ++k) {
       const uint32_t d = g * (DP / 4) + k * 8;
-      qf[q][k] = load_q8<E>(p + d, r < rows && d < D, a.q_vec);
+      qf[q][k] = flipped<E>(load_q8<E>(p + d, r < rows && d < D, a.q_vec), a.flip);
     }
   }
 
@@ -486,54 +495,70 @@ __global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
   const uint32_t k0 = k0_64 < space ? (uint32_t)k0_64 : space, k1 = share < space - k0 ? k0 + share : space;
   const int32_t* table = a.s.table + b * a.s.table_stride;
   const int32_t* sel = SEL ? a.sel + ((uint64_t)(first + tok0) * H + h) * a.count : nullptr;
-  for (uint32_t k = k0 + (KVW > 1 ? wave * 32 : 0); k < k1; k += 32 * KVW) {
-    uint32_t pos[2];
-    const uint8_t* rec[2];
-    uint32_t slot[2];
-    bool ok[2];
-    float ks[2], vs[2];
+  const uint32_t head_off = h * T * D, k_lane = c * D + g * (DP / 4), v_lane = 4 * g * D + c * VJ;
+  bool bad = false;
+
+  // Three steps are under way at a time: the page numbers of one, the codes and scales of the next, the sums of a third.
+  struct Where { uint32_t pos[2], page[2], off[2]; bool ok[2]; };
+  const auto look_up = [&](uint32_t k) {
+    Where w;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const uint32_t v = k + 16 * t, j = v / T, off = v - j * T;
+      const uint32_t v = k + 16 * t, tl = v >> 4, j = a.per_page == 1 ? tl : __umulhi(tl, a.per_page_inv), slot = (tl - j * a.per_page) << 4;
       uint32_t at = j;
-      ok[t] = v < space;
+      bool ok = v < k1;
       if (SEL) {
-        const int32_t sj = ok[t] ? sel[j] : -1;
-        ok[t] = sj >= 0 && (uint32_t)sj < a.s.width;
-        at = ok[t] ? (uint32_t)sj : 0;
+        const int32_t sj = ok ? sel[j] : -1;
+        ok = sj >= 0 && (uint32_t)sj < a.s.width;
+        at = ok ? (uint32_t)sj : 0;
       }
-      pos[t] = at * T + off;
-      ok[t] = ok[t] && pos[t] < l_max;
-      const int32_t pg = ok[t] ? table[at] : 0;
-      if (pg < 0 || (uint32_t)pg >= a.c.n_pages) { ok[t] = false; if (lane == 0) report(a.s.status); }
-      rec[t] = a.c.pages + (ok[t] ? (uint64_t)pg * a.c.stride : 0);
-      slot[t] = off;
-      const float* sc = reinterpret_cast<const float*>(rec[t] + a.c.scales) + 2 * h;
-      ks[t] = sc[0];
-      vs[t] = sc[1];
+      w.pos[t] = at * T + slot;
+      ok = ok && w.pos[t] < l_max;
+      const uint32_t pg = ok ? (uint32_t)table[at] : 0;
+      const bool there = pg < a.c.n_pages;
+      bad |= !there;
+      w.ok[t] = ok && there;
+      w.page[t] = w.ok[t] ? pg : 0;
+      w.off[t] = head_off + slot * D;
     }
-    if (!ok[0] && !ok[1]) continue;
-    uint32_t kw[2][KW], vw[8][VW];
+    return w;
+  };
+  struct Stage { uint32_t kw[2][KW], vw[8][VW], pos[2]; float ks[2], vs[2]; bool ok[2]; };
+  const auto fetch = [&](Stage& s, const Where& w) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const uint8_t* base = rec[t] + (uint64_t)(h * T + slot[t]) * D;
-      const uint32_t d = g * (DP / 4);
+      s.pos[t] = w.pos[t];
+      s.ok[t] = w.ok[t];
+      const uint8_t* rec = a.c.pages + (uint64_t)w.page[t] * a.c.stride;
+      const float* sc = reinterpret_cast<const float*>(rec + a.c.scales) + 2 * h;
+      s.ks[t] = sc[0];
+      s.vs[t] = sc[1];
+      const uint8_t* base = rec + w.off[t];
 #pragma unroll
       for (int i = 0; i < KW / 4; ++i) {
-        u32x4 w = {0, 0, 0, 0};
-        if (d + 16 * i < D) w = *reinterpret_cast<const u32x4*>(base + c * D + d + 16 * i);
+        u32x4 x = {0, 0, 0, 0};
+        if (g * (DP / 4) + 16 * i < D) x = *reinterpret_cast<const u32x4*>(base + k_lane + 16 * i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) kw[t][4 * i + e] = w[e];
+        for (int e = 0; e < 4; ++e) s.kw[t][4 * i + e] = x[e];
       }
+      const uint8_t* vb = base + a.c.side;
+      const uint32_t in = (uint32_t)(c * VJ) < D ? v_lane : 0;   // lanes beyond D read what they will not write
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint8_t* p = base + a.c.side + (4 * g + i) * D + c * VJ;
-        const bool in = (uint32_t)(c * VJ) < D;
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(vb + in + i * D);
+        if constexpr (VW == 1) s.vw[4 * t + i][0] = p[0];
+        else if constexpr (VW == 2) { const u2 x = *reinterpret_cast<const u2*>(p); s.vw[4 * t + i][0] = x[0]; s.vw[4 * t + i][1] = x[1]; }
+        else {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(p);
 #pragma unroll
-        for (int e = 0; e < VW; ++e) vw[4 * t + i][e] = in ? reinterpret_cast<const uint32_t*>(p)[e] : 0;
+          for (int e = 0; e < 4; ++e) s.vw[4 * t + i][e] = x[e];
+        }
       }
     }
-    const bool masked = !ok[0] || !ok[1] || pos[0] + 16 > l_min || pos[1] + 16 > l_min;
+  };
+  const auto work = [&](Stage& x, uint32_t k) {
+    if (!x.ok[0] && !x.ok[1]) return;
+    const bool masked = !x.ok[0] || !x.ok[1] || x.pos[0] + 16 > l_min || x.pos[1] + 16 > l_min;
 
     f4 s[NQ][2];
 #pragma unroll
@@ -542,7 +567,7 @@ __global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
       for (int q = 0; q < NQ; ++q) s[q][t] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
-        const v8 kf = codes8<E>(kw[t][2 * kk], kw[t][2 * kk + 1]);
+        const v8 kf = codes8<E>(x.kw[t][2 * kk], x.kw[t][2 * kk + 1]);
 #pragma unroll
         for (int q = 0; q < NQ; ++q) s[q][t] = Frag<E>::mfma(kf, qf[q][kk], s[q][t]);
       }
@@ -556,23 +581,27 @@ __global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t p = pos[t] + 4 * g + i;
-          const bool keep = ok[t] && p < l_max;
+          const uint32_t p = x.pos[t] + 4 * g + i;
+          const bool keep = x.ok[t] && p < l_max;
+#pragma unroll
+          for (int q = 0; q < NQ; ++q)
+            if (!(x.ok[t] && p < lim[q])) s[q][t][i] = -kInf;
 #pragma unroll
           for (int e = 0; e < VW; ++e) {
-            uint32_t w = keep ? vw[4 * t + i][e] : 0;
+            uint32_t w = keep ? x.vw[4 * t + i][e] : 0;
             const uint32_t mag = w & 0x7f7f7f7fu;
             const uint32_t nan = (mag + 0x01010101u) & 0x80808080u;   // bytes whose magnitude is 0x7f
             seen_nan |= nan;
             w &= ~((nan >> 7) * 0xffu);
-            vw[4 * t + i][e] = w;
+            x.vw[4 * t + i][e] = w;
           }
         }
       if (__ballot(seen_nan != 0)) {
+        const Where w = look_up(k);
         for (int t = 0; t < 2; ++t) {
-          if (!ok[t]) continue;
-          const uint8_t* base = rec[t] + a.c.side + (uint64_t)(h * T + slot[t]) * D;
-          for (uint32_t kx = 0; kx < 16 && pos[t] + kx < l_max; ++kx)
+          if (!w.ok[t]) continue;
+          const uint8_t* base = a.c.pages + (uint64_t)w.page[t] * a.c.stride + a.c.side + w.off[t];
+          for (uint32_t kx = 0; kx < 16 && w.pos[t] + kx < l_max; ++kx)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -581,17 +610,17 @@ __global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
                 if (d < D && (base[kx * D + d] & 0x7f) == 0x7f) {
 #pragma unroll
                   for (int q = 0; q < NQ; ++q)
-                    if (pos[t] + kx < lim[q]) o[q][j][i] = kNan;
+                    if (w.pos[t] + kx < lim[q]) o[q][j][i] = kNan;
                 }
               }
         }
       }
     }
 
-    const float vmax = fmaxf(vs[0], vs[1]);
+    const float vmax = fmaxf(x.vs[0], x.vs[1]);
     if (vmax > 0.f && !(vmax <= vref * 64.f && vmax * 64.f >= vref)) {
-      const float f = vref > 0.f ? vref / vmax : 0.f;
       if (vref > 0.f) {
+        const float f = vref / vmax;
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
@@ -601,27 +630,20 @@ __global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
     }
     const float inv_ref = inverse(vref);
 
+    // the floor keeps -inf what it is under a block of zeros; what it multiplies otherwise is zero all the same
+    const float kc0 = fmaxf(x.ks[0] * a.scale2, 1e-37f), kc1 = fmaxf(x.ks[1] * a.scale2, 1e-37f);
     h8 pf[NQ];
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
-      float xs[8], mx = -kInf;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float v = s[q][t][i] * (ks[t] * a.scale2);
-          if (masked && !(ok[t] && pos[t] + 4 * g + i < lim[q])) v = -kInf;
-          xs[4 * t + i] = v;
-          mx = fmaxf(mx, v);
-        }
-      mx = column_max(mx);
-      const float mn = fmaxf(m[q], mx), ref = mn == -kInf ? 0.f : mn - 14.f;
-      const float alpha = exp2_fast(m[q] - (mn == -kInf ? 0.f : mn));
+      const float m0 = fmaxf(fmaxf(s[q][0][0], s[q][0][1]), fmaxf(s[q][0][2], s[q][0][3]));
+      const float m1 = fmaxf(fmaxf(s[q][1][0], s[q][1][1]), fmaxf(s[q][1][2], s[q][1][3]));
+      const float mn = fmaxf(m[q], column_max(fmaxf(m0 * kc0, m1 * kc1)));
+      const float top = mn == -kInf ? 0.f : mn, ref = top - 14.f, alpha = exp2_fast(m[q] - top);
       m[q] = mn;
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float p = exp2_fast(xs[i] - ref);
+        const float p = exp2_fast(__builtin_fmaf(s[q][i >> 2][i & 3], i < 4 ? kc0 : kc1, -ref));
         sum += p;
         pf[q][i] = (_Float16)p;
       }
@@ -632,49 +654,78 @@ __global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
       }
     }
 
-    h8 vf[VJ];
-    const float f0 = vs[0] * inv_ref, f1 = vs[1] * inv_ref;
+    const float f0 = x.vs[0] * inv_ref, f1 = x.vs[1] * inv_ref;
 #pragma unroll
-    for (int pr = 0; pr < 4; ++pr) {
-      const float f = pr < 2 ? f0 : f1;
+    for (int e = 0; e < VW; ++e) {
+      h8 vf[4];
 #pragma unroll
-      for (int e = 0; e < VW; ++e) {
-        const uint32_t lo = __builtin_amdgcn_perm(vw[2 * pr + 1][e], vw[2 * pr][e], 0x05010400u), hi = __builtin_amdgcn_perm(vw[2 * pr + 1][e], vw[2 * pr][e], 0x07030602u);
+      for (int pr = 0; pr < 4; ++pr) {
+        const float f = pr < 2 ? f0 : f1;
+        const uint32_t lo = __builtin_amdgcn_perm(x.vw[2 * pr + 1][e], x.vw[2 * pr][e], 0x05010400u), hi = __builtin_amdgcn_perm(x.vw[2 * pr + 1][e], x.vw[2 * pr][e], 0x07030602u);
         const h2 x0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, f, false), x1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, f, true);
         const h2 x2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, f, false), x3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, f, true);
-        vf[4 * e][2 * pr] = x0[0]; vf[4 * e][2 * pr + 1] = x0[1];
-        vf[4 * e + 1][2 * pr] = x1[0]; vf[4 * e + 1][2 * pr + 1] = x1[1];
-        vf[4 * e + 2][2 * pr] = x2[0]; vf[4 * e + 2][2 * pr + 1] = x2[1];
-        vf[4 * e + 3][2 * pr] = x3[0]; vf[4 * e + 3][2 * pr + 1] = x3[1];
+        vf[0][2 * pr] = x0[0]; vf[0][2 * pr + 1] = x0[1];
+        vf[1][2 * pr] = x1[0]; vf[1][2 * pr + 1] = x1[1];
+        vf[2][2 * pr] = x2[0]; vf[2][2 * pr + 1] = x2[1];
+        vf[3][2 * pr] = x3[0]; vf[3][2 * pr + 1] = x3[1];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) o[q][4 * e + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[j], pf[q], o[q][4 * e + j], 0, 0, 0);
+    }
+  };
+
+  {
+    constexpr uint32_t kStep = 32 * KVW;
+    uint32_t k = k0 + (KVW > 1 ? wave * 32 : 0);
+    if (k < k1) {
+      Stage now, next;
+      Where w = look_up(k);
+      fetch(next, w);
+      w = look_up(k + kStep);
+      for (; k < k1; k += kStep) {
+        now = next;
+        if (k + kStep < k1) fetch(next, w);
+        w = look_up(k + 2 * kStep);
+        work(now, k);
       }
     }
-#pragma unroll
-    for (int j = 0; j < VJ; ++j)
-#pragma unroll
-      for (int q = 0; q < NQ; ++q) o[q][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[j], pf[q], o[q][j], 0, 0, 0);
   }
+  if (bad && lane == 0) report(a.s.status);
 #pragma unroll
   for (int q = 0; q < NQ; ++q) l[q] = column_sum(l[q]);
 
-  // a row's result: dims [d, d + 4 VJ) of lane group g, in order i, j
+  // eight dims of a row's result
   const uint64_t row_out = (uint64_t)a.s.n_tokens * H * G;
-  const auto emit = [&](uint32_t r, float mm, float ll, const float* v, uint32_t d, uint32_t cnt, bool head) {
+  const auto emit = [&](uint32_t r, float mm, float ll, const float* v, uint32_t d, bool head) {
     const uint32_t i = r / G;
     const uint64_t tok = first + i, hq = h * G + (r - i * G);
     const float lg = ll > 0.f ? mm + __builtin_amdgcn_logf(ll) - 14.f : (ll == 0.f ? -kInf : kNan);
     if (a.splits > 1) {
       const uint64_t at = split * row_out + tok * H * G + hq;
       if (head) a.part_l[at] = lg;
-      for (uint32_t e = 0; e < cnt; ++e)
-        if (d + e < D) a.part_o[at * D + d + e] = v[e];
+      if (d < D) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) *reinterpret_cast<f4*>(a.part_o + at * D + d + e) = f4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+      }
     } else {
       if (head) {
         if (a.lse) a.lse[tok * H * G + hq] = lg * 0.6931471805599453f;
         if (a.lse2) a.lse2[tok * H * G + hq] = lg;
       }
-      E* p = reinterpret_cast<E*>(a.out) + tok * a.o_token + hq * a.o_head;
-      for (uint32_t e = 0; e < cnt; ++e)
-        if (d + e < D) p[d + e] = (E)v[e];
+      E* p = reinterpret_cast<E*>(a.out) + tok * a.o_token + hq * a.o_head + d;
+      if (d < D) {
+        v8 y;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = (E)v[e];
+        if (a.o_vec) {
+          *reinterpret_cast<v8*>(p) = y;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) p[e] = y[e];
+        }
+      }
     }
   };
 
@@ -688,7 +739,10 @@ __global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < VJ; ++j) v[i * VJ + j] = o[q][j][i] * f;
-      if (r < rows) emit(r, m[q], l[q], v, g * 4 * VJ, 4 * VJ, g == 0);
+      if (r < rows) {
+#pragma unroll
+        for (int u = 0; u < 4 * VJ; u += 8) emit(r, m[q], l[q], v + u, g * 4 * VJ + u, g == 0 && u == 0);
+      }
     }
   } else {
 #pragma unroll
@@ -719,7 +773,7 @@ __global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
       const float f = ll == 0.f ? 0.f : 1.f / ll;
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] *= f;
-      emit(r, mm, ll, v, d, 8, d == 0);
+      emit(r, mm, ll, v, d, d == 0);
     }
   }
 }
@@ -824,7 +878,7 @@ __global__ __launch_bounds__(256) void fl_kv_weights(const AttendArgs a) {
           const E* p = reinterpret_cast<const E*>(a.q) + tok * a.q_token + hq * a.q_head;
           f4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int k = 0; k < KK; ++k) s = Frag<E>::mfma(kf[k], load_q8<E>(p + d0 + k * 8, in && d0 + k * 8 < D, a.q_vec), s);
+          for (int k = 0; k < KK; ++k) s = Frag<E>::mfma(kf[k], flipped<E>(load_q8<E>(p + d0 + k * 8, in && d0 + k * 8 < D, a.q_vec), a.flip), s);
           int64_t lim = !in ? 0 : a.causal ? (int64_t)len - n + i + 1 : len;
           const float lg = in ? a.lse2[tok * H * G + hq] : 0.f;
 #pragma unroll
@@ -1103,6 +1157,8 @@ __global__ __launch_bounds__(1024) void fl_kv_keep(const KeepArgs a) {
 // ------------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------------
+constexpr uint32_t kMaxPages = (1u << 23) - 1;   // of a sequence: positions fit 31 bits
+
 bool aligned(const void* p, uint64_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 int check_cache(const flh_kv_cache* k, Cache* c, const char* what) {
@@ -1130,7 +1186,7 @@ int check_cache(const flh_kv_cache* k, Cache* c, const char* what) {
 int check_seqs(const flh_kv_seqs* k, Seqs* s, int32_t* d_status, const char* what) {
   if (!k->d_lens || !k->d_table || !d_status) return fl_set_error(FLH_E_ARG, "%s: lens, page table and status are required", what);
   if (k->n_seqs == 0 || k->n_seqs > 65535) return fl_set_error(FLH_E_ARG, "%s: %u sequences (1..65535)", what, k->n_seqs);
-  if (k->table_width == 0 || k->table_stride < k->table_width || k->table_width > (0x7fffffffu >> 8))
+  if (k->table_width == 0 || k->table_stride < k->table_width || k->table_width > kMaxPages)
     return fl_set_error(FLH_E_ARG, "%s: page table of %u columns, stride %llu", what, k->table_width, (unsigned long long)k->table_stride);
   if (k->n_tokens > (1u << 24)) return fl_set_error(FLH_E_ARG, "%s: %u tokens in one call (up to 2^24)", what, k->n_tokens);
   if (!k->d_starts && k->n_tokens % k->n_seqs) return fl_set_error(FLH_E_ARG, "%s: %u tokens do not divide into %u sequences; give starts", what, k->n_tokens, k->n_seqs);
@@ -1295,8 +1351,7 @@ int flh_kv_attend(const flh_kv_attend_params* p, void* stream) {
   if (rc) return rc;
   if (p->type != FLH_KV_BF16 && p->type != FLH_KV_FP16) return fl_set_error(FLH_E_ARG, "flh_kv_attend: type %u (bf16 or fp16)", p->type);
   if (p->seqs.n_tokens && (!p->d_q || !p->d_out || !aligned(p->d_q, 2) || !aligned(p->d_out, 2))) return fl_set_error(FLH_E_ARG, "flh_kv_attend: queries and output are required");
-  if (p->d_selected && (p->n_selected == 0 || p->n_selected > p->seqs.table_width))
-    return fl_set_error(FLH_E_ARG, "flh_kv_attend: %u selected pages of a table of %u", p->n_selected, p->seqs.table_width);
+  if (p->d_selected && (p->n_selected == 0 || p->n_selected > kMaxPages)) return fl_set_error(FLH_E_ARG, "flh_kv_attend: %u selected pages", p->n_selected);
   if (p->d_selected && p->d_weights) return fl_set_error(FLH_E_ARG, "flh_kv_attend: weights are kept over all pages, not over selected ones");
   if (!p->d_weights && p->d_weights_in) return fl_set_error(FLH_E_ARG, "flh_kv_attend: weights to start from, but none to write");
   if (p->d_weights && p->weights_width == 0) return fl_set_error(FLH_E_ARG, "flh_kv_attend: weights of no positions");
@@ -1316,7 +1371,10 @@ int flh_kv_attend(const flh_kv_attend_params* p, void* stream) {
   a.G = p->q_heads / p->cache.heads;
   a.tiles_x = pl.tiles_x;
   a.splits = pl.splits;
-  a.scale2 = p->scale * 1.4426950408889634f;
+  a.per_page = a.c.T / 16;
+  a.per_page_inv = 0xffffffffu / a.per_page + 1;   // (one tile a page: not used)
+  a.scale2 = fabsf(p->scale) * 1.4426950408889634f;
+  a.flip = p->scale < 0.f ? 0x80008000u : 0u;
   a.causal = p->causal != 0;
   a.q_vec = aligned(p->d_q, 16) && (p->q_token_stride | p->q_head_stride) % 8 == 0;
   a.o_vec = aligned(p->d_out, 16) && (p->out_token_stride | p->out_head_stride) % 8 == 0;

@@ -87,7 +87,7 @@ WIDE = dict(table_width=400, table_stride=400)
 CALLS = [("flh_kv_store", dict(type=3)), ("flh_kv_store", dict(d_k=None)), ("flh_kv_store", dict(d_v=None)), ("flh_kv_store", dict(d_k=P + 1)),
          ("flh_kv_attend", dict(type=2)), ("flh_kv_attend", dict(d_q=None)), ("flh_kv_attend", dict(d_out=None)), ("flh_kv_attend", dict(d_q=P + 1)),
          ("flh_kv_attend", dict(q_heads=0)), ("flh_kv_attend", dict(q_heads=33)), ("flh_kv_attend", dict(s=seqs(**WIDE), d_workspace=None)), ("flh_kv_attend", dict(s=seqs(**WIDE), workspace_bytes=64)),
-         ("flh_kv_attend", dict(s=seqs(**WIDE), d_workspace=P + 4)), ("flh_kv_attend", dict(d_selected=P)), ("flh_kv_attend", dict(d_selected=P, n_selected=5)),
+         ("flh_kv_attend", dict(s=seqs(**WIDE), d_workspace=P + 4)), ("flh_kv_attend", dict(d_selected=P)), ("flh_kv_attend", dict(d_selected=P, n_selected=1 << 23)),
          ("flh_kv_attend", dict(d_selected=P, n_selected=2, d_weights=P, weights_width=64)), ("flh_kv_attend", dict(d_weights_in=P)), ("flh_kv_attend", dict(d_weights=P)),
          ("flh_kv_select", dict(type=2)), ("flh_kv_select", dict(d_q=None)), ("flh_kv_select", dict(d_out=None)), ("flh_kv_select", dict(q_heads=9)), ("flh_kv_select", dict(count=0)),
          ("flh_kv_select", dict(first=3)), ("flh_kv_select", dict(last=0xffffffff)), ("flh_kv_select", dict(d_workspace=None)), ("flh_kv_select", dict(workspace_bytes=100)),
