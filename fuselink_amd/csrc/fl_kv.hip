@@ -43,6 +43,14 @@ struct Seqs {
   int32_t* status;
 };
 
+// What no launch writes while it runs -- page tables, counts, scales of the records it reads -- at a uniform address:
+// through the constant address space these are scalar loads, which do not queue behind the vector loads of the codes.
+template <class T>
+__device__ __forceinline__ T scalar_load(const T* p) {
+  typedef const T __attribute__((address_space(4))) * P;
+  return *(P)(uintptr_t)p;
+}
+
 __device__ __forceinline__ void report(int32_t* status) { *status = FLH_E_RANGE; }
 
 __device__ __forceinline__ void seq_tokens(const Seqs& s, uint32_t b, uint32_t& first, uint32_t& n) {
@@ -421,11 +429,12 @@ __device__ __forceinline__ typename Frag<E>::v8 flipped(typename Frag<E>::v8 x, 
 // other rows, and S^T leaves the first product in the very lanes and order in which the second one wants P^T if the
 // 32 keys of a step are numbered (two tiles of 16) x (four lane groups) x 4 -- an order that sums do not see.  K and V
 // come as rows of codes straight into registers; V's bytes are interleaved token against token on the way to pairs.
-// P is rounded to 16-bit floats with 11 bits of mantissa at 2^14 times its value relative to the row's maximum so
-// far, normal down to 2^-28 of it; V's codes are multiplied there by their block's scale over a reference that moves
-// only when the scales leave 2^+-6 of it.  Sums, maxima and the accumulators are 32 bits wide.
+// P is rounded to 16-bit floats (11 bits of mantissa) as 2^8 times its value relative to a reference of the row that
+// follows its maximum only when that has grown by 2^7: at most 2^15, normal down to 2^-22 of the reference.  V's codes
+// are multiplied there by their block's scale over a reference that moves only when the scales leave 2^+-6 of it.  So
+// the accumulators are rarely rescaled; they, sums and references are 32 bits wide.
 template <class E, int DP, int NQ, int KVW, bool SEL>
-__global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
+__global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) void fl_kv_attend(const AttendArgs a) {
   constexpr int KK = DP / 32, KW = DP / 16, VJ = DP / 16, VW = DP / 64;
   constexpr uint32_t TR = 16 * NQ * (4 / KVW);
   typedef typename Frag<E>::v8 v8;
@@ -478,11 +487,11 @@ __global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
   }
 
   f4 o[NQ][VJ];
-  float m[NQ], l[NQ];
+  float top[NQ], ref[NQ], l[NQ];   // the maximum that ref = top - 8 comes from; sum of exp2(x - ref)
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
-    m[q] = -kInf;
-    l[q] = 0.f;
+    top[q] = -kInf;
+    ref[q] = l[q] = 0.f;
 #pragma unroll
     for (int j = 0; j < VJ; ++j) o[q][j] = f4{0.f, 0.f, 0.f, 0.f};
   }
@@ -495,31 +504,44 @@ __global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
   const uint32_t k0 = k0_64 < space ? (uint32_t)k0_64 : space, k1 = share < space - k0 ? k0 + share : space;
   const int32_t* table = a.s.table + b * a.s.table_stride;
   const int32_t* sel = SEL ? a.sel + ((uint64_t)(first + tok0) * H + h) * a.count : nullptr;
-  const uint32_t head_off = h * T * D, k_lane = c * D + g * (DP / 4), v_lane = 4 * g * D + c * VJ;
-  bool bad = false;
+  const uint32_t head_off = h * T * D;
+  uint32_t k_lane[KW / 4], v_lane[4];   // this lane's bytes of a tile; lanes beyond D read what no one multiplies or writes
+#pragma unroll
+  for (int i = 0; i < KW / 4; ++i) k_lane[i] = c * D + (g * (DP / 4) + 16 * i < D ? g * (DP / 4) + 16 * i : 0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v_lane[i] = (4 * g + i) * D + ((uint32_t)(c * VJ) < D ? c * VJ : 0);
+  uint32_t bad = 0, nan_steps = 0;
 
-  // Three steps are under way at a time: the page numbers of one, the codes and scales of the next, the sums of a third.
+  // Four steps are under way at a time: the choice of a page (a load if pages were selected), its number, the codes and
+  // scales, the sums.  Nothing in the first three branches: past the end they look at the last tile again.
+  struct Choice { uint32_t at[2], slot[2]; bool ok[2]; };
   struct Where { uint32_t pos[2], page[2], off[2]; bool ok[2]; };
-  const auto look_up = [&](uint32_t k) {
+  const uint32_t last_tile = (k1 - 1) >> 4;   // (used when there are keys)
+  const auto choose = [&](uint32_t k) {
+    Choice r;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint32_t tv = (k >> 4) + t, tl = tv < last_tile ? tv : last_tile, j = a.per_page == 1 ? tl : __umulhi(tl, a.per_page_inv);
+      r.slot[t] = (tl - j * a.per_page) << 4;
+      r.at[t] = SEL ? (uint32_t)scalar_load(sel + j) : j;
+      r.ok[t] = tv <= last_tile;
+    }
+    return r;
+  };
+  const auto look_up = [&](const Choice& r) {
     Where w;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const uint32_t v = k + 16 * t, tl = v >> 4, j = a.per_page == 1 ? tl : __umulhi(tl, a.per_page_inv), slot = (tl - j * a.per_page) << 4;
-      uint32_t at = j;
-      bool ok = v < k1;
+      uint32_t at = r.at[t];
+      w.ok[t] = r.ok[t];
       if (SEL) {
-        const int32_t sj = ok ? sel[j] : -1;
-        ok = sj >= 0 && (uint32_t)sj < a.s.width;
-        at = ok ? (uint32_t)sj : 0;
+        w.ok[t] = w.ok[t] && at < a.s.width;
+        at = at < a.s.width ? at : 0;
       }
-      w.pos[t] = at * T + slot;
-      ok = ok && w.pos[t] < l_max;
-      const uint32_t pg = ok ? (uint32_t)table[at] : 0;
-      const bool there = pg < a.c.n_pages;
-      bad |= !there;
-      w.ok[t] = ok && there;
-      w.page[t] = w.ok[t] ? pg : 0;
-      w.off[t] = head_off + slot * D;
+      w.pos[t] = at * T + r.slot[t];
+      w.ok[t] = w.ok[t] && w.pos[t] < l_max;
+      w.off[t] = head_off + r.slot[t] * D;
+      w.page[t] = (uint32_t)scalar_load(table + at);
     }
     return w;
   };
@@ -527,25 +549,25 @@ __global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
   const auto fetch = [&](Stage& s, const Where& w) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
+      const bool there = w.page[t] < a.c.n_pages;
+      bad |= w.ok[t] && !there ? 1 : 0;
       s.pos[t] = w.pos[t];
-      s.ok[t] = w.ok[t];
-      const uint8_t* rec = a.c.pages + (uint64_t)w.page[t] * a.c.stride;
+      s.ok[t] = w.ok[t] && there;
+      const uint8_t* rec = a.c.pages + (uint64_t)(there ? w.page[t] : 0) * a.c.stride;
       const float* sc = reinterpret_cast<const float*>(rec + a.c.scales) + 2 * h;
-      s.ks[t] = sc[0];
-      s.vs[t] = sc[1];
-      const uint8_t* base = rec + w.off[t];
+      s.ks[t] = scalar_load(sc);
+      s.vs[t] = scalar_load(sc + 1);
+      const uint8_t *base = rec + w.off[t], *vb = base + a.c.side;
+      asm("" : "+s"(base), "+s"(vb));   // scalar bases, so that a load's address is one register of this lane
 #pragma unroll
       for (int i = 0; i < KW / 4; ++i) {
-        u32x4 x = {0, 0, 0, 0};
-        if (g * (DP / 4) + 16 * i < D) x = *reinterpret_cast<const u32x4*>(base + k_lane + 16 * i);
+        const u32x4 x = *reinterpret_cast<const u32x4*>(base + k_lane[i]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) s.kw[t][4 * i + e] = x[e];
       }
-      const uint8_t* vb = base + a.c.side;
-      const uint32_t in = (uint32_t)(c * VJ) < D ? v_lane : 0;   // lanes beyond D read what they will not write
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t* p = reinterpret_cast<const uint32_t*>(vb + in + i * D);
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(vb + v_lane[i]);
         if constexpr (VW == 1) s.vw[4 * t + i][0] = p[0];
         else if constexpr (VW == 2) { const u2 x = *reinterpret_cast<const u2*>(p); s.vw[4 * t + i][0] = x[0]; s.vw[4 * t + i][1] = x[1]; }
         else {
@@ -556,7 +578,7 @@ __global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
       }
     }
   };
-  const auto work = [&](Stage& x, uint32_t k) {
+  const auto work = [&](Stage& x) {
     if (!x.ok[0] && !x.ok[1]) return;
     const bool masked = !x.ok[0] || !x.ok[1] || x.pos[0] + 16 > l_min || x.pos[1] + 16 > l_min;
 
@@ -574,6 +596,7 @@ __global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
     }
 
     if (masked) {
+      asm volatile("");   // a branch, not selects on every step's way
       // A row that does not see a key must not see its value either, and 0 * NaN is NaN: values nobody sees become
       // zero, and a NaN that some rows see goes into their sums by hand.
       uint32_t seen_nan = 0;
@@ -596,61 +619,45 @@ __global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
             x.vw[4 * t + i][e] = w;
           }
         }
-      if (__ballot(seen_nan != 0)) {
-        const Where w = look_up(k);
-        for (int t = 0; t < 2; ++t) {
-          if (!w.ok[t]) continue;
-          const uint8_t* base = a.c.pages + (uint64_t)w.page[t] * a.c.stride + a.c.side + w.off[t];
-          for (uint32_t kx = 0; kx < 16 && w.pos[t] + kx < l_max; ++kx)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-              for (int j = 0; j < VJ; ++j) {
-                const uint32_t d = (4 * g + i) * VJ + j;
-                if (d < D && (base[kx * D + d] & 0x7f) == 0x7f) {
-#pragma unroll
-                  for (int q = 0; q < NQ; ++q)
-                    if (w.pos[t] + kx < lim[q]) o[q][j][i] = kNan;
-                }
-              }
-        }
-      }
+      if (__ballot(seen_nan != 0)) nan_steps = 1;
     }
-
-    const float vmax = fmaxf(x.vs[0], x.vs[1]);
-    if (vmax > 0.f && !(vmax <= vref * 64.f && vmax * 64.f >= vref)) {
-      if (vref > 0.f) {
-        const float f = vref / vmax;
-#pragma unroll
-        for (int q = 0; q < NQ; ++q)
-#pragma unroll
-          for (int j = 0; j < VJ; ++j) o[q][j] *= f;
-      }
-      vref = vmax;
-    }
-    const float inv_ref = inverse(vref);
 
     // the floor keeps -inf what it is under a block of zeros; what it multiplies otherwise is zero all the same
     const float kc0 = fmaxf(x.ks[0] * a.scale2, 1e-37f), kc1 = fmaxf(x.ks[1] * a.scale2, 1e-37f);
-    h8 pf[NQ];
+    const float vmax = fmaxf(x.vs[0], x.vs[1]);
+    float mx[NQ];
+    bool move = vmax > 0.f && !(vmax <= vref * 64.f && vmax * 64.f >= vref);
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
       const float m0 = fmaxf(fmaxf(s[q][0][0], s[q][0][1]), fmaxf(s[q][0][2], s[q][0][3]));
       const float m1 = fmaxf(fmaxf(s[q][1][0], s[q][1][1]), fmaxf(s[q][1][2], s[q][1][3]));
-      const float mn = fmaxf(m[q], column_max(fmaxf(m0 * kc0, m1 * kc1)));
-      const float top = mn == -kInf ? 0.f : mn, ref = top - 14.f, alpha = exp2_fast(m[q] - top);
-      m[q] = mn;
-      float sum = 0.f;
+      mx[q] = column_max(fmaxf(m0 * kc0, m1 * kc1));
+      move |= mx[q] > top[q] + 7.f;
+    }
+    if (__ballot(move)) {
+      const float vnew = vmax > 0.f && !(vmax <= vref * 64.f && vmax * 64.f >= vref) ? vmax : vref;
+      const float fv = vref > 0.f ? vref / vnew : 1.f;
+      vref = vnew;
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        const float t = fmaxf(top[q], mx[q]), f = top[q] == -kInf ? 0.f : exp2_fast(top[q] - t);
+        top[q] = t;
+        ref[q] = t == -kInf ? 0.f : t - 8.f;
+        l[q] *= f;
+#pragma unroll
+        for (int j = 0; j < VJ; ++j) o[q][j] *= f * fv;
+      }
+    }
+    const float inv_ref = inverse(vref);
+
+    h8 pf[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float p = exp2_fast(__builtin_fmaf(s[q][i >> 2][i & 3], i < 4 ? kc0 : kc1, -ref));
-        sum += p;
+        const float p = exp2_fast(__builtin_fmaf(s[q][i >> 2][i & 3], i < 4 ? kc0 : kc1, -ref[q]));
+        l[q] += p;
         pf[q][i] = (_Float16)p;
-      }
-      l[q] = l[q] * alpha + sum;
-      if (__ballot(alpha != 1.f)) {
-#pragma unroll
-        for (int j = 0; j < VJ; ++j) o[q][j] *= alpha;
       }
     }
 
@@ -680,15 +687,49 @@ __global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
     constexpr uint32_t kStep = 32 * KVW;
     uint32_t k = k0 + (KVW > 1 ? wave * 32 : 0);
     if (k < k1) {
-      Stage now, next;
-      Where w = look_up(k);
-      fetch(next, w);
-      w = look_up(k + kStep);
-      for (; k < k1; k += kStep) {
-        now = next;
-        if (k + kStep < k1) fetch(next, w);
-        w = look_up(k + 2 * kStep);
-        work(now, k);
+      // The fetch is unconditional: behind a branch, the wait for this step's codes would have to cover the next ones'
+      // as well.
+      Stage s0, s1;
+      Where w = look_up(choose(k));
+      Choice r = choose(k + kStep);
+      fetch(s0, w);
+      w = look_up(r);
+      r = choose(k + 2 * kStep);
+      for (;;) {
+        fetch(s1, w);
+        w = look_up(r);
+        r = choose(k + 3 * kStep);
+        work(s0);
+        k += kStep;
+        if (k >= k1) break;
+        fetch(s0, w);
+        w = look_up(r);
+        r = choose(k + 3 * kStep);
+        work(s1);
+        k += kStep;
+        if (k >= k1) break;
+      }
+    }
+    if (nan_steps) {   // a NaN value that not every row of the tile sees: into the sums of those that do
+      for (k = k0 + (KVW > 1 ? wave * 32 : 0); k < k1; k += kStep) {
+        Where w = look_up(choose(k));
+#pragma unroll
+        for (int t = 0; t < 2; ++t) w.ok[t] = w.ok[t] && w.page[t] < a.c.n_pages;
+        if (w.ok[0] && w.ok[1] && w.pos[0] + 16 <= l_min && w.pos[1] + 16 <= l_min) continue;
+        for (int t = 0; t < 2; ++t) {
+          if (!w.ok[t]) continue;
+          const uint8_t* base = a.c.pages + (uint64_t)w.page[t] * a.c.stride + a.c.side + w.off[t];
+          for (uint32_t kx = 0; kx < 16 && w.pos[t] + kx < l_max; ++kx)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int j = 0; j < VJ; ++j) {
+                const uint32_t d = (4 * g + i) * VJ + j;
+                const bool nan = d < D && (base[kx * D + d] & 0x7f) == 0x7f;
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) o[q][j][i] += nan && w.pos[t] + kx < lim[q] ? kNan : 0.f;
+              }
+        }
       }
     }
   }
@@ -701,7 +742,7 @@ __global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
   const auto emit = [&](uint32_t r, float mm, float ll, const float* v, uint32_t d, bool head) {
     const uint32_t i = r / G;
     const uint64_t tok = first + i, hq = h * G + (r - i * G);
-    const float lg = ll > 0.f ? mm + __builtin_amdgcn_logf(ll) - 14.f : (ll == 0.f ? -kInf : kNan);
+    const float lg = ll > 0.f ? mm + __builtin_amdgcn_logf(ll) : (ll == 0.f ? -kInf : kNan);
     if (a.splits > 1) {
       const uint64_t at = split * row_out + tok * H * G + hq;
       if (head) a.part_l[at] = lg;
@@ -741,14 +782,14 @@ __global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
         for (int j = 0; j < VJ; ++j) v[i * VJ + j] = o[q][j][i] * f;
       if (r < rows) {
 #pragma unroll
-        for (int u = 0; u < 4 * VJ; u += 8) emit(r, m[q], l[q], v + u, g * 4 * VJ + u, g == 0 && u == 0);
+        for (int u = 0; u < 4 * VJ; u += 8) emit(r, ref[q], l[q], v + u, g * 4 * VJ + u, g == 0 && u == 0);
       }
     }
   } else {
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
       const int w = (int)wave * 16 * NQ + q * 16 + c;
-      if (g == 0) { sm_m[w] = m[q]; sm_l[w] = l[q]; }
+      if (g == 0) { sm_m[w] = l[q] == 0.f ? -kInf : ref[q]; sm_l[w] = l[q]; }
       float* p = sm_o + w * (DP + 4) + g * 4 * VJ;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -778,11 +819,12 @@ __global__ __launch_bounds__(256) void fl_kv_attend(const AttendArgs a) {
   }
 }
 
-// The splits' results of every row, weighted by what their shares of the keys add up to.  Same rows per workgroup as
-// in fl_kv_attend: rows of no sequence are not touched.
+// The splits' results of every row, weighted by what their shares of the keys add up to.  Rows are numbered as in
+// fl_kv_attend, so those of no sequence are not touched.  A wavefront joins one row: with DL = D / 4 lanes to a split it
+// reads 64 / DL splits at a time, none of the loads waiting for another.
 template <class E, bool SEL>
 __global__ __launch_bounds__(256) void fl_kv_join(const AttendArgs a, uint32_t TR) {
-  const uint32_t H = a.c.H, G = a.G, D = a.c.D, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t H = a.c.H, G = a.G, D = a.c.D, lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const uint32_t h = blockIdx.x % H, x = blockIdx.x / H;
   uint32_t b, tile, first, n, r0, rows, tok0 = 0;
   if constexpr (SEL) {
@@ -797,39 +839,45 @@ __global__ __launch_bounds__(256) void fl_kv_join(const AttendArgs a, uint32_t T
   seq_tokens(a.s, b, first, n);
   if constexpr (SEL) { r0 = tok0 * G + tile * TR; rows = (tok0 + 1) * G; } else { r0 = tile * TR; rows = n * G; }
   const uint64_t row_out = (uint64_t)a.s.n_tokens * H * G;
-  for (uint32_t r = r0 + wave; r < r0 + TR && r < rows; r += 4) {
-    const uint32_t i = r / G;
-    const uint64_t tok = first + i, hq = h * G + (r - i * G), at = tok * H * G + hq;
-    float top = -kInf, bad = 0.f;
-    for (uint32_t s = lane; s < a.splits; s += 64) {
-      const float v = a.part_l[s * row_out + at];
-      top = fmaxf(top, v);
-      bad += v != v ? 1.f : 0.f;
-    }
+  const uint32_t r = r0 + blockIdx.y * 4 + wave;
+  if (r >= rows) return;
+  const uint32_t i = r / G;
+  const uint64_t tok = first + i, hq = h * G + (r - i * G), at = tok * H * G + hq;
+  const uint32_t DL = D <= 64 ? 16 : D <= 128 ? 32 : 64, SP = 64 / DL, d = (lane & (DL - 1)) * 4, sub = lane / DL;
+
+  float top = -kInf;
+  for (uint32_t s = lane; s < a.splits; s += 64) top = fmaxf(top, a.part_l[s * row_out + at]);
 #pragma unroll
-    for (int o = 32; o; o >>= 1) { top = fmaxf(top, __shfl_xor(top, o)); bad += __shfl_xor(bad, o); }
-    float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    if (top != -kInf || bad > 0.f) {
-      for (uint32_t s = 0; s < a.splits; ++s) {
-        const float v = a.part_l[s * row_out + at];
-        if (v == -kInf) continue;
-        const float w = exp2_fast(v - (top == -kInf ? 0.f : top));
-        sum += w;
-        const float* p = a.part_o + (s * row_out + at) * D;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (lane + 64 * e < D) acc[e] += p[lane + 64 * e] * w;
-      }
+  for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  const float base = top == -kInf ? 0.f : top;
+  float sum = 0.f;
+  f4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (uint32_t s0 = 0; s0 < a.splits; s0 += 64) {
+    const float part = s0 + lane < a.splits ? a.part_l[(s0 + lane) * row_out + at] : -kInf;
+    const float w = part == -kInf ? 0.f : exp2_fast(part - base);
+    sum += w;
+    const uint32_t cnt = a.splits - s0 < 64 ? a.splits - s0 : 64;
+#pragma unroll 4
+    for (uint32_t s = 0; s < cnt; s += SP) {
+      const uint32_t mine = s + sub;
+      const float ws = __shfl(w, (int)(mine & 63));
+      if (mine < cnt && ws != 0.f && d < D) acc += *reinterpret_cast<const f4*>(a.part_o + ((s0 + mine) * row_out + at) * D + d) * ws;
     }
-    const float f = sum == 0.f ? 0.f : 1.f / sum, lg = sum == 0.f ? -kInf : top + __builtin_amdgcn_logf(sum);
-    if (lane == 0) {
-      if (a.lse) a.lse[at] = lg * 0.6931471805599453f;
-      if (a.lse2) a.lse2[at] = lg;
-    }
-    E* p = reinterpret_cast<E*>(a.out) + tok * a.o_token + hq * a.o_head;
+  }
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (lane + 64 * e < D) p[lane + 64 * e] = (E)(acc[e] * f);
+  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    for (uint32_t o = DL; o < 64; o <<= 1) acc[e] += __shfl_xor(acc[e], (int)o);
+  const float f = sum == 0.f ? 0.f : 1.f / sum, lg = sum == 0.f ? -kInf : base + __builtin_amdgcn_logf(sum);
+  if (lane == 0) {
+    if (a.lse) a.lse[at] = lg * 0.6931471805599453f;
+    if (a.lse2) a.lse2[at] = lg;
+  }
+  if (sub == 0 && d < D) {
+    E* p = reinterpret_cast<E*>(a.out) + tok * a.o_token + hq * a.o_head + d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) p[e] = (E)(acc[e] * f);
   }
 }
 
@@ -1224,7 +1272,7 @@ int make_plan(const flh_kv_attend_params* p, Plan* pl) {
   const bool sel = p->d_selected != nullptr;
   const uint64_t rows = sel ? G : ((uint64_t)n * G + B - 1) / B;   // of a sequence, on average
   pl->kvw = rows <= 32 || sel ? 4 : 1;
-  pl->nq = pl->kvw == 4 ? (rows <= 16 || pl->dp == 256 ? 1 : 2) : (pl->dp == 256 ? 2 : 4);
+  pl->nq = pl->dp == 256 || (pl->kvw == 4 && rows <= 16) ? 1 : 2;
   pl->tr = 16 * pl->nq * (4 / pl->kvw);
   uint64_t tiles, est;
   if (sel) tiles = est = (uint64_t)n * ((G + pl->tr - 1) / pl->tr);
@@ -1264,20 +1312,21 @@ void launch_attend(const AttendArgs& a, hipStream_t st) {
 template <class E>
 void run_attend(const AttendArgs& a, const Plan& pl, hipStream_t st) {
   if (pl.dp == 64) {
-    if (pl.kvw == 1) launch_attend<E, 64, 4, 1>(a, st);
+    if (pl.kvw == 1) launch_attend<E, 64, 2, 1>(a, st);
     else if (pl.nq == 1) launch_attend<E, 64, 1, 4>(a, st);
     else launch_attend<E, 64, 2, 4>(a, st);
   } else if (pl.dp == 128) {
-    if (pl.kvw == 1) launch_attend<E, 128, 4, 1>(a, st);
+    if (pl.kvw == 1) launch_attend<E, 128, 2, 1>(a, st);
     else if (pl.nq == 1) launch_attend<E, 128, 1, 4>(a, st);
     else launch_attend<E, 128, 2, 4>(a, st);
   } else {
-    if (pl.kvw == 1) launch_attend<E, 256, 2, 1>(a, st);
+    if (pl.kvw == 1) launch_attend<E, 256, 1, 1>(a, st);
     else launch_attend<E, 256, 1, 4>(a, st);
   }
   if (pl.splits > 1 && a.tiles_x) {
-    if (a.sel) FL_LAUNCH((fl_kv_join<E, true>), dim3(a.tiles_x * a.c.H), dim3(256), 0, st, a, pl.tr);
-    else FL_LAUNCH((fl_kv_join<E, false>), dim3(a.tiles_x * a.c.H), dim3(256), 0, st, a, pl.tr);
+    const dim3 grid(a.tiles_x * a.c.H, pl.tr / 4);
+    if (a.sel) FL_LAUNCH((fl_kv_join<E, true>), grid, dim3(256), 0, st, a, pl.tr);
+    else FL_LAUNCH((fl_kv_join<E, false>), grid, dim3(256), 0, st, a, pl.tr);
   }
   if (a.w_out) {
     const uint64_t span = (uint64_t)a.s.width * a.c.T > a.w_width ? (uint64_t)a.s.width * a.c.T : a.w_width;
