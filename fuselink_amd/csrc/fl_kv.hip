@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstring>
+#include <type_traits>
 
 #include "fl_device.h"
 #include "fl_internal.h"
@@ -66,6 +67,22 @@ __device__ __forceinline__ uint32_t seq_len(const Seqs& s, uint32_t T, uint32_t 
   const int32_t len = s.lens[b];
   const uint64_t most = (uint64_t)s.width * T;
   if (len < 0 || (uint64_t)len > most) { report(s.status); return len < 0 ? 0u : (uint32_t)most; }
+  return (uint32_t)len;
+}
+
+// the same for a sequence that the whole wavefront looks at
+__device__ __forceinline__ void uniform_tokens(const Seqs& s, uint32_t b, uint32_t& first, uint32_t& n) {
+  if (!s.starts) { first = b * s.per; n = s.per; return; }
+  const int32_t lo = scalar_load(s.starts + b), hi = scalar_load(s.starts + b + 1);
+  const bool ok = lo >= 0 && hi >= lo && (uint32_t)hi <= s.n_tokens;
+  if (!ok) report(s.status);
+  first = ok ? (uint32_t)lo : 0;
+  n = ok ? (uint32_t)(hi - lo) : 0;
+}
+__device__ __forceinline__ uint32_t uniform_len(const Seqs& s, uint32_t T, uint32_t b) {
+  const int32_t len = scalar_load(s.lens + b);
+  const uint32_t most = s.width * T;   // (the host keeps it within 31 bits)
+  if (len < 0 || (uint32_t)len > most) { report(s.status); return len < 0 ? 0u : most; }
   return (uint32_t)len;
 }
 
@@ -139,67 +156,68 @@ struct PackArgs {
   uint32_t budget, per_seq;
 };
 
+// Eight neighbouring channels of a token as they lie in memory, and as numbers.
+template <class E> struct Raw { uint32_t w[sizeof(E) * 2]; };
+struct Code { uint32_t w[2]; float s; };
+
 template <class E>
-__device__ __forceinline__ void load8(const E* p, bool vec, float* x);
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, bool vec, float* x) {
+__device__ __forceinline__ void load_raw(Raw<E>& r, const E* p, bool vec) {
+  constexpr int W = sizeof(E) * 2;
   if (vec) {
-    const f4 a = *reinterpret_cast<const f4*>(p), b = *reinterpret_cast<const f4*>(p + 4);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[4 + i] = b[i]; }
+    for (int i = 0; i < W; i += 4) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint32_t*>(p) + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r.w[i + e] = x[e];
+    }
+  } else if constexpr (sizeof(E) == 4) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) r.w[i] = reinterpret_cast<const uint32_t*>(p)[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = p[i];
+    for (int i = 0; i < W; ++i) r.w[i] = reinterpret_cast<const uint16_t*>(p)[2 * i] | (uint32_t)reinterpret_cast<const uint16_t*>(p)[2 * i + 1] << 16;
   }
 }
-template <>
-__device__ __forceinline__ void load8<_Float16>(const _Float16* p, bool vec, float* x) {
-  if (vec) {
-    const h8 a = *reinterpret_cast<const h8*>(p);
+template <class E>
+__device__ __forceinline__ void numbers(const Raw<E>& r, float* x) {   // what is not finite becomes NaN
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (float)p[i];
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (sizeof(E) == 4) x[i] = __uint_as_float(r.w[i]);
+    else if constexpr (__is_same(E, __bf16)) x[i] = __uint_as_float(i & 1 ? r.w[i >> 1] & 0xffff0000u : r.w[i >> 1] << 16);
+    else x[i] = (float)__builtin_bit_cast(h2, r.w[i >> 1])[i & 1];
+    x[i] = __builtin_isfinite(x[i]) ? x[i] : kNan;
   }
 }
-template <>
-__device__ __forceinline__ void load8<__bf16>(const __bf16* p, bool vec, float* x) {
-  if (vec) {
-    const u32x4 a = *reinterpret_cast<const u32x4*>(p);
+__device__ __forceinline__ void numbers(const Code& r, float* x) {
+  unpack4(r.w[0], x);
+  unpack4(r.w[1], x + 4);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(a[i] << 16); x[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u); }
-  } else {
-    const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float((uint32_t)q[i] << 16);
-  }
+  for (int i = 0; i < 8; ++i) x[i] *= r.s;
 }
 
-// One wavefront packs one side (K or V) of one head of one page.  A lane holds 8 neighbouring channels of every
-// RP-th token (RP = 64 / (D / 8) tokens at a time), so both the codes' rows and the channels' bounds come out of
-// registers.  The largest magnitude of the new tokens fixes the scale, then the same rows become codes.  Up to
-// kRows rows per lane stay in registers between the two; longer blocks are read twice (the second time from cache).
-// In evict the rows are codes of other records under their own scales.
-constexpr int kRows = 8;
-
-template <class E, bool EVICT, bool ONE>
+// One wavefront packs K and V of one head of one page.  A lane holds 8 neighbouring channels of every RP-th token
+// (RP = 64 / (D / 8) tokens at a time), so both the codes' rows and the channels' bounds come out of registers.  The
+// largest magnitude of the new tokens fixes the scale, then the same rows become codes.  Up to ROWS rows a lane stay in
+// registers between the two, as they were loaded; longer blocks are read twice, the second time from cache.  In evict the rows
+// are codes of other records under their own scales.
+template <class E, bool EVICT, int ROWS, bool ONE>
 __global__ __launch_bounds__(256) void fl_kv_pack(const PackArgs a) {
+  typedef typename std::conditional<EVICT, Code, Raw<E>>::type Row;
   const int lane = threadIdx.x & 63;
-  const uint32_t unit = blockIdx.y * 4 + uniform(threadIdx.x >> 6);
   const Cache& c = a.c;
-  if (unit >= 2 * c.H) return;
-  const uint32_t h = unit >> 1, side = unit & 1, T = c.T, D = c.D;
+  const uint32_t h = blockIdx.y * 4 + uniform(threadIdx.x >> 6);
+  if (h >= c.H) return;
+  const uint32_t T = c.T, D = c.D;
   uint32_t b, j, first = 0, n, held;
   int32_t page;
   if constexpr (EVICT) {
     b = blockIdx.x / a.per_seq;
     j = blockIdx.x - b * a.per_seq;
-    n = seq_len(a.s, a.from.T, b);
+    n = uniform_len(a.s, a.from.T, b);
     if (n > a.budget) n = a.budget;
     held = 0;
     if (j * T >= n) return;
-    page = a.to_table[b * a.to_stride + j];
+    page = scalar_load(a.to_table + b * a.to_stride + j);
   } else {
     const auto items = [&](uint32_t q) {
       uint32_t f, m;
@@ -209,11 +227,11 @@ __global__ __launch_bounds__(256) void fl_kv_pack(const PackArgs a) {
     };
     if (!find_seq(a.s.n_seqs, blockIdx.x, items, b, j)) return;
     b = uniform(b);
-    seq_tokens(a.s, b, first, n);
-    held = seq_len(a.s, T, b);
-    j += held / T;
+    uniform_tokens(a.s, b, first, n);
+    held = uniform_len(a.s, T, b);
+    j = uniform(j) + held / T;
     if (j >= a.s.width) { if (lane == 0) report(a.s.status); return; }
-    page = a.s.table[b * a.s.table_stride + j];
+    page = scalar_load(a.s.table + b * a.s.table_stride + j);
   }
   if (page < 0 || (uint32_t)page >= c.n_pages) { if (lane == 0) report(a.s.status); return; }
   const uint32_t at = j * T;                                   // position of the page's first slot
@@ -221,121 +239,147 @@ __global__ __launch_bounds__(256) void fl_kv_pack(const PackArgs a) {
   const uint64_t end64 = (uint64_t)held + n - at;
   const uint32_t fill = end64 < T ? (uint32_t)end64 : T;       // slots that hold one afterwards
   uint8_t* rec = c.pages + (uint64_t)page * c.stride;
-  uint8_t* codes = rec + side * c.side + (uint64_t)h * T * D;
-  float* scale_at = reinterpret_cast<float*>(rec + c.scales) + 2 * h + side;
+  float* scale_at = reinterpret_cast<float*>(rec + c.scales) + 2 * h;
 
   const uint32_t CG = D >> 3, RP = 64 / CG, grp = (uint32_t)lane / CG, cg = (uint32_t)lane - grp * CG;
   const bool on = grp < RP;
   const uint32_t passes = (T + RP - 1) / RP;
-  const float s_old = !EVICT && old ? *scale_at : 0.f;
+  float s_old[2] = {0.f, 0.f};
+  if (!EVICT && old) { s_old[0] = scale_at[0]; s_old[1] = scale_at[1]; }
 
-  float x[kRows][8];
-  const auto load = [&](uint32_t p0) {   // rows (p0 + i) * RP + grp: new tokens' values (evict: all of them), 0 elsewhere
+  Row x[2][ROWS];
+  const auto load = [&](uint32_t p0) {   // rows (p0 + i) * RP + grp: new tokens (evict: all of them), 0 elsewhere
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
+    for (int i = 0; i < ROWS; ++i) {
       const uint32_t r = (p0 + i) * RP + grp;
+      const bool in = on && r < fill && r >= old;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
-      if (!on || r >= fill || r < old) continue;
+      for (int side = 0; side < 2; ++side) x[side][i] = Row{};
+      if (!in) continue;
       if constexpr (EVICT) {
-        const int32_t pos = a.kept[b * a.kept_stride * c.H + (uint64_t)h * a.kept_stride + at + r];
+        const int32_t pos = a.kept[(b * (uint64_t)c.H + h) * a.kept_stride + at + r];
         const uint32_t slot = (uint32_t)pos / a.from.T;
         const int32_t pg = pos >= 0 && slot < a.s.width ? a.s.table[b * a.s.table_stride + slot] : -1;
         if (pg < 0 || (uint32_t)pg >= a.from.n_pages) { report(a.s.status); continue; }
         const uint8_t* f = a.from.pages + (uint64_t)pg * a.from.stride;
-        const float s = reinterpret_cast<const float*>(f + a.from.scales)[2 * h + side];
-        const u2 w = *reinterpret_cast<const u2*>(f + side * a.from.side + ((uint64_t)h * a.from.T + ((uint32_t)pos - slot * a.from.T)) * D + cg * 8);
-        unpack4(w[0], x[i]);
-        unpack4(w[1], x[i] + 4);
+        const u2 s = *reinterpret_cast<const u2*>(f + a.from.scales + 8 * h);
+        const uint64_t off = ((uint64_t)h * a.from.T + ((uint32_t)pos - slot * a.from.T)) * D + cg * 8;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[i][e] *= s;
+        for (int side = 0; side < 2; ++side) {
+          const u2 w = *reinterpret_cast<const u2*>(f + side * a.from.side + off);
+          x[side][i] = Code{{w[0], w[1]}, __uint_as_float(s[side])};
+        }
       } else {
-        const E* p = reinterpret_cast<const E*>(a.src[side]) + (uint64_t)(first + at + r - held) * a.token_stride[side] + h * a.head_stride[side] + cg * 8;
-        load8<E>(p, a.vec, x[i]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[i][e] = __builtin_isfinite(x[i][e]) ? x[i][e] : kNan;
+        for (int side = 0; side < 2; ++side)
+          load_raw<E>(x[side][i], reinterpret_cast<const E*>(a.src[side]) + (uint64_t)(first + at + r - held) * a.token_stride[side] + h * a.head_stride[side] + cg * 8, a.vec);
       }
     }
   };
 
-  float amax = 0.f;
-  for (uint32_t p0 = 0; p0 < passes; p0 += kRows) {
+  float amax[2] = {0.f, 0.f};
+  for (uint32_t p0 = 0; p0 < passes; p0 += ROWS) {
     load(p0);
 #pragma unroll
-    for (int i = 0; i < kRows; ++i)
+    for (int side = 0; side < 2; ++side)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[i][e]));   // fmaxf passes over NaN
+      for (int i = 0; i < ROWS; ++i) {
+        float y[8];
+        numbers(x[side][i], y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax[side] = fmaxf(amax[side], fabsf(y[e]));   // fmaxf passes over NaN
+      }
   }
 #pragma unroll
-  for (int o = 32; o; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
-  const float s = fmaxf(s_old, block_scale(amax)), inv = inverse(s);
-  const bool grown = old && s != s_old;
-  const float ratio = s_old * inv;
+  for (int o = 32; o; o >>= 1) {
+    amax[0] = fmaxf(amax[0], __shfl_xor(amax[0], o));
+    amax[1] = fmaxf(amax[1], __shfl_xor(amax[1], o));
+  }
+  float s[2];
+#pragma unroll
+  for (int side = 0; side < 2; ++side) s[side] = fmaxf(s_old[side], block_scale(amax[side]));
 
+  if constexpr (ONE) {   // what waits in registers for the scale is the rows as loaded, not their numbers
+#pragma unroll
+    for (int side = 0; side < 2; ++side)
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+        for (int e = 0; e < (int)(sizeof(x[0][0].w) / 4); ++e) asm("" : "+v"(x[side][i].w[e]));
+  }
   float lo[8], hi[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) { lo[e] = kInf; hi[e] = -kInf; }
-  for (uint32_t p0 = 0; p0 < passes; p0 += kRows) {
+  for (uint32_t p0 = 0; p0 < passes; p0 += ROWS) {
     if (!ONE) load(p0);
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const uint32_t r = (p0 + i) * RP + grp;
-      if (!on || r >= T) continue;
-      u2* row = reinterpret_cast<u2*>(codes + (uint64_t)r * D + cg * 8);
-      float y[8];
-      if (r < old) {
-        if (side == 1 && !grown) continue;
-        const u2 w = *row;
-        unpack4(w[0], y);
-        unpack4(w[1], y + 4);
-        if (grown) {
+    for (int side = 0; side < 2; ++side) {
+      const float inv = inverse(s[side]), ratio = s_old[side] * inv;
+      const bool grown = old && s[side] != s_old[side];
+      uint8_t* codes = rec + side * c.side + (uint64_t)h * T * D;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] *= ratio;
+      for (int i = 0; i < ROWS; ++i) {
+        const uint32_t r = (p0 + i) * RP + grp;
+        if (!on || r >= T) continue;
+        u2* row = reinterpret_cast<u2*>(codes + (uint64_t)r * D + cg * 8);
+        float y[8];
+        if (r < old) {
+          if (side == 1 && !grown) continue;
+          const u2 w = *row;
+          unpack4(w[0], y);
+          unpack4(w[1], y + 4);
+          if (grown) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] *= ratio;
+          }
+        } else {
+          numbers(x[side][i], y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] *= inv;
         }
-      } else {
+        if (side == 0 && r < fill) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = x[i][e] * inv;
-      }
-      if (r < fill) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) { lo[e] = fminf(lo[e], y[e]); hi[e] = fmaxf(hi[e], y[e]); }
-      }
-      if (r < old ? grown : (r < fill || !old)) {   // slots behind the tokens of a page that this call opens are zero
-        u2 w;
-        w[0] = pack4(y);
-        w[1] = pack4(y + 4);
-        *row = w;
+          for (int e = 0; e < 8; ++e) { lo[e] = fminf(lo[e], y[e]); hi[e] = fmaxf(hi[e], y[e]); }
+        }
+        if (r < old ? grown : (r < fill || !old)) {   // slots behind the tokens of a page that this call opens are zero
+          u2 w;
+          w[0] = pack4(y);
+          w[1] = pack4(y + 4);
+          *row = w;
+        }
       }
     }
   }
-  if (lane == 0) *scale_at = s;
-  if (side == 0) {
+  if (lane == 0) *reinterpret_cast<u2*>(scale_at) = u2{__float_as_uint(s[0]), __float_as_uint(s[1])};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float l = lo[e], u = hi[e];
+    if ((CG & (CG - 1)) == 0) {
+      for (uint32_t o = CG; o < 64; o <<= 1) {
+        l = fminf(l, __shfl_xor(l, (int)o));
+        u = fmaxf(u, __shfl_xor(u, (int)o));
+      }
+    } else {
+      for (uint32_t k = 1; k < RP; ++k) {
+        l = fminf(l, __shfl(lo[e], (int)(cg + k * CG)));
+        u = fmaxf(u, __shfl(hi[e], (int)(cg + k * CG)));
+      }
+    }
+    lo[e] = l;
+    hi[e] = u;
+  }
+  if (lane < (int)CG) {   // rounding is monotonic: the smallest value's code is the smallest code
+    u2 wl = {0, 0}, wh = {0, 0};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      float l = lo[e], u = hi[e];
-      for (uint32_t k = 1; k < RP; ++k) {
-        l = fminf(l, __shfl(lo[e], cg + k * CG));
-        u = fmaxf(u, __shfl(hi[e], cg + k * CG));
-      }
-      lo[e] = l;
-      hi[e] = u;
+      const bool any = lo[e] <= hi[e];
+      const uint32_t two = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(any ? lo[e] : 0.f, any ? hi[e] : 0.f, 0, false);
+      const int li = (int)floorf(__builtin_amdgcn_cvt_f32_fp8((int)two, 0) * 0.25f), ui = (int)ceilf(__builtin_amdgcn_cvt_f32_fp8((int)two, 1) * 0.25f);
+      wl[e >> 2] |= (uint32_t)(li & 0xff) << (8 * (e & 3));
+      wh[e >> 2] |= (uint32_t)(ui & 0xff) << (8 * (e & 3));
     }
-    if (lane < (int)CG) {   // rounding is monotonic: the smallest value's code is the smallest code
-      uint32_t wl[2] = {0, 0}, wh[2] = {0, 0};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const bool any = lo[e] <= hi[e];
-        const uint32_t two = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(any ? lo[e] : 0.f, any ? hi[e] : 0.f, 0, false);
-        const int li = (int)floorf(__builtin_amdgcn_cvt_f32_fp8((int)two, 0) * 0.25f), hi_i = (int)ceilf(__builtin_amdgcn_cvt_f32_fp8((int)two, 1) * 0.25f);
-        wl[e >> 2] |= (uint32_t)(li & 0xff) << (8 * (e & 3));
-        wh[e >> 2] |= (uint32_t)(hi_i & 0xff) << (8 * (e & 3));
-      }
-      u2 w;
-      w[0] = wl[0]; w[1] = wl[1];
-      *reinterpret_cast<u2*>(rec + c.low + (uint64_t)h * D + cg * 8) = w;
-      w[0] = wh[0]; w[1] = wh[1];
-      *reinterpret_cast<u2*>(rec + c.high + (uint64_t)h * D + cg * 8) = w;
-    }
+    *reinterpret_cast<u2*>(rec + c.low + (uint64_t)h * D + cg * 8) = wl;
+    *reinterpret_cast<u2*>(rec + c.high + (uint64_t)h * D + cg * 8) = wh;
   }
 }
 
@@ -456,9 +500,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) 
     if (!find_seq(a.s.n_seqs, x, items, b, tile)) return;
     b = uniform(b); tile = uniform(tile);
   }
-  seq_tokens(a.s, b, first, n);
-  first = uniform(first); n = uniform(n);
-  len = uniform(seq_len(a.s, T, b));
+  uniform_tokens(a.s, b, first, n);
+  len = uniform_len(a.s, T, b);
   // rows of this workgroup: (query token, head of the group), tokens first
   if constexpr (SEL) { r0 = tok0 * G + tile * TR; rows = (tok0 + 1) * G; } else { r0 = tile * TR; rows = n * G; }
   const uint32_t wr0 = r0 + (KVW == 1 ? wave * 16 * NQ : 0);
@@ -831,12 +874,14 @@ __global__ __launch_bounds__(256) void fl_kv_join(const AttendArgs a, uint32_t T
     const uint32_t per = (G + TR - 1) / TR, t = x / per;
     const auto items = [&](uint32_t q) { uint32_t f, m; seq_tokens(a.s, q, f, m); return m; };
     if (!find_seq(a.s.n_seqs, t, items, b, tok0)) return;
+    b = uniform(b);
     tile = x - t * per;
   } else {
     const auto items = [&](uint32_t q) { uint32_t f, m; seq_tokens(a.s, q, f, m); return (m * G + TR - 1) / TR; };
     if (!find_seq(a.s.n_seqs, x, items, b, tile)) return;
+    b = uniform(b);
   }
-  seq_tokens(a.s, b, first, n);
+  uniform_tokens(a.s, b, first, n);
   if constexpr (SEL) { r0 = tok0 * G + tile * TR; rows = (tok0 + 1) * G; } else { r0 = tile * TR; rows = n * G; }
   const uint64_t row_out = (uint64_t)a.s.n_tokens * H * G;
   const uint32_t r = r0 + blockIdx.y * 4 + wave;
@@ -891,58 +936,87 @@ __global__ __launch_bounds__(256) void fl_kv_weights(const AttendArgs a) {
   const uint32_t wave = uniform(threadIdx.x >> 6), H = a.c.H, G = a.G, T = a.c.T, D = a.c.D, h = blockIdx.y, b = blockIdx.z;
   const uint32_t k0 = (blockIdx.x * 4 + wave) * 64;
   uint32_t first, n;
-  seq_tokens(a.s, b, first, n);
-  first = uniform(first); n = uniform(n);
-  const uint32_t len = uniform(seq_len(a.s, T, b)), rows = n * G;
+  uniform_tokens(a.s, b, first, n);
+  const uint32_t len = uniform_len(a.s, T, b), rows = n * G;
   const float* w_in = a.w_in ? a.w_in + b * a.wi_seq + h * a.wi_head : nullptr;
   float* w_out = a.w_out + b * a.wo_seq + h * a.wo_head;
   if (len > a.w_width && lane == 0) report(a.s.status);
-  const int32_t* table = a.s.table + b * a.s.table_stride;
+  float acc[4][4];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const uint32_t v = k0 + 16 * t, j = v / T, off = v - j * T;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    if (v < len && rows) {
-      const int32_t pg = table[j];
-      if (pg < 0 || (uint32_t)pg >= a.c.n_pages) {
-        if (lane == 0) report(a.s.status);
-      } else {
-        const uint8_t* rec = a.c.pages + (uint64_t)pg * a.c.stride;
-        const float kc = reinterpret_cast<const float*>(rec + a.c.scales)[2 * h] * a.scale2;
-        const uint8_t* base = rec + (uint64_t)(h * T + off + c) * D;
-        const uint32_t d0 = g * (DP / 4);
-        v8 kf[KK];
+  for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < KW / 4; ++i) {
-          u32x4 w = {0, 0, 0, 0};
-          if (d0 + 16 * i < D) w = *reinterpret_cast<const u32x4*>(base + d0 + 16 * i);
-          kf[2 * i] = codes8<E>(w[0], w[1]);
-          kf[2 * i + 1] = codes8<E>(w[2], w[3]);
-        }
-        for (uint32_t r0 = 0; r0 < rows; r0 += 16) {
-          const uint32_t r = r0 + c, i = r / G;
-          const bool in = r < rows;
-          const uint64_t tok = first + i, hq = h * G + (r - i * G);
-          const E* p = reinterpret_cast<const E*>(a.q) + tok * a.q_token + hq * a.q_head;
-          f4 s = {0.f, 0.f, 0.f, 0.f};
+    for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
+  if (k0 < len && rows) {
+    const int32_t* table = a.s.table + b * a.s.table_stride;
+    const uint32_t last_tile = (len - 1) >> 4;
+    uint32_t kw[4][KW], bad = 0;
+    float kc[4];
+    bool ok[4];
+    uint32_t k_lane[KW / 4];
 #pragma unroll
-          for (int k = 0; k < KK; ++k) s = Frag<E>::mfma(kf[k], flipped<E>(load_q8<E>(p + d0 + k * 8, in && d0 + k * 8 < D, a.q_vec), a.flip), s);
-          int64_t lim = !in ? 0 : a.causal ? (int64_t)len - n + i + 1 : len;
-          const float lg = in ? a.lse2[tok * H * G + hq] : 0.f;
+    for (int i = 0; i < KW / 4; ++i) k_lane[i] = c * D + (g * (DP / 4) + 16 * i < D ? g * (DP / 4) + 16 * i : 0);
+    uint32_t page[4], slot[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if ((int64_t)(v + 4 * g + e) < lim) acc[e] += exp2_fast(s[e] * kc - lg);
-        }
+    for (int t = 0; t < 4; ++t) {
+      const uint32_t tv = (k0 >> 4) + t, tl = tv < last_tile ? tv : last_tile, j = a.per_page == 1 ? tl : __umulhi(tl, a.per_page_inv);
+      slot[t] = (tl - j * a.per_page) << 4;
+      page[t] = (uint32_t)scalar_load(table + j);
+      ok[t] = tv <= last_tile;
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const bool there = page[t] < a.c.n_pages;
+      bad |= ok[t] && !there ? 1 : 0;
+      ok[t] = ok[t] && there;
+      const uint8_t* rec = a.c.pages + (uint64_t)(there ? page[t] : 0) * a.c.stride;
+      kc[t] = scalar_load(reinterpret_cast<const float*>(rec + a.c.scales) + 2 * h) * a.scale2;
+      const uint8_t* base = rec + (uint64_t)(h * T + slot[t]) * D;
+      asm("" : "+s"(base));
+#pragma unroll
+      for (int i = 0; i < KW / 4; ++i) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(base + k_lane[i]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) kw[t][4 * i + e] = w[e];
       }
     }
+    if (bad && lane == 0) report(a.s.status);
+    for (uint32_t r0 = 0; r0 < rows; r0 += 16) {
+      const uint32_t r = r0 + c, i = r / G;
+      const bool in = r < rows;
+      const uint64_t tok = first + i, hq = h * G + (r - i * G);
+      const E* p = reinterpret_cast<const E*>(a.q) + tok * a.q_token + hq * a.q_head;
+      v8 qf[KK];
+#pragma unroll
+      for (int k = 0; k < KK; ++k) qf[k] = flipped<E>(load_q8<E>(p + g * (DP / 4) + k * 8, in && g * (DP / 4) + k * 8 < D, a.q_vec), a.flip);
+      const float lg = in ? a.lse2[tok * H * G + hq] : 0.f;
+      const int64_t lim64 = !in ? 0 : a.causal ? (int64_t)len - n + i + 1 : len;
+      const uint32_t lim = lim64 > 0 ? (uint32_t)lim64 : 0;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        f4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KK; ++k) s = Frag<E>::mfma(codes8<E>(kw[t][2 * k], kw[t][2 * k + 1]), qf[k], s);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (ok[t] && k0 + 16 * t + 4 * g + e < lim) acc[t][e] += exp2_fast(__builtin_fmaf(s[e], kc[t], -lg));
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
 #pragma unroll
-      for (int o = 8; o; o >>= 1) acc[e] += __shfl_xor(acc[e], o);
-      const uint32_t p = v + 4 * g + e;
-      if (c == 0 && p < a.w_width && (p < len || w_in != w_out)) w_out[p] = (w_in ? w_in[p] : 0.f) + (p < len ? acc[e] : 0.f);
+      for (int o = 8; o; o >>= 1) acc[t][e] += __shfl_xor(acc[t][e], o);
     }
-  }
+  // lane c of group g writes position 4 g + (c & 3) of tile c >> 2
+  float mine = 0.f;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) mine = c == 4 * t + e ? acc[t][e] : mine;
+  const uint32_t p = k0 + 16 * (c >> 2) + 4 * g + (c & 3);
+  if (p < a.w_width && (p < len || w_in != w_out)) w_out[p] = (w_in ? w_in[p] : 0.f) + (p < len ? mine : 0.f);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -953,7 +1027,7 @@ struct SelectArgs {
   Seqs s;
   const void* q;
   uint64_t q_token, q_head;
-  uint32_t G, causal, q_vec, first, last, count;
+  uint32_t G, causal, q_vec, first, last, count, parts;
   float* scores;              // [n_tokens][H][width]
   int32_t* out;               // [n_tokens][H][count]
 };
@@ -973,59 +1047,77 @@ template <class E, int DP>
 __global__ __launch_bounds__(256) void fl_kv_score(const SelectArgs a) {
   constexpr int KK = DP / 64;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-  const uint32_t wave = uniform(threadIdx.x >> 6), H = a.c.H, G = a.G, T = a.c.T, D = a.c.D, h = blockIdx.y;
+  const uint32_t wave = uniform(threadIdx.x >> 6), H = a.c.H, G = a.G, T = a.c.T, D = a.c.D, h = blockIdx.x % H, part = blockIdx.x / H;
   uint32_t b, i, first, n;
   const auto items = [&](uint32_t q) { uint32_t f, m; seq_tokens(a.s, q, f, m); return m; };
-  if (!find_seq(a.s.n_seqs, blockIdx.z, items, b, i)) return;
+  if (!find_seq(a.s.n_seqs, blockIdx.y, items, b, i)) return;
   b = uniform(b);
-  seq_tokens(a.s, b, first, n);
-  const uint32_t lim = token_limit(a, seq_len(a.s, T, b), n, i), pages = (lim + T - 1) / T;
-  const uint32_t p0 = (blockIdx.x * 4 + wave) * 64;
+  i = uniform(i);
+  uniform_tokens(a.s, b, first, n);
+  const uint32_t lim = token_limit(a, uniform_len(a.s, T, b), n, i), pages = (lim + T - 1) / T;
+  const uint32_t step = a.parts * 4 * 32;                  // 32 pages to a wavefront at a time
+  uint32_t p0 = (part * 4 + wave) * 32;
   if (p0 >= pages) return;
   const uint64_t tok = first + i;
-  float best[4][4];
-#pragma unroll
-  for (int t = 0; t < 4; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) best[t][e] = -kInf;
   const int32_t* table = a.s.table + b * a.s.table_stride;
-  const uint8_t* rec[4];
+  float* out = a.scores + (tok * H + h) * a.s.width;
+
+  struct Bounds { i4 lo[2][KK], hi[2][KK]; float ks[2]; };
+  uint32_t d_lane[KK];   // dims beyond D meet zeros of the query
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const uint32_t p = p0 + 16 * t + c;
-    const int32_t pg = p < pages ? table[p] : 0;
-    const bool ok = pg >= 0 && (uint32_t)pg < a.c.n_pages;
-    if (!ok) report(a.s.status);
-    rec[t] = ok ? a.c.pages + (uint64_t)pg * a.c.stride : nullptr;
-  }
-  for (uint32_t h0 = 0; h0 < G; h0 += 16) {
+  for (int k = 0; k < KK; ++k) d_lane[k] = k * 64 + g * 16 < D ? k * 64 + g * 16 : 0;
+  uint32_t bad = 0;
+  const auto number = [&](uint32_t p, int32_t* pg) {       // page numbers of rows c of the two tiles
+#pragma unroll
+    for (int t = 0; t < 2; ++t) pg[t] = table[p + 16 * t + c < pages ? p + 16 * t + c : pages - 1];
+  };
+  const auto fetch = [&](const int32_t* pg, Bounds& x) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const bool there = (uint32_t)pg[t] < a.c.n_pages;
+      bad |= there ? 0 : 1;
+      const uint8_t* rec = a.c.pages + (uint64_t)(there ? (uint32_t)pg[t] : 0) * a.c.stride;
+      const uint8_t *lo = rec + a.c.low + h * D, *hi = rec + a.c.high + h * D;
+#pragma unroll
+      for (int k = 0; k < KK; ++k) {
+        x.hi[t][k] = *reinterpret_cast<const i4*>(hi + d_lane[k]);
+        x.lo[t][k] = *reinterpret_cast<const i4*>(lo + d_lane[k]);
+      }
+      x.ks[t] = *(reinterpret_cast<const float*>(rec + a.c.scales) + 2 * h);
+      if (!there) x.ks[t] = kNan;
+    }
+  };
+  int32_t pg[2];
+  number(p0, pg);
+
+  // the queries of up to 16 heads as 8-bit whole numbers, split by sign (more heads: one round for each 16)
+  i4 up[KK], dn[KK];
+  float scale = 0.f;
+  const auto queries = [&](uint32_t h0) {
     const bool in = h0 + c < G;
     const E* q = reinterpret_cast<const E*>(a.q) + tok * a.q_token + (uint64_t)(h * G + h0 + c) * a.q_head;
-    float x[KK][16], amax = 0.f;
+    typename Frag<E>::v8 x[KK][2];
 #pragma unroll
     for (int k = 0; k < KK; ++k)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t d = k * 64 + g * 16 + u * 8;
-        const typename Frag<E>::v8 w = load_q8<E>(q + d, in && d < D, a.q_vec);
+      for (int u = 0; u < 2; ++u) x[k][u] = load_q8<E>(q + k * 64 + g * 16 + u * 8, in && k * 64 + g * 16 < D, a.q_vec);
+    float amax = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float v = (float)w[e];
-          if (!__builtin_isfinite(v)) v = 0.f;
-          x[k][8 * u + e] = v;
-          amax = fmaxf(amax, fabsf(v));
-        }
+    for (int k = 0; k < KK; ++k)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float v = (float)x[k][e >> 3][e & 7];
+        amax = fmaxf(amax, __builtin_isfinite(v) ? fabsf(v) : 0.f);
       }
     amax = column_max(amax);
-    float step = 0.f;   // smallest 2^e >= amax / 127, 127 = 1.984375 * 2^6
+    scale = 0.f;   // smallest 2^e >= amax / 127, 127 = 1.984375 * 2^6
     if (amax > 0.f) {
       const uint32_t u = __float_as_uint(amax);
       int e = (int)(u >> 23) - 127 - ((u & 0x7fffffu) <= 0x7e0000u ? 6 : 5);
       if (e < -126 || u < 0x800000u) e = -126;
-      step = pow2f(e);
+      scale = pow2f(e);
     }
-    const float inv = inverse(step);
-    i4 up[KK], dn[KK];
+    const float inv = inverse(scale);
 #pragma unroll
     for (int k = 0; k < KK; ++k)
 #pragma unroll
@@ -1033,49 +1125,59 @@ __global__ __launch_bounds__(256) void fl_kv_score(const SelectArgs a) {
         uint32_t pu = 0, pd = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int v = (int)rintf(x[k][4 * w + e] * inv);
+          float f = (float)x[k][w >> 1][(4 * w + e) & 7];
+          f = __builtin_isfinite(f) ? f : 0.f;
+          const int v = (int)rintf(f * inv);
           pu |= (uint32_t)(v > 0 ? v : 0) << (8 * e);
           pd |= (uint32_t)((v < 0 ? v : 0) & 0xff) << (8 * e);
         }
         up[k][w] = (int)pu;
         dn[k][w] = (int)pd;
       }
+    return in;
+  };
+
+  Bounds now;
+  fetch(pg, now);
+  bool in = queries(0);
+  for (; p0 < pages; p0 += step) {
+    number(p0 + step < pages ? p0 + step : p0, pg);
+    float best[2][4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      if (p0 + 16 * t >= pages) break;
-      i4 sum = {0, 0, 0, 0};
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int k = 0; k < KK; ++k) {
-        const uint32_t d = k * 64 + g * 16;
-        i4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-        if (rec[t] && d < D) {
-          lo = *reinterpret_cast<const i4*>(rec[t] + a.c.low + (uint64_t)h * D + d);
-          hi = *reinterpret_cast<const i4*>(rec[t] + a.c.high + (uint64_t)h * D + d);
+      for (int e = 0; e < 4; ++e) best[t][e] = -kInf;
+    for (uint32_t h0 = 0; h0 < G; h0 += 16) {
+      if (G > 16) in = queries(h0);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        i4 sum = {0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < KK; ++k) {
+          sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(now.hi[t][k], up[k], sum, 0, 0, 0);
+          sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(now.lo[t][k], dn[k], sum, 0, 0, 0);
         }
-        sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(hi, up[k], sum, 0, 0, 0);
-        sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(lo, dn[k], sum, 0, 0, 0);
-      }
-      // row 4 g + e: a page; column c: a head
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (in) best[t][e] = fmaxf(best[t][e], (float)sum[e] * step);
+        for (int e = 0; e < 4; ++e) best[t][e] = in ? fmaxf(best[t][e], (float)sum[e] * scale) : best[t][e];   // row 4 g + e: a page; column c: a head
+      }
     }
+    const float ks0 = now.ks[0], ks1 = now.ks[1];
+    fetch(pg, now);
+    float mine = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v = best[t][e];
+#pragma unroll
+        for (int o = 8; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+        v *= __shfl(t ? ks1 : ks0, 4 * g + e);
+        mine = c == 4 * t + e ? (v != v ? -kInf : v) : mine;
+      }
+    const uint32_t p = p0 + 16 * (c >> 2) + 4 * g + (c & 3);
+    if (c < 8 && p < pages) out[p] = mine;
   }
-  float* out = a.scores + (tok * H + h) * a.s.width;
-#pragma unroll
-  for (int t = 0; t < 4; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float v = best[t][e];
-#pragma unroll
-      for (int o = 8; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-      const uint32_t p = p0 + 16 * t + 4 * g + e;
-      if (c == 0 && p < pages) {
-        const int32_t pg = table[p];
-        const bool ok = pg >= 0 && (uint32_t)pg < a.c.n_pages;
-        out[p] = ok ? v * reinterpret_cast<const float*>(a.c.pages + (uint64_t)pg * a.c.stride + a.c.scales)[2 * h] : -kInf;
-      }
-    }
+  if (bad) report(a.s.status);
 }
 
 // Numbers in their order as unsigned integers; NaN before all of them, what has to stay behind.
@@ -1087,77 +1189,99 @@ __device__ __forceinline__ uint32_t order_key(float f) {
 }
 
 struct Pick { uint32_t key, need; };
+constexpr int kHeld = 16;   // keys a thread holds: 16384 in a workgroup of 1024
 
-// The k-th largest of n keys (k < n), by its bytes from the top: key, and how many of its equals belong to the k.
-// One workgroup of 1024.
-template <class Key>
-__device__ Pick kth_largest(uint32_t n, uint32_t k, Key key, uint32_t* hist, uint32_t* word) {
+struct PickShared { uint32_t hist[2048], word[2], sums[2][kHeld * 16], wave[16]; };
+
+// The k-th largest of n keys (k < n), by 11, 11 and 10 of its bits from the top, and how many of its equals belong to
+// the k.  The first digit holds the exponent and two bits of the mantissa, so that numbers of like size do not all
+// count into a few bins.  One workgroup of 1024; ONE: the keys stay in registers.
+template <bool ONE, class Load>
+__device__ Pick kth_largest(uint32_t n, uint32_t k, uint32_t* keys, Load load, PickShared& sh) {
   uint32_t prefix = 0, mask = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (threadIdx.x < 256) hist[threadIdx.x] = 0;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const uint32_t shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, ones = pass == 2 ? 1023 : 2047;
+    sh.hist[tid] = 0;
+    sh.hist[1024 + tid] = 0;
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += 1024) {
-      const uint32_t u = key(i);
-      if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift) & 255], 1u);
+    for (uint32_t base = 0; base < n; base += 1024 * kHeld) {
+      if (!ONE) load(base);
+#pragma unroll
+      for (int j = 0; j < kHeld; ++j)
+        if (base + j * 1024 + tid < n && (keys[j] & mask) == prefix) atomicAdd(&sh.hist[(keys[j] >> shift) & ones], 1u);
     }
     __syncthreads();
-    if (threadIdx.x < 64) {   // lane l looks at bins 255 - 4 l ... 252 - 4 l
-      const uint32_t l = threadIdx.x;
-      uint32_t cnt[4], sum = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) { cnt[e] = hist[255 - 4 * l - e]; sum += cnt[e]; }
-      const uint32_t incl = wave_incl_sum_u32(sum, (int)l);
-      uint32_t before = incl - sum;
-      if (before < k && k <= incl) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (before < k && k <= before + cnt[e]) { word[0] = 255 - 4 * l - e; word[1] = k - before; }
-          before += cnt[e];
-        }
-      }
-    }
+    // thread t owns bins 2047 - 2 t and 2046 - 2 t: a scan from the top
+    const uint32_t c0 = sh.hist[2047 - 2 * tid], c1 = sh.hist[2046 - 2 * tid], incl = wave_incl_sum_u32(c0 + c1, (int)lane);
+    if (lane == 63) sh.wave[wave] = incl;
     __syncthreads();
-    prefix |= word[0] << shift;
-    mask |= 255u << shift;
-    k = word[1];
+    uint32_t before = incl - c0 - c1;
+    for (uint32_t w = 0; w < wave; ++w) before += sh.wave[w];
+    if (before < k && k <= before + c0) { sh.word[0] = 2047 - 2 * tid; sh.word[1] = k - before; }
+    else if (before + c0 < k && k <= before + c0 + c1) { sh.word[0] = 2046 - 2 * tid; sh.word[1] = k - before - c0; }
+    __syncthreads();
+    prefix |= sh.word[0] << shift;
+    mask |= ones << shift;
+    k = sh.word[1];
     __syncthreads();
   }
   return {prefix, k};
 }
 
-// Indices of the keys above the pick and of the first `need` equal to it, in ascending order.
-template <class Key, class Put>
-__device__ void put_picked(uint32_t n, Pick pick, Key key, Put put, uint32_t* sums) {
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// Indices of the keys above the pick and of the first `need` equal to it, in ascending order: put(place, index, j).
+template <bool ONE, class Load, class Put>
+__device__ void put_picked(uint32_t n, Pick pick, const uint32_t* keys, Load load, Put put, PickShared& sh) {
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   uint32_t above = 0, equal = 0;   // in all rounds so far
-  for (uint32_t base = 0; base < n; base += 1024) {
-    const uint32_t i = base + threadIdx.x;
-    const uint32_t u = i < n ? key(i) : 0;
-    const bool gt = i < n && u > pick.key, eq = i < n && u == pick.key;
-    const uint64_t bg = __ballot(gt), be = __ballot(eq), below = (1ull << lane) - 1;
-    if (lane == 0) { sums[wave] = (uint32_t)__popcll(bg); sums[16 + wave] = (uint32_t)__popcll(be); }
-    __syncthreads();
-    uint32_t g0 = above, e0 = equal;
-    for (uint32_t w = 0; w < 16; ++w) {
-      if (w < wave) { g0 += sums[w]; e0 += sums[16 + w]; }
-      above += sums[w];
-      equal += sums[16 + w];
+  for (uint32_t base = 0; base < n; base += 1024 * kHeld) {
+    if (!ONE) load(base);
+    uint32_t before[kHeld];        // of this wavefront's 64 keys: those above in the low half, those equal in the high half
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      const bool in = base + j * 1024 + tid < n;
+      const uint64_t bg = __ballot(in && keys[j] > pick.key), be = __ballot(in && keys[j] == pick.key);
+      before[j] = (uint32_t)__popcll(bg & below) | (uint32_t)__popcll(be & below) << 16;
+      if (lane == 0) { sh.sums[0][j * 16 + wave] = (uint32_t)__popcll(bg); sh.sums[1][j * 16 + wave] = (uint32_t)__popcll(be); }
     }
-    g0 += (uint32_t)__popcll(bg & below);
-    e0 += (uint32_t)__popcll(be & below);
-    if (gt || (eq && e0 < pick.need)) put(g0 + (e0 < pick.need ? e0 : pick.need), i);
+    __syncthreads();
+    if (wave < 2) {                // 256 counts in the order of the keys, four to a lane: exclusive sums in place
+      uint32_t c[4], sum = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { c[e] = sh.sums[wave][4 * lane + e]; sum += c[e]; }
+      const uint32_t incl = wave_incl_sum_u32(sum, (int)lane);
+      uint32_t run = incl - sum;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { sh.sums[wave][4 * lane + e] = run; run += c[e]; }
+      if (lane == 63) sh.word[wave] = incl;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      const uint32_t i = base + j * 1024 + tid;
+      if (i < n && keys[j] >= pick.key) {
+        const uint32_t g0 = above + sh.sums[0][j * 16 + wave] + (before[j] & 0xffffu), e0 = equal + sh.sums[1][j * 16 + wave] + (before[j] >> 16);
+        if (keys[j] > pick.key || e0 < pick.need) put(g0 + (e0 < pick.need ? e0 : pick.need), i);
+      }
+    }
+    above += sh.word[0];
+    equal += sh.word[1];
     __syncthreads();
   }
 }
 
+template <bool ONE>
 __global__ __launch_bounds__(1024) void fl_kv_pick_pages(const SelectArgs a) {
-  __shared__ uint32_t hist[256], word[2], sums[32];
+  __shared__ PickShared sh;
   const uint32_t h = blockIdx.x % a.c.H, t = blockIdx.x / a.c.H;
   uint32_t b, i, first, n;
   const auto items = [&](uint32_t q) { uint32_t f, m; seq_tokens(a.s, q, f, m); return m; };
   if (!find_seq(a.s.n_seqs, t, items, b, i)) return;
-  seq_tokens(a.s, b, first, n);
-  const uint32_t lim = token_limit(a, seq_len(a.s, a.c.T, b), n, i), pages = (lim + a.c.T - 1) / a.c.T;
+  b = uniform(b);
+  uniform_tokens(a.s, b, first, n);
+  const uint32_t lim = token_limit(a, uniform_len(a.s, a.c.T, b), n, uniform(i)), pages = (lim + a.c.T - 1) / a.c.T;
   const uint64_t row = (uint64_t)(first + i) * a.c.H + h;
   const float* score = a.scores + row * a.s.width;
   int32_t* out = a.out + row * a.count;
@@ -1166,9 +1290,17 @@ __global__ __launch_bounds__(1024) void fl_kv_pick_pages(const SelectArgs a) {
     for (uint32_t k = threadIdx.x; k < pages; k += 1024) out[k] = (int32_t)k;
     return;
   }
-  const auto key = [&](uint32_t p) { return p < a.first || p + a.last >= pages ? 0xffffffffu : order_key(score[p]); };
-  const Pick pick = kth_largest(pages, a.count, key, hist, word);
-  put_picked(pages, pick, key, [&](uint32_t at, uint32_t p) { out[at] = (int32_t)p; }, sums);
+  uint32_t keys[kHeld];
+  const auto load = [&](uint32_t base) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      const uint32_t p = base + j * 1024 + threadIdx.x;
+      keys[j] = p >= pages ? 0 : p < a.first || p + a.last >= pages ? 0xffffffffu : order_key(score[p]);
+    }
+  };
+  if (ONE) load(0);
+  const Pick pick = kth_largest<ONE>(pages, a.count, keys, load, sh);
+  put_picked<ONE>(pages, pick, keys, load, [&](uint32_t at, uint32_t p) { out[at] = (int32_t)p; }, sh);
 }
 
 struct KeepArgs {
@@ -1181,10 +1313,11 @@ struct KeepArgs {
   int32_t* new_lens;
 };
 
+template <bool ONE>
 __global__ __launch_bounds__(1024) void fl_kv_keep(const KeepArgs a) {
-  __shared__ uint32_t hist[256], word[2], sums[32];
+  __shared__ PickShared sh;
   const uint32_t h = blockIdx.x % a.H, b = blockIdx.x / a.H;
-  uint32_t len = seq_len(a.s, a.T, b);
+  uint32_t len = uniform_len(a.s, a.T, b);
   if (len > a.w_width) { if (threadIdx.x == 0) report(a.s.status); len = a.w_width; }
   const float* w = a.w + b * a.w_seq + h * a.w_head;
   float* nw = a.nw + b * a.nw_seq + h * a.nw_head;
@@ -1197,9 +1330,17 @@ __global__ __launch_bounds__(1024) void fl_kv_keep(const KeepArgs a) {
     for (uint32_t k = threadIdx.x; k < len; k += 1024) { kept[k] = (int32_t)k; nw[k] = w[k]; }
     return;
   }
-  const auto key = [&](uint32_t p) { return p < a.first || p + a.recent >= len ? 0xffffffffu : order_key(w[p]); };
-  const Pick pick = kth_largest(len, m, key, hist, word);
-  put_picked(len, pick, key, [&](uint32_t at, uint32_t p) { kept[at] = (int32_t)p; nw[at] = w[p]; }, sums);
+  uint32_t keys[kHeld];
+  const auto load = [&](uint32_t base) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      const uint32_t p = base + j * 1024 + threadIdx.x;
+      keys[j] = p >= len ? 0 : p < a.first || p + a.recent >= len ? 0xffffffffu : order_key(w[p]);
+    }
+  };
+  if (ONE) load(0);
+  const Pick pick = kth_largest<ONE>(len, m, keys, load, sh);
+  put_picked<ONE>(len, pick, keys, load, [&](uint32_t at, uint32_t p) { kept[at] = (int32_t)p; nw[at] = w[p]; }, sh);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1337,12 +1478,14 @@ void run_attend(const AttendArgs& a, const Plan& pl, hipStream_t st) {
   }
 }
 
+// Rows of a page that stay in a lane's registers: 4 or 8 (pages of 16 and 32 tokens of 128 channels), else the page is read twice.
 template <class E, bool EVICT>
 void launch_pack(const PackArgs& a, uint32_t items, hipStream_t st) {
-  const uint32_t rp = 64 / (a.c.D / 8);
-  const dim3 grid(items, (2 * a.c.H + 3) / 4);
-  if ((a.c.T + rp - 1) / rp <= (uint32_t)kRows) FL_LAUNCH((fl_kv_pack<E, EVICT, true>), grid, dim3(256), 0, st, a);
-  else FL_LAUNCH((fl_kv_pack<E, EVICT, false>), grid, dim3(256), 0, st, a);
+  const uint32_t rp = 64 / (a.c.D / 8), rows = (a.c.T + rp - 1) / rp;
+  const dim3 grid(items, (a.c.H + 3) / 4);
+  if (rows <= 4) FL_LAUNCH((fl_kv_pack<E, EVICT, 4, true>), grid, dim3(256), 0, st, a);
+  else if (rows <= 8) FL_LAUNCH((fl_kv_pack<E, EVICT, 8, true>), grid, dim3(256), 0, st, a);
+  else FL_LAUNCH((fl_kv_pack<E, EVICT, 4, false>), grid, dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -1481,12 +1624,17 @@ int flh_kv_select(const flh_kv_select_params* p, void* stream) {
   a.out = p->d_out;
   fl_prof().kid = 10;
   const hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((a.s.width + 255) / 256, a.c.H, a.s.n_tokens);
+  // workgroups to a row of scores: enough for 8 a compute unit between all rows, each with 128 pages at least
+  const uint64_t rows = (uint64_t)a.s.n_tokens * a.c.H;
+  const uint32_t want = (uint32_t)((2048 + rows - 1) / rows), most = (a.s.width + 127) / 128;
+  a.parts = want < most ? want : most;
+  const dim3 grid(a.parts * a.c.H, a.s.n_tokens);
   const bool bf = p->type == FLH_KV_BF16;
   if (a.c.D <= 64) { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 64>), grid, dim3(256), 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 64>), grid, dim3(256), 0, st, a); }
   else if (a.c.D <= 128) { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 128>), grid, dim3(256), 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 128>), grid, dim3(256), 0, st, a); }
   else { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 256>), grid, dim3(256), 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 256>), grid, dim3(256), 0, st, a); }
-  FL_LAUNCH(fl_kv_pick_pages, dim3(a.s.n_tokens * a.c.H), dim3(1024), 0, st, a);
+  if (a.s.width <= 1024 * kHeld) FL_LAUNCH((fl_kv_pick_pages<true>), dim3(a.s.n_tokens * a.c.H), dim3(1024), 0, st, a);
+  else FL_LAUNCH((fl_kv_pick_pages<false>), dim3(a.s.n_tokens * a.c.H), dim3(1024), 0, st, a);
   return finish("flh_kv_select");
 }
 
@@ -1535,7 +1683,8 @@ int flh_kv_evict(const flh_kv_evict_params* p, void* stream) {
   a.per_seq = per;
   fl_prof().kid = 11;
   const hipStream_t st = (hipStream_t)stream;
-  FL_LAUNCH(fl_kv_keep, dim3(a.s.n_seqs * a.c.H), dim3(1024), 0, st, k);
+  if (k.w_width <= 1024 * kHeld) FL_LAUNCH((fl_kv_keep<true>), dim3(a.s.n_seqs * a.c.H), dim3(1024), 0, st, k);
+  else FL_LAUNCH((fl_kv_keep<false>), dim3(a.s.n_seqs * a.c.H), dim3(1024), 0, st, k);
   launch_pack<__bf16, true>(a, per * a.s.n_seqs, st);
   return finish("flh_kv_evict");
 }
