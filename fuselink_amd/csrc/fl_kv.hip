@@ -108,6 +108,29 @@ __device__ __forceinline__ bool find_seq(uint32_t n_seqs, uint32_t x, Count coun
 
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 
+// the four lanes that share a column of a 16 x 16 result: l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float column_max(float v) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float column_sum(float v) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// all lanes get the largest of the 64 (a row of 16 by DPP, the four rows as above)
+__device__ __forceinline__ float wave_max_f32(float v) {
+  v = fmaxf(v, __uint_as_float(dpp_u32<0xb1>(__float_as_uint(v))));    // quad_perm 1 0 3 2
+  v = fmaxf(v, __uint_as_float(dpp_u32<0x4e>(__float_as_uint(v))));    // quad_perm 2 3 0 1
+  v = fmaxf(v, __uint_as_float(dpp_u32<0x141>(__float_as_uint(v))));   // mirrored in 8
+  v = fmaxf(v, __uint_as_float(dpp_u32<0x140>(__float_as_uint(v))));   // mirrored in 16
+  return column_max(v);
+}
+
 // ------------------------------------------------------------------------------------------------
 // e4m3 codes under a power-of-two scale
 // ------------------------------------------------------------------------------------------------
@@ -124,16 +147,6 @@ __device__ __forceinline__ float block_scale(float amax) {
 }
 __device__ __forceinline__ float inverse(float s) {   // of a power of two, exact; 0 for 0
   return s > 0.f ? __uint_as_float((254u << 23) - __float_as_uint(s)) : 0.f;
-}
-__device__ __forceinline__ void unpack4(uint32_t w, float* x) {
-  x[0] = __builtin_amdgcn_cvt_f32_fp8((int)w, 0);
-  x[1] = __builtin_amdgcn_cvt_f32_fp8((int)w, 1);
-  x[2] = __builtin_amdgcn_cvt_f32_fp8((int)w, 2);
-  x[3] = __builtin_amdgcn_cvt_f32_fp8((int)w, 3);
-}
-__device__ __forceinline__ uint32_t pack4(const float* x) {
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -179,20 +192,98 @@ __device__ __forceinline__ void load_raw(Raw<E>& r, const E* p, bool vec) {
   }
 }
 template <class E>
-__device__ __forceinline__ void numbers(const Raw<E>& r, float* x) {   // what is not finite becomes NaN
+__device__ __forceinline__ float number(const Raw<E>& r, int i) {
+  if constexpr (sizeof(E) == 4) return __uint_as_float(r.w[i]);
+  else if constexpr (__is_same(E, __bf16)) return __uint_as_float(i & 1 ? r.w[i >> 1] & 0xffff0000u : r.w[i >> 1] << 16);
+  else return (float)__builtin_bit_cast(h2, r.w[i >> 1])[i & 1];
+}
+
+// The largest magnitude as bits, which order as magnitudes do, two 16-bit ones to a word.  Infinities and NaN come
+// above all that is finite: finite_amax() goes over the row again if there are any.
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+template <class E>
+__device__ __forceinline__ void max_bits(uint32_t& m, const Raw<E>& r) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if constexpr (sizeof(E) == 4) x[i] = __uint_as_float(r.w[i]);
-    else if constexpr (__is_same(E, __bf16)) x[i] = __uint_as_float(i & 1 ? r.w[i >> 1] & 0xffff0000u : r.w[i >> 1] << 16);
-    else x[i] = (float)__builtin_bit_cast(h2, r.w[i >> 1])[i & 1];
-    x[i] = __builtin_isfinite(x[i]) ? x[i] : kNan;
+  for (int i = 0; i < (int)(sizeof(E) * 2); ++i) {
+    if constexpr (sizeof(E) == 4) { const uint32_t v = r.w[i] & 0x7fffffffu; m = v > m ? v : m; }
+    else m = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, m), __builtin_bit_cast(us2, r.w[i] & 0x7fff7fffu)));
   }
 }
-__device__ __forceinline__ void numbers(const Code& r, float* x) {
-  unpack4(r.w[0], x);
-  unpack4(r.w[1], x + 4);
+template <class E>
+__device__ __forceinline__ float max_of_bits(uint32_t m) {
+  if constexpr (sizeof(E) == 4) return __uint_as_float(m);
+  const uint32_t v = (m & 0xffffu) > (m >> 16) ? m & 0xffffu : m >> 16;
+  if constexpr (__is_same(E, __bf16)) return __uint_as_float(v << 16);
+  else return (float)__builtin_bit_cast(h2, v)[0];
+}
+template <class E>
+__device__ __forceinline__ float finite_amax(const Raw<E>& r) {
+  float m = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] *= r.s;
+  for (int i = 0; i < 8; ++i) { const float v = fabsf(number(r, i)); m = v < kInf && v > m ? v : m; }
+  return m;
+}
+
+// Eight channels as codes under a power-of-two scale.  The conversions divide by it and round to nearest even; what is
+// not finite becomes NaN.
+typedef short s2 __attribute__((ext_vector_type(2)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float s) {
+  s2 r = {0, 0};
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, a, b, s, false);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c, d, s, true);
+  return __builtin_bit_cast(uint32_t, r);
+}
+template <class E>
+__device__ __forceinline__ u2 encode(const Raw<E>& x, float s) {
+  u2 w;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    s2 r = {0, 0};
+    if constexpr (__is_same(E, __bf16)) {
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(b2, x.w[2 * i]), s, false);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(b2, x.w[2 * i + 1]), s, true);
+      w[i] = __builtin_bit_cast(uint32_t, r);
+    } else if constexpr (__is_same(E, _Float16)) {
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(h2, x.w[2 * i]), s, false);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(h2, x.w[2 * i + 1]), s, true);
+      w[i] = __builtin_bit_cast(uint32_t, r);
+    } else {
+      w[i] = encode4(__uint_as_float(x.w[4 * i]), __uint_as_float(x.w[4 * i + 1]), __uint_as_float(x.w[4 * i + 2]), __uint_as_float(x.w[4 * i + 3]), s);
+    }
+  }
+  return w;
+}
+// codes under one scale as codes under another
+__device__ __forceinline__ u2 recode(const uint32_t* w, float from, float to) {
+  u2 r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const f2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i], from, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i], from, true);
+    r[i] = encode4(a[0], a[1], b[0], b[1], to);
+  }
+  return r;
+}
+__device__ __forceinline__ u2 encode(const Code& x, float s) { return recode(x.w, x.s, s); }
+__device__ __forceinline__ float amax_of(const Code& x) {   // (fmaxf passes over NaN)
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const f2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(x.w[i], x.s, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(x.w[i], x.s, true);
+    m = fmaxf(m, fmaxf(fmaxf(fabsf(a[0]), fabsf(a[1])), fmaxf(fabsf(b[0]), fabsf(b[1]))));
+  }
+  return m;
+}
+__device__ __forceinline__ h2 least(h2 a, h2 b) { return __builtin_elementwise_min(a, b); }
+__device__ __forceinline__ h2 most(h2 a, h2 b) { return __builtin_elementwise_max(a, b); }
+// over the four lanes l, l ^ 16, l ^ 32, l ^ 48
+template <class F>
+__device__ __forceinline__ h2 column_pair(h2 v, F f) {
+  uint32_t u = __builtin_bit_cast(uint32_t, v);
+  auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  u = __builtin_bit_cast(uint32_t, f(__builtin_bit_cast(h2, (uint32_t)r[0]), __builtin_bit_cast(h2, (uint32_t)r[1])));
+  r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return f(__builtin_bit_cast(h2, (uint32_t)r[0]), __builtin_bit_cast(h2, (uint32_t)r[1]));
 }
 
 // One wavefront packs K and V of one head of one page.  A lane holds 8 neighbouring channels of every RP-th token
@@ -239,148 +330,134 @@ __global__ __launch_bounds__(256) void fl_kv_pack(const PackArgs a) {
   const uint64_t end64 = (uint64_t)held + n - at;
   const uint32_t fill = end64 < T ? (uint32_t)end64 : T;       // slots that hold one afterwards
   uint8_t* rec = c.pages + (uint64_t)page * c.stride;
-  float* scale_at = reinterpret_cast<float*>(rec + c.scales) + 2 * h;
 
   const uint32_t CG = D >> 3, RP = 64 / CG, grp = (uint32_t)lane / CG, cg = (uint32_t)lane - grp * CG;
   const bool on = grp < RP;
   const uint32_t passes = (T + RP - 1) / RP;
-  float s_old[2] = {0.f, 0.f};
-  if (!EVICT && old) { s_old[0] = scale_at[0]; s_old[1] = scale_at[1]; }
 
+  // Rows (p0 + i) * RP + grp: new tokens (evict: all of them), 0 elsewhere.  sides: 1 K, 2 V, 3 both
   Row x[2][ROWS];
-  const auto load = [&](uint32_t p0) {   // rows (p0 + i) * RP + grp: new tokens (evict: all of them), 0 elsewhere
+  const auto load = [&](uint32_t p0, const int sides) {
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       const uint32_t r = (p0 + i) * RP + grp;
-      const bool in = on && r < fill && r >= old;
 #pragma unroll
-      for (int side = 0; side < 2; ++side) x[side][i] = Row{};
-      if (!in) continue;
+      for (int side = 0; side < 2; ++side)
+        if (sides >> side & 1) x[side][i] = Row{};
+      if (!on || r >= fill || r < old) continue;
       if constexpr (EVICT) {
         const int32_t pos = a.kept[(b * (uint64_t)c.H + h) * a.kept_stride + at + r];
         const uint32_t slot = (uint32_t)pos / a.from.T;
         const int32_t pg = pos >= 0 && slot < a.s.width ? a.s.table[b * a.s.table_stride + slot] : -1;
         if (pg < 0 || (uint32_t)pg >= a.from.n_pages) { report(a.s.status); continue; }
         const uint8_t* f = a.from.pages + (uint64_t)pg * a.from.stride;
-        const u2 s = *reinterpret_cast<const u2*>(f + a.from.scales + 8 * h);
         const uint64_t off = ((uint64_t)h * a.from.T + ((uint32_t)pos - slot * a.from.T)) * D + cg * 8;
+        const u2 s = *reinterpret_cast<const u2*>(f + a.from.scales + 8 * h);
 #pragma unroll
-        for (int side = 0; side < 2; ++side) {
-          const u2 w = *reinterpret_cast<const u2*>(f + side * a.from.side + off);
-          x[side][i] = Code{{w[0], w[1]}, __uint_as_float(s[side])};
-        }
+        for (int side = 0; side < 2; ++side)
+          if (sides >> side & 1) {
+            const u2 w = *reinterpret_cast<const u2*>(f + side * a.from.side + off);
+            x[side][i] = Code{{w[0], w[1]}, __uint_as_float(s[side])};
+          }
       } else {
 #pragma unroll
         for (int side = 0; side < 2; ++side)
-          load_raw<E>(x[side][i], reinterpret_cast<const E*>(a.src[side]) + (uint64_t)(first + at + r - held) * a.token_stride[side] + h * a.head_stride[side] + cg * 8, a.vec);
+          if (sides >> side & 1)
+            load_raw<E>(x[side][i], reinterpret_cast<const E*>(a.src[side]) + (uint64_t)(first + at + r - held) * a.token_stride[side] + h * a.head_stride[side] + cg * 8, a.vec);
       }
     }
   };
-
-  float amax[2] = {0.f, 0.f};
-  for (uint32_t p0 = 0; p0 < passes; p0 += ROWS) {
-    load(p0);
+  const auto pack = [&](const int side) {
+    float* scale_at = reinterpret_cast<float*>(rec + c.scales) + 2 * h + side;
+    const float s_old = !EVICT && old ? *scale_at : 0.f;
+    float amax = 0.f;
+    if constexpr (EVICT) {
+      for (uint32_t p0 = 0; p0 < passes; p0 += ROWS) {
+        if (!ONE) load(p0, 1 << side);
 #pragma unroll
-    for (int side = 0; side < 2; ++side)
-#pragma unroll
-      for (int i = 0; i < ROWS; ++i) {
-        float y[8];
-        numbers(x[side][i], y);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) amax[side] = fmaxf(amax[side], fabsf(y[e]));   // fmaxf passes over NaN
+        for (int i = 0; i < ROWS; ++i) amax = fmaxf(amax, amax_of(x[side][i]));
       }
-  }
+    } else {
+      uint32_t bits = 0;
+      for (uint32_t p0 = 0; p0 < passes; p0 += ROWS) {
+        if (!ONE) load(p0, 1 << side);
 #pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    amax[0] = fmaxf(amax[0], __shfl_xor(amax[0], o));
-    amax[1] = fmaxf(amax[1], __shfl_xor(amax[1], o));
-  }
-  float s[2];
+        for (int i = 0; i < ROWS; ++i) max_bits<E>(bits, x[side][i]);
+      }
+      amax = max_of_bits<E>(bits);
+      if (__ballot(!(amax < kInf))) {
+        amax = 0.f;
+        for (uint32_t p0 = 0; p0 < passes; p0 += ROWS) {
+          if (!ONE) load(p0, 1 << side);
 #pragma unroll
-  for (int side = 0; side < 2; ++side) s[side] = fmaxf(s_old[side], block_scale(amax[side]));
-
-  if constexpr (ONE) {   // what waits in registers for the scale is the rows as loaded, not their numbers
+          for (int i = 0; i < ROWS; ++i) amax = fmaxf(amax, finite_amax<E>(x[side][i]));
+        }
+      }
+    }
+    const float s = fmaxf(s_old, block_scale(wave_max_f32(amax)));
+    const bool grown = old && s != s_old;
+    h2 lo[4], hi[4];
 #pragma unroll
-    for (int side = 0; side < 2; ++side)
-#pragma unroll
-      for (int i = 0; i < ROWS; ++i)
-#pragma unroll
-        for (int e = 0; e < (int)(sizeof(x[0][0].w) / 4); ++e) asm("" : "+v"(x[side][i].w[e]));
-  }
-  float lo[8], hi[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) { lo[e] = kInf; hi[e] = -kInf; }
-  for (uint32_t p0 = 0; p0 < passes; p0 += ROWS) {
-    if (!ONE) load(p0);
-#pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      const float inv = inverse(s[side]), ratio = s_old[side] * inv;
-      const bool grown = old && s[side] != s_old[side];
-      uint8_t* codes = rec + side * c.side + (uint64_t)h * T * D;
+    for (int e = 0; e < 4; ++e) { lo[e] = h2{(_Float16)kInf, (_Float16)kInf}; hi[e] = -lo[e]; }
+    uint8_t* codes = rec + side * c.side + (uint64_t)h * T * D;
+    for (uint32_t p0 = 0; p0 < passes; p0 += ROWS) {
+      if (!ONE) load(p0, 1 << side);
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
         const uint32_t r = (p0 + i) * RP + grp;
         if (!on || r >= T) continue;
-        u2* row = reinterpret_cast<u2*>(codes + (uint64_t)r * D + cg * 8);
-        float y[8];
+        u2* row = reinterpret_cast<u2*>(codes + r * D + cg * 8);
+        u2 w;
         if (r < old) {
           if (side == 1 && !grown) continue;
-          const u2 w = *row;
-          unpack4(w[0], y);
-          unpack4(w[1], y + 4);
-          if (grown) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] *= ratio;
-          }
+          w = *row;
+          if (grown) { const uint32_t t[2] = {w[0], w[1]}; w = recode(t, s_old, s); }
         } else {
-          numbers(x[side][i], y);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] *= inv;
+          w = encode(x[side][i], s);
         }
+        if (r < old ? grown : (r < fill || !old)) *row = w;   // slots behind the tokens of a page that this call opens are zero
         if (side == 0 && r < fill) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) { lo[e] = fminf(lo[e], y[e]); hi[e] = fmaxf(hi[e], y[e]); }
-        }
-        if (r < old ? grown : (r < fill || !old)) {   // slots behind the tokens of a page that this call opens are zero
-          u2 w;
-          w[0] = pack4(y);
-          w[1] = pack4(y + 4);
-          *row = w;
+          for (int e = 0; e < 4; ++e) {
+            const h2 v = e & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[e >> 1], 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[e >> 1], 1.f, false);
+            lo[e] = least(lo[e], v);
+            hi[e] = most(hi[e], v);
+          }
         }
       }
     }
-  }
-  if (lane == 0) *reinterpret_cast<u2*>(scale_at) = u2{__float_as_uint(s[0]), __float_as_uint(s[1])};
+    if (lane == 0) *scale_at = s;
+    if (side == 1) return;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float l = lo[e], u = hi[e];
-    if ((CG & (CG - 1)) == 0) {
-      for (uint32_t o = CG; o < 64; o <<= 1) {
-        l = fminf(l, __shfl_xor(l, (int)o));
-        u = fmaxf(u, __shfl_xor(u, (int)o));
-      }
-    } else {
-      for (uint32_t k = 1; k < RP; ++k) {
-        l = fminf(l, __shfl(lo[e], (int)(cg + k * CG)));
-        u = fmaxf(u, __shfl(hi[e], (int)(cg + k * CG)));
+    for (int e = 0; e < 4; ++e) {
+      if (CG == 16) {
+        lo[e] = column_pair(lo[e], least);
+        hi[e] = column_pair(hi[e], most);
+      } else {
+        const uint32_t l0 = __builtin_bit_cast(uint32_t, lo[e]), u0 = __builtin_bit_cast(uint32_t, hi[e]);
+        for (uint32_t k = 1; k < RP; ++k) {
+          lo[e] = least(lo[e], __builtin_bit_cast(h2, __shfl((int)l0, (int)(cg + k * CG))));
+          hi[e] = most(hi[e], __builtin_bit_cast(h2, __shfl((int)u0, (int)(cg + k * CG))));
+        }
       }
     }
-    lo[e] = l;
-    hi[e] = u;
-  }
-  if (lane < (int)CG) {   // rounding is monotonic: the smallest value's code is the smallest code
-    u2 wl = {0, 0}, wh = {0, 0};
+    if (lane < (int)CG) {
+      u2 wl = {0, 0}, wh = {0, 0};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const bool any = lo[e] <= hi[e];
-      const uint32_t two = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(any ? lo[e] : 0.f, any ? hi[e] : 0.f, 0, false);
-      const int li = (int)floorf(__builtin_amdgcn_cvt_f32_fp8((int)two, 0) * 0.25f), ui = (int)ceilf(__builtin_amdgcn_cvt_f32_fp8((int)two, 1) * 0.25f);
-      wl[e >> 2] |= (uint32_t)(li & 0xff) << (8 * (e & 3));
-      wh[e >> 2] |= (uint32_t)(ui & 0xff) << (8 * (e & 3));
+      for (int e = 0; e < 8; ++e) {
+        const float l = (float)lo[e >> 1][e & 1], u = (float)hi[e >> 1][e & 1];
+        const int li = l <= u ? (int)floorf(l * 0.25f) : 0, ui = l <= u ? (int)ceilf(u * 0.25f) : 0;   // (not so: no finite one)
+        wl[e >> 2] |= (uint32_t)(li & 0xff) << (8 * (e & 3));
+        wh[e >> 2] |= (uint32_t)(ui & 0xff) << (8 * (e & 3));
+      }
+      *reinterpret_cast<u2*>(rec + c.low + (uint64_t)h * D + cg * 8) = wl;
+      *reinterpret_cast<u2*>(rec + c.high + (uint64_t)h * D + cg * 8) = wh;
     }
-    *reinterpret_cast<u2*>(rec + c.low + (uint64_t)h * D + cg * 8) = wl;
-    *reinterpret_cast<u2*>(rec + c.high + (uint64_t)h * D + cg * 8) = wh;
-  }
+  };
+
+  if (ONE) load(0, 3);
+  pack(0);
+  pack(1);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -430,20 +507,6 @@ __device__ __forceinline__ typename Frag<E>::v8 codes8(uint32_t w0, uint32_t w1)
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// the four lanes that share a column of a 16 x 16 result: l, l ^ 16, l ^ 32, l ^ 48
-__device__ __forceinline__ float column_max(float v) {
-  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float column_sum(float v) {
-  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
 
 template <class E>
 __device__ __forceinline__ typename Frag<E>::v8 load_q8(const E* p, bool ok, bool vec) {
@@ -1027,7 +1090,7 @@ struct SelectArgs {
   Seqs s;
   const void* q;
   uint64_t q_token, q_head;
-  uint32_t G, causal, q_vec, first, last, count, parts;
+  uint32_t G, causal, q_vec, first, last, count, parts, heads_wg;
   float* scores;              // [n_tokens][H][width]
   int32_t* out;               // [n_tokens][H][count]
 };
@@ -1047,7 +1110,9 @@ template <class E, int DP>
 __global__ __launch_bounds__(256) void fl_kv_score(const SelectArgs a) {
   constexpr int KK = DP / 64;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-  const uint32_t wave = uniform(threadIdx.x >> 6), H = a.c.H, G = a.G, T = a.c.T, D = a.c.D, h = blockIdx.x % H, part = blockIdx.x / H;
+  const uint32_t wave = uniform(threadIdx.x >> 6), H = a.c.H, G = a.G, T = a.c.T, D = a.c.D, HW = a.heads_wg, groups = (H + HW - 1) / HW;
+  const uint32_t h = blockIdx.x % groups * HW + wave % HW, part = blockIdx.x / groups;
+  if (h >= H) return;
   uint32_t b, i, first, n;
   const auto items = [&](uint32_t q) { uint32_t f, m; seq_tokens(a.s, q, f, m); return m; };
   if (!find_seq(a.s.n_seqs, blockIdx.y, items, b, i)) return;
@@ -1055,8 +1120,8 @@ __global__ __launch_bounds__(256) void fl_kv_score(const SelectArgs a) {
   i = uniform(i);
   uniform_tokens(a.s, b, first, n);
   const uint32_t lim = token_limit(a, uniform_len(a.s, T, b), n, i), pages = (lim + T - 1) / T;
-  const uint32_t step = a.parts * 4 * 32;                  // 32 pages to a wavefront at a time
-  uint32_t p0 = (part * 4 + wave) * 32;
+  const uint32_t subs = 4 / HW, step = a.parts * subs * 32;   // 32 pages to a wavefront at a time
+  uint32_t p0 = (part * subs + wave / HW) * 32;
   if (p0 >= pages) return;
   const uint64_t tok = first + i;
   const int32_t* table = a.s.table + b * a.s.table_stride;
@@ -1189,91 +1254,172 @@ __device__ __forceinline__ uint32_t order_key(float f) {
 }
 
 struct Pick { uint32_t key, need; };
-constexpr int kHeld = 16;   // keys a thread holds: 16384 in a workgroup of 1024
+constexpr int kHeld = 16;      // keys a thread holds
+constexpr uint32_t kFew = 256;
 
-struct PickShared { uint32_t hist[2048], word[2], sums[2][kHeld * 16], wave[16]; };
+struct PickShared { uint32_t hist[2048], word[4], sums[2][256], wave[2][16]; alignas(16) uint32_t few[kFew + 16]; };
 
-// The k-th largest of n keys (k < n), by 11, 11 and 10 of its bits from the top, and how many of its equals belong to
-// the k.  The first digit holds the exponent and two bits of the mantissa, so that numbers of like size do not all
-// count into a few bins.  One workgroup of 1024; ONE: the keys stay in registers.
-template <bool ONE, class Load>
+// all lanes get the largest of the 64
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+  uint32_t t = dpp_u32<0xb1>(v);
+  v = t > v ? t : v;
+  t = dpp_u32<0x4e>(v);
+  v = t > v ? t : v;
+  t = dpp_u32<0x141>(v);
+  v = t > v ? t : v;
+  t = dpp_u32<0x140>(v);
+  v = t > v ? t : v;
+  auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  v = r[0] > r[1] ? r[0] : r[1];
+  r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return r[0] > r[1] ? r[0] : r[1];
+}
+
+// The k-th largest of n keys (k < n), and how many of its equals belong to the k.  2048 equal bins over the range that
+// the keys span, so that keys of like size do not all count into a few; the bin that holds the k-th is taken for the
+// next range until few keys are left in it (or one value), and those are ranked against each other.  Keys of all ones
+// (what has to be among the k) are counted apart and do not stretch the range.  NT threads; ONE: the keys stay in
+// registers.
+template <int NT, bool ONE, class Load>
 __device__ Pick kth_largest(uint32_t n, uint32_t k, uint32_t* keys, Load load, PickShared& sh) {
-  uint32_t prefix = 0, mask = 0;
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-#pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const uint32_t shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, ones = pass == 2 ? 1023 : 2047;
-    sh.hist[tid] = 0;
-    sh.hist[1024 + tid] = 0;
+  uint32_t lo = 0xffffffffu, hi = 0, forced = 0;
+  for (uint32_t base = 0; base < n; base += NT * kHeld) {
+    if (!ONE) load(base);
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      if (ONE && j * (uint32_t)NT >= n) break;
+      const bool in = base + j * NT + tid < n, all = in && keys[j] == 0xffffffffu;
+      forced += all ? 1 : 0;
+      if (in && !all) { lo = keys[j] < lo ? keys[j] : lo; hi = keys[j] > hi ? keys[j] : hi; }
+    }
+  }
+  lo = ~wave_max_u32(~lo);
+  hi = wave_max_u32(hi);
+  forced = wave_incl_sum_u32(forced, (int)lane);
+  if (lane == 63) { sh.wave[0][wave] = lo; sh.wave[1][wave] = hi; sh.hist[wave] = forced; }
+  __syncthreads();
+  {
+    const uint32_t w = lane & (NT / 64 - 1);
+    lo = ~wave_max_u32(~sh.wave[0][w]);
+    hi = wave_max_u32(sh.wave[1][w]);
+    forced = bcast_lane_u32(wave_incl_sum_u32(lane < NT / 64 ? sh.hist[w] : 0, (int)lane), 63);
+  }
+  if (forced >= k) return {0xffffffffu, k};
+  k -= forced;
+  for (;;) {                     // keys in [lo, hi], the k-th largest of them wanted; the range shrinks by 2048 each time
+    if (lo == hi) return {lo, k};
+    const int bits = 32 - __builtin_clz(hi - lo), shift = bits > 11 ? bits - 11 : 0;
     __syncthreads();
-    for (uint32_t base = 0; base < n; base += 1024 * kHeld) {
+    for (uint32_t i = tid; i < 2048; i += NT) sh.hist[i] = 0;
+    if (tid == 0) sh.word[2] = 0;
+    __syncthreads();
+    for (uint32_t base = 0; base < n; base += NT * kHeld) {
       if (!ONE) load(base);
 #pragma unroll
-      for (int j = 0; j < kHeld; ++j)
-        if (base + j * 1024 + tid < n && (keys[j] & mask) == prefix) atomicAdd(&sh.hist[(keys[j] >> shift) & ones], 1u);
+      for (int j = 0; j < kHeld; ++j) {
+        if (ONE && j * (uint32_t)NT >= n) break;
+        if (base + j * NT + tid < n && keys[j] >= lo && keys[j] <= hi) atomicAdd(&sh.hist[(keys[j] - lo) >> shift], 1u);
+      }
     }
     __syncthreads();
-    // thread t owns bins 2047 - 2 t and 2046 - 2 t: a scan from the top
-    const uint32_t c0 = sh.hist[2047 - 2 * tid], c1 = sh.hist[2046 - 2 * tid], incl = wave_incl_sum_u32(c0 + c1, (int)lane);
-    if (lane == 63) sh.wave[wave] = incl;
+    // thread t owns the OWN bins from 2047 - OWN t downwards: a scan from the top
+    constexpr int OWN = 2048 / NT;
+    uint32_t cnt[OWN], own = 0;
+#pragma unroll
+    for (int e = 0; e < OWN; ++e) { cnt[e] = sh.hist[2047 - OWN * tid - e]; own += cnt[e]; }
+    const uint32_t incl = wave_incl_sum_u32(own, (int)lane);
+    if (lane == 63) sh.wave[0][wave] = incl;
     __syncthreads();
-    uint32_t before = incl - c0 - c1;
-    for (uint32_t w = 0; w < wave; ++w) before += sh.wave[w];
-    if (before < k && k <= before + c0) { sh.word[0] = 2047 - 2 * tid; sh.word[1] = k - before; }
-    else if (before + c0 < k && k <= before + c0 + c1) { sh.word[0] = 2046 - 2 * tid; sh.word[1] = k - before - c0; }
+    const uint32_t waves = wave_incl_sum_u32(lane < NT / 64 ? sh.wave[0][lane] : 0, (int)lane);
+    uint32_t before = (wave ? bcast_lane_u32(waves, (int)uniform(wave) - 1) : 0) + incl - own;
+#pragma unroll
+    for (int e = 0; e < OWN; ++e) {
+      if (before < k && k <= before + cnt[e]) { sh.word[0] = 2047 - OWN * tid - e; sh.word[1] = k - before; sh.word[3] = cnt[e]; }
+      before += cnt[e];
+    }
     __syncthreads();
-    prefix |= sh.word[0] << shift;
-    mask |= ones << shift;
+    const uint32_t left = sh.word[3];
+    lo += sh.word[0] << shift;
+    hi = shift ? lo + ((1u << shift) - 1) : lo;
     k = sh.word[1];
-    __syncthreads();
+    if (lo == hi) return {lo, k};
+    if (left <= kFew) {
+      for (uint32_t base = 0; base < n; base += NT * kHeld) {
+        if (!ONE) load(base);
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+          if (ONE && j * (uint32_t)NT >= n) break;
+          if (base + j * NT + tid < n && keys[j] >= lo && keys[j] <= hi) sh.few[atomicAdd(&sh.word[2], 1u)] = keys[j];
+        }
+      }
+      __syncthreads();
+      if (tid < 16) sh.few[left + tid] = 0;   // (nothing is below it; equals are looked for among the `left` only)
+      __syncthreads();
+      if (tid < left) {
+        const uint32_t mine = sh.few[tid];
+        uint32_t above = 0, equal = 0;
+        for (uint32_t i = 0; i < left; i += 16) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(&sh.few[i + e]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) { above += v[u] > mine ? 1 : 0; equal += v[u] == mine && i + e + u < left ? 1 : 0; }
+          }
+        }
+        if (above < k && k <= above + equal) { sh.word[0] = mine; sh.word[1] = k - above; }   // all equals write the same
+      }
+      __syncthreads();
+      return {sh.word[0], sh.word[1]};
+    }
   }
-  return {prefix, k};
 }
 
 // Indices of the keys above the pick and of the first `need` equal to it, in ascending order: put(place, index, j).
-template <bool ONE, class Load, class Put>
+template <int NT, bool ONE, class Load, class Put>
 __device__ void put_picked(uint32_t n, Pick pick, const uint32_t* keys, Load load, Put put, PickShared& sh) {
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   uint32_t above = 0, equal = 0;   // in all rounds so far
-  for (uint32_t base = 0; base < n; base += 1024 * kHeld) {
+  for (uint32_t base = 0; base < n; base += NT * kHeld) {
     if (!ONE) load(base);
     uint32_t before[kHeld];        // of this wavefront's 64 keys: those above in the low half, those equal in the high half
     const uint64_t below = (1ull << lane) - 1;
+    __syncthreads();
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) {
-      const bool in = base + j * 1024 + tid < n;
+      const bool in = base + j * NT + tid < n;
       const uint64_t bg = __ballot(in && keys[j] > pick.key), be = __ballot(in && keys[j] == pick.key);
       before[j] = (uint32_t)__popcll(bg & below) | (uint32_t)__popcll(be & below) << 16;
-      if (lane == 0) { sh.sums[0][j * 16 + wave] = (uint32_t)__popcll(bg); sh.sums[1][j * 16 + wave] = (uint32_t)__popcll(be); }
+      if (lane == 0) { sh.sums[0][j * (NT / 64) + wave] = (uint32_t)__popcll(bg); sh.sums[1][j * (NT / 64) + wave] = (uint32_t)__popcll(be); }
     }
     __syncthreads();
-    if (wave < 2) {                // 256 counts in the order of the keys, four to a lane: exclusive sums in place
-      uint32_t c[4], sum = 0;
+    if (wave < 2) {                // the counts in the order of the keys, PER to a lane: exclusive sums in place
+      constexpr int PER = kHeld * (NT / 64) / 64;
+      uint32_t c[PER], sum = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { c[e] = sh.sums[wave][4 * lane + e]; sum += c[e]; }
+      for (int e = 0; e < PER; ++e) { c[e] = sh.sums[wave][PER * lane + e]; sum += c[e]; }
       const uint32_t incl = wave_incl_sum_u32(sum, (int)lane);
       uint32_t run = incl - sum;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { sh.sums[wave][4 * lane + e] = run; run += c[e]; }
+      for (int e = 0; e < PER; ++e) { sh.sums[wave][PER * lane + e] = run; run += c[e]; }
       if (lane == 63) sh.word[wave] = incl;
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) {
-      const uint32_t i = base + j * 1024 + tid;
+      const uint32_t i = base + j * NT + tid;
       if (i < n && keys[j] >= pick.key) {
-        const uint32_t g0 = above + sh.sums[0][j * 16 + wave] + (before[j] & 0xffffu), e0 = equal + sh.sums[1][j * 16 + wave] + (before[j] >> 16);
+        const uint32_t g0 = above + sh.sums[0][j * (NT / 64) + wave] + (before[j] & 0xffffu), e0 = equal + sh.sums[1][j * (NT / 64) + wave] + (before[j] >> 16);
         if (keys[j] > pick.key || e0 < pick.need) put(g0 + (e0 < pick.need ? e0 : pick.need), i);
       }
     }
     above += sh.word[0];
     equal += sh.word[1];
-    __syncthreads();
   }
 }
 
-template <bool ONE>
-__global__ __launch_bounds__(1024) void fl_kv_pick_pages(const SelectArgs a) {
+template <int NT, bool ONE>
+__global__ __launch_bounds__(NT) void fl_kv_pick_pages(const SelectArgs a) {
   __shared__ PickShared sh;
   const uint32_t h = blockIdx.x % a.c.H, t = blockIdx.x / a.c.H;
   uint32_t b, i, first, n;
@@ -1285,22 +1431,22 @@ __global__ __launch_bounds__(1024) void fl_kv_pick_pages(const SelectArgs a) {
   const uint64_t row = (uint64_t)(first + i) * a.c.H + h;
   const float* score = a.scores + row * a.s.width;
   int32_t* out = a.out + row * a.count;
-  for (uint32_t k = (pages < a.count ? pages : a.count) + threadIdx.x; k < a.count; k += 1024) out[k] = -1;
+  for (uint32_t k = (pages < a.count ? pages : a.count) + threadIdx.x; k < a.count; k += NT) out[k] = -1;
   if (pages <= a.count) {
-    for (uint32_t k = threadIdx.x; k < pages; k += 1024) out[k] = (int32_t)k;
+    for (uint32_t k = threadIdx.x; k < pages; k += NT) out[k] = (int32_t)k;
     return;
   }
   uint32_t keys[kHeld];
   const auto load = [&](uint32_t base) {
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) {
-      const uint32_t p = base + j * 1024 + threadIdx.x;
+      const uint32_t p = base + j * NT + threadIdx.x;
       keys[j] = p >= pages ? 0 : p < a.first || p + a.last >= pages ? 0xffffffffu : order_key(score[p]);
     }
   };
   if (ONE) load(0);
-  const Pick pick = kth_largest<ONE>(pages, a.count, keys, load, sh);
-  put_picked<ONE>(pages, pick, keys, load, [&](uint32_t at, uint32_t p) { out[at] = (int32_t)p; }, sh);
+  const Pick pick = kth_largest<NT, ONE>(pages, a.count, keys, load, sh);
+  put_picked<NT, ONE>(pages, pick, keys, load, [&](uint32_t at, uint32_t p) { out[at] = (int32_t)p; }, sh);
 }
 
 struct KeepArgs {
@@ -1313,8 +1459,8 @@ struct KeepArgs {
   int32_t* new_lens;
 };
 
-template <bool ONE>
-__global__ __launch_bounds__(1024) void fl_kv_keep(const KeepArgs a) {
+template <int NT, bool ONE>
+__global__ __launch_bounds__(NT) void fl_kv_keep(const KeepArgs a) {
   __shared__ PickShared sh;
   const uint32_t h = blockIdx.x % a.H, b = blockIdx.x / a.H;
   uint32_t len = uniform_len(a.s, a.T, b);
@@ -1324,23 +1470,23 @@ __global__ __launch_bounds__(1024) void fl_kv_keep(const KeepArgs a) {
   int32_t* kept = a.kept + ((uint64_t)b * a.H + h) * a.kept_stride;
   const uint32_t m = len < a.budget ? len : a.budget;
   if (h == 0 && threadIdx.x == 0) a.new_lens[b] = (int32_t)m;
-  for (uint32_t k = m + threadIdx.x; k < a.budget; k += 1024) kept[k] = -1;
-  for (uint32_t k = m + threadIdx.x; k < a.nw_width; k += 1024) nw[k] = 0.f;
+  for (uint32_t k = m + threadIdx.x; k < a.budget; k += NT) kept[k] = -1;
+  for (uint32_t k = m + threadIdx.x; k < a.nw_width; k += NT) nw[k] = 0.f;
   if (len <= a.budget) {
-    for (uint32_t k = threadIdx.x; k < len; k += 1024) { kept[k] = (int32_t)k; nw[k] = w[k]; }
+    for (uint32_t k = threadIdx.x; k < len; k += NT) { kept[k] = (int32_t)k; nw[k] = w[k]; }
     return;
   }
   uint32_t keys[kHeld];
   const auto load = [&](uint32_t base) {
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) {
-      const uint32_t p = base + j * 1024 + threadIdx.x;
+      const uint32_t p = base + j * NT + threadIdx.x;
       keys[j] = p >= len ? 0 : p < a.first || p + a.recent >= len ? 0xffffffffu : order_key(w[p]);
     }
   };
   if (ONE) load(0);
-  const Pick pick = kth_largest<ONE>(len, m, keys, load, sh);
-  put_picked<ONE>(len, pick, keys, load, [&](uint32_t at, uint32_t p) { kept[at] = (int32_t)p; nw[at] = w[p]; }, sh);
+  const Pick pick = kth_largest<NT, ONE>(len, m, keys, load, sh);
+  put_picked<NT, ONE>(len, pick, keys, load, [&](uint32_t at, uint32_t p) { kept[at] = (int32_t)p; nw[at] = w[p]; }, sh);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1624,17 +1770,21 @@ int flh_kv_select(const flh_kv_select_params* p, void* stream) {
   a.out = p->d_out;
   fl_prof().kid = 10;
   const hipStream_t st = (hipStream_t)stream;
-  // workgroups to a row of scores: enough for 8 a compute unit between all rows, each with 128 pages at least
-  const uint64_t rows = (uint64_t)a.s.n_tokens * a.c.H;
-  const uint32_t want = (uint32_t)((2048 + rows - 1) / rows), most = (a.s.width + 127) / 128;
+  // The wavefronts of a workgroup take up to four heads of the same pages, whose scales lie in one line (a head to a
+  // workgroup fetched that line once for each: 41 -> TBD us at 65536 pages of 8 heads).  As many workgroups as stay
+  // resident, or 128 pages each.
+  a.heads_wg = a.c.H >= 4 ? 4 : a.c.H >= 2 ? 2 : 1;
+  const uint64_t rows = (uint64_t)a.s.n_tokens * ((a.c.H + a.heads_wg - 1) / a.heads_wg);
+  const uint32_t per = 32 * (4 / a.heads_wg), want = (uint32_t)((1024 + rows - 1) / rows), most = (a.s.width + per - 1) / per;
   a.parts = want < most ? want : most;
-  const dim3 grid(a.parts * a.c.H, a.s.n_tokens);
+  const dim3 grid(a.parts * ((a.c.H + a.heads_wg - 1) / a.heads_wg), a.s.n_tokens);
   const bool bf = p->type == FLH_KV_BF16;
   if (a.c.D <= 64) { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 64>), grid, dim3(256), 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 64>), grid, dim3(256), 0, st, a); }
   else if (a.c.D <= 128) { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 128>), grid, dim3(256), 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 128>), grid, dim3(256), 0, st, a); }
   else { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 256>), grid, dim3(256), 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 256>), grid, dim3(256), 0, st, a); }
-  if (a.s.width <= 1024 * kHeld) FL_LAUNCH((fl_kv_pick_pages<true>), dim3(a.s.n_tokens * a.c.H), dim3(1024), 0, st, a);
-  else FL_LAUNCH((fl_kv_pick_pages<false>), dim3(a.s.n_tokens * a.c.H), dim3(1024), 0, st, a);
+  if (a.s.width <= 256 * kHeld) FL_LAUNCH((fl_kv_pick_pages<256, true>), dim3(a.s.n_tokens * a.c.H), dim3(256), 0, st, a);
+  else if (a.s.width <= 1024 * kHeld) FL_LAUNCH((fl_kv_pick_pages<1024, true>), dim3(a.s.n_tokens * a.c.H), dim3(1024), 0, st, a);
+  else FL_LAUNCH((fl_kv_pick_pages<1024, false>), dim3(a.s.n_tokens * a.c.H), dim3(1024), 0, st, a);
   return finish("flh_kv_select");
 }
 
@@ -1683,8 +1833,9 @@ int flh_kv_evict(const flh_kv_evict_params* p, void* stream) {
   a.per_seq = per;
   fl_prof().kid = 11;
   const hipStream_t st = (hipStream_t)stream;
-  if (k.w_width <= 1024 * kHeld) FL_LAUNCH((fl_kv_keep<true>), dim3(a.s.n_seqs * a.c.H), dim3(1024), 0, st, k);
-  else FL_LAUNCH((fl_kv_keep<false>), dim3(a.s.n_seqs * a.c.H), dim3(1024), 0, st, k);
+  if (k.w_width <= 256 * kHeld) FL_LAUNCH((fl_kv_keep<256, true>), dim3(a.s.n_seqs * a.c.H), dim3(256), 0, st, k);
+  else if (k.w_width <= 1024 * kHeld) FL_LAUNCH((fl_kv_keep<1024, true>), dim3(a.s.n_seqs * a.c.H), dim3(1024), 0, st, k);
+  else FL_LAUNCH((fl_kv_keep<1024, false>), dim3(a.s.n_seqs * a.c.H), dim3(1024), 0, st, k);
   launch_pack<__bf16, true>(a, per * a.s.n_seqs, st);
   return finish("flh_kv_evict");
 }
