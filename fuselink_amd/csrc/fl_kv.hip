@@ -293,6 +293,7 @@ __device__ __forceinline__ h2 column_pair(h2 v, F f) {
 // are codes of other records under their own scales.
 template <class E, bool EVICT, int ROWS, bool ONE>
 __global__ __launch_bounds__(256) void fl_kv_pack(const PackArgs a) {
+  warm_kernel_args(a);
   typedef typename std::conditional<EVICT, Code, Raw<E>>::type Row;
   const int lane = threadIdx.x & 63;
   const Cache& c = a.c;
@@ -542,6 +543,7 @@ __device__ __forceinline__ typename Frag<E>::v8 flipped(typename Frag<E>::v8 x, 
 // the accumulators are rarely rescaled; they, sums and references are 32 bits wide.
 template <class E, int DP, int NQ, int KVW, bool SEL>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) void fl_kv_attend(const AttendArgs a) {
+  warm_kernel_args(a);
   constexpr int KK = DP / 32, KW = DP / 16, VJ = DP / 16, VW = DP / 64;
   constexpr uint32_t TR = 16 * NQ * (4 / KVW);
   typedef typename Frag<E>::v8 v8;
@@ -930,6 +932,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) 
 // reads 64 / DL splits at a time, none of the loads waiting for another.
 template <class E, bool SEL>
 __global__ __launch_bounds__(256) void fl_kv_join(const AttendArgs a, uint32_t TR) {
+  warm_kernel_args(a);
   const uint32_t H = a.c.H, G = a.G, D = a.c.D, lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const uint32_t h = blockIdx.x % H, x = blockIdx.x / H;
   uint32_t b, tile, first, n, r0, rows, tok0 = 0;
@@ -993,6 +996,7 @@ __global__ __launch_bounds__(256) void fl_kv_join(const AttendArgs a, uint32_t T
 // its key-value head, on top of w_in.  One wavefront owns 64 keys and walks over all rows, so the sums need no atomics.
 template <class E, int DP>
 __global__ __launch_bounds__(256) void fl_kv_weights(const AttendArgs a) {
+  warm_kernel_args(a);
   constexpr int KK = DP / 32, KW = DP / 16;
   typedef typename Frag<E>::v8 v8;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
@@ -1108,6 +1112,7 @@ __device__ __forceinline__ uint32_t token_limit(const SelectArgs& a, uint32_t le
 // bytes of the record as they lie.
 template <class E, int DP>
 __global__ __launch_bounds__(256) void fl_kv_score(const SelectArgs a) {
+  warm_kernel_args(a);
   constexpr int KK = DP / 64;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const uint32_t wave = uniform(threadIdx.x >> 6), H = a.c.H, G = a.G, T = a.c.T, D = a.c.D, HW = a.heads_wg, groups = (H + HW - 1) / HW;
@@ -1254,10 +1259,12 @@ __device__ __forceinline__ uint32_t order_key(float f) {
 }
 
 struct Pick { uint32_t key, need; };
-constexpr int kHeld = 16;      // keys a thread holds
-constexpr uint32_t kFew = 256;
+constexpr uint32_t kHeld = 16;     // keys in shared memory for each thread of a workgroup; longer rows are read again
 
-struct PickShared { uint32_t hist[2048], word[4], sums[2][256], wave[2][16]; alignas(16) uint32_t few[kFew + 16]; };
+template <int NT, bool ONE>
+struct PickShared {
+  uint32_t keys[ONE ? NT * kHeld : 1], hist[2048], word[4], wave[3][NT / 64];
+};
 
 // all lanes get the largest of the 64
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
@@ -1277,50 +1284,52 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 
 // The k-th largest of n keys (k < n), and how many of its equals belong to the k.  2048 equal bins over the range that
 // the keys span, so that keys of like size do not all count into a few; the bin that holds the k-th is taken for the
-// next range until few keys are left in it (or one value), and those are ranked against each other.  Keys of all ones
-// (what has to be among the k) are counted apart and do not stretch the range.  NT threads; ONE: the keys stay in
-// registers.
-template <int NT, bool ONE, class Load>
-__device__ Pick kth_largest(uint32_t n, uint32_t k, uint32_t* keys, Load load, PickShared& sh) {
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// next range until all of it belongs to the k (then the key returned is the one below it) or it is one value.  Keys of all
+// ones (what has to be among the k) are counted apart and do not stretch the range.  The loops are short and rolled:
+// with a few rows to a call, fetching straight-line code for keys in registers took longer than all else here.
+template <int NT, bool ONE, class Key>
+__device__ Pick kth_largest(uint32_t n, uint32_t k, Key key, PickShared<NT, ONE>& sh) {
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   uint32_t lo = 0xffffffffu, hi = 0, forced = 0;
-  for (uint32_t base = 0; base < n; base += NT * kHeld) {
-    if (!ONE) load(base);
+  for (uint32_t base = tid; base < n; base += 8 * NT) {   // eight loads at a time, none behind a branch
+    uint32_t u[8];
 #pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-      if (ONE && j * (uint32_t)NT >= n) break;
-      const bool in = base + j * NT + tid < n, all = in && keys[j] == 0xffffffffu;
-      forced += all ? 1 : 0;
-      if (in && !all) { lo = keys[j] < lo ? keys[j] : lo; hi = keys[j] > hi ? keys[j] : hi; }
+    for (int e = 0; e < 8; ++e) u[e] = key(base + e * NT < n ? base + e * NT : n - 1);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const bool in = base + e * NT < n, all = u[e] == 0xffffffffu;
+      if (ONE && in) sh.keys[base + e * NT] = u[e];
+      forced += in && all ? 1 : 0;
+      lo = !all && u[e] < lo ? u[e] : lo;
+      hi = !all && u[e] > hi ? u[e] : hi;
     }
   }
+  const auto held = [&](uint32_t i) { return ONE ? sh.keys[i] : key(i); };
   lo = ~wave_max_u32(~lo);
   hi = wave_max_u32(hi);
   forced = wave_incl_sum_u32(forced, (int)lane);
-  if (lane == 63) { sh.wave[0][wave] = lo; sh.wave[1][wave] = hi; sh.hist[wave] = forced; }
+  if (lane == 63) { sh.wave[0][wave] = lo; sh.wave[1][wave] = hi; sh.wave[2][wave] = forced; }
   __syncthreads();
   {
     const uint32_t w = lane & (NT / 64 - 1);
     lo = ~wave_max_u32(~sh.wave[0][w]);
     hi = wave_max_u32(sh.wave[1][w]);
-    forced = bcast_lane_u32(wave_incl_sum_u32(lane < NT / 64 ? sh.hist[w] : 0, (int)lane), 63);
+    forced = bcast_lane_u32(wave_incl_sum_u32(lane < NT / 64 ? sh.wave[2][w] : 0, (int)lane), 63);
   }
   if (forced >= k) return {0xffffffffu, k};
   k -= forced;
   for (;;) {                     // keys in [lo, hi], the k-th largest of them wanted; the range shrinks by 2048 each time
     if (lo == hi) return {lo, k};
     const int bits = 32 - __builtin_clz(hi - lo), shift = bits > 11 ? bits - 11 : 0;
-    __syncthreads();
     for (uint32_t i = tid; i < 2048; i += NT) sh.hist[i] = 0;
-    if (tid == 0) sh.word[2] = 0;
     __syncthreads();
-    for (uint32_t base = 0; base < n; base += NT * kHeld) {
-      if (!ONE) load(base);
+    for (uint32_t base = tid; base < n; base += 8 * NT) {
+      uint32_t u[8];
 #pragma unroll
-      for (int j = 0; j < kHeld; ++j) {
-        if (ONE && j * (uint32_t)NT >= n) break;
-        if (base + j * NT + tid < n && keys[j] >= lo && keys[j] <= hi) atomicAdd(&sh.hist[(keys[j] - lo) >> shift], 1u);
-      }
+      for (int e = 0; e < 8; ++e) u[e] = held(base + e * NT < n ? base + e * NT : n - 1);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (base + e * NT < n && u[e] >= lo && u[e] <= hi) atomicAdd(&sh.hist[(u[e] - lo) >> shift], 1u);
     }
     __syncthreads();
     // thread t owns the OWN bins from 2047 - OWN t downwards: a scan from the top
@@ -1332,7 +1341,7 @@ __device__ Pick kth_largest(uint32_t n, uint32_t k, uint32_t* keys, Load load, P
     if (lane == 63) sh.wave[0][wave] = incl;
     __syncthreads();
     const uint32_t waves = wave_incl_sum_u32(lane < NT / 64 ? sh.wave[0][lane] : 0, (int)lane);
-    uint32_t before = (wave ? bcast_lane_u32(waves, (int)uniform(wave) - 1) : 0) + incl - own;
+    uint32_t before = (wave ? bcast_lane_u32(waves, (int)wave - 1) : 0) + incl - own;
 #pragma unroll
     for (int e = 0; e < OWN; ++e) {
       if (before < k && k <= before + cnt[e]) { sh.word[0] = 2047 - OWN * tid - e; sh.word[1] = k - before; sh.word[3] = cnt[e]; }
@@ -1344,83 +1353,59 @@ __device__ Pick kth_largest(uint32_t n, uint32_t k, uint32_t* keys, Load load, P
     hi = shift ? lo + ((1u << shift) - 1) : lo;
     k = sh.word[1];
     if (lo == hi) return {lo, k};
-    if (left <= kFew) {
-      for (uint32_t base = 0; base < n; base += NT * kHeld) {
-        if (!ONE) load(base);
-#pragma unroll
-        for (int j = 0; j < kHeld; ++j) {
-          if (ONE && j * (uint32_t)NT >= n) break;
-          if (base + j * NT + tid < n && keys[j] >= lo && keys[j] <= hi) sh.few[atomicAdd(&sh.word[2], 1u)] = keys[j];
-        }
-      }
-      __syncthreads();
-      if (tid < 16) sh.few[left + tid] = 0;   // (nothing is below it; equals are looked for among the `left` only)
-      __syncthreads();
-      if (tid < left) {
-        const uint32_t mine = sh.few[tid];
-        uint32_t above = 0, equal = 0;
-        for (uint32_t i = 0; i < left; i += 16) {
-#pragma unroll
-          for (int e = 0; e < 16; e += 4) {
-            const u32x4 v = *reinterpret_cast<const u32x4*>(&sh.few[i + e]);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) { above += v[u] > mine ? 1 : 0; equal += v[u] == mine && i + e + u < left ? 1 : 0; }
-          }
-        }
-        if (above < k && k <= above + equal) { sh.word[0] = mine; sh.word[1] = k - above; }   // all equals write the same
-      }
-      __syncthreads();
-      return {sh.word[0], sh.word[1]};
-    }
+    if (k == left) return lo ? Pick{lo - 1, 0} : Pick{0, 0xffffffffu};   // all of the bin
+    __syncthreads();
   }
 }
 
-// Indices of the keys above the pick and of the first `need` equal to it, in ascending order: put(place, index, j).
-template <int NT, bool ONE, class Load, class Put>
-__device__ void put_picked(uint32_t n, Pick pick, const uint32_t* keys, Load load, Put put, PickShared& sh) {
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  uint32_t above = 0, equal = 0;   // in all rounds so far
-  for (uint32_t base = 0; base < n; base += NT * kHeld) {
-    if (!ONE) load(base);
-    uint32_t before[kHeld];        // of this wavefront's 64 keys: those above in the low half, those equal in the high half
-    const uint64_t below = (1ull << lane) - 1;
-    __syncthreads();
+// Indices of the keys above the pick and of the first `need` equal to it, in ascending order: put(place, index, what
+// `along` loads for the index).  Every wavefront looks over a run of the keys twice, for its counts and, once all counts are
+// known, for its places, four times 64 at a time, so that the loads do not wait for the stores.
+template <int NT, bool ONE, class Key, class Along, class Put>
+__device__ void put_picked(uint32_t n, Pick pick, Key key, Along along, Put put, PickShared<NT, ONE>& sh) {
+  const uint32_t lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), run = (n + NT - 1) / NT * 64;
+  const uint32_t i0 = wave * run < n ? wave * run : n, i1 = n - i0 < run ? n : i0 + run;
+  const auto held = [&](uint32_t i) { return ONE ? sh.keys[i < n ? i : n - 1] : key(i < n ? i : n - 1); };
+  uint32_t above = 0, equal = 0;
+  __syncthreads();
+#pragma unroll 2
+  for (uint32_t i = i0; i < i1; i += 64) {
+    const uint32_t u = held(i + lane);
+    above += (uint32_t)__popcll(__ballot(i + lane < i1 && u > pick.key));
+    equal += (uint32_t)__popcll(__ballot(i + lane < i1 && u == pick.key));
+  }
+  if (lane == 0) { sh.wave[0][wave] = above; sh.wave[1][wave] = equal; }
+  __syncthreads();
+  const uint32_t sa = wave_incl_sum_u32(lane < NT / 64 ? sh.wave[0][lane] : 0, (int)lane), se = wave_incl_sum_u32(lane < NT / 64 ? sh.wave[1][lane] : 0, (int)lane);
+  above = bcast_lane_u32(sa, (int)wave) - above;
+  equal = bcast_lane_u32(se, (int)wave) - equal;
+  const uint64_t below = (1ull << lane) - 1;
+  for (uint32_t base = i0; base < i1; base += 256) {
+    uint32_t u[4];
+    float with[4];
 #pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-      const bool in = base + j * NT + tid < n;
-      const uint64_t bg = __ballot(in && keys[j] > pick.key), be = __ballot(in && keys[j] == pick.key);
-      before[j] = (uint32_t)__popcll(bg & below) | (uint32_t)__popcll(be & below) << 16;
-      if (lane == 0) { sh.sums[0][j * (NT / 64) + wave] = (uint32_t)__popcll(bg); sh.sums[1][j * (NT / 64) + wave] = (uint32_t)__popcll(be); }
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t i = base + 64 * e + lane;
+      with[e] = along(i < i1 ? i : i1 - 1);
+      u[e] = held(i);
     }
-    __syncthreads();
-    if (wave < 2) {                // the counts in the order of the keys, PER to a lane: exclusive sums in place
-      constexpr int PER = kHeld * (NT / 64) / 64;
-      uint32_t c[PER], sum = 0;
 #pragma unroll
-      for (int e = 0; e < PER; ++e) { c[e] = sh.sums[wave][PER * lane + e]; sum += c[e]; }
-      const uint32_t incl = wave_incl_sum_u32(sum, (int)lane);
-      uint32_t run = incl - sum;
-#pragma unroll
-      for (int e = 0; e < PER; ++e) { sh.sums[wave][PER * lane + e] = run; run += c[e]; }
-      if (lane == 63) sh.word[wave] = incl;
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t i = base + 64 * e + lane;
+      const bool in = i < i1, gt = in && u[e] > pick.key, eq = in && u[e] == pick.key;
+      const uint64_t bg = __ballot(gt), be = __ballot(eq);
+      const uint32_t g0 = above + (uint32_t)__popcll(bg & below), e0 = equal + (uint32_t)__popcll(be & below);
+      if (gt || (eq && e0 < pick.need)) put(g0 + (e0 < pick.need ? e0 : pick.need), i, with[e]);
+      above += (uint32_t)__popcll(bg);
+      equal += (uint32_t)__popcll(be);
     }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-      const uint32_t i = base + j * NT + tid;
-      if (i < n && keys[j] >= pick.key) {
-        const uint32_t g0 = above + sh.sums[0][j * (NT / 64) + wave] + (before[j] & 0xffffu), e0 = equal + sh.sums[1][j * (NT / 64) + wave] + (before[j] >> 16);
-        if (keys[j] > pick.key || e0 < pick.need) put(g0 + (e0 < pick.need ? e0 : pick.need), i);
-      }
-    }
-    above += sh.word[0];
-    equal += sh.word[1];
   }
 }
 
 template <int NT, bool ONE>
 __global__ __launch_bounds__(NT) void fl_kv_pick_pages(const SelectArgs a) {
-  __shared__ PickShared sh;
+  warm_kernel_args(a);
+  __shared__ PickShared<NT, ONE> sh;
   const uint32_t h = blockIdx.x % a.c.H, t = blockIdx.x / a.c.H;
   uint32_t b, i, first, n;
   const auto items = [&](uint32_t q) { uint32_t f, m; seq_tokens(a.s, q, f, m); return m; };
@@ -1436,17 +1421,9 @@ __global__ __launch_bounds__(NT) void fl_kv_pick_pages(const SelectArgs a) {
     for (uint32_t k = threadIdx.x; k < pages; k += NT) out[k] = (int32_t)k;
     return;
   }
-  uint32_t keys[kHeld];
-  const auto load = [&](uint32_t base) {
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-      const uint32_t p = base + j * NT + threadIdx.x;
-      keys[j] = p >= pages ? 0 : p < a.first || p + a.last >= pages ? 0xffffffffu : order_key(score[p]);
-    }
-  };
-  if (ONE) load(0);
-  const Pick pick = kth_largest<NT, ONE>(pages, a.count, keys, load, sh);
-  put_picked<NT, ONE>(pages, pick, keys, load, [&](uint32_t at, uint32_t p) { out[at] = (int32_t)p; }, sh);
+  const auto key = [&](uint32_t p) { const uint32_t u = order_key(score[p]); return p < a.first || p + a.last >= pages ? 0xffffffffu : u; };
+  const Pick pick = kth_largest<NT, ONE>(pages, a.count, key, sh);
+  put_picked<NT, ONE>(pages, pick, key, [](uint32_t) { return 0.f; }, [&](uint32_t at, uint32_t p, float) { out[at] = (int32_t)p; }, sh);
 }
 
 struct KeepArgs {
@@ -1461,7 +1438,8 @@ struct KeepArgs {
 
 template <int NT, bool ONE>
 __global__ __launch_bounds__(NT) void fl_kv_keep(const KeepArgs a) {
-  __shared__ PickShared sh;
+  warm_kernel_args(a);
+  __shared__ PickShared<NT, ONE> sh;
   const uint32_t h = blockIdx.x % a.H, b = blockIdx.x / a.H;
   uint32_t len = uniform_len(a.s, a.T, b);
   if (len > a.w_width) { if (threadIdx.x == 0) report(a.s.status); len = a.w_width; }
@@ -1476,17 +1454,9 @@ __global__ __launch_bounds__(NT) void fl_kv_keep(const KeepArgs a) {
     for (uint32_t k = threadIdx.x; k < len; k += NT) { kept[k] = (int32_t)k; nw[k] = w[k]; }
     return;
   }
-  uint32_t keys[kHeld];
-  const auto load = [&](uint32_t base) {
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-      const uint32_t p = base + j * NT + threadIdx.x;
-      keys[j] = p >= len ? 0 : p < a.first || p + a.recent >= len ? 0xffffffffu : order_key(w[p]);
-    }
-  };
-  if (ONE) load(0);
-  const Pick pick = kth_largest<NT, ONE>(len, m, keys, load, sh);
-  put_picked<NT, ONE>(len, pick, keys, load, [&](uint32_t at, uint32_t p) { kept[at] = (int32_t)p; nw[at] = w[p]; }, sh);
+  const auto key = [&](uint32_t p) { const uint32_t u = order_key(w[p]); return p < a.first || p + a.recent >= len ? 0xffffffffu : u; };
+  const Pick pick = kth_largest<NT, ONE>(len, m, key, sh);
+  put_picked<NT, ONE>(len, pick, key, [&](uint32_t p) { return w[p]; }, [&](uint32_t at, uint32_t p, float v) { kept[at] = (int32_t)p; nw[at] = v; }, sh);
 }
 
 // ------------------------------------------------------------------------------------------------
