@@ -175,13 +175,14 @@ SIGNATURES = {
     "flh_region_refs": (C.c_int, [C.c_void_p]),
     "flh_region_windows": (C.c_int, [C.c_void_p, C.POINTER(Windows)]),
     "flh_region_translate": (C.c_void_p, [C.c_void_p, C.c_uint32, C.c_void_p]),
+    # parameter blocks: the structures above by reference, or their bytes
     "flh_kv_page_bytes": (C.c_uint64, [C.c_uint32, C.c_uint32, C.c_uint32]),
-    "flh_kv_store": (C.c_int, [C.POINTER(KvStoreParams), C.c_void_p]),
-    "flh_kv_attend_workspace_bytes": (C.c_int64, [C.POINTER(KvAttendParams)]),
-    "flh_kv_attend": (C.c_int, [C.POINTER(KvAttendParams), C.c_void_p]),
+    "flh_kv_store": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "flh_kv_attend_workspace_bytes": (C.c_int64, [C.c_void_p]),
+    "flh_kv_attend": (C.c_int, [C.c_void_p, C.c_void_p]),
     "flh_kv_select_workspace_bytes": (C.c_uint64, [C.c_uint32, C.c_uint32, C.c_uint32]),
-    "flh_kv_select": (C.c_int, [C.POINTER(KvSelectParams), C.c_void_p]),
-    "flh_kv_evict": (C.c_int, [C.POINTER(KvEvictParams), C.c_void_p]),
+    "flh_kv_select": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "flh_kv_evict": (C.c_int, [C.c_void_p, C.c_void_p]),
     "flh_tune": (C.c_int, [C.c_char_p, C.c_int64]),
     "flh_prof_begin": (C.c_int, [C.c_int]),
     "flh_prof_end": (C.c_int, [C.POINTER(C.c_double), C.POINTER(C.c_int), C.c_int]),

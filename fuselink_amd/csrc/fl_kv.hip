@@ -62,14 +62,6 @@ __device__ __forceinline__ void seq_tokens(const Seqs& s, uint32_t b, uint32_t& 
   n = (uint32_t)(hi - lo);
 }
 
-// tokens that sequence b holds, at most what its row of the page table can name
-__device__ __forceinline__ uint32_t seq_len(const Seqs& s, uint32_t T, uint32_t b) {
-  const int32_t len = s.lens[b];
-  const uint64_t most = (uint64_t)s.width * T;
-  if (len < 0 || (uint64_t)len > most) { report(s.status); return len < 0 ? 0u : (uint32_t)most; }
-  return (uint32_t)len;
-}
-
 // the same for a sequence that the whole wavefront looks at
 __device__ __forceinline__ void uniform_tokens(const Seqs& s, uint32_t b, uint32_t& first, uint32_t& n) {
   if (!s.starts) { first = b * s.per; n = s.per; return; }
@@ -86,19 +78,42 @@ __device__ __forceinline__ uint32_t uniform_len(const Seqs& s, uint32_t T, uint3
   return (uint32_t)len;
 }
 
-// Item x of the sequences' items laid end to end: which sequence, and which of its items.  A wavefront looks at 64
-// sequences at a time.  False if there are fewer items.
-template <class Count>
-__device__ __forceinline__ bool find_seq(uint32_t n_seqs, uint32_t x, Count count, uint32_t& b, uint32_t& local) {
+// Item x of the sequences' items laid end to end: its sequence, which of that one's items it is, and the sequence's
+// tokens.  A wavefront looks at 64 sequences at a time, all it needs to know of them loaded at once.  False if there
+// are fewer items.  LONGEST: the sequences of 64 are laid out by length, the longest first, so that what is handed out
+// last is short.
+struct Item { uint32_t b, local, first, n, len; };
+template <bool LONGEST = false, class Count>
+__device__ __forceinline__ bool find_item(const Seqs& s, uint32_t T, uint32_t x, Count count, Item& it) {
   const int lane = threadIdx.x & 63;
-  for (uint32_t base = 0; base < n_seqs; base += 64) {
-    const uint32_t c = base + lane < n_seqs ? count(base + lane) : 0;
-    const uint32_t incl = wave_incl_sum_u32(c, lane);
+  for (uint32_t base = 0; base < s.n_seqs; base += 64) {
+    uint32_t first = 0, n = 0, len = 0, c = 0;
+    if (base + lane < s.n_seqs) {
+      const int32_t held = s.lens[base + lane];
+      seq_tokens(s, base + lane, first, n);
+      const uint32_t most = s.width * T;   // (the host keeps it within 31 bits)
+      len = held < 0 ? 0u : (uint32_t)held > most ? most : (uint32_t)held;
+      if ((uint32_t)held != len) report(s.status);
+      c = count(n, len);
+    }
+    uint32_t incl = wave_incl_sum_u32(c, lane);
     const uint32_t total = bcast_lane_u32(incl, 63);
     if (x < total) {
-      const int l = __builtin_ctzll(__ballot(incl > x));
-      b = base + (uint32_t)l;
-      local = x - (bcast_lane_u32(incl, l) - bcast_lane_u32(c, l));
+      if (LONGEST) {
+        incl = c;
+        const uint32_t cnt = s.n_seqs - base < 64 ? s.n_seqs - base : 64;
+#pragma unroll 1
+        for (uint32_t j = 0; j < cnt; ++j) {
+          const uint32_t lj = bcast_lane_u32(len, (int)j), cj = bcast_lane_u32(c, (int)j);
+          incl += lj > len || (lj == len && j < (uint32_t)lane) ? cj : 0;
+        }
+      }
+      const int l = __builtin_ctzll(__ballot(incl > x && incl - c <= x));
+      it.b = base + (uint32_t)l;
+      it.local = x - (bcast_lane_u32(incl, l) - bcast_lane_u32(c, l));
+      it.first = bcast_lane_u32(first, l);
+      it.n = bcast_lane_u32(n, l);
+      it.len = bcast_lane_u32(len, l);
       return true;
     }
     x -= total;
@@ -108,12 +123,16 @@ __device__ __forceinline__ bool find_seq(uint32_t n_seqs, uint32_t x, Count coun
 
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 
+// The larger of two as one instruction: the median with infinity.  (fmaxf also quiets each operand that may be a
+// signalling NaN, which everything is that comes from a matrix instruction or another lane.)  A NaN gives way to a number.
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, kInf); }
+
 // the four lanes that share a column of a 16 x 16 result: l, l ^ 16, l ^ 32, l ^ 48
 __device__ __forceinline__ float column_max(float v) {
   auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  v = larger(__uint_as_float(r[0]), __uint_as_float(r[1]));
   r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  return larger(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float column_sum(float v) {
   auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -311,17 +330,13 @@ __global__ __launch_bounds__(256) void fl_kv_pack(const PackArgs a) {
     if (j * T >= n) return;
     page = scalar_load(a.to_table + b * a.to_stride + j);
   } else {
-    const auto items = [&](uint32_t q) {
-      uint32_t f, m;
-      seq_tokens(a.s, q, f, m);
-      const uint32_t l = seq_len(a.s, T, q);
-      return m ? (l + m + T - 1) / T - l / T : 0;
-    };
-    if (!find_seq(a.s.n_seqs, blockIdx.x, items, b, j)) return;
-    b = uniform(b);
-    uniform_tokens(a.s, b, first, n);
-    held = uniform_len(a.s, T, b);
-    j = uniform(j) + held / T;
+    Item it;
+    if (!find_item(a.s, T, blockIdx.x, [&](uint32_t m, uint32_t l) { return m ? (l + m + T - 1) / T - l / T : 0; }, it)) return;
+    b = it.b;
+    first = it.first;
+    n = it.n;
+    held = it.len;
+    j = it.local + held / T;
     if (j >= a.s.width) { if (lane == 0) report(a.s.status); return; }
     page = scalar_load(a.s.table + b * a.s.table_stride + j);
   }
@@ -532,58 +547,175 @@ __device__ __forceinline__ typename Frag<E>::v8 flipped(typename Frag<E>::v8 x, 
   return __builtin_bit_cast(typename Frag<E>::v8, w);
 }
 
+// What a wavefront carries for its NQ x 16 rows: O^T in units of vref, the maximum that ref = top - 8 comes from, and
+// each lane's part of the sum of exp2(x - ref).
+template <int NQ, int VJ>
+struct Rows {
+  f4 o[NQ][VJ];
+  float top[NQ], ref[NQ], l[NQ], vref, vlow;
+};
+template <int NQ, int VJ>
+__device__ __forceinline__ void clear(Rows<NQ, VJ>& r) {
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    r.top[q] = -kInf;
+    r.ref[q] = r.l[q] = 0.f;
+#pragma unroll
+    for (int j = 0; j < VJ; ++j) r.o[q][j] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  r.vref = r.vlow = 0.f;
+}
+// The scale that values are counted in: that of the larger of the blocks at hand, kept while it stays within 2^6 below it.
+// It does not fall by more than 2^60 below the largest so far (vlow), or what the sums hold would overflow in its units.
+__device__ __forceinline__ float next_vref(float vref, float vlow, float vmax) {
+  const float v = larger(vmax, vlow);
+  return vmax > 0.f && !(v <= vref && v * 64.f >= vref) ? v : vref;
+}
+
+// One step of the softmax: scores of 32 keys (two tiles under k scales kc0 and kc1, base 2) to probabilities, the rows'
+// state moved where a maximum has grown too far or vref has changed.  The tiles' value scales v0 and v1 go into the
+// probabilities as powers of two of vref (exact, and free in the exponent), so that codes meet them as they are; the
+// rows' sums take them out again.
+template <int NQ, int VJ>
+__device__ __forceinline__ void soften(Rows<NQ, VJ>& r, const f4 (&s)[NQ][2], float kc0, float kc1, float v0, float v1, h8 (&pf)[NQ]) {
+  float mx[NQ];
+  const float vnew = next_vref(r.vref, r.vlow, larger(v0, v1));
+  bool move = vnew != r.vref;
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    // (where all are NaN this is infinity, and the row's sum NaN one way or the other)
+    const float m0 = larger(larger(s[q][0][0], s[q][0][1]), larger(s[q][0][2], s[q][0][3]));
+    const float m1 = larger(larger(s[q][1][0], s[q][1][1]), larger(s[q][1][2], s[q][1][3]));
+    mx[q] = column_max(larger(m0 * kc0, m1 * kc1));
+    move |= mx[q] > r.top[q] + 7.f;
+  }
+  if (__ballot(move)) {
+    const float fv = r.vref > 0.f ? r.vref * inverse(vnew) : 1.f;
+    r.vref = vnew;
+    r.vlow = larger(r.vlow, vnew * 0x1p-60f);
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const float t = fmaxf(r.top[q], mx[q]), f = r.top[q] == -kInf ? 0.f : exp2_fast(r.top[q] - t);
+      r.top[q] = t;
+      r.ref[q] = t == -kInf ? 0.f : t - 8.f;
+      r.l[q] *= f;
+#pragma unroll
+      for (int j = 0; j < VJ; ++j) r.o[q][j] *= f * fv;
+    }
+  }
+  // exponents of the tiles' scales over vref's (a block of zeros has the least there is, and adds zeros)
+  const int ev = (int)(__float_as_uint(vnew) >> 23), d0 = (int)(__float_as_uint(v0) >> 23) - ev, d1 = (int)(__float_as_uint(v1) >> 23) - ev;
+  const float e0 = (float)(d0 < -64 ? -64 : d0), e1 = (float)(d1 < -64 ? -64 : d1), u0 = exp2_fast(-e0), u1 = exp2_fast(-e1);
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      p[i] = exp2_fast(__builtin_fmaf(s[q][i >> 2][i & 3], i < 4 ? kc0 : kc1, (i < 4 ? e0 : e1) - r.ref[q]));
+      pf[q][i] = (_Float16)p[i];
+    }
+    r.l[q] = __builtin_fmaf((p[0] + p[1]) + (p[2] + p[3]), u0, r.l[q]);
+    r.l[q] = __builtin_fmaf((p[4] + p[5]) + (p[6] + p[7]), u1, r.l[q]);
+  }
+}
+
+// four codes of each of two tokens as pairs: v[j] gets (first token's, second's) of code j
+__device__ __forceinline__ void interleave(uint32_t w0, uint32_t w1, h2 (&v)[4]) {
+  const uint32_t lo = __builtin_amdgcn_perm(w1, w0, 0x05010400u), hi = __builtin_amdgcn_perm(w1, w0, 0x07030602u);
+  v[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false);
+  v[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
+  v[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false);
+  v[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true);
+}
+// codes of NaN become zero; what was found is or-ed into `seen`
+__device__ __forceinline__ uint32_t without_nan(uint32_t w, uint32_t& seen) {
+  const uint32_t nan = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;   // bytes whose magnitude is 0x7f
+  seen |= nan;
+  return w & ~((nan >> 7) * 0xffu);
+}
+
+// eight dims of row r's result, to the output or, if there are splits, to this split's part of the workspace
+template <class E>
+__device__ __forceinline__ void emit8(const AttendArgs& a, uint32_t split, uint32_t first, uint32_t h, uint32_t r, float mm, float ll, const float* v, uint32_t d, bool head) {
+  const uint32_t H = a.c.H, G = a.G, D = a.c.D, i = r / G;
+  const uint64_t tok = first + i, hq = h * G + (r - i * G);
+  const float lg = ll > 0.f ? mm + __builtin_amdgcn_logf(ll) : (ll == 0.f ? -kInf : kNan);
+  if (a.splits > 1) {
+    const uint64_t at = (uint64_t)split * a.s.n_tokens * H * G + tok * H * G + hq;
+    if (head) a.part_l[at] = lg;
+    if (d < D) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) *reinterpret_cast<f4*>(a.part_o + at * D + d + e) = f4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+    }
+  } else {
+    if (head) {
+      if (a.lse) a.lse[tok * H * G + hq] = lg * 0.6931471805599453f;
+      if (a.lse2) a.lse2[tok * H * G + hq] = lg;
+    }
+    E* p = reinterpret_cast<E*>(a.out) + tok * a.o_token + hq * a.o_head + d;
+    if (d < D) {
+      typename Frag<E>::v8 y;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = (E)v[e];
+      if (a.o_vec) {
+        *reinterpret_cast<typename Frag<E>::v8*>(p) = y;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = y[e];
+      }
+    }
+  }
+}
+
 // Softmax and both products in one pass over the keys.  S^T = K Q^T and O^T = V^T P^T on 16 x 16 x 32 matrix
 // instructions: a lane's column is one query row in both, so the row's maximum, sum and rescaling need no data from
 // other rows, and S^T leaves the first product in the very lanes and order in which the second one wants P^T if the
 // 32 keys of a step are numbered (two tiles of 16) x (four lane groups) x 4 -- an order that sums do not see.  K and V
 // come as rows of codes straight into registers; V's bytes are interleaved token against token on the way to pairs.
 // P is rounded to 16-bit floats (11 bits of mantissa) as 2^8 times its value relative to a reference of the row that
-// follows its maximum only when that has grown by 2^7: at most 2^15, normal down to 2^-22 of the reference.  V's codes
-// are multiplied there by their block's scale over a reference that moves only when the scales leave 2^+-6 of it.  So
-// the accumulators are rarely rescaled; they, sums and references are 32 bits wide.
-template <class E, int DP, int NQ, int KVW, bool SEL>
+// follows its maximum only when that has grown by 2^7, times its block's value scale over a reference that moves only
+// when the scales leave 2^-6 ... 1 of it: at most 2^15, normal down to 2^-22 of the reference for the larger scale of a
+// step.  So the accumulators are rarely rescaled; they, sums and references are 32 bits wide.
+template <class E, int DP, int NQ, bool SEL>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) void fl_kv_attend(const AttendArgs a) {
   warm_kernel_args(a);
   constexpr int KK = DP / 32, KW = DP / 16, VJ = DP / 16, VW = DP / 64;
-  constexpr uint32_t TR = 16 * NQ * (4 / KVW);
+  constexpr uint32_t KVW = 4, TR = 16 * NQ;
   typedef typename Frag<E>::v8 v8;
-  __shared__ float sm_o[KVW > 1 ? KVW * 16 * NQ * (DP + 4) : 1];
-  __shared__ float sm_m[KVW > 1 ? KVW * 16 * NQ : 1], sm_l[KVW > 1 ? KVW * 16 * NQ : 1];
+  __shared__ float sm_o[KVW * 16 * NQ * (DP + 4)];
+  __shared__ float sm_m[KVW * 16 * NQ], sm_l[KVW * 16 * NQ];
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const uint32_t wave = uniform(threadIdx.x >> 6), H = a.c.H, G = a.G, T = a.c.T, D = a.c.D;
   const uint32_t h = blockIdx.x % H, rest = blockIdx.x / H, split = rest / a.tiles_x, x = rest - split * a.tiles_x;
 
-  uint32_t b, tile, first, n, len, r0, rows, tok0 = 0;
+  uint32_t tile, r0, rows, tok0 = 0;
+  Item it;
   if constexpr (SEL) {
     const uint32_t per = (G + TR - 1) / TR, t = x / per;
-    const auto items = [&](uint32_t q) { uint32_t f, m; seq_tokens(a.s, q, f, m); return m; };
-    if (!find_seq(a.s.n_seqs, t, items, b, tok0)) return;
-    b = uniform(b); tok0 = uniform(tok0);
+    if (!find_item(a.s, T, t, [](uint32_t m, uint32_t) { return m; }, it)) return;
+    tok0 = it.local;
     tile = x - t * per;
   } else {
-    const auto items = [&](uint32_t q) { uint32_t f, m; seq_tokens(a.s, q, f, m); return (m * G + TR - 1) / TR; };
-    if (!find_seq(a.s.n_seqs, x, items, b, tile)) return;
-    b = uniform(b); tile = uniform(tile);
+    if (!find_item(a.s, T, x, [&](uint32_t m, uint32_t) { return (m * G + TR - 1) / TR; }, it)) return;
+    tile = it.local;
   }
-  uniform_tokens(a.s, b, first, n);
-  len = uniform_len(a.s, T, b);
+  const uint32_t b = it.b, first = it.first, n = it.n, len = it.len;
   // rows of this workgroup: (query token, head of the group), tokens first
   if constexpr (SEL) { r0 = tok0 * G + tile * TR; rows = (tok0 + 1) * G; } else { r0 = tile * TR; rows = n * G; }
-  const uint32_t wr0 = r0 + (KVW == 1 ? wave * 16 * NQ : 0);
   const auto limit = [&](uint32_t r) -> uint32_t {   // keys that row r sees
     if (r >= rows) return 0;
     if (!a.causal) return len;
     const int64_t l = (int64_t)len - n + r / G + 1;
     return l > 0 ? (uint32_t)l : 0;
   };
-  const uint32_t last_row = wr0 + 16 * NQ - 1 < rows ? wr0 + 16 * NQ - 1 : rows - 1;
-  const uint32_t l_min = uniform(wr0 < rows ? limit(wr0) : 0), l_max = uniform(wr0 < rows ? limit(last_row) : 0);
+  const uint32_t last_row = r0 + 16 * NQ - 1 < rows ? r0 + 16 * NQ - 1 : rows - 1;
+  const uint32_t l_min = uniform(r0 < rows ? limit(r0) : 0), l_max = uniform(r0 < rows ? limit(last_row) : 0);
 
   v8 qf[NQ][KK];
   uint32_t lim[NQ];
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
-    const uint32_t r = wr0 + q * 16 + c;
+    const uint32_t r = r0 + q * 16 + c;
     lim[q] = limit(r);
     const uint32_t i = r / G;
     const E* p = reinterpret_cast<const E*>(a.q) + (uint64_t)(first + i) * a.q_token + (uint64_t)(h * G + (r - i * G)) * a.q_head;
@@ -594,16 +726,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) 
     }
   }
 
-  f4 o[NQ][VJ];
-  float top[NQ], ref[NQ], l[NQ];   // the maximum that ref = top - 8 comes from; sum of exp2(x - ref)
-#pragma unroll
-  for (int q = 0; q < NQ; ++q) {
-    top[q] = -kInf;
-    ref[q] = l[q] = 0.f;
-#pragma unroll
-    for (int j = 0; j < VJ; ++j) o[q][j] = f4{0.f, 0.f, 0.f, 0.f};
-  }
-  float vref = 0.f;
+  Rows<NQ, VJ> st;
+  clear(st);
 
   // The keys of this split, in steps of 32.  The host knows how many splits there are, the device how long the sequence
   // is: every split takes an equal share of it in whole rounds of the workgroup's wavefronts.
@@ -718,82 +842,36 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) 
           for (int q = 0; q < NQ; ++q)
             if (!(x.ok[t] && p < lim[q])) s[q][t][i] = -kInf;
 #pragma unroll
-          for (int e = 0; e < VW; ++e) {
-            uint32_t w = keep ? x.vw[4 * t + i][e] : 0;
-            const uint32_t mag = w & 0x7f7f7f7fu;
-            const uint32_t nan = (mag + 0x01010101u) & 0x80808080u;   // bytes whose magnitude is 0x7f
-            seen_nan |= nan;
-            w &= ~((nan >> 7) * 0xffu);
-            x.vw[4 * t + i][e] = w;
-          }
+          for (int e = 0; e < VW; ++e) x.vw[4 * t + i][e] = without_nan(keep ? x.vw[4 * t + i][e] : 0, seen_nan);
         }
       if (__ballot(seen_nan != 0)) nan_steps = 1;
     }
 
     // the floor keeps -inf what it is under a block of zeros; what it multiplies otherwise is zero all the same
     const float kc0 = fmaxf(x.ks[0] * a.scale2, 1e-37f), kc1 = fmaxf(x.ks[1] * a.scale2, 1e-37f);
-    const float vmax = fmaxf(x.vs[0], x.vs[1]);
-    float mx[NQ];
-    bool move = vmax > 0.f && !(vmax <= vref * 64.f && vmax * 64.f >= vref);
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      const float m0 = fmaxf(fmaxf(s[q][0][0], s[q][0][1]), fmaxf(s[q][0][2], s[q][0][3]));
-      const float m1 = fmaxf(fmaxf(s[q][1][0], s[q][1][1]), fmaxf(s[q][1][2], s[q][1][3]));
-      mx[q] = column_max(fmaxf(m0 * kc0, m1 * kc1));
-      move |= mx[q] > top[q] + 7.f;
-    }
-    if (__ballot(move)) {
-      const float vnew = vmax > 0.f && !(vmax <= vref * 64.f && vmax * 64.f >= vref) ? vmax : vref;
-      const float fv = vref > 0.f ? vref / vnew : 1.f;
-      vref = vnew;
-#pragma unroll
-      for (int q = 0; q < NQ; ++q) {
-        const float t = fmaxf(top[q], mx[q]), f = top[q] == -kInf ? 0.f : exp2_fast(top[q] - t);
-        top[q] = t;
-        ref[q] = t == -kInf ? 0.f : t - 8.f;
-        l[q] *= f;
-#pragma unroll
-        for (int j = 0; j < VJ; ++j) o[q][j] *= f * fv;
-      }
-    }
-    const float inv_ref = inverse(vref);
-
     h8 pf[NQ];
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float p = exp2_fast(__builtin_fmaf(s[q][i >> 2][i & 3], i < 4 ? kc0 : kc1, -ref[q]));
-        l[q] += p;
-        pf[q][i] = (_Float16)p;
-      }
-    }
+    soften(st, s, kc0, kc1, x.vs[0], x.vs[1], pf);
 
-    const float f0 = x.vs[0] * inv_ref, f1 = x.vs[1] * inv_ref;
 #pragma unroll
     for (int e = 0; e < VW; ++e) {
       h8 vf[4];
 #pragma unroll
       for (int pr = 0; pr < 4; ++pr) {
-        const float f = pr < 2 ? f0 : f1;
-        const uint32_t lo = __builtin_amdgcn_perm(x.vw[2 * pr + 1][e], x.vw[2 * pr][e], 0x05010400u), hi = __builtin_amdgcn_perm(x.vw[2 * pr + 1][e], x.vw[2 * pr][e], 0x07030602u);
-        const h2 x0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, f, false), x1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, f, true);
-        const h2 x2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, f, false), x3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, f, true);
-        vf[0][2 * pr] = x0[0]; vf[0][2 * pr + 1] = x0[1];
-        vf[1][2 * pr] = x1[0]; vf[1][2 * pr + 1] = x1[1];
-        vf[2][2 * pr] = x2[0]; vf[2][2 * pr + 1] = x2[1];
-        vf[3][2 * pr] = x3[0]; vf[3][2 * pr + 1] = x3[1];
+        h2 v[4];
+        interleave(x.vw[2 * pr][e], x.vw[2 * pr + 1][e], v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { vf[j][2 * pr] = v[j][0]; vf[j][2 * pr + 1] = v[j][1]; }
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) o[q][4 * e + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[j], pf[q], o[q][4 * e + j], 0, 0, 0);
+        for (int q = 0; q < NQ; ++q) st.o[q][4 * e + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[j], pf[q], st.o[q][4 * e + j], 0, 0, 0);
     }
   };
 
   {
     constexpr uint32_t kStep = 32 * KVW;
-    uint32_t k = k0 + (KVW > 1 ? wave * 32 : 0);
+    uint32_t k = k0 + (wave * 32);
     if (k < k1) {
       // The fetch is unconditional: behind a branch, the wait for this step's codes would have to cover the next ones'
       // as well.
@@ -819,7 +897,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) 
       }
     }
     if (nan_steps) {   // a NaN value that not every row of the tile sees: into the sums of those that do
-      for (k = k0 + (KVW > 1 ? wave * 32 : 0); k < k1; k += kStep) {
+      for (k = k0 + (wave * 32); k < k1; k += kStep) {
         Where w = look_up(choose(k));
 #pragma unroll
         for (int t = 0; t < 2; ++t) w.ok[t] = w.ok[t] && w.page[t] < a.c.n_pages;
@@ -835,7 +913,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) 
                 const uint32_t d = (4 * g + i) * VJ + j;
                 const bool nan = d < D && (base[kx * D + d] & 0x7f) == 0x7f;
 #pragma unroll
-                for (int q = 0; q < NQ; ++q) o[q][j][i] += nan && w.pos[t] + kx < lim[q] ? kNan : 0.f;
+                for (int q = 0; q < NQ; ++q) st.o[q][j][i] += nan && w.pos[t] + kx < lim[q] ? kNan : 0.f;
               }
         }
       }
@@ -843,87 +921,250 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) 
   }
   if (bad && lane == 0) report(a.s.status);
 #pragma unroll
-  for (int q = 0; q < NQ; ++q) l[q] = column_sum(l[q]);
+  for (int q = 0; q < NQ; ++q) {
+    const float l = column_sum(st.l[q]);
+    const int w = (int)wave * 16 * NQ + q * 16 + c;
+    if (g == 0) { sm_m[w] = l == 0.f ? -kInf : st.ref[q]; sm_l[w] = l; }
+    float* p = sm_o + w * (DP + 4) + g * 4 * VJ;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < VJ; ++j) p[i * VJ + j] = st.o[q][j][i] * st.vref;
+  }
+  __syncthreads();
+  for (uint32_t u = threadIdx.x; u < 16 * NQ * (DP / 8); u += 256) {
+    const uint32_t rr = u / (DP / 8), d = (u - rr * (DP / 8)) * 8, r = r0 + rr;
+    if (r >= rows || d >= D) continue;
+    float mm = -kInf, ll = 0.f, v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    for (uint32_t w = 0; w < KVW; ++w) mm = fmaxf(mm, sm_m[w * 16 * NQ + rr]);
+    for (uint32_t w = 0; w < KVW; ++w) {
+      const float f = mm == -kInf ? 1.f : exp2_fast(sm_m[w * 16 * NQ + rr] - mm);
+      ll += sm_l[w * 16 * NQ + rr] * f;
+      const float* p = sm_o + (w * 16 * NQ + rr) * (DP + 4) + d;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += p[e] * f;
+    }
+    const float f = ll == 0.f ? 0.f : 1.f / ll;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= f;
+    emit8<E>(a, split, first, h, r, mm, ll, v, d, d == 0);
+  }
+}
 
-  // eight dims of a row's result
-  const uint64_t row_out = (uint64_t)a.s.n_tokens * H * G;
-  const auto emit = [&](uint32_t r, float mm, float ll, const float* v, uint32_t d, bool head) {
+// The same for many rows to a key-value head, where the matrix instructions and the exponentials bound it: each of the
+// four wavefronts owns 32 rows and all walk over the keys together, 64 at a time.  Every wavefront looks up, fetches and
+// converts one tile of 16 and leaves it in shared memory as the operands of the matrix instructions, with its scales, so
+// that a code is converted once for 128 rows instead of once for 32 and the registers hold a quarter of the codes on
+// their way.  Two barriers to 64 keys; the three workgroups of a compute unit fill each other's waits.
+template <class E, int DP>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void fl_kv_attend_rows(const AttendArgs a) {
+  warm_kernel_args(a);
+  constexpr int NQ = 2, KK = DP / 32, KW = DP / 16, VJ = DP / 16, VW = DP / 64;
+  constexpr uint32_t TR = 64 * NQ;
+  typedef typename Frag<E>::v8 v8;
+  __shared__ v8 sm_k[4 * KK * 64];                     // [tile][kk][lane]
+  __shared__ h8 sm_v[2 * VJ * 64];                     // [pair of tiles][j][lane]
+  __shared__ f4 sm_tile[4];                            // K scale * scale2, V scale, there is such a tile
+  __shared__ uint32_t sm_nan;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const uint32_t wave = uniform(threadIdx.x >> 6), H = a.c.H, G = a.G, T = a.c.T, D = a.c.D;
+  const uint32_t h = blockIdx.x % H, rest = blockIdx.x / H, split = rest / a.tiles_x, x = rest - split * a.tiles_x;
+  Item it;
+  if (!find_item<true>(a.s, T, x, [&](uint32_t m, uint32_t) { return (m * G + TR - 1) / TR; }, it)) return;
+  const uint32_t b = it.b, first = it.first, n = it.n, len = it.len, r0 = it.local * TR, rows = n * G, wr0 = r0 + wave * 16 * NQ;
+  const auto limit = [&](uint32_t r) -> uint32_t {   // keys that row r sees
+    if (r >= rows) return 0;
+    if (!a.causal) return len;
+    const int64_t l = (int64_t)len - n + r / G + 1;
+    return l > 0 ? (uint32_t)l : 0;
+  };
+  const auto last_of = [&](uint32_t from, uint32_t cnt) { return from >= rows ? 0 : limit(from + cnt - 1 < rows ? from + cnt - 1 : rows - 1); };
+  const uint32_t l_min = limit(r0), l_max = last_of(r0, TR), mine = last_of(wr0, 16 * NQ), mine_min = limit(wr0);
+
+  v8 qf[NQ][KK];
+  uint32_t lim[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const uint32_t r = wr0 + q * 16 + c;
+    lim[q] = limit(r);
     const uint32_t i = r / G;
-    const uint64_t tok = first + i, hq = h * G + (r - i * G);
-    const float lg = ll > 0.f ? mm + __builtin_amdgcn_logf(ll) : (ll == 0.f ? -kInf : kNan);
-    if (a.splits > 1) {
-      const uint64_t at = split * row_out + tok * H * G + hq;
-      if (head) a.part_l[at] = lg;
-      if (d < D) {
+    const E* p = reinterpret_cast<const E*>(a.q) + (uint64_t)(first + i) * a.q_token + (uint64_t)(h * G + (r - i * G)) * a.q_head;
 #pragma unroll
-        for (int e = 0; e < 8; e += 4) *reinterpret_cast<f4*>(a.part_o + at * D + d + e) = f4{v[e], v[e + 1], v[e + 2], v[e + 3]};
-      }
-    } else {
-      if (head) {
-        if (a.lse) a.lse[tok * H * G + hq] = lg * 0.6931471805599453f;
-        if (a.lse2) a.lse2[tok * H * G + hq] = lg;
-      }
-      E* p = reinterpret_cast<E*>(a.out) + tok * a.o_token + hq * a.o_head + d;
-      if (d < D) {
-        v8 y;
+    for (int k = 0; k < KK; ++k) {
+      const uint32_t d = g * (DP / 4) + k * 8;
+      qf[q][k] = flipped<E>(load_q8<E>(p + d, r < rows && d < D, a.q_vec), a.flip);
+    }
+  }
+  Rows<NQ, VJ> st;
+  clear(st);
+
+  const uint32_t share = 64 * ((l_max + a.splits * 64 - 1) / (a.splits * 64));
+  const uint64_t k0_64 = (uint64_t)split * share;
+  const uint32_t k0 = k0_64 < l_max ? (uint32_t)k0_64 : l_max, k1 = share < l_max - k0 ? k0 + share : l_max;
+  const int32_t* table = a.s.table + b * a.s.table_stride;
+  const uint32_t head_off = h * T * D;
+  uint32_t k_lane[KW / 4], v_lane[4];   // this lane's bytes of a tile, as in fl_kv_attend
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = (E)v[e];
-        if (a.o_vec) {
-          *reinterpret_cast<v8*>(p) = y;
-        } else {
+  for (int i = 0; i < KW / 4; ++i) k_lane[i] = c * D + (g * (DP / 4) + 16 * i < D ? g * (DP / 4) + 16 * i : 0);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) p[e] = y[e];
-        }
+  for (int i = 0; i < 4; ++i) v_lane[i] = (4 * g + i) * D + ((uint32_t)(c * VJ) < D ? c * VJ : 0);
+  uint32_t bad = 0, nan_steps = 0;
+
+  // this wavefront's tile of the 64 keys from k on: where it lies, its codes, its operands
+  struct Where { uint32_t pos, page, off; bool ok; };
+  const uint32_t last_tile = (k1 - 1) >> 4;            // (used when there are keys)
+  const auto look_up = [&](uint32_t tv) {
+    Where w;
+    const uint32_t tl = tv < last_tile ? tv : last_tile, j = a.per_page == 1 ? tl : __umulhi(tl, a.per_page_inv);
+    w.ok = tv <= last_tile;
+    w.pos = tl << 4;
+    w.off = head_off + ((tl - j * a.per_page) << 4) * D;
+    w.page = (uint32_t)scalar_load(table + j);
+    return w;
+  };
+  struct Stage { uint32_t kw[KW], vw[4][VW], pos; float ks, vs; bool ok; };
+  const auto fetch = [&](Stage& s, const Where& w) {
+    const bool there = w.page < a.c.n_pages;
+    bad |= w.ok && !there ? 1 : 0;
+    s.pos = w.pos;
+    s.ok = w.ok && there;
+    const uint8_t* rec = a.c.pages + (uint64_t)(there ? w.page : 0) * a.c.stride;
+    const float* sc = reinterpret_cast<const float*>(rec + a.c.scales) + 2 * h;
+    s.ks = scalar_load(sc);
+    s.vs = scalar_load(sc + 1);
+    const uint8_t *base = rec + w.off, *vb = base + a.c.side;
+    asm("" : "+s"(base), "+s"(vb));
+#pragma unroll
+    for (int i = 0; i < KW / 4; ++i) {
+      const u32x4 y = *reinterpret_cast<const u32x4*>(base + k_lane[i]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s.kw[4 * i + e] = y[e];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(vb + v_lane[i]);
+      if constexpr (VW == 1) s.vw[i][0] = p[0];
+      else if constexpr (VW == 2) { const u2 y = *reinterpret_cast<const u2*>(p); s.vw[i][0] = y[0]; s.vw[i][1] = y[1]; }
+      else {
+        const u32x4 y = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s.vw[i][e] = y[e];
       }
     }
   };
+  const auto stage = [&](Stage& s) {
+    if (!s.ok || s.pos + 16 > l_min) {   // as in fl_kv_attend: values nobody sees, and NaN, are left out
+      asm volatile("");
+      uint32_t seen = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool keep = s.ok && s.pos + 4 * g + i < l_max;
+#pragma unroll
+        for (int e = 0; e < VW; ++e) s.vw[i][e] = without_nan(keep ? s.vw[i][e] : 0, seen);
+      }
+      if (__ballot(seen != 0)) nan_steps = 1;
+    }
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) sm_k[(wave * KK + kk) * 64 + lane] = codes8<E>(s.kw[2 * kk], s.kw[2 * kk + 1]);
+#pragma unroll
+    for (int e = 0; e < VW; ++e) {
+      h2 v[2][4];
+      interleave(s.vw[0][e], s.vw[1][e], v[0]);
+      interleave(s.vw[2][e], s.vw[3][e], v[1]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        u2* at = reinterpret_cast<u2*>(&sm_v[((wave >> 1) * VJ + 4 * e + j) * 64 + lane]) + (wave & 1);
+        *at = u2{__builtin_bit_cast(uint32_t, v[0][j]), __builtin_bit_cast(uint32_t, v[1][j])};
+      }
+    }
+    if (lane == 0) sm_tile[wave] = f4{fmaxf(s.ks * a.scale2, 1e-37f), s.ok ? s.vs : 0.f, s.ok ? 1.f : 0.f, 0.f};
+  };
 
-  if constexpr (KVW == 1) {
+  if (threadIdx.x == 0) sm_nan = 0;
+  if (k0 < k1) {
+    Stage s;
+    Where w = look_up((k0 >> 4) + wave);
+    fetch(s, w);
+    w = look_up((k0 >> 4) + 4 + wave);
+    for (uint32_t k = k0; k < k1; k += 64) {
+      __syncthreads();                                 // the last 64 keys have been used
+      stage(s);
+      fetch(s, w);
+      w = look_up((k >> 4) + 8 + wave);
+      __syncthreads();
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      const uint32_t r = wr0 + q * 16 + c;
-      const float f = l[q] == 0.f ? 0.f : vref / l[q];
-      float v[4 * VJ];
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t p0 = k + 32 * u;
+        if (p0 >= mine || p0 >= k1) break;
+        const f4 t0 = sm_tile[2 * u], t1 = sm_tile[2 * u + 1];
+        f4 sc[NQ][2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int t = 0; t < 2; ++t) {
 #pragma unroll
-        for (int j = 0; j < VJ; ++j) v[i * VJ + j] = o[q][j][i] * f;
-      if (r < rows) {
+          for (int q = 0; q < NQ; ++q) sc[q][t] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int u = 0; u < 4 * VJ; u += 8) emit(r, ref[q], l[q], v + u, g * 4 * VJ + u, g == 0 && u == 0);
+          for (int kk = 0; kk < KK; ++kk) {
+            const v8 kf = sm_k[((2 * u + t) * KK + kk) * 64 + lane];
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) sc[q][t] = Frag<E>::mfma(kf, qf[q][kk], sc[q][t]);
+          }
+        }
+        if (p0 + 32 > mine_min || __ballot(t0[2] * t1[2] == 0.f)) {
+          asm volatile("");
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int q = 0; q < NQ; ++q)
+                if (!((t ? t1 : t0)[2] != 0.f && p0 + 16 * t + 4 * g + i < lim[q])) sc[q][t][i] = -kInf;
+        }
+        h8 pf[NQ];
+        soften(st, sc, t0[0], t1[0], t0[1], t1[1], pf);
+#pragma unroll
+        for (int j = 0; j < VJ; ++j) {
+          const h8 vf = sm_v[(u * VJ + j) * 64 + lane];
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) st.o[q][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[q], st.o[q][j], 0, 0, 0);
+        }
       }
     }
-  } else {
+  }
+  if (nan_steps) sm_nan = 1;
+  __syncthreads();
+  if (sm_nan) {   // a NaN value that not every row of the workgroup sees: into the sums of those that do
+    for (uint32_t tv = k0 >> 4; tv << 4 < k1; ++tv) {
+      const Where w = look_up(tv);
+      const bool ok = w.page < a.c.n_pages;
+      if (!ok || w.pos + 16 <= l_min) continue;
+      const uint8_t* base = a.c.pages + (uint64_t)w.page * a.c.stride + a.c.side + w.off;
+      for (uint32_t kx = 0; kx < 16 && w.pos + kx < l_max; ++kx)
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      const int w = (int)wave * 16 * NQ + q * 16 + c;
-      if (g == 0) { sm_m[w] = l[q] == 0.f ? -kInf : ref[q]; sm_l[w] = l[q]; }
-      float* p = sm_o + w * (DP + 4) + g * 4 * VJ;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+          for (int j = 0; j < VJ; ++j) {
+            const uint32_t d = (4 * g + i) * VJ + j;
+            const bool nan = d < D && (base[kx * D + d] & 0x7f) == 0x7f;
 #pragma unroll
-        for (int j = 0; j < VJ; ++j) p[i * VJ + j] = o[q][j][i] * vref;
+            for (int q = 0; q < NQ; ++q) st.o[q][j][i] += nan && w.pos + kx < lim[q] ? kNan : 0.f;
+          }
     }
-    __syncthreads();
-    for (uint32_t u = threadIdx.x; u < 16 * NQ * (DP / 8); u += 256) {
-      const uint32_t rr = u / (DP / 8), d = (u - rr * (DP / 8)) * 8, r = r0 + rr;
-      if (r >= rows || d >= D) continue;
-      float mm = -kInf, ll = 0.f, v[8];
+  }
+  if (bad && lane == 0) report(a.s.status);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
-      for (int w = 0; w < KVW; ++w) mm = fmaxf(mm, sm_m[w * 16 * NQ + rr]);
-      for (int w = 0; w < KVW; ++w) {
-        const float f = mm == -kInf ? 1.f : exp2_fast(sm_m[w * 16 * NQ + rr] - mm);
-        ll += sm_l[w * 16 * NQ + rr] * f;
-        const float* p = sm_o + (w * 16 * NQ + rr) * (DP + 4) + d;
+  for (int q = 0; q < NQ; ++q) {
+    const uint32_t r = wr0 + q * 16 + c;
+    const float l = column_sum(st.l[q]), f = l == 0.f ? 0.f : st.vref / l;
+    if (r >= rows) continue;
+    float v[4 * VJ];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += p[e] * f;
-      }
-      const float f = ll == 0.f ? 0.f : 1.f / ll;
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= f;
-      emit(r, mm, ll, v, d, d == 0);
-    }
+      for (int j = 0; j < VJ; ++j) v[i * VJ + j] = st.o[q][j][i] * f;
+#pragma unroll
+    for (int u = 0; u < 4 * VJ; u += 8) emit8<E>(a, split, first, h, r, l == 0.f ? -kInf : st.ref[q], l, v + u, g * 4 * VJ + u, g == 0 && u == 0);
   }
 }
 
@@ -935,19 +1176,18 @@ __global__ __launch_bounds__(256) void fl_kv_join(const AttendArgs a, uint32_t T
   warm_kernel_args(a);
   const uint32_t H = a.c.H, G = a.G, D = a.c.D, lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const uint32_t h = blockIdx.x % H, x = blockIdx.x / H;
-  uint32_t b, tile, first, n, r0, rows, tok0 = 0;
+  uint32_t tile, r0, rows, tok0 = 0;
+  Item it;
   if constexpr (SEL) {
     const uint32_t per = (G + TR - 1) / TR, t = x / per;
-    const auto items = [&](uint32_t q) { uint32_t f, m; seq_tokens(a.s, q, f, m); return m; };
-    if (!find_seq(a.s.n_seqs, t, items, b, tok0)) return;
-    b = uniform(b);
+    if (!find_item(a.s, a.c.T, t, [](uint32_t m, uint32_t) { return m; }, it)) return;
+    tok0 = it.local;
     tile = x - t * per;
   } else {
-    const auto items = [&](uint32_t q) { uint32_t f, m; seq_tokens(a.s, q, f, m); return (m * G + TR - 1) / TR; };
-    if (!find_seq(a.s.n_seqs, x, items, b, tile)) return;
-    b = uniform(b);
+    if (!find_item(a.s, a.c.T, x, [&](uint32_t m, uint32_t) { return (m * G + TR - 1) / TR; }, it)) return;
+    tile = it.local;
   }
-  uniform_tokens(a.s, b, first, n);
+  const uint32_t first = it.first, n = it.n;
   if constexpr (SEL) { r0 = tok0 * G + tile * TR; rows = (tok0 + 1) * G; } else { r0 = tile * TR; rows = n * G; }
   const uint64_t row_out = (uint64_t)a.s.n_tokens * H * G;
   const uint32_t r = r0 + blockIdx.y * 4 + wave;
@@ -1118,13 +1358,9 @@ __global__ __launch_bounds__(256) void fl_kv_score(const SelectArgs a) {
   const uint32_t wave = uniform(threadIdx.x >> 6), H = a.c.H, G = a.G, T = a.c.T, D = a.c.D, HW = a.heads_wg, groups = (H + HW - 1) / HW;
   const uint32_t h = blockIdx.x % groups * HW + wave % HW, part = blockIdx.x / groups;
   if (h >= H) return;
-  uint32_t b, i, first, n;
-  const auto items = [&](uint32_t q) { uint32_t f, m; seq_tokens(a.s, q, f, m); return m; };
-  if (!find_seq(a.s.n_seqs, blockIdx.y, items, b, i)) return;
-  b = uniform(b);
-  i = uniform(i);
-  uniform_tokens(a.s, b, first, n);
-  const uint32_t lim = token_limit(a, uniform_len(a.s, T, b), n, i), pages = (lim + T - 1) / T;
+  Item it;
+  if (!find_item(a.s, T, blockIdx.y, [](uint32_t m, uint32_t) { return m; }, it)) return;
+  const uint32_t b = it.b, i = it.local, first = it.first, n = it.n, lim = token_limit(a, it.len, n, i), pages = (lim + T - 1) / T;
   const uint32_t subs = 4 / HW, step = a.parts * subs * 32;   // 32 pages to a wavefront at a time
   uint32_t p0 = (part * subs + wave / HW) * 32;
   if (p0 >= pages) return;
@@ -1407,13 +1643,10 @@ __global__ __launch_bounds__(NT) void fl_kv_pick_pages(const SelectArgs a) {
   warm_kernel_args(a);
   __shared__ PickShared<NT, ONE> sh;
   const uint32_t h = blockIdx.x % a.c.H, t = blockIdx.x / a.c.H;
-  uint32_t b, i, first, n;
-  const auto items = [&](uint32_t q) { uint32_t f, m; seq_tokens(a.s, q, f, m); return m; };
-  if (!find_seq(a.s.n_seqs, t, items, b, i)) return;
-  b = uniform(b);
-  uniform_tokens(a.s, b, first, n);
-  const uint32_t lim = token_limit(a, uniform_len(a.s, a.c.T, b), n, uniform(i)), pages = (lim + a.c.T - 1) / a.c.T;
-  const uint64_t row = (uint64_t)(first + i) * a.c.H + h;
+  Item it;
+  if (!find_item(a.s, a.c.T, t, [](uint32_t m, uint32_t) { return m; }, it)) return;
+  const uint32_t lim = token_limit(a, it.len, it.n, it.local), pages = (lim + a.c.T - 1) / a.c.T;
+  const uint64_t row = (uint64_t)(it.first + it.local) * a.c.H + h;
   const float* score = a.scores + row * a.s.width;
   int32_t* out = a.out + row * a.count;
   for (uint32_t k = (pages < a.count ? pages : a.count) + threadIdx.x; k < a.count; k += NT) out[k] = -1;
@@ -1529,8 +1762,10 @@ int make_plan(const flh_kv_attend_params* p, Plan* pl) {
   const bool sel = p->d_selected != nullptr;
   const uint64_t rows = sel ? G : ((uint64_t)n * G + B - 1) / B;   // of a sequence, on average
   pl->kvw = rows <= 32 || sel ? 4 : 1;
-  pl->nq = pl->dp == 256 || (pl->kvw == 4 && rows <= 16) ? 1 : 2;
+  pl->nq = pl->kvw == 4 && (pl->dp == 256 || rows <= 16) ? 1 : 2;
   pl->tr = 16 * pl->nq * (4 / pl->kvw);
+  // workgroups that stay resident together: what their registers allow, on 256 compute units
+  const uint32_t seats = 256 * (pl->kvw == 1 ? (pl->dp == 256 ? 1 : 3) : pl->dp == 256 ? 1 : pl->dp == 64 ? (pl->nq == 1 ? 5 : 3) : pl->nq == 1 ? 3 : 2);
   uint64_t tiles, est;
   if (sel) tiles = est = (uint64_t)n * ((G + pl->tr - 1) / pl->tr);
   else if (!p->seqs.d_starts) tiles = est = (uint64_t)B * (((uint64_t)(n / B) * G + pl->tr - 1) / pl->tr);
@@ -1539,9 +1774,17 @@ int make_plan(const flh_kv_attend_params* p, Plan* pl) {
     est = (uint64_t)n * G / pl->tr > B ? (uint64_t)n * G / pl->tr : B;
   }
   const uint64_t space = sel ? (uint64_t)p->n_selected * p->cache.tokens : (uint64_t)p->seqs.table_width * p->cache.tokens;
-  const uint64_t want = est * H ? (1024 + est * H - 1) / (est * H) : 1, most = (space + 127) / 128;
-  pl->splits = (uint32_t)(want < most ? want : most);
-  if (pl->kvw == 1 || pl->splits < 1) pl->splits = 1;
+  // Splits: rounds of workgroups times the longest share (in whole rounds of their wavefronts), a start and an end worth
+  // some 384 keys each time, and the join, worth as much again.
+  const uint32_t round = pl->kvw == 4 ? 128 : 64;
+  uint64_t best = ~0ull;
+  pl->splits = 1;
+  const uint64_t top = pl->kvw == 4 ? 256 : est * H < seats ? seats / (est * H ? est * H : 1) : 1;   // (many rows: until the seats are taken)
+  for (uint32_t sp = 1; sp <= top && (sp == 1 || (uint64_t)(sp - 1) * round < space); ++sp) {
+    const uint64_t rounds = (est * H * sp + seats - 1) / seats, share = (space + (uint64_t)sp * round - 1) / ((uint64_t)sp * round) * round;
+    const uint64_t cost = rounds * (share + 384) + (sp > 1 ? 384 : 0);
+    if (cost < best) { best = cost; pl->splits = sp; }
+  }
   if (tiles * H * pl->splits > kMaxGroups) return fl_set_error(FLH_E_ARG, "flh_kv_attend: too much for one launch");
   pl->tiles_x = (uint32_t)tiles;
   pl->rows = (uint64_t)n * p->q_heads;
@@ -1556,29 +1799,26 @@ int make_plan(const flh_kv_attend_params* p, Plan* pl) {
   return FLH_OK;
 }
 
-template <class E, int DP, int NQ, int KVW>
-void launch_attend(const AttendArgs& a, hipStream_t st) {
+template <class E, int DP, int NQ>
+void launch_attend(const AttendArgs& a, const Plan& pl, hipStream_t st) {
   const dim3 grid(a.tiles_x * a.c.H * a.splits);
-  if (a.tiles_x == 0) return;
-  if constexpr (KVW == 4) {
-    if (a.sel) { FL_LAUNCH((fl_kv_attend<E, DP, NQ, KVW, true>), grid, dim3(256), 0, st, a); return; }
-  }
-  FL_LAUNCH((fl_kv_attend<E, DP, NQ, KVW, false>), grid, dim3(256), 0, st, a);
+  if (pl.kvw == 1) FL_LAUNCH((fl_kv_attend_rows<E, DP>), grid, dim3(256), 0, st, a);
+  else if (a.sel) FL_LAUNCH((fl_kv_attend<E, DP, NQ, true>), grid, dim3(256), 0, st, a);
+  else FL_LAUNCH((fl_kv_attend<E, DP, NQ, false>), grid, dim3(256), 0, st, a);
 }
 
 template <class E>
 void run_attend(const AttendArgs& a, const Plan& pl, hipStream_t st) {
-  if (pl.dp == 64) {
-    if (pl.kvw == 1) launch_attend<E, 64, 2, 1>(a, st);
-    else if (pl.nq == 1) launch_attend<E, 64, 1, 4>(a, st);
-    else launch_attend<E, 64, 2, 4>(a, st);
-  } else if (pl.dp == 128) {
-    if (pl.kvw == 1) launch_attend<E, 128, 2, 1>(a, st);
-    else if (pl.nq == 1) launch_attend<E, 128, 1, 4>(a, st);
-    else launch_attend<E, 128, 2, 4>(a, st);
-  } else {
-    if (pl.kvw == 1) launch_attend<E, 256, 1, 1>(a, st);
-    else launch_attend<E, 256, 1, 4>(a, st);
+  if (a.tiles_x) {
+    if (pl.dp == 64) {
+      if (pl.nq == 1) launch_attend<E, 64, 1>(a, pl, st);
+      else launch_attend<E, 64, 2>(a, pl, st);
+    } else if (pl.dp == 128) {
+      if (pl.nq == 1) launch_attend<E, 128, 1>(a, pl, st);
+      else launch_attend<E, 128, 2>(a, pl, st);
+    } else {
+      launch_attend<E, 256, 1>(a, pl, st);
+    }
   }
   if (pl.splits > 1 && a.tiles_x) {
     const dim3 grid(a.tiles_x * a.c.H, pl.tr / 4);

@@ -11,14 +11,25 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import math
+import struct
 from typing import Optional
 
 import torch
 
 from . import _lib
-from ._lib import KvAttendParams, KvCache, KvEvictParams, KvSelectParams, KvSeqs, KvStoreParams, check
+from ._lib import KvAttendParams, KvEvictParams, KvSelectParams, KvStoreParams, check
 
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_I32, _F32 = torch.int32, torch.float32
+
+# The parameter blocks as struct formats: filling a ctypes structure field by field took longer than the launch.
+_CACHE, _SEQS = "QQIIII", "QQQQIIII"
+_STORE = struct.Struct("=" + _CACHE + _SEQS + "QQ" + "QQQQ" + "II" + "Q")
+_ATTEND = struct.Struct("=" + _CACHE + _SEQS + "QQ" + "QQQQ" + "Q" + "IIfI" + "QQQ" + "QQQQ" + "II" + "QQQ")
+_SELECT = struct.Struct("=" + _CACHE + _SEQS + "Q" + "QQ" + "IIIIII" + "Q" + "QQQ")
+_EVICT = struct.Struct("=" + _CACHE + _CACHE + _SEQS + "QQ" + "QQQ" + "QQQ" + "QQ" + "IIIIII" + "Q")
+for _f, _c in ((_STORE, KvStoreParams), (_ATTEND, KvAttendParams), (_SELECT, KvSelectParams), (_EVICT, KvEvictParams)):
+    assert _f.size == C.sizeof(_c), _c
 
 
 def page_bytes(tokens: int, heads: int, dim: int) -> int:
@@ -41,7 +52,8 @@ class PageCache:
         _need(pages.shape[1] >= need and stride >= need and stride % 16 == 0 and pages.data_ptr() % 16 == 0,
               f"records of {need} bytes in rows of {pages.shape[1]}, {stride} apart")
         self.pages, self.tokens, self.heads, self.dim = pages, tokens, heads, dim
-        self.c = KvCache(pages.data_ptr(), stride, pages.shape[0], tokens, heads, dim)
+        self.c = (pages.data_ptr(), stride, pages.shape[0], tokens, heads, dim)
+        self.device, self.index = pages.device, pages.get_device()
 
     def codes(self):
         """K and V codes, float8_e4m3fn views [n_pages, heads, tokens, dim] of the pool."""
@@ -64,10 +76,17 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _check(dev: torch.device, name: str, t: torch.Tensor, dtype, dims: int) -> None:
-    if t.device != dev or t.dim() != dims or (t.dtype != dtype if dtype is not None else t.dtype not in TYPES) or (t.shape[-1] > 1 and t.stride(-1) != 1):
-        raise ValueError(f"{name}: a tensor of {dims} dimensions on {dev}, {dtype or 'bf16, fp16 or fp32'}, its last dimension contiguous; "
-                         f"not {tuple(t.shape)} {t.dtype} on {t.device}")
+def _wrong(cache: PageCache, name: str, t, what: str) -> None:
+    _need(cache.index >= 0, "the pool must be on a GPU: there is no CPU path")
+    raise ValueError(f"{name}: {what}, its last dimension contiguous, on {cache.device}; not {tuple(t.shape)} {t.dtype}, strides {t.stride()}, on {t.device}")
+
+
+def _check(cache: PageCache, name: str, t: torch.Tensor, dtype, dims: int):
+    """Shape and strides of a tensor that is what it has to be."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not dtype or len(shape) != dims or (stride[-1] != 1 and shape[-1] > 1) or t.get_device() != cache.index:
+        _wrong(cache, name, t, f"{dims} dimensions of {dtype}")
+    return shape, stride
 
 
 def _check_written(name: str, t: torch.Tensor) -> None:
@@ -75,42 +94,51 @@ def _check_written(name: str, t: torch.Tensor) -> None:
         raise ValueError(f"{name}: written, but some of its elements share memory")
 
 
-def _seqs(cache: PageCache, table, lens, status, starts, n_tokens: int) -> KvSeqs:
-    dev = cache.pages.device
-    _need(dev.type == "cuda", "the pool must be on a GPU: there is no CPU path")
-    _check(dev, "page_table", table, torch.int32, 2)
-    _check(dev, "lens", lens, torch.int32, 1)
-    _check(dev, "status", status, torch.int32, 1)
-    _need(status.numel() >= 1, "status: one word at least")
-    n = table.shape[0]
-    _need(n > 0 and table.shape[1] > 0 and lens.shape[0] == n, f"page_table of {tuple(table.shape)} for {lens.shape[0]} lens")
-    stride = table.stride(0) if n > 1 else table.shape[1]
-    _need(stride >= table.shape[1], "page_table: its rows overlap")
+def _seqs(cache: PageCache, table, lens, status, starts, n_tokens: int):
+    """The fields of flh_kv_seqs, and the status word's address."""
+    _need(cache.index >= 0, "the pool must be on a GPU: there is no CPU path")
+    (n, width), (stride, _) = _check(cache, "page_table", table, _I32, 2)
+    (n_lens,), _ = _check(cache, "lens", lens, _I32, 1)
+    (words,), _ = _check(cache, "status", status, _I32, 1)
+    if n == 1:
+        stride = width
+    if not (n > 0 and width > 0 and n_lens == n and stride >= width and words > 0):
+        raise ValueError(f"page_table of {tuple(table.shape)} (rows {stride} apart) for {n_lens} lens, {words} words of status")
     if starts is not None:
-        _check(dev, "starts", starts, torch.int32, 1)
-        _need(starts.shape[0] == n + 1, f"{starts.shape[0]} starts for {n} sequences (one more than sequences)")
+        (n_starts,), _ = _check(cache, "starts", starts, _I32, 1)
+        if n_starts != n + 1:
+            raise ValueError(f"{n_starts} starts for {n} sequences (one more than sequences)")
         sp = starts.data_ptr()
     else:
-        _need(n_tokens % n == 0, f"{n_tokens} tokens do not divide into {n} sequences; give starts")
-        sp = None
-    return KvSeqs(sp, lens.data_ptr(), table.data_ptr(), stride, table.shape[1], n, n_tokens, 0)
+        if n_tokens % n:
+            raise ValueError(f"{n_tokens} tokens do not divide into {n} sequences; give starts")
+        sp = 0
+    return (sp, lens.data_ptr(), table.data_ptr(), stride, width, n, n_tokens, 0), status.data_ptr()
+
+
+def _queries(cache: PageCache, q: torch.Tensor):
+    """Tokens, query heads, strides and type of the queries."""
+    if q.dtype is not torch.bfloat16 and q.dtype is not torch.float16:
+        _wrong(cache, "q", q, "bf16 or fp16")
+    (n, hq, d), (st, sh, _) = _check(cache, "q", q, q.dtype, 3)
+    if d != cache.dim or hq == 0 or hq % cache.heads:
+        raise ValueError(f"q {tuple(q.shape)} over {cache.heads} heads of {cache.dim}")
+    return n, hq, st, sh, 0 if q.dtype is torch.bfloat16 else 1
 
 
 class _On:
-    """Device and stream of a call: allocations inside belong to the stream, tensors given are marked as used on it."""
+    """Device and stream of a call that names a stream, or whose tensors are not on the current device: allocations inside belong
+    to the stream, and the tensors given are marked as used on it."""
 
-    def __init__(self, dev: torch.device, stream: Optional[torch.cuda.Stream], *tensors):
-        self.stack = None
-        if stream is None:
-            if torch.cuda.current_device() != dev.index:
-                self.stack = contextlib.ExitStack()
-                self.stack.enter_context(torch.cuda.device(dev))
-            self.ptr = C.c_void_p(torch._C._cuda_getCurrentRawStream(dev.index))
-            return
-        _need(stream.device == dev, f"stream of {stream.device}, tensors of {dev}")
+    def __init__(self, cache: PageCache, stream: Optional[torch.cuda.Stream], *tensors):
         self.stack = contextlib.ExitStack()
+        if stream is None:
+            self.stack.enter_context(torch.cuda.device(cache.device))
+            self.ptr = torch.cuda.current_stream(cache.device).cuda_stream
+            return
+        _need(stream.device == cache.device, f"stream of {stream.device}, tensors of {cache.device}")
         self.stack.enter_context(torch.cuda.stream(stream))
-        self.ptr = C.c_void_p(stream.cuda_stream)
+        self.ptr = stream.cuda_stream
         if not torch.cuda.is_current_stream_capturing():
             for t in tensors:
                 if t is not None:
@@ -120,32 +148,56 @@ class _On:
         return self.ptr
 
     def __exit__(self, *exc):
-        if self.stack is not None:
-            self.stack.close()
+        self.stack.close()
 
 
-def _workspace(given: Optional[torch.Tensor], need: int, dev: torch.device) -> Optional[torch.Tensor]:
+class _Here:
+    """The current stream of the current device."""
+
+    def __init__(self, index: int):
+        self.ptr = torch._C._cuda_getCurrentRawStream(index)
+
+    def __enter__(self):
+        return self.ptr
+
+    def __exit__(self, *exc):
+        pass
+
+
+def _on(cache: PageCache, stream, *tensors):
+    if stream is None and torch.cuda.current_device() == cache.index:
+        return _Here(cache.index)
+    return _On(cache, stream, *tensors)
+
+
+def _workspace(cache: PageCache, given: Optional[torch.Tensor], need: int):
+    """Address and bytes of a workspace, and what owns it."""
     if need == 0:
-        return None
+        return 0, 0, None
     if given is None:
-        return torch.empty(need, dtype=torch.uint8, device=dev)
+        given = torch.empty(need, dtype=torch.uint8, device=cache.device)
+        return given.data_ptr(), need, given
     nbytes = given.numel() * given.element_size()
-    _need(given.device == dev and given.is_contiguous() and nbytes >= need and given.data_ptr() % 16 == 0, f"workspace: {need} contiguous bytes on {dev}, 16-byte aligned")
-    return given
+    _need(given.get_device() == cache.index and given.is_contiguous() and nbytes >= need and given.data_ptr() % 16 == 0,
+          f"workspace: {need} contiguous bytes on {cache.device}, 16-byte aligned")
+    return given.data_ptr(), nbytes, given
 
 
 def store(cache: PageCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor, status: torch.Tensor, *,
           starts: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> None:
     """flh_kv_store: appends k and v [n_tokens, heads, dim] (bf16, fp16 or fp32) to sequences that hold `lens` tokens
     before the call.  `starts` [n_seqs + 1] says whose tokens are whose; without it every sequence has equally many."""
-    dev = cache.pages.device
-    _check(dev, "k", k, None, 3)
-    _check(dev, "v", v, k.dtype, 3)
-    _need(k.shape == v.shape and tuple(k.shape[1:]) == (cache.heads, cache.dim), f"k {tuple(k.shape)} and v {tuple(v.shape)} for {cache.heads} heads of {cache.dim}")
-    p = KvStoreParams(cache.c, _seqs(cache, page_table, lens, status, starts, k.shape[0]), k.data_ptr(), v.data_ptr(),
-                      k.stride(0), k.stride(1), v.stride(0), v.stride(1), TYPES[k.dtype], 0, status.data_ptr())
-    with _On(dev, stream, cache.pages, k, v, page_table, lens, status, starts) as sp:
-        check(_lib.load().flh_kv_store(C.byref(p), sp))
+    kind = TYPES.get(k.dtype)
+    if kind is None:
+        _wrong(cache, "k", k, "bf16, fp16 or fp32")
+    shape, (kt, kh, _) = _check(cache, "k", k, k.dtype, 3)
+    v_shape, (vt, vh, _) = _check(cache, "v", v, k.dtype, 3)
+    if shape != v_shape or shape[1] != cache.heads or shape[2] != cache.dim:
+        raise ValueError(f"k {tuple(shape)} and v {tuple(v_shape)} for {cache.heads} heads of {cache.dim}")
+    seqs, word = _seqs(cache, page_table, lens, status, starts, shape[0])
+    p = _STORE.pack(*cache.c, *seqs, k.data_ptr(), v.data_ptr(), kt, kh, vt, vh, kind, 0, word)
+    with _on(cache, stream, cache.pages, k, v, page_table, lens, status, starts) as sp:
+        check(_lib.load().flh_kv_store(p, sp))
 
 
 def attend(cache: PageCache, q: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor, status: torch.Tensor, *,
@@ -158,53 +210,51 @@ def attend(cache: PageCache, q: torch.Tensor, page_table: torch.Tensor, lens: to
     contiguous) receives the logarithms of the rows' sums.  `selected` (from select_pages) restricts every query token and head to
     those pages.  `weights` (float32 [n_seqs, heads, positions]) gains what attention every key drew: it is added to in
     place, or written as `weights_in` plus the gain when that is given."""
-    dev = cache.pages.device
-    _check(dev, "q", q, None, 3)
-    _need(q.dtype != torch.float32, "q: bf16 or fp16")
-    n, hq = q.shape[0], q.shape[1]
-    _need(q.shape[2] == cache.dim and hq > 0 and hq % cache.heads == 0, f"q {tuple(q.shape)} over {cache.heads} heads of {cache.dim}")
-    s = _seqs(cache, page_table, lens, status, starts, n)
-    p = KvAttendParams()
+    n, hq, qt, qh, kind = _queries(cache, q)
+    seqs, word = _seqs(cache, page_table, lens, status, starts, n)
+    n_seqs, heads = seqs[5], cache.heads
+    lse_p = sel_p = count = win_p = w_p = wis = wih = ws = wh = width = 0
     if lse is not None:
-        _check(dev, "lse", lse, torch.float32, 2)
-        _need(lse.is_contiguous() and lse.shape == q.shape[:2], f"lse: contiguous {tuple(q.shape[:2])}")
-        p.d_lse = lse.data_ptr()
+        shape, _ = _check(cache, "lse", lse, _F32, 2)
+        _need(lse.is_contiguous() and shape == q.shape[:2], f"lse: contiguous {tuple(q.shape[:2])}")
+        lse_p = lse.data_ptr()
     if selected is not None:
-        _check(dev, "selected", selected, torch.int32, 3)
-        _need(selected.is_contiguous() and tuple(selected.shape[:2]) == (n, cache.heads), f"selected: contiguous [{n}, {cache.heads}, pages]")
+        (a, b, count), _ = _check(cache, "selected", selected, _I32, 3)
         _need(weights is None, "weights are kept over all pages, not over selected ones")
-        _need(selected.shape[2] > 0, "selected: no pages")
-        p.d_selected, p.n_selected = selected.data_ptr(), min(selected.shape[2], 0xffffffff)
-    if weights_in is not None:
-        _need(weights is not None, "weights_in without weights")
+        _need(a == n and b == heads and count > 0 and selected.is_contiguous(), f"selected: contiguous [{n}, {heads}, pages]")
+        sel_p = selected.data_ptr()
     if weights is not None:
-        src = weights if weights_in is None else weights_in
-        for name, w in (("weights", weights), ("weights_in", src)):
-            _check(dev, name, w, torch.float32, 3)
-            _need(tuple(w.shape[:2]) == (s.n_seqs, cache.heads) and w.shape == weights.shape and w.shape[2] > 0, f"{name}: [{s.n_seqs}, {cache.heads}, positions]")
+        (a, b, width), (ws, wh, _) = _check(cache, "weights", weights, _F32, 3)
+        _need(a == n_seqs and b == heads and width > 0, f"weights: [{n_seqs}, {heads}, positions]")
         _check_written("weights", weights)
-        p.d_weights, p.d_weights_in, p.weights_width = weights.data_ptr(), src.data_ptr(), weights.shape[2]
-        p.weights_seq_stride, p.weights_head_stride = weights.stride(0), weights.stride(1)
-        p.weights_in_seq_stride, p.weights_in_head_stride = src.stride(0), src.stride(1)
-    p.cache, p.seqs = cache.c, s
-    p.d_q, p.q_token_stride, p.q_head_stride = q.data_ptr(), q.stride(0), q.stride(1)
-    p.type, p.q_heads, p.causal, p.d_status = TYPES[q.dtype], hq, int(causal), status.data_ptr()
-    p.scale = 1.0 / math.sqrt(cache.dim) if scale is None else scale
+        w_p, win_p, wis, wih = weights.data_ptr(), weights.data_ptr(), ws, wh
+        if weights_in is not None:
+            shape, (wis, wih, _) = _check(cache, "weights_in", weights_in, _F32, 3)
+            _need(shape == weights.shape, f"weights_in: [{n_seqs}, {heads}, {width}]")
+            win_p = weights_in.data_ptr()
+    else:
+        _need(weights_in is None, "weights_in without weights")
     lib = _lib.load()
-    with _On(dev, stream, cache.pages, q, page_table, lens, status, starts, lse, selected, weights, weights_in, out, workspace) as sp:
+    with _on(cache, stream, cache.pages, q, page_table, lens, status, starts, lse, selected, weights, weights_in, out, workspace) as sp:
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
-            _check(dev, "out", out, q.dtype, 3)
+            _check(cache, "out", out, q.dtype, 3)
             _check_written("out", out)
             _need(out.shape == q.shape, f"out {tuple(out.shape)} for q {tuple(q.shape)}")
-        p.d_out, p.out_token_stride, p.out_head_stride = out.data_ptr(), out.stride(0), out.stride(1)
-        need = check(lib.flh_kv_attend_workspace_bytes(C.byref(p)))
-        if need:
-            workspace = _workspace(workspace, need, dev)
-            p.d_workspace, p.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        check(lib.flh_kv_attend(C.byref(p), sp))
+        ot, oh, _ = out.stride()
+        head = (*cache.c, *seqs, q.data_ptr(), out.data_ptr(), qt, qh, ot, oh, lse_p, kind, hq,
+                1.0 / math.sqrt(cache.dim) if scale is None else scale, 1 if causal else 0, sel_p, win_p, w_p, wis, wih, ws, wh, count, width)
+        sizes = (cache.c[3:], seqs[4:7], seqs[0] != 0, hq, count, w_p != 0)
+        need = _needs.get(sizes)
+        if need is None:
+            need = _needs[sizes] = check(lib.flh_kv_attend_workspace_bytes(_ATTEND.pack(*head, 0, 0, word)))
+        wp, wb, owner = _workspace(cache, workspace, need)
+        check(lib.flh_kv_attend(_ATTEND.pack(*head, wp, wb, word), sp))
     return out
+
+
+_needs: dict = {}    # sizes of a call -> bytes of its workspace
 
 
 def select_pages(cache: PageCache, q: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor, count: int, status: torch.Tensor, *,
@@ -212,25 +262,18 @@ def select_pages(cache: PageCache, q: torch.Tensor, page_table: torch.Tensor, le
                  workspace: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """flh_kv_select: for every query token and key-value head the `count` pages (int32 [n_tokens, heads, count], ascending, -1 behind
     them) whose keys may weigh most, the first `first` and last `last` ones always among them."""
-    dev = cache.pages.device
-    _check(dev, "q", q, None, 3)
-    _need(q.dtype != torch.float32, "q: bf16 or fp16")
-    n, hq = q.shape[0], q.shape[1]
-    _need(q.shape[2] == cache.dim and hq > 0 and hq % cache.heads == 0, f"q {tuple(q.shape)} over {cache.heads} heads of {cache.dim}")
+    n, hq, qt, qh, kind = _queries(cache, q)
     _need(0 < count < 2 ** 31 and first >= 0 and last >= 0 and first + last <= count, f"{count} pages with {first} first and {last} last ones")
-    s = _seqs(cache, page_table, lens, status, starts, n)
-    lib = _lib.load()
-    with _On(dev, stream, cache.pages, q, page_table, lens, status, starts, out, workspace) as sp:
+    seqs, word = _seqs(cache, page_table, lens, status, starts, n)
+    with _on(cache, stream, cache.pages, q, page_table, lens, status, starts, out, workspace) as sp:
         if out is None:
-            out = torch.empty((n, cache.heads, count), dtype=torch.int32, device=dev)
+            out = torch.empty((n, cache.heads, count), dtype=_I32, device=cache.device)
         else:
-            _check(dev, "out", out, torch.int32, 3)
-            _need(out.is_contiguous() and tuple(out.shape) == (n, cache.heads, count), f"out: contiguous [{n}, {cache.heads}, {count}]")
-        workspace = _workspace(workspace, int(lib.flh_kv_select_workspace_bytes(n, cache.heads, s.table_width)), dev)
-        p = KvSelectParams(cache.c, s, q.data_ptr(), q.stride(0), q.stride(1), TYPES[q.dtype], hq, count, first, last, int(causal), out.data_ptr(),
-                           workspace.data_ptr() if workspace is not None else None,
-                           workspace.numel() * workspace.element_size() if workspace is not None else 0, status.data_ptr())
-        check(lib.flh_kv_select(C.byref(p), sp))
+            shape, _ = _check(cache, "out", out, _I32, 3)
+            _need(out.is_contiguous() and tuple(shape) == (n, cache.heads, count), f"out: contiguous [{n}, {cache.heads}, {count}]")
+        wp, wb, owner = _workspace(cache, workspace, 4 * n * cache.heads * seqs[4])     # flh_kv_select_workspace_bytes
+        check(_lib.load().flh_kv_select(_SELECT.pack(*cache.c, *seqs, q.data_ptr(), qt, qh, kind, hq, count, first, last, 1 if causal else 0,
+                                                     out.data_ptr(), wp, wb, word), sp))
     return out
 
 
@@ -241,33 +284,36 @@ def evict(cache: PageCache, page_table: torch.Tensor, lens: torch.Tensor, weight
     `weights` [n_seqs, heads, positions] -- packed into the pages of `to` that `to_table` [n_seqs, pages] names, none of which may be
     among those that are read.  Returns (kept, new_weights, new_lens): positions [n_seqs, heads, budget] with -1 behind
     them, the weights kept with zeros behind them ([n_seqs, heads, >= budget]), and the new lengths."""
-    dev = cache.pages.device
-    s = _seqs(cache, page_table, lens, status, None, 0)
-    b, h = s.n_seqs, cache.heads
-    _need(to.pages.device == dev and to.heads == h and to.dim == cache.dim, "the new cache differs in device, heads or head dim")
-    _check(dev, "weights", weights, torch.float32, 3)
-    _need(tuple(weights.shape[:2]) == (b, h) and weights.shape[2] > 0, f"weights: [{b}, {h}, positions]")
+    seqs, word = _seqs(cache, page_table, lens, status, None, 0)
+    b, h = seqs[5], cache.heads
+    _need(to.index == cache.index and to.heads == h and to.dim == cache.dim, "the new cache differs in device, heads or head dim")
+    (wb, wh, width), (ws_s, ws_h, _) = _check(cache, "weights", weights, _F32, 3)
+    _need(wb == b and wh == h and width > 0, f"weights: [{b}, {h}, positions]")
     _need(0 < budget <= 1 << 30 and first >= 0 and recent >= 0 and first + recent <= budget, f"a budget of {budget} with {first} first and {recent} recent tokens")
-    _check(dev, "to_table", to_table, torch.int32, 2)
-    per = (budget + to.tokens - 1) // to.tokens
-    stride = to_table.stride(0) if b > 1 else to_table.shape[1]
-    _need(to_table.shape[0] == b and to_table.shape[1] >= per and stride >= to_table.shape[1], f"to_table: [{b}, >= {per}]")
-    with _On(dev, stream, cache.pages, to.pages, page_table, lens, weights, to_table, status, kept, new_weights, new_lens) as sp:
+    (tb, to_width), (stride, _) = _check(cache, "to_table", to_table, _I32, 2)
+    if b == 1:
+        stride = to_width
+    _need(tb == b and to_width >= (budget + to.tokens - 1) // to.tokens and stride >= to_width, f"to_table: [{b}, >= {(budget + to.tokens - 1) // to.tokens}]")
+    with _on(cache, stream, cache.pages, to.pages, page_table, lens, weights, to_table, status, kept, new_weights, new_lens) as sp:
         if kept is None:
-            kept = torch.empty((b, h, budget), dtype=torch.int32, device=dev)
+            kept = torch.empty((b, h, budget), dtype=_I32, device=cache.device)
+        else:
+            shape, _ = _check(cache, "kept", kept, _I32, 3)
+            _need(kept.is_contiguous() and tuple(shape) == (b, h, budget), f"kept: contiguous [{b}, {h}, {budget}]")
         if new_weights is None:
-            new_weights = torch.empty((b, h, budget), dtype=torch.float32, device=dev)
+            new_weights = torch.empty((b, h, budget), dtype=_F32, device=cache.device)
+            ns, nh, nw = h * budget, budget, budget
+        else:
+            (nb, nhh, nw), (ns, nh, _) = _check(cache, "new_weights", new_weights, _F32, 3)
+            _check_written("new_weights", new_weights)
+            _need(nb == b and nhh == h and nw >= budget, f"new_weights: [{b}, {h}, >= {budget}]")
         if new_lens is None:
-            new_lens = torch.empty(b, dtype=torch.int32, device=dev)
-        _check(dev, "kept", kept, torch.int32, 3)
-        _check(dev, "new_weights", new_weights, torch.float32, 3)
-        _check(dev, "new_lens", new_lens, torch.int32, 1)
-        _need(kept.is_contiguous() and tuple(kept.shape) == (b, h, budget), f"kept: contiguous [{b}, {h}, {budget}]")
-        _need(tuple(new_weights.shape[:2]) == (b, h) and new_weights.shape[2] >= budget, f"new_weights: [{b}, {h}, >= {budget}]")
-        _check_written("new_weights", new_weights)
-        _need(new_lens.shape[0] == b, f"new_lens: [{b}]")
-        p = KvEvictParams(cache.c, to.c, s, to_table.data_ptr(), stride, weights.data_ptr(), weights.stride(0), weights.stride(1),
-                          new_weights.data_ptr(), new_weights.stride(0), new_weights.stride(1), kept.data_ptr(), new_lens.data_ptr(),
-                          to_table.shape[1], weights.shape[2], new_weights.shape[2], budget, first, recent, status.data_ptr())
-        check(_lib.load().flh_kv_evict(C.byref(p), sp))
+            new_lens = torch.empty(b, dtype=_I32, device=cache.device)
+        else:
+            (nl,), _ = _check(cache, "new_lens", new_lens, _I32, 1)
+            _check_written("new_lens", new_lens)
+            _need(nl == b, f"new_lens: [{b}]")
+        check(_lib.load().flh_kv_evict(_EVICT.pack(*cache.c, *to.c, *seqs, to_table.data_ptr(), stride, weights.data_ptr(), ws_s, ws_h,
+                                                   new_weights.data_ptr(), ns, nh, kept.data_ptr(), new_lens.data_ptr(), to_width, width, nw,
+                                                   budget, first, recent, word), sp))
     return kept, new_weights, new_lens

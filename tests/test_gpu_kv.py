@@ -311,9 +311,10 @@ def test_attend_scales_far_apart(fl, T):
     q = dev(torch, rng.standard_normal((1, G, D)) * 4, torch.float32).to(torch.float16)
     out = kv.attend(cache, q.expand(1, G, D), dev(torch, table), dev(torch, np.array([x], np.int32)), core.new_status()).cpu().double().numpy()
     r = ref.attend(c, q.cpu().double().numpy(), table, [x], [0, 1], 1 / np.sqrt(D))
-    big = np.abs(r["out"]) > 65000
+    # what is computed lies within tol of the definition before it becomes 16 bits wide; from 65520 on that is infinity
     tol = ref.out_tolerance(r, torch.finfo(torch.float16).eps, x)
-    assert (np.abs(out - r["out"])[~big] <= tol[~big]).all() and (np.abs(out[big]) >= 65000).all()
+    low, high = np.abs(r["out"]) - tol, np.abs(r["out"]) + tol
+    assert (np.abs(out - r["out"])[high < 65504] <= tol[high < 65504]).all() and np.isinf(out[low > 65520]).all() and not np.isnan(out).any()
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.3, 40.0])
