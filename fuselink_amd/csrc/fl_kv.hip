@@ -20,6 +20,7 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef int i4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 
 constexpr float kInf = __builtin_inff();
 constexpr float kNan = __builtin_nanf("");
@@ -219,7 +220,6 @@ __device__ __forceinline__ float number(const Raw<E>& r, int i) {
 
 // The largest magnitude as bits, which order as magnitudes do, two 16-bit ones to a word.  Infinities and NaN come
 // above all that is finite: finite_amax() goes over the row again if there are any.
-typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 template <class E>
 __device__ __forceinline__ void max_bits(uint32_t& m, const Raw<E>& r) {
 #pragma unroll
@@ -547,76 +547,95 @@ __device__ __forceinline__ typename Frag<E>::v8 flipped(typename Frag<E>::v8 x, 
   return __builtin_bit_cast(typename Frag<E>::v8, w);
 }
 
-// What a wavefront carries for its NQ x 16 rows: O^T in units of vref, the maximum that ref = top - 8 comes from, and
-// each lane's part of the sum of exp2(x - ref).
+// What a wavefront carries for its NQ x 16 rows: O^T in units of 2^(ev - 127), each lane's part of the rows' sums of
+// exp2(x - ref), the maximum that ref = top - 8 comes from.  fresh: a row that may see keys has not seen
+// one.  elow: ev does not fall below it.
 template <int NQ, int VJ>
 struct Rows {
   f4 o[NQ][VJ];
-  float top[NQ], ref[NQ], l[NQ], vref, vlow;
+  float top[NQ], ref[NQ], l[NQ];
+  int ev, elow;
+  bool fresh;
 };
 template <int NQ, int VJ>
-__device__ __forceinline__ void clear(Rows<NQ, VJ>& r) {
+__device__ __forceinline__ void clear(Rows<NQ, VJ>& r, const uint32_t (&lim)[NQ], uint32_t k0) {
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
-    r.top[q] = -kInf;
+    r.top[q] = lim[q] > k0 ? -kInf : 0.f;
     r.ref[q] = r.l[q] = 0.f;
 #pragma unroll
     for (int j = 0; j < VJ; ++j) r.o[q][j] = f4{0.f, 0.f, 0.f, 0.f};
   }
-  r.vref = r.vlow = 0.f;
+  r.ev = r.elow = 0;
+  r.fresh = true;
 }
-// The scale that values are counted in: that of the larger of the blocks at hand, kept while it stays within 2^6 below it.
-// It does not fall by more than 2^60 below the largest so far (vlow), or what the sums hold would overflow in its units.
-__device__ __forceinline__ float next_vref(float vref, float vlow, float vmax) {
-  const float v = larger(vmax, vlow);
-  return vmax > 0.f && !(v <= vref && v * 64.f >= vref) ? v : vref;
-}
+__device__ __forceinline__ float scale_of(int ev) { return ev > 0 ? __uint_as_float((uint32_t)ev << 23) : 0.f; }
 
-// One step of the softmax: scores of 32 keys (two tiles under k scales kc0 and kc1, base 2) to probabilities, the rows'
-// state moved where a maximum has grown too far or vref has changed.  The tiles' value scales v0 and v1 go into the
-// probabilities as powers of two of vref (exact, and free in the exponent), so that codes meet them as they are; the
-// rows' sums take them out again.
+// One step of the softmax: scores of 32 keys (two tiles under K scales kc0 and kc1, base 2, and value scales v0 and v1) to
+// probabilities and their sums.
+//
+// A row's probabilities are exp2(x - ref) with a reference that follows its maximum only when one of them would pass 2^15,
+// which is seen from the rounded ones themselves, two to a word; the maximum proper is taken in that case only.  The
+// tiles' value scales go into the probabilities as powers of two of the scale that O counts in (exact, and free in the
+// exponent), so that V's codes meet them as they are.  That scale is the larger of the two blocks', kept while it stays
+// within 2^6 below; it never falls more than 2^60 below the largest so far, or what O holds would overflow.  The sums
+// take the probabilities before they are rounded: logarithms and weights are 32 bits wide and come from them.
 template <int NQ, int VJ>
 __device__ __forceinline__ void soften(Rows<NQ, VJ>& r, const f4 (&s)[NQ][2], float kc0, float kc1, float v0, float v1, h8 (&pf)[NQ]) {
-  float mx[NQ];
-  const float vnew = next_vref(r.vref, r.vlow, larger(v0, v1));
-  bool move = vnew != r.vref;
+  const int x0 = (int)(uniform(__float_as_uint(v0)) >> 23), x1 = (int)(uniform(__float_as_uint(v1)) >> 23), xm = x0 > x1 ? x0 : x1, xt = xm > r.elow ? xm : r.elow;
+  const int enew = xm > 0 && !(xt <= r.ev && xt + 6 >= r.ev) ? xt : r.ev;
+  const int d0 = x0 - enew < -64 ? -64 : x0 - enew, d1 = x1 - enew < -64 ? -64 : x1 - enew;   // (a block of zeros: the least)
+  const float e0 = (float)d0, e1 = (float)d1;
+  if (enew != r.ev) {
+    asm volatile("");
+    const int dv = r.ev - enew;
+    const float fv = r.ev == 0 ? 1.f : dv < -126 ? 0.f : pow2f(dv);
+    r.ev = enew;
+    if (enew - 60 > r.elow) r.elow = enew - 60;
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+      for (int j = 0; j < VJ; ++j) r.o[q][j] *= fv;
+  }
+  const float u0 = pow2f(-d0), u1 = pow2f(-d1);
+  bool none = false;
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
-    // (where all are NaN this is infinity, and the row's sum NaN one way or the other)
-    const float m0 = larger(larger(s[q][0][0], s[q][0][1]), larger(s[q][0][2], s[q][0][3]));
-    const float m1 = larger(larger(s[q][1][0], s[q][1][1]), larger(s[q][1][2], s[q][1][3]));
-    mx[q] = column_max(larger(m0 * kc0, m1 * kc1));
-    move |= mx[q] > r.top[q] + 7.f;
-  }
-  if (__ballot(move)) {
-    const float fv = r.vref > 0.f ? r.vref * inverse(vnew) : 1.f;
-    r.vref = vnew;
-    r.vlow = larger(r.vlow, vnew * 0x1p-60f);
+    float sum;
+    uint32_t high;
+    const auto exponentials = [&]() {
+      const float r0 = e0 - r.ref[q], r1 = e1 - r.ref[q];
+      float p[8];
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      const float t = fmaxf(r.top[q], mx[q]), f = r.top[q] == -kInf ? 0.f : exp2_fast(r.top[q] - t);
+      for (int i = 0; i < 8; ++i) {
+        p[i] = exp2_fast(__builtin_fmaf(s[q][i >> 2][i & 3], i < 4 ? kc0 : kc1, i < 4 ? r0 : r1));
+        pf[q][i] = (_Float16)p[i];
+      }
+      sum = ((p[0] + p[1]) + (p[2] + p[3])) * u0 + ((p[4] + p[5]) + (p[6] + p[7])) * u1;
+      const u32x4 w = __builtin_bit_cast(u32x4, pf[q]);
+      const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3];   // (a bit cast of a vector's element takes the first one's bits)
+      const us2 m = __builtin_elementwise_max(__builtin_elementwise_max(__builtin_bit_cast(us2, w0), __builtin_bit_cast(us2, w1)),
+                                              __builtin_elementwise_max(__builtin_bit_cast(us2, w2), __builtin_bit_cast(us2, w3)));
+      high = __builtin_bit_cast(uint32_t, m) + 0x08000800u;   // bit 15 of a half: 2^15 or more, or no number
+    };
+    exponentials();
+    if (r.fresh || __ballot((high & 0x80008000u) != 0)) {
+      asm volatile("");
+      // (where all are NaN this is infinity, and the row's sum NaN one way or the other)
+      const float m0 = larger(larger(s[q][0][0], s[q][0][1]), larger(s[q][0][2], s[q][0][3]));
+      const float m1 = larger(larger(s[q][1][0], s[q][1][1]), larger(s[q][1][2], s[q][1][3]));
+      const float t = larger(r.top[q], column_max(larger(m0 * kc0, m1 * kc1))), f = r.top[q] == -kInf ? 0.f : exp2_fast(r.top[q] - t);
       r.top[q] = t;
       r.ref[q] = t == -kInf ? 0.f : t - 8.f;
+      none |= t == -kInf;
       r.l[q] *= f;
 #pragma unroll
-      for (int j = 0; j < VJ; ++j) r.o[q][j] *= f * fv;
+      for (int j = 0; j < VJ; ++j) r.o[q][j] *= f;
+      exponentials();
     }
+    r.l[q] += sum;
   }
-  // exponents of the tiles' scales over vref's (a block of zeros has the least there is, and adds zeros)
-  const int ev = (int)(__float_as_uint(vnew) >> 23), d0 = (int)(__float_as_uint(v0) >> 23) - ev, d1 = (int)(__float_as_uint(v1) >> 23) - ev;
-  const float e0 = (float)(d0 < -64 ? -64 : d0), e1 = (float)(d1 < -64 ? -64 : d1), u0 = exp2_fast(-e0), u1 = exp2_fast(-e1);
-#pragma unroll
-  for (int q = 0; q < NQ; ++q) {
-    float p[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      p[i] = exp2_fast(__builtin_fmaf(s[q][i >> 2][i & 3], i < 4 ? kc0 : kc1, (i < 4 ? e0 : e1) - r.ref[q]));
-      pf[q][i] = (_Float16)p[i];
-    }
-    r.l[q] = __builtin_fmaf((p[0] + p[1]) + (p[2] + p[3]), u0, r.l[q]);
-    r.l[q] = __builtin_fmaf((p[4] + p[5]) + (p[6] + p[7]), u1, r.l[q]);
-  }
+  if (r.fresh) r.fresh = __ballot(none) != 0;
 }
 
 // four codes of each of two tokens as pairs: v[j] gets (first token's, second's) of code j
@@ -672,10 +691,9 @@ __device__ __forceinline__ void emit8(const AttendArgs& a, uint32_t split, uint3
 // other rows, and S^T leaves the first product in the very lanes and order in which the second one wants P^T if the
 // 32 keys of a step are numbered (two tiles of 16) x (four lane groups) x 4 -- an order that sums do not see.  K and V
 // come as rows of codes straight into registers; V's bytes are interleaved token against token on the way to pairs.
-// P is rounded to 16-bit floats (11 bits of mantissa) as 2^8 times its value relative to a reference of the row that
-// follows its maximum only when that has grown by 2^7, times its block's value scale over a reference that moves only
-// when the scales leave 2^-6 ... 1 of it: at most 2^15, normal down to 2^-22 of the reference for the larger scale of a
-// step.  So the accumulators are rarely rescaled; they, sums and references are 32 bits wide.
+// P is rounded to 16-bit floats (11 bits of mantissa) at 2^8 times its value relative to the row's reference and up to 2^15,
+// normal down to 2^-22 of it (for the tile with the larger value scale of a step).  Sums, references and accumulators
+// are 32 bits wide and rarely rescaled.
 template <class E, int DP, int NQ, bool SEL>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) void fl_kv_attend(const AttendArgs a) {
   warm_kernel_args(a);
@@ -726,14 +744,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) 
     }
   }
 
-  Rows<NQ, VJ> st;
-  clear(st);
-
   // The keys of this split, in steps of 32.  The host knows how many splits there are, the device how long the sequence
   // is: every split takes an equal share of it in whole rounds of the workgroup's wavefronts.
   const uint32_t space = SEL ? a.count * T : l_max, share = KVW * 32 * ((space + a.splits * KVW * 32 - 1) / (a.splits * KVW * 32));
   const uint64_t k0_64 = (uint64_t)split * share;
   const uint32_t k0 = k0_64 < space ? (uint32_t)k0_64 : space, k1 = share < space - k0 ? k0 + share : space;
+  Rows<NQ, VJ> st;
+  clear(st, lim, SEL ? 0 : k0);
   const int32_t* table = a.s.table + b * a.s.table_stride;
   const int32_t* sel = SEL ? a.sel + ((uint64_t)(first + tok0) * H + h) * a.count : nullptr;
   const uint32_t head_off = h * T * D;
@@ -922,14 +939,14 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) 
   if (bad && lane == 0) report(a.s.status);
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
-    const float l = column_sum(st.l[q]);
+    const float l = column_sum(st.l[q]), vref = scale_of(st.ev);
     const int w = (int)wave * 16 * NQ + q * 16 + c;
     if (g == 0) { sm_m[w] = l == 0.f ? -kInf : st.ref[q]; sm_l[w] = l; }
     float* p = sm_o + w * (DP + 4) + g * 4 * VJ;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < VJ; ++j) p[i * VJ + j] = st.o[q][j][i] * st.vref;
+      for (int j = 0; j < VJ; ++j) p[i * VJ + j] = st.o[q][j][i] * vref;
   }
   __syncthreads();
   for (uint32_t u = threadIdx.x; u < 16 * NQ * (DP / 8); u += 256) {
@@ -997,12 +1014,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void fl_kv_attend_rows(cons
       qf[q][k] = flipped<E>(load_q8<E>(p + d, r < rows && d < D, a.q_vec), a.flip);
     }
   }
-  Rows<NQ, VJ> st;
-  clear(st);
-
   const uint32_t share = 64 * ((l_max + a.splits * 64 - 1) / (a.splits * 64));
   const uint64_t k0_64 = (uint64_t)split * share;
   const uint32_t k0 = k0_64 < l_max ? (uint32_t)k0_64 : l_max, k1 = share < l_max - k0 ? k0 + share : l_max;
+  Rows<NQ, VJ> st;
+  clear(st, lim, k0);
   const int32_t* table = a.s.table + b * a.s.table_stride;
   const uint32_t head_off = h * T * D;
   uint32_t k_lane[KW / 4], v_lane[4];   // this lane's bytes of a tile, as in fl_kv_attend
@@ -1156,7 +1172,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void fl_kv_attend_rows(cons
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
     const uint32_t r = wr0 + q * 16 + c;
-    const float l = column_sum(st.l[q]), f = l == 0.f ? 0.f : st.vref / l;
+    const float l = column_sum(st.l[q]), f = l == 0.f ? 0.f : scale_of(st.ev) / l;
     if (r >= rows) continue;
     float v[4 * VJ];
 #pragma unroll
