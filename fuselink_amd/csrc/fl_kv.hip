@@ -1249,97 +1249,120 @@ __global__ __launch_bounds__(256) void fl_kv_join(const AttendArgs a, uint32_t T
 }
 
 // What every key of a sequence was worth to the call's queries: the probabilities exp2(s - lse) summed over the rows of
-// its key-value head, on top of w_in.  One wavefront owns 64 keys and walks over all rows, so the sums need no atomics.
+// its key-value head, on top of w_in.  A wavefront owns NT tiles of 16 keys at a time and walks over all rows, so the
+// sums need no atomics; the next tiles' codes are on their way meanwhile.  Rows that fit one tile are loaded once.
 template <class E, int DP>
 __global__ __launch_bounds__(256) void fl_kv_weights(const AttendArgs a) {
   warm_kernel_args(a);
-  constexpr int KK = DP / 32, KW = DP / 16;
+  constexpr int KK = DP / 32, KW = DP / 16, NT = 2;
   typedef typename Frag<E>::v8 v8;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-  const uint32_t wave = uniform(threadIdx.x >> 6), H = a.c.H, G = a.G, T = a.c.T, D = a.c.D, h = blockIdx.y, b = blockIdx.z;
-  const uint32_t k0 = (blockIdx.x * 4 + wave) * 64;
+  const uint32_t H = a.c.H, G = a.G, T = a.c.T, D = a.c.D, h = blockIdx.y, b = blockIdx.z;
+  const uint32_t wave = blockIdx.x * 4 + uniform(threadIdx.x >> 6), step = gridDim.x * 4 * NT;   // in tiles
   uint32_t first, n;
   uniform_tokens(a.s, b, first, n);
-  const uint32_t len = uniform_len(a.s, T, b), rows = n * G;
+  const uint32_t len = uniform_len(a.s, T, b), rows = n * G, tiles = rows ? (len + 15) >> 4 : 0, last_tile = tiles - 1, span = (a.w_width + 15) >> 4;
   const float* w_in = a.w_in ? a.w_in + b * a.wi_seq + h * a.wi_head : nullptr;
   float* w_out = a.w_out + b * a.wo_seq + h * a.wo_head;
   if (len > a.w_width && lane == 0) report(a.s.status);
-  float acc[4][4];
+  const int32_t* table = a.s.table + b * a.s.table_stride;
+  uint32_t k_lane[KW / 4], bad = 0;
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int i = 0; i < KW / 4; ++i) k_lane[i] = c * D + (g * (DP / 4) + 16 * i < D ? g * (DP / 4) + 16 * i : 0);
+
+  struct Stage { uint32_t kw[NT][KW]; float kc[NT]; bool ok[NT]; };
+  const auto fetch = [&](Stage& s, uint32_t t0) {     // (past the end: the last tile again)
+    uint32_t page[NT], slot[NT];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
-  if (k0 < len && rows) {
-    const int32_t* table = a.s.table + b * a.s.table_stride;
-    const uint32_t last_tile = (len - 1) >> 4;
-    uint32_t kw[4][KW], bad = 0;
-    float kc[4];
-    bool ok[4];
-    uint32_t k_lane[KW / 4];
-#pragma unroll
-    for (int i = 0; i < KW / 4; ++i) k_lane[i] = c * D + (g * (DP / 4) + 16 * i < D ? g * (DP / 4) + 16 * i : 0);
-    uint32_t page[4], slot[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const uint32_t tv = (k0 >> 4) + t, tl = tv < last_tile ? tv : last_tile, j = a.per_page == 1 ? tl : __umulhi(tl, a.per_page_inv);
+    for (int t = 0; t < NT; ++t) {
+      const uint32_t tl = t0 + t < tiles ? t0 + t : last_tile, j = a.per_page == 1 ? tl : __umulhi(tl, a.per_page_inv);
       slot[t] = (tl - j * a.per_page) << 4;
       page[t] = (uint32_t)scalar_load(table + j);
-      ok[t] = tv <= last_tile;
     }
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < NT; ++t) {
       const bool there = page[t] < a.c.n_pages;
-      bad |= ok[t] && !there ? 1 : 0;
-      ok[t] = ok[t] && there;
+      s.ok[t] = t0 + t < tiles && there;
+      bad |= there ? 0 : 1;
       const uint8_t* rec = a.c.pages + (uint64_t)(there ? page[t] : 0) * a.c.stride;
-      kc[t] = scalar_load(reinterpret_cast<const float*>(rec + a.c.scales) + 2 * h) * a.scale2;
+      s.kc[t] = scalar_load(reinterpret_cast<const float*>(rec + a.c.scales) + 2 * h) * a.scale2;
       const uint8_t* base = rec + (uint64_t)(h * T + slot[t]) * D;
       asm("" : "+s"(base));
 #pragma unroll
       for (int i = 0; i < KW / 4; ++i) {
         const u32x4 w = *reinterpret_cast<const u32x4*>(base + k_lane[i]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) kw[t][4 * i + e] = w[e];
+        for (int e = 0; e < 4; ++e) s.kw[t][4 * i + e] = w[e];
       }
     }
-    if (bad && lane == 0) report(a.s.status);
-    for (uint32_t r0 = 0; r0 < rows; r0 += 16) {
-      const uint32_t r = r0 + c, i = r / G;
-      const bool in = r < rows;
-      const uint64_t tok = first + i, hq = h * G + (r - i * G);
-      const E* p = reinterpret_cast<const E*>(a.q) + tok * a.q_token + hq * a.q_head;
-      v8 qf[KK];
+  };
+  v8 qf[KK];
+  float lg = 0.f;
+  uint32_t lim = 0;
+  const auto load_rows = [&](uint32_t r0) {
+    const uint32_t r = r0 + c, i = r / G;
+    const bool in = r < rows;
+    const uint64_t tok = first + i, hq = h * G + (r - i * G);
+    const E* p = reinterpret_cast<const E*>(a.q) + tok * a.q_token + hq * a.q_head;
 #pragma unroll
-      for (int k = 0; k < KK; ++k) qf[k] = flipped<E>(load_q8<E>(p + g * (DP / 4) + k * 8, in && g * (DP / 4) + k * 8 < D, a.q_vec), a.flip);
-      const float lg = in ? a.lse2[tok * H * G + hq] : 0.f;
-      const int64_t lim64 = !in ? 0 : a.causal ? (int64_t)len - n + i + 1 : len;
-      const uint32_t lim = lim64 > 0 ? (uint32_t)lim64 : 0;
+    for (int k = 0; k < KK; ++k) qf[k] = flipped<E>(load_q8<E>(p + g * (DP / 4) + k * 8, in && g * (DP / 4) + k * 8 < D, a.q_vec), a.flip);
+    lg = in ? a.lse2[tok * H * G + hq] : 0.f;
+    const int64_t l = !in ? 0 : a.causal ? (int64_t)len - n + i + 1 : len;
+    lim = l > 0 ? (uint32_t)l : 0;
+  };
+  const auto work = [&](const Stage& s, uint32_t t0) {
+    float acc[NT][4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        f4 s = {0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int k = 0; k < KK; ++k) s = Frag<E>::mfma(codes8<E>(kw[t][2 * k], kw[t][2 * k + 1]), qf[k], s);
+      for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
+    if (t0 < tiles) {
+      for (uint32_t r0 = 0; r0 < rows; r0 += 16) {
+        if (rows > 16) load_rows(r0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (ok[t] && k0 + 16 * t + 4 * g + e < lim) acc[t][e] += exp2_fast(__builtin_fmaf(s[e], kc[t], -lg));
+        for (int t = 0; t < NT; ++t) {
+          f4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < KK; ++k) x = Frag<E>::mfma(codes8<E>(s.kw[t][2 * k], s.kw[t][2 * k + 1]), qf[k], x);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p = exp2_fast(__builtin_fmaf(x[e], s.kc[t], -lg));
+            acc[t][e] += s.ok[t] && ((t0 + t) << 4) + 4 * g + e < lim ? p : 0.f;
+          }
+        }
       }
     }
+    // lane c of group g writes position 4 g + (c & 3) of tile c >> 2
+    float mine = 0.f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v = acc[t][e];
+        v += __uint_as_float(dpp_u32<0xb1>(__float_as_uint(v)));    // quad_perm 1 0 3 2
+        v += __uint_as_float(dpp_u32<0x4e>(__float_as_uint(v)));    // quad_perm 2 3 0 1
+        v += __uint_as_float(dpp_u32<0x141>(__float_as_uint(v)));   // mirrored in 8
+        v += __uint_as_float(dpp_u32<0x140>(__float_as_uint(v)));   // mirrored in 16
+        mine = c == 4 * t + e ? v : mine;
+      }
+    const uint32_t p = (t0 << 4) + 16 * (c >> 2) + 4 * g + (c & 3);
+    if (c < 4 * NT && p < a.w_width && (p < len || w_in != w_out)) w_out[p] = (w_in ? w_in[p] : 0.f) + (p < len ? mine : 0.f);
+  };
+
+  const uint32_t end = tiles > span ? tiles : span;
+  uint32_t t0 = wave * NT;
+  if (t0 >= end) return;
+  Stage now, next;
+  if (tiles) {
+    fetch(now, t0);
+    load_rows(0);
   }
-#pragma unroll
-  for (int t = 0; t < 4; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-#pragma unroll
-      for (int o = 8; o; o >>= 1) acc[t][e] += __shfl_xor(acc[t][e], o);
-    }
-  // lane c of group g writes position 4 g + (c & 3) of tile c >> 2
-  float mine = 0.f;
-#pragma unroll
-  for (int t = 0; t < 4; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) mine = c == 4 * t + e ? acc[t][e] : mine;
-  const uint32_t p = k0 + 16 * (c >> 2) + 4 * g + (c & 3);
-  if (p < a.w_width && (p < len || w_in != w_out)) w_out[p] = (w_in ? w_in[p] : 0.f) + (p < len ? mine : 0.f);
+  for (; t0 < end; t0 += step) {
+    if (tiles) fetch(next, t0 + step);
+    work(now, t0);
+    now = next;
+  }
+  if (bad && lane == 0) report(a.s.status);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1364,10 +1387,10 @@ __device__ __forceinline__ uint32_t token_limit(const SelectArgs& a, uint32_t le
 // score(page) = max over the group's heads of ks * qs * sum_d q8_d (q8_d > 0 ? high_d : low_d): an estimate of the
 // largest product that a key of the page can have with the query, in whole numbers (8-bit queries against the page's
 // 8-bit bounds), so equal scores are equal and the choice does not depend on the order of a sum.  The sum splits into
-// max(q8, 0) . high + min(q8, 0) . low, two runs of 16 x 16 x 64 integer matrix instructions whose operands are the
+// max(q8, 0) . high - max(-q8, 0) . low, two runs of 16 x 16 x 64 integer matrix instructions whose operands are the
 // bytes of the record as they lie.
 template <class E, int DP>
-__global__ __launch_bounds__(256) void fl_kv_score(const SelectArgs a) {
+__global__ __launch_bounds__(512) void fl_kv_score(const SelectArgs a) {
   warm_kernel_args(a);
   constexpr int KK = DP / 64;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
@@ -1377,7 +1400,7 @@ __global__ __launch_bounds__(256) void fl_kv_score(const SelectArgs a) {
   Item it;
   if (!find_item(a.s, T, blockIdx.y, [](uint32_t m, uint32_t) { return m; }, it)) return;
   const uint32_t b = it.b, i = it.local, first = it.first, n = it.n, lim = token_limit(a, it.len, n, i), pages = (lim + T - 1) / T;
-  const uint32_t subs = 4 / HW, step = a.parts * subs * 32;   // 32 pages to a wavefront at a time
+  const uint32_t subs = (blockDim.x >> 6) / HW, step = a.parts * subs * 32;   // 32 pages to a wavefront at a time
   uint32_t p0 = (part * subs + wave / HW) * 32;
   if (p0 >= pages) return;
   const uint64_t tok = first + i;
@@ -1444,14 +1467,14 @@ __global__ __launch_bounds__(256) void fl_kv_score(const SelectArgs a) {
     for (int k = 0; k < KK; ++k)
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        uint32_t pu = 0, pd = 0;
+        uint32_t pu = 0, pd = 0;   // positive ones, magnitudes of negative ones: the conversion to a byte cuts off below zero
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float f = (float)x[k][w >> 1][(4 * w + e) & 7];
           f = __builtin_isfinite(f) ? f : 0.f;
-          const int v = (int)rintf(f * inv);
-          pu |= (uint32_t)(v > 0 ? v : 0) << (8 * e);
-          pd |= (uint32_t)((v < 0 ? v : 0) & 0xff) << (8 * e);
+          f = rintf(f * inv);
+          pu = __builtin_amdgcn_cvt_pk_u8_f32(f, e, pu);
+          pd = __builtin_amdgcn_cvt_pk_u8_f32(-f, e, pd);
         }
         up[k][w] = (int)pu;
         dn[k][w] = (int)pd;
@@ -1473,12 +1496,13 @@ __global__ __launch_bounds__(256) void fl_kv_score(const SelectArgs a) {
       if (G > 16) in = queries(h0);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        i4 sum = {0, 0, 0, 0};
+        i4 sum = {0, 0, 0, 0}, less = {0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < KK; ++k) {
           sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(now.hi[t][k], up[k], sum, 0, 0, 0);
-          sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(now.lo[t][k], dn[k], sum, 0, 0, 0);
+          less = __builtin_amdgcn_mfma_i32_16x16x64_i8(now.lo[t][k], dn[k], less, 0, 0, 0);
         }
+        sum -= less;
 #pragma unroll
         for (int e = 0; e < 4; ++e) best[t][e] = in ? fmaxf(best[t][e], (float)sum[e] * scale) : best[t][e];   // row 4 g + e: a page; column c: a head
       }
@@ -1491,8 +1515,10 @@ __global__ __launch_bounds__(256) void fl_kv_score(const SelectArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float v = best[t][e];
-#pragma unroll
-        for (int o = 8; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+        v = larger(v, __uint_as_float(dpp_u32<0xb1>(__float_as_uint(v))));
+        v = larger(v, __uint_as_float(dpp_u32<0x4e>(__float_as_uint(v))));
+        v = larger(v, __uint_as_float(dpp_u32<0x141>(__float_as_uint(v))));
+        v = larger(v, __uint_as_float(dpp_u32<0x140>(__float_as_uint(v))));
         v *= __shfl(t ? ks1 : ks0, 4 * g + e);
         mine = c == 4 * t + e ? (v != v ? -kInf : v) : mine;
       }
@@ -1842,8 +1868,10 @@ void run_attend(const AttendArgs& a, const Plan& pl, hipStream_t st) {
     else FL_LAUNCH((fl_kv_join<E, false>), grid, dim3(256), 0, st, a, pl.tr);
   }
   if (a.w_out) {
-    const uint64_t span = (uint64_t)a.s.width * a.c.T > a.w_width ? (uint64_t)a.s.width * a.c.T : a.w_width;
-    const dim3 grid((uint32_t)((span + 255) / 256), a.c.H, a.s.n_seqs);
+    // as many workgroups as stay resident, or what there is to do
+    const uint64_t span = (uint64_t)a.s.width * a.c.T > a.w_width ? (uint64_t)a.s.width * a.c.T : a.w_width, rows = (uint64_t)a.s.n_seqs * a.c.H;
+    const uint64_t most = (span + 127) / 128, want = (1024 + rows - 1) / rows;
+    const dim3 grid((uint32_t)(want < most ? want : most), a.c.H, a.s.n_seqs);
     if (pl.dp == 64) FL_LAUNCH((fl_kv_weights<E, 64>), grid, dim3(256), 0, st, a);
     else if (pl.dp == 128) FL_LAUNCH((fl_kv_weights<E, 128>), grid, dim3(256), 0, st, a);
     else FL_LAUNCH((fl_kv_weights<E, 256>), grid, dim3(256), 0, st, a);
@@ -1996,18 +2024,20 @@ int flh_kv_select(const flh_kv_select_params* p, void* stream) {
   a.out = p->d_out;
   fl_prof().kid = 10;
   const hipStream_t st = (hipStream_t)stream;
-  // The wavefronts of a workgroup take up to four heads of the same pages, whose scales lie in one line (a head to a
-  // workgroup fetched that line once for each: 41 -> TBD us at 65536 pages of 8 heads).  As many workgroups as stay
-  // resident, or 128 pages each.
-  a.heads_wg = a.c.H >= 4 ? 4 : a.c.H >= 2 ? 2 : 1;
-  const uint64_t rows = (uint64_t)a.s.n_tokens * ((a.c.H + a.heads_wg - 1) / a.heads_wg);
-  const uint32_t per = 32 * (4 / a.heads_wg), want = (uint32_t)((1024 + rows - 1) / rows), most = (a.s.width + per - 1) / per;
+  // The wavefronts of a workgroup take up to eight heads of the same pages: the pages' translations and the line that
+  // holds their scales are then fetched by one compute unit (65536 pages of 8 heads: a head to a workgroup 41 us, four
+  // 31, eight TBD).  As many workgroups as stay resident, or 32 pages to a wavefront.
+  const uint32_t waves = a.c.H >= 8 ? 8 : 4;
+  a.heads_wg = a.c.H >= 8 ? 8 : a.c.H >= 4 ? 4 : a.c.H >= 2 ? 2 : 1;
+  const uint32_t groups = (a.c.H + a.heads_wg - 1) / a.heads_wg;
+  const uint64_t rows = (uint64_t)a.s.n_tokens * groups;
+  const uint32_t per = 32 * (waves / a.heads_wg), want = (uint32_t)((512 + rows - 1) / rows), most = (a.s.width + per - 1) / per;
   a.parts = want < most ? want : most;
-  const dim3 grid(a.parts * ((a.c.H + a.heads_wg - 1) / a.heads_wg), a.s.n_tokens);
+  const dim3 grid(a.parts * groups, a.s.n_tokens), block(64 * waves);
   const bool bf = p->type == FLH_KV_BF16;
-  if (a.c.D <= 64) { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 64>), grid, dim3(256), 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 64>), grid, dim3(256), 0, st, a); }
-  else if (a.c.D <= 128) { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 128>), grid, dim3(256), 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 128>), grid, dim3(256), 0, st, a); }
-  else { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 256>), grid, dim3(256), 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 256>), grid, dim3(256), 0, st, a); }
+  if (a.c.D <= 64) { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 64>), grid, block, 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 64>), grid, block, 0, st, a); }
+  else if (a.c.D <= 128) { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 128>), grid, block, 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 128>), grid, block, 0, st, a); }
+  else { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 256>), grid, block, 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 256>), grid, block, 0, st, a); }
   if (a.s.width <= 256 * kHeld) FL_LAUNCH((fl_kv_pick_pages<256, true>), dim3(a.s.n_tokens * a.c.H), dim3(256), 0, st, a);
   else if (a.s.width <= 1024 * kHeld) FL_LAUNCH((fl_kv_pick_pages<1024, true>), dim3(a.s.n_tokens * a.c.H), dim3(1024), 0, st, a);
   else FL_LAUNCH((fl_kv_pick_pages<1024, false>), dim3(a.s.n_tokens * a.c.H), dim3(1024), 0, st, a);
