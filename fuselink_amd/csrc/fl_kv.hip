@@ -1432,8 +1432,9 @@ __global__ __launch_bounds__(512) void fl_kv_score(const SelectArgs a) {
       if (!there) x.ks[t] = kNan;
     }
   };
-  int32_t pg[2];
+  int32_t pg[2], later[2];
   number(p0, pg);
+  number(p0 + step < pages ? p0 + step : p0, later);
 
   // the queries of up to 16 heads as 8-bit whole numbers, split by sign (more heads: one round for each 16)
   i4 up[KK], dn[KK];
@@ -1450,10 +1451,24 @@ __global__ __launch_bounds__(512) void fl_kv_score(const SelectArgs a) {
 #pragma unroll
     for (int k = 0; k < KK; ++k)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float v = (float)x[k][e >> 3][e & 7];
-        amax = fmaxf(amax, __builtin_isfinite(v) ? fabsf(v) : 0.f);
-      }
+      for (int e = 0; e < 16; ++e) amax = larger(amax, fabsf((float)x[k][e >> 3][e & 7]));
+    bool odd = !(amax < kInf);   // (a NaN alone gives way to the numbers: it is looked for below)
+#pragma unroll
+    for (int k = 0; k < KK; ++k)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) odd |= x[k][e >> 3][e & 7] != x[k][e >> 3][e & 7];
+    if (__ballot(odd)) {         // what is not finite counts as 0
+      asm volatile("");
+      amax = 0.f;
+#pragma unroll
+      for (int k = 0; k < KK; ++k)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float v = (float)x[k][e >> 3][e & 7];
+          if (!__builtin_isfinite(v)) x[k][e >> 3][e & 7] = (E)0.f;
+          else amax = larger(amax, fabsf(v));
+        }
+    }
     amax = column_max(amax);
     scale = 0.f;   // smallest 2^e >= amax / 127, 127 = 1.984375 * 2^6
     if (amax > 0.f) {
@@ -1471,7 +1486,6 @@ __global__ __launch_bounds__(512) void fl_kv_score(const SelectArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float f = (float)x[k][w >> 1][(4 * w + e) & 7];
-          f = __builtin_isfinite(f) ? f : 0.f;
           f = rintf(f * inv);
           pu = __builtin_amdgcn_cvt_pk_u8_f32(f, e, pu);
           pd = __builtin_amdgcn_cvt_pk_u8_f32(-f, e, pd);
@@ -1486,7 +1500,9 @@ __global__ __launch_bounds__(512) void fl_kv_score(const SelectArgs a) {
   fetch(pg, now);
   bool in = queries(0);
   for (; p0 < pages; p0 += step) {
-    number(p0 + step < pages ? p0 + step : p0, pg);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) pg[t] = later[t];
+    number(p0 + 2 * step < pages ? p0 + 2 * step : p0, later);
     float best[2][4];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -1569,12 +1585,12 @@ template <int NT, bool ONE, class Key>
 __device__ Pick kth_largest(uint32_t n, uint32_t k, Key key, PickShared<NT, ONE>& sh) {
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   uint32_t lo = 0xffffffffu, hi = 0, forced = 0;
-  for (uint32_t base = tid; base < n; base += 8 * NT) {   // eight loads at a time, none behind a branch
-    uint32_t u[8];
+  for (uint32_t base = tid; base < n; base += 4 * NT) {   // four loads at a time, none behind a branch
+    uint32_t u[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) u[e] = key(base + e * NT < n ? base + e * NT : n - 1);
+    for (int e = 0; e < 4; ++e) u[e] = key(base + e * NT < n ? base + e * NT : n - 1);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < 4; ++e) {
       const bool in = base + e * NT < n, all = u[e] == 0xffffffffu;
       if (ONE && in) sh.keys[base + e * NT] = u[e];
       forced += in && all ? 1 : 0;
@@ -1601,12 +1617,12 @@ __device__ Pick kth_largest(uint32_t n, uint32_t k, Key key, PickShared<NT, ONE>
     const int bits = 32 - __builtin_clz(hi - lo), shift = bits > 11 ? bits - 11 : 0;
     for (uint32_t i = tid; i < 2048; i += NT) sh.hist[i] = 0;
     __syncthreads();
-    for (uint32_t base = tid; base < n; base += 8 * NT) {
-      uint32_t u[8];
+    for (uint32_t base = tid; base < n; base += 4 * NT) {
+      uint32_t u[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) u[e] = held(base + e * NT < n ? base + e * NT : n - 1);
+      for (int e = 0; e < 4; ++e) u[e] = held(base + e * NT < n ? base + e * NT : n - 1);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
+      for (int e = 0; e < 4; ++e)
         if (base + e * NT < n && u[e] >= lo && u[e] <= hi) atomicAdd(&sh.hist[(u[e] - lo) >> shift], 1u);
     }
     __syncthreads();
@@ -1646,7 +1662,7 @@ __device__ void put_picked(uint32_t n, Pick pick, Key key, Along along, Put put,
   const auto held = [&](uint32_t i) { return ONE ? sh.keys[i < n ? i : n - 1] : key(i < n ? i : n - 1); };
   uint32_t above = 0, equal = 0;
   __syncthreads();
-#pragma unroll 2
+#pragma unroll 1
   for (uint32_t i = i0; i < i1; i += 64) {
     const uint32_t u = held(i + lane);
     above += (uint32_t)__popcll(__ballot(i + lane < i1 && u > pick.key));
@@ -1658,17 +1674,17 @@ __device__ void put_picked(uint32_t n, Pick pick, Key key, Along along, Put put,
   above = bcast_lane_u32(sa, (int)wave) - above;
   equal = bcast_lane_u32(se, (int)wave) - equal;
   const uint64_t below = (1ull << lane) - 1;
-  for (uint32_t base = i0; base < i1; base += 256) {
-    uint32_t u[4];
-    float with[4];
+  for (uint32_t base = i0; base < i1; base += 128) {
+    uint32_t u[2];
+    float with[2];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 2; ++e) {
       const uint32_t i = base + 64 * e + lane;
       with[e] = along(i < i1 ? i : i1 - 1);
       u[e] = held(i);
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 2; ++e) {
       const uint32_t i = base + 64 * e + lane;
       const bool in = i < i1, gt = in && u[e] > pick.key, eq = in && u[e] == pick.key;
       const uint64_t bg = __ballot(gt), be = __ballot(eq);
@@ -2026,12 +2042,12 @@ int flh_kv_select(const flh_kv_select_params* p, void* stream) {
   const hipStream_t st = (hipStream_t)stream;
   // The wavefronts of a workgroup take up to eight heads of the same pages: the pages' translations and the line that
   // holds their scales are then fetched by one compute unit (65536 pages of 8 heads: a head to a workgroup 41 us, four
-  // 31, eight TBD).  As many workgroups as stay resident, or 32 pages to a wavefront.
+  // 31, eight 29).  As many workgroups as stay resident, or 32 pages to a wavefront.
   const uint32_t waves = a.c.H >= 8 ? 8 : 4;
   a.heads_wg = a.c.H >= 8 ? 8 : a.c.H >= 4 ? 4 : a.c.H >= 2 ? 2 : 1;
   const uint32_t groups = (a.c.H + a.heads_wg - 1) / a.heads_wg;
   const uint64_t rows = (uint64_t)a.s.n_tokens * groups;
-  const uint32_t per = 32 * (waves / a.heads_wg), want = (uint32_t)((512 + rows - 1) / rows), most = (a.s.width + per - 1) / per;
+  const uint32_t per = 32 * (waves / a.heads_wg), want = (uint32_t)((256 + rows - 1) / rows), most = (a.s.width + per - 1) / per;
   a.parts = want < most ? want : most;
   const dim3 grid(a.parts * groups, a.s.n_tokens), block(64 * waves);
   const bool bf = p->type == FLH_KV_BF16;

@@ -249,6 +249,8 @@ ATTEND = [  # T, H, G, D, lens, query tokens
     (16, 2, 40, 64, [70], [1]), (16, 1, 2, 16, [40], [3]), (16, 1, 2, 48, [600, 33], [1, 1]), (16, 2, 4, 128, [50, 20, 7], [5, 20, 7]),
     (32, 1, 4, 128, [90, 33], [33, 16]), (16, 1, 3, 64, [150, 40], [70, 40]), (16, 1, 1, 112, [200], [130]), (64, 1, 2, 256, [100, 64], [50, 64]),
     (128, 2, 1, 144, [129], [100]), (16, 1, 4, 128, [3, 10], [9, 10]), (16, 1, 1, 128, [2100], [1]),
+    (16, 1, 2, 64, [9000], [1]), (16, 1, 2, 128, list(range(0, 70)), [1] * 70), (16, 1, 4, 64, [(37 * i) % 90 for i in range(70)], [(5 * i) % 11 for i in range(70)]),
+    (32, 1, 2, 80, [700, 40], [90, 40]), (16, 1, 8, 128, [1100], [40]),
 ]
 
 
@@ -266,14 +268,16 @@ def test_attend_weights(fl, case):
     run_attend(fl, T, H, G, D, lens, news, "bf16", weights=True)
 
 
-def test_attend_nan_is_seen_by_those_who_may(fl):
+@pytest.mark.parametrize("n", [3, 5, 20])
+def test_attend_nan_is_seen_by_those_who_may(fl, n):
     """A NaN among the values reaches exactly the queries that see its token; one among the keys likewise, whole rows."""
     core, kv, torch = fl
-    T, H, G, D, x, n = 16, 2, 4, 64, 40, 20
+    T, H, G, D, x = 16, 2, 4, 64, 40
     rng = np.random.default_rng(3)
     for side in (1, 0):
         cache, c, table = make(fl, rng, [x], T, H, D)
-        at = x - 9
+        late = min(9, n - 1)               # the last `late` queries see the token
+        at = x - late
         raw = cache.pages
         off = side * H * T * D + (1 * T + at % T) * D + 5
         raw[int(table[0, at // T]), off] = 0x7f
@@ -287,9 +291,9 @@ def test_attend_nan_is_seen_by_those_who_may(fl):
         o = out.cpu().double().numpy()
         nan = np.zeros(o.shape, bool)
         if side:
-            nan[n - 9:, G:, 5] = True
+            nan[n - late:, G:, 5] = True
         else:
-            nan[n - 9:, G:, :] = True
+            nan[n - late:, G:, :] = True
         np.testing.assert_array_equal(np.isnan(o), nan)
         tol = ref.out_tolerance(r, torch.finfo(torch.bfloat16).eps, x)
         assert (np.abs(o - r["out"])[~nan] <= tol[~nan]).all()
@@ -342,6 +346,38 @@ def test_attend_strided_and_uniform(fl):
         r = ref.attend(c, q.cpu().double().numpy(), table, lens, [0, 2, 4, 6], 1 / np.sqrt(D))
         check_out(torch, out, None, r, torch.float16, lens, [0, 2, 4, 6])
         assert (res[:, :, :shift] == 7).all() and (res[:, :, shift + D:] == 7).all()
+
+
+def test_pool_past_four_gigabytes(fl):
+    """Pages at the far end of a pool of 4.5 GiB: store, attention, the choice of pages and eviction."""
+    core, kv, torch = fl
+    T, H, G, D, x = 16, 8, 2, 128, 150
+    pb = kv.page_bytes(T, H, D)
+    n = (9 << 29) // pb
+    cache = kv.PageCache(torch.empty(n, pb, dtype=torch.uint8, device="cuda"), T, H, D)
+    rng = np.random.default_rng(8)
+    table = np.array([list(range(n - 1, n - 6, -1)) + list(range(5))], np.int32)
+    k, v = (dev(torch, rng.standard_normal((x, H, D)), torch.float32) for _ in range(2))
+    status, lens = core.new_status(), dev(torch, np.array([x], np.int32))
+    kv.store(cache, k, v, dev(torch, table), torch.zeros_like(lens), status)
+    c = ref.empty(10, T, H, D)
+    small = np.arange(10, dtype=np.int32)[None]
+    ref.store(c, k.cpu().double().numpy(), v.cpu().double().numpy(), small, [0], [0, x])
+    got = ref.unpack(cache.pages[dev(torch, table[0]).long()].cpu().numpy(), T, H, D)
+    same_cache(got, c)
+    q = dev(torch, rng.standard_normal((1, H * G, D)), torch.float32).to(torch.bfloat16)
+    out = kv.attend(cache, q, dev(torch, table), lens, status)
+    check_out(torch, out, None, ref.attend(c, q.cpu().double().numpy(), small, [x], [0, 1], 1 / np.sqrt(D)), torch.bfloat16, [x], [0, 1])
+    sel = kv.select_pages(cache, q, dev(torch, table), lens, 4, status)
+    np.testing.assert_array_equal(sel.cpu().numpy(), ref.select(c, q.cpu().double().numpy(), small, [x], [0, 1], 4, 1, 1))
+    w = dev(torch, rng.random((1, H, x)).astype(np.float32))
+    to_table = np.array([[n // 2, n - 7, n - 9]], np.int32)
+    kept, _, _ = kv.evict(cache, dev(torch, table), lens, w, 40, cache, dev(torch, to_table), status)
+    exp = ref.empty(3, T, H, D)
+    k_exp, _ = ref.evict(c, small, [x], w.cpu().numpy(), 40, 0, 0, exp, np.arange(3)[None])
+    np.testing.assert_array_equal(kept.cpu().numpy(), k_exp)
+    same_cache(ref.unpack(cache.pages[dev(torch, to_table[0]).long()].cpu().numpy(), T, H, D), exp)
+    assert int(status) == 0
 
 
 # ---- selected pages -------------------------------------------------------------------------------------------------
@@ -402,10 +438,26 @@ def test_select_ties_and_odd_queries(fl):
         assert int(status) == 0
 
 
+def test_select_among_very_many(fl):
+    """More pages than a workgroup keeps keys of, few of them different."""
+    core, kv, torch = fl
+    T, H, G, D, n = 16, 1, 1, 32, 17001
+    rng = np.random.default_rng(1)
+    cache, c, table = make(fl, rng, [16 * 40], T, H, D)
+    table = table[:, rng.integers(0, 40, n)].astype(np.int32)
+    q = dev(torch, rng.standard_normal((1, H * G, D)), torch.float32).to(torch.bfloat16)
+    status = core.new_status()
+    for count in (100, 1000, 16999):
+        got = kv.select_pages(cache, q, dev(torch, table), dev(torch, np.array([16 * n - 3], np.int32)), count, status, first=3, last=7)
+        np.testing.assert_array_equal(got.cpu().numpy(), ref.select(c, q.cpu().double().numpy(), table, [16 * n - 3], [0, 1], count, 3, 7))
+    assert int(status) == 0
+
+
 # ---- eviction -------------------------------------------------------------------------------------------------------
 EVICT = [  # T, T of the new pages, H, D, lens, budget, first, recent
     (16, 16, 2, 64, [100, 40, 41], 40, 4, 8), (16, 32, 1, 80, [300, 0, 1], 33, 0, 0), (32, 16, 3, 128, [200], 100, 0, 100), (256, 48, 1, 256, [700], 300, 2, 5),
     (16, 16, 1, 16, [2500, 1100], 1029, 1, 28), (16, 256, 2, 128, [600, 16], 1, 0, 1), (48, 16, 1, 96, [50], 64, 64, 0), (16, 128, 1, 256, [9000], 260, 3, 3),
+    (64, 64, 1, 16, [17000, 16384, 16385], 5000, 2, 9), (16, 16, 1, 16, [(i * 13) % 80 for i in range(70)], 30, 1, 2),
 ]
 
 
