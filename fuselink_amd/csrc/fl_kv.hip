@@ -305,18 +305,22 @@ __device__ __forceinline__ h2 column_pair(h2 v, F f) {
   return f(__builtin_bit_cast(h2, (uint32_t)r[0]), __builtin_bit_cast(h2, (uint32_t)r[1]));
 }
 
-// One wavefront packs K and V of one head of one page.  A lane holds 8 neighbouring channels of every RP-th token
+// W wavefronts pack K and V of one head of one page.  A lane holds 8 neighbouring channels of every RP-th token
 // (RP = 64 / (D / 8) tokens at a time), so both the codes' rows and the channels' bounds come out of registers.  The
-// largest magnitude of the new tokens fixes the scale, then the same rows become codes.  Up to ROWS rows a lane stay in
-// registers between the two, as they were loaded; longer blocks are read twice, the second time from cache.  In evict the rows
-// are codes of other records under their own scales.
-template <class E, bool EVICT, int ROWS, bool ONE>
-__global__ __launch_bounds__(256) void fl_kv_pack(const PackArgs a) {
+// largest magnitude of the new tokens fixes the scale, then the same rows become codes: every row is read once and stays
+// in registers between the two, as it was loaded, ROWS of them a lane.  More than one wavefront exchange their largest
+// magnitude and their bounds through shared memory.  In evict the rows are codes of other records under their own scales.
+template <class E, bool EVICT, int ROWS, int W>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fl_kv_pack(const PackArgs a) {
   warm_kernel_args(a);
   typedef typename std::conditional<EVICT, Code, Raw<E>>::type Row;
+  constexpr bool kBoth = sizeof(Row) * ROWS * 2 <= (W == 16 ? 256 : 512);   // rows of K and of V fit the registers together
+  __shared__ float part_max[2][W];
+  __shared__ h2 part_low[W][32][4], part_high[W][32][4];
   const int lane = threadIdx.x & 63;
   const Cache& c = a.c;
-  const uint32_t h = blockIdx.y * 4 + uniform(threadIdx.x >> 6);
+  const uint32_t wave = uniform(threadIdx.x >> 6), part = W == 1 ? 0 : wave;
+  const uint32_t h = W == 1 ? blockIdx.y * 4 + wave : blockIdx.y;
   if (h >= c.H) return;
   const uint32_t T = c.T, D = c.D;
   uint32_t b, j, first = 0, n, held;
@@ -349,14 +353,13 @@ __global__ __launch_bounds__(256) void fl_kv_pack(const PackArgs a) {
 
   const uint32_t CG = D >> 3, RP = 64 / CG, grp = (uint32_t)lane / CG, cg = (uint32_t)lane - grp * CG;
   const bool on = grp < RP;
-  const uint32_t passes = (T + RP - 1) / RP;
 
-  // Rows (p0 + i) * RP + grp: new tokens (evict: all of them), 0 elsewhere.  sides: 1 K, 2 V, 3 both
+  // Rows (i * W + part) * RP + grp: new tokens (evict: all of them), 0 elsewhere.  sides: 1 K, 2 V, 3 both
   Row x[2][ROWS];
-  const auto load = [&](uint32_t p0, const int sides) {
+  const auto load = [&](const int sides) {
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-      const uint32_t r = (p0 + i) * RP + grp;
+      const uint32_t r = (i * W + part) * RP + grp;
 #pragma unroll
       for (int side = 0; side < 2; ++side)
         if (sides >> side & 1) x[side][i] = Row{};
@@ -387,62 +390,57 @@ __global__ __launch_bounds__(256) void fl_kv_pack(const PackArgs a) {
     float* scale_at = reinterpret_cast<float*>(rec + c.scales) + 2 * h + side;
     const float s_old = !EVICT && old ? *scale_at : 0.f;
     float amax = 0.f;
+    if (!kBoth) load(1 << side);
     if constexpr (EVICT) {
-      for (uint32_t p0 = 0; p0 < passes; p0 += ROWS) {
-        if (!ONE) load(p0, 1 << side);
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) amax = fmaxf(amax, amax_of(x[side][i]));
-      }
+      for (int i = 0; i < ROWS; ++i) amax = fmaxf(amax, amax_of(x[side][i]));
     } else {
       uint32_t bits = 0;
-      for (uint32_t p0 = 0; p0 < passes; p0 += ROWS) {
-        if (!ONE) load(p0, 1 << side);
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) max_bits<E>(bits, x[side][i]);
-      }
+      for (int i = 0; i < ROWS; ++i) max_bits<E>(bits, x[side][i]);
       amax = max_of_bits<E>(bits);
       if (__ballot(!(amax < kInf))) {
         amax = 0.f;
-        for (uint32_t p0 = 0; p0 < passes; p0 += ROWS) {
-          if (!ONE) load(p0, 1 << side);
 #pragma unroll
-          for (int i = 0; i < ROWS; ++i) amax = fmaxf(amax, finite_amax<E>(x[side][i]));
-        }
+        for (int i = 0; i < ROWS; ++i) amax = fmaxf(amax, finite_amax<E>(x[side][i]));
       }
     }
-    const float s = fmaxf(s_old, block_scale(wave_max_f32(amax)));
+    amax = wave_max_f32(amax);
+    if constexpr (W > 1) {
+      if (lane == 0) part_max[side][part] = amax;
+      __syncthreads();
+      amax = wave_max_f32(part_max[side][lane & (W - 1)]);
+    }
+    const float s = fmaxf(s_old, block_scale(amax));
     const bool grown = old && s != s_old;
     h2 lo[4], hi[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) { lo[e] = h2{(_Float16)kInf, (_Float16)kInf}; hi[e] = -lo[e]; }
     uint8_t* codes = rec + side * c.side + (uint64_t)h * T * D;
-    for (uint32_t p0 = 0; p0 < passes; p0 += ROWS) {
-      if (!ONE) load(p0, 1 << side);
 #pragma unroll
-      for (int i = 0; i < ROWS; ++i) {
-        const uint32_t r = (p0 + i) * RP + grp;
-        if (!on || r >= T) continue;
-        u2* row = reinterpret_cast<u2*>(codes + r * D + cg * 8);
-        u2 w;
-        if (r < old) {
-          if (side == 1 && !grown) continue;
-          w = *row;
-          if (grown) { const uint32_t t[2] = {w[0], w[1]}; w = recode(t, s_old, s); }
-        } else {
-          w = encode(x[side][i], s);
-        }
-        if (r < old ? grown : (r < fill || !old)) *row = w;   // slots behind the tokens of a page that this call opens are zero
-        if (side == 0 && r < fill) {
+    for (int i = 0; i < ROWS; ++i) {
+      const uint32_t r = (i * W + part) * RP + grp;
+      if (!on || r >= T) continue;
+      u2* row = reinterpret_cast<u2*>(codes + r * D + cg * 8);
+      u2 w;
+      if (r < old) {
+        if (side == 1 && !grown) continue;
+        w = *row;
+        if (grown) { const uint32_t t[2] = {w[0], w[1]}; w = recode(t, s_old, s); }
+      } else {
+        w = encode(x[side][i], s);
+      }
+      if (r < old ? grown : (r < fill || !old)) *row = w;   // slots behind the tokens of a page that this call opens are zero
+      if (side == 0 && r < fill) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const h2 v = e & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[e >> 1], 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[e >> 1], 1.f, false);
-            lo[e] = least(lo[e], v);
-            hi[e] = most(hi[e], v);
-          }
+        for (int e = 0; e < 4; ++e) {
+          const h2 v = e & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[e >> 1], 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[e >> 1], 1.f, false);
+          lo[e] = least(lo[e], v);
+          hi[e] = most(hi[e], v);
         }
       }
     }
-    if (lane == 0) *scale_at = s;
+    if (lane == 0 && part == 0) *scale_at = s;
     if (side == 1) return;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -457,7 +455,18 @@ __global__ __launch_bounds__(256) void fl_kv_pack(const PackArgs a) {
         }
       }
     }
-    if (lane < (int)CG) {
+    if constexpr (W > 1) {
+      if (lane < (int)CG)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { part_low[part][lane][e] = lo[e]; part_high[part][lane][e] = hi[e]; }
+      __syncthreads();
+      if (part == 0 && lane < (int)CG)
+#pragma unroll 3
+        for (int k = 1; k < W; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { lo[e] = least(lo[e], part_low[k][lane][e]); hi[e] = most(hi[e], part_high[k][lane][e]); }
+    }
+    if (part == 0 && lane < (int)CG) {
       u2 wl = {0, 0}, wh = {0, 0};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -471,7 +480,7 @@ __global__ __launch_bounds__(256) void fl_kv_pack(const PackArgs a) {
     }
   };
 
-  if (ONE) load(0, 3);
+  if (kBoth) load(3);
   pack(0);
   pack(1);
 }
@@ -1894,14 +1903,20 @@ void run_attend(const AttendArgs& a, const Plan& pl, hipStream_t st) {
   }
 }
 
-// Rows of a page that stay in a lane's registers: 4 or 8 (pages of 16 and 32 tokens of 128 channels), else the page is read twice.
+// As many wavefronts to a head of a page as keep its rows in registers, 8 of them a lane at most.  (One wavefront that
+// reads longer blocks twice, four rows at a time, against four: 29 sequences of 1634 tokens, 12 heads of 256 channels,
+// evicted into pages of 32 tokens 235 us, 123; 33 of up to 4140, 8 heads of 128, stored in pages of 64 146 us, 117; against
+// sixteen, pages of 256 193 us, 147.  Eight wavefronts with four rows a lane each in place of four with eight: the same.)
 template <class E, bool EVICT>
 void launch_pack(const PackArgs& a, uint32_t items, hipStream_t st) {
-  const uint32_t rp = 64 / (a.c.D / 8), rows = (a.c.T + rp - 1) / rp;
-  const dim3 grid(items, (a.c.H + 3) / 4);
-  if (rows <= 4) FL_LAUNCH((fl_kv_pack<E, EVICT, 4, true>), grid, dim3(256), 0, st, a);
-  else if (rows <= 8) FL_LAUNCH((fl_kv_pack<E, EVICT, 8, true>), grid, dim3(256), 0, st, a);
-  else FL_LAUNCH((fl_kv_pack<E, EVICT, 4, false>), grid, dim3(256), 0, st, a);
+  const uint32_t rp = 64 / (a.c.D / 8), rows = (a.c.T + rp - 1) / rp;   // 128 at most
+  const dim3 heads4(items, (a.c.H + 3) / 4), heads(items, a.c.H);
+  if (rows <= 4) FL_LAUNCH((fl_kv_pack<E, EVICT, 4, 1>), heads4, dim3(256), 0, st, a);
+  else if (rows <= 8) FL_LAUNCH((fl_kv_pack<E, EVICT, 8, 1>), heads4, dim3(256), 0, st, a);
+  else if (rows <= 16) FL_LAUNCH((fl_kv_pack<E, EVICT, 4, 4>), heads, dim3(256), 0, st, a);
+  else if (rows <= 32) FL_LAUNCH((fl_kv_pack<E, EVICT, 8, 4>), heads, dim3(256), 0, st, a);
+  else if (rows <= 64) FL_LAUNCH((fl_kv_pack<E, EVICT, 4, 16>), heads, dim3(1024), 0, st, a);
+  else FL_LAUNCH((fl_kv_pack<E, EVICT, 8, 16>), heads, dim3(1024), 0, st, a);
 }
 
 }  // namespace

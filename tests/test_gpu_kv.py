@@ -126,10 +126,11 @@ def test_store(fl, case, kind):
     same_cache(held(cache, T, H, D), exp)
 
 
-def test_store_values_at_the_edges(fl):
+@pytest.mark.parametrize("tokens,dim", [(16, 32), (64, 32), (16, 256), (64, 128), (128, 144), (128, 256)])
+def test_store_values_at_the_edges(fl, tokens, dim):
     """Blocks of zeros, numbers that are not finite, the largest and smallest of a type, magnitudes at 448 * 2^e."""
     core, kv, torch = fl
-    T, H, D = 16, 2, 32
+    T, H, D = tokens, 2, dim
     n = 16 * 8
     x = np.zeros((n, H, D))
     rng = np.random.default_rng(0)
@@ -457,6 +458,7 @@ def test_select_among_very_many(fl):
 EVICT = [  # T, T of the new pages, H, D, lens, budget, first, recent
     (16, 16, 2, 64, [100, 40, 41], 40, 4, 8), (16, 32, 1, 80, [300, 0, 1], 33, 0, 0), (32, 16, 3, 128, [200], 100, 0, 100), (256, 48, 1, 256, [700], 300, 2, 5),
     (16, 16, 1, 16, [2500, 1100], 1029, 1, 28), (16, 256, 2, 128, [600, 16], 1, 0, 1), (48, 16, 1, 96, [50], 64, 64, 0), (16, 128, 1, 256, [9000], 260, 3, 3),
+    (16, 64, 3, 128, [500, 70], 150, 4, 8), (32, 256, 1, 256, [700, 40], 520, 1, 9),
     (64, 64, 1, 16, [17000, 16384, 16385], 5000, 2, 9), (16, 16, 1, 16, [(i * 13) % 80 for i in range(70)], 30, 1, 2),
 ]
 
