@@ -2091,7 +2091,7 @@ int flh_kv_evict(const flh_kv_evict_params* p, void* stream) {
   if (p->to_table_width < per || p->to_table_stride < p->to_table_width)
     return fl_set_error(FLH_E_ARG, "flh_kv_evict: %u tokens need %u pages, the new table has %u", p->budget, per, p->to_table_width);
   if (p->weights_width == 0 || p->new_weights_width < p->budget) return fl_set_error(FLH_E_ARG, "flh_kv_evict: weights of %u positions, new ones of %u", p->weights_width, p->new_weights_width);
-  if ((uint64_t)per * a.s.n_seqs > kMaxGroups || (uint64_t)a.s.n_seqs * a.c.H > kMaxGroups / 4) return fl_set_error(FLH_E_ARG, "flh_kv_evict: too much for one launch");
+  if ((uint64_t)per * a.s.n_seqs > kMaxGroups / 4 || (uint64_t)a.s.n_seqs * a.c.H > kMaxGroups / 4) return fl_set_error(FLH_E_ARG, "flh_kv_evict: too much for one launch");
   if ((rc = fl_need_init())) return rc;
   KeepArgs k;
   memset(&k, 0, sizeof(k));

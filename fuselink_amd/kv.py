@@ -3,8 +3,9 @@ record of a page and every operator's definition).  The pages are ordinary pool 
 core.scatter_pages, so a cache filled on one node moves and is read on another as it is.
 
 Every call launches on `stream` (default: the current stream of the tensors' device) and returns at once; what it
-allocates -- results that were not given, workspaces -- comes from that stream's pool.  Tensors that belong to another
-stream are marked as used on this one.  What is wrong with device-resident page numbers, lengths and starts shows as
+allocates -- results that were not given, workspaces -- comes from that stream's pool.  A call that names a stream marks the
+tensors given as used on it.  A workspace that is given belongs to one call at a time: calls on two streams, or two
+graphs that may run at once, need one each.  What is wrong with device-resident page numbers, lengths and starts shows as
 FLH_E_RANGE in `status` (core.new_status())."""
 from __future__ import annotations
 
@@ -92,6 +93,21 @@ def _check(cache: PageCache, name: str, t: torch.Tensor, dtype, dims: int):
 def _check_written(name: str, t: torch.Tensor) -> None:
     if any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
         raise ValueError(f"{name}: written, but some of its elements share memory")
+
+
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """No element of one is an element of the other: their extents are disjoint, or rows a common stride apart lie between each other."""
+    if a.numel() == 0 or b.numel() == 0:
+        return True
+    inner = [t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape[1:], t.stride()[1:]))) for t in (a, b)]
+    pa, pb = a.data_ptr(), b.data_ptr()
+    row = a.stride(0) * a.element_size()
+    if pa + (a.shape[0] - 1) * row + inner[0] <= pb or pb + (b.shape[0] - 1) * b.stride(0) * b.element_size() + inner[1] <= pa:
+        return True
+    if row == 0 or row != b.stride(0) * b.element_size():
+        return False
+    d = (pb - pa) % row
+    return d >= inner[0] and row - d >= inner[1]
 
 
 def _seqs(cache: PageCache, table, lens, status, starts, n_tokens: int):
@@ -232,6 +248,7 @@ def attend(cache: PageCache, q: torch.Tensor, page_table: torch.Tensor, lens: to
             shape, (wis, wih, _) = _check(cache, "weights_in", weights_in, _F32, 3)
             _need(shape == weights.shape, f"weights_in: [{n_seqs}, {heads}, {width}]")
             win_p = weights_in.data_ptr()
+            _need((win_p == w_p and (wis, wih) == (ws, wh)) or _apart(weights, weights_in), "weights and weights_in overlap without being the same")
     else:
         _need(weights_in is None, "weights_in without weights")
     lib = _lib.load()
@@ -242,12 +259,15 @@ def attend(cache: PageCache, q: torch.Tensor, page_table: torch.Tensor, lens: to
             _check(cache, "out", out, q.dtype, 3)
             _check_written("out", out)
             _need(out.shape == q.shape, f"out {tuple(out.shape)} for q {tuple(q.shape)}")
+            _need(_apart(out, q), "out overlaps q")
         ot, oh, _ = out.stride()
         head = (*cache.c, *seqs, q.data_ptr(), out.data_ptr(), qt, qh, ot, oh, lse_p, kind, hq,
                 1.0 / math.sqrt(cache.dim) if scale is None else scale, 1 if causal else 0, sel_p, win_p, w_p, wis, wih, ws, wh, count, width)
         sizes = (cache.c[3:], seqs[4:7], seqs[0] != 0, hq, count, w_p != 0)
         need = _needs.get(sizes)
         if need is None:
+            if len(_needs) >= 4096:
+                _needs.clear()
             need = _needs[sizes] = check(lib.flh_kv_attend_workspace_bytes(_ATTEND.pack(*head, 0, 0, word)))
         wp, wb, owner = _workspace(cache, workspace, need)
         check(lib.flh_kv_attend(_ATTEND.pack(*head, wp, wb, word), sp))
@@ -307,6 +327,7 @@ def evict(cache: PageCache, page_table: torch.Tensor, lens: torch.Tensor, weight
             (nb, nhh, nw), (ns, nh, _) = _check(cache, "new_weights", new_weights, _F32, 3)
             _check_written("new_weights", new_weights)
             _need(nb == b and nhh == h and nw >= budget, f"new_weights: [{b}, {h}, >= {budget}]")
+            _need(_apart(new_weights, weights), "new_weights overlaps weights")
         if new_lens is None:
             new_lens = torch.empty(b, dtype=_I32, device=cache.device)
         else:

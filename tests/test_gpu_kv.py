@@ -142,7 +142,8 @@ def test_store_values_at_the_edges(fl, tokens, dim):
     x[80:96] = rng.uniform(-1, 1, (16, H, D)); x[80, 0, 0], x[81, 1, 1] = np.nextafter(np.float32(448), np.float32(500)), np.nextafter(np.float32(1.75), np.float32(2))
     x[96:112] = np.nan
     x[112:128] = rng.standard_normal((16, H, D)) * np.exp(8 * rng.standard_normal((16, H, D)))
-    x = x.astype(np.float32)
+    with np.errstate(over="ignore"):        # what passes the largest number becomes an infinity, one more value to test
+        x = x.astype(np.float32)
     cache = kv.PageCache(torch.full((9, kv.page_bytes(T, H, D)), 0xA5, dtype=torch.uint8, device="cuda"), T, H, D)
     table = np.array([[7, 3, 1, 0, 8, 2, 5, 4]], np.int32)
     exp = held(cache, T, H, D)
@@ -347,6 +348,54 @@ def test_attend_strided_and_uniform(fl):
         r = ref.attend(c, q.cpu().double().numpy(), table, lens, [0, 2, 4, 6], 1 / np.sqrt(D))
         check_out(torch, out, None, r, torch.float16, lens, [0, 2, 4, 6])
         assert (res[:, :, :shift] == 7).all() and (res[:, :, shift + D:] == 7).all()
+
+
+@pytest.mark.parametrize("n,x", [(1, 50), (1, 5000), (3, 50), (40, 90), (40, 1500)])
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+def test_attend_queries_that_are_not_finite(fl, n, x, kind):
+    """A NaN or an infinity in a query makes its own row NaN -- with keys of both signs an infinite channel gives an
+    infinite largest score -- and touches no other row."""
+    core, kv, torch = fl
+    T, H, G, D = 16, 2, 4, 128
+    rng = np.random.default_rng(n + x)
+    cache, c, table = make(fl, rng, [x], T, H, D)
+    q = dev(torch, rng.standard_normal((n, H * G, D)), torch.float32).to({"bf16": torch.bfloat16, "fp16": torch.float16}[kind])
+    bad = np.zeros((n, H * G), bool)
+    for i, (t, h, value) in enumerate([(0, 1, np.nan), (n // 2, 2, np.inf), (n - 1, 6, -np.inf)]):
+        q[t, h, 17 * i + 3] = value
+        bad[t, h] = True
+    status, lse = core.new_status(), torch.zeros(n, H * G, device="cuda")
+    out = kv.attend(cache, q, dev(torch, table), dev(torch, np.array([x], np.int32)), status, lse=lse)
+    r = ref.attend(c, np.where(bad[:, :, None], 0, q.cpu().double().numpy()), table, [x], [0, n], 1 / np.sqrt(D))
+    o, s = out.cpu().double().numpy(), lse.cpu().double().numpy()
+    assert int(status) == 0 and np.isnan(o[bad]).all() and np.isnan(s[bad]).all()
+    assert (np.abs(o - r["out"]) <= ref.out_tolerance(r, torch.finfo(out.dtype).eps, x))[~bad].all()
+
+
+def test_views_that_overlap(fl):
+    """What a call writes may lie between what it reads, but not on it."""
+    core, kv, torch = fl
+    T, H, G, D, x = 16, 2, 4, 64, 40
+    rng = np.random.default_rng(2)
+    cache, c, table = make(fl, rng, [x, x], T, H, D)
+    wide = dev(torch, rng.standard_normal((2, 2 * H * G * D)), torch.float32).to(torch.bfloat16)
+    q, between = (wide[:, i * H * G * D:(i + 1) * H * G * D].unflatten(1, (H * G, D)) for i in (0, 1))
+    args = dev(torch, table), dev(torch, np.array([x, x], np.int32)), core.new_status()
+    exp = kv.attend(cache, q, *args)
+    for out in (q, wide[:, D:D + H * G * D].unflatten(1, (H * G, D)), wide.view(-1)[8:8 + 2 * H * G * D].view(2, H * G, D)):
+        with pytest.raises(ValueError, match="overlaps q"):
+            kv.attend(cache, q, *args, out=out)
+    kv.attend(cache, q, *args, out=between)
+    assert torch.equal(between, exp)
+    w = torch.zeros(2, H, 2 * 64, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        kv.attend(cache, q, *args, weights=w[:, :, :64], weights_in=w[:, :, 1:65])
+    kv.attend(cache, q, *args, weights=w[:, :, :64], weights_in=w[:, :, :64])
+    to = kv.PageCache(torch.zeros(4, kv.page_bytes(T, H, D), dtype=torch.uint8, device="cuda"), T, H, D)
+    to_table = dev(torch, np.arange(4, dtype=np.int32).reshape(2, 2))
+    with pytest.raises(ValueError, match="overlaps weights"):
+        kv.evict(cache, args[0], args[1], w[:, :, :64], 20, to, to_table, args[2], new_weights=w[:, :, 40:104])
+    assert int(args[2]) == 0
 
 
 def test_pool_past_four_gigabytes(fl):
