@@ -1316,6 +1316,7 @@ __global__ __launch_bounds__(256) void fl_kv_weights(const AttendArgs a) {
 #pragma unroll
     for (int k = 0; k < KK; ++k) qf[k] = flipped<E>(load_q8<E>(p + g * (DP / 4) + k * 8, in && g * (DP / 4) + k * 8 < D, a.q_vec), a.flip);
     lg = in ? a.lse2[tok * H * G + hq] : 0.f;
+    lg = lg == -kInf ? kInf : lg;                     // no key is worth anything to such a row
     const int64_t l = !in ? 0 : a.causal ? (int64_t)len - n + i + 1 : len;
     lim = l > 0 ? (uint32_t)l : 0;
   };

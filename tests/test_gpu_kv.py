@@ -372,6 +372,29 @@ def test_attend_queries_that_are_not_finite(fl, n, x, kind):
     assert (np.abs(o - r["out"]) <= ref.out_tolerance(r, torch.finfo(out.dtype).eps, x))[~bad].all()
 
 
+@pytest.mark.parametrize("n,x", [(1, 50), (1, 5000), (3, 50), (20, 90), (40, 1500)])
+def test_attend_scores_that_are_all_minus_infinity(fl, n, x):
+    """Such a row draws nothing from any key: zeros, a log-sum of -inf, and the others' weights as without it."""
+    core, kv, torch = fl
+    T, H, G, D = 16, 1, 4, 64
+    rng = np.random.default_rng(n + x)
+    cache = kv.PageCache(torch.zeros(-(-x // T), kv.page_bytes(T, H, D), dtype=torch.uint8, device="cuda"), T, H, D)
+    k, v = (dev(torch, rng.uniform(0.5, 1, (x, H, D)), torch.float32) for _ in range(2))
+    table, lens, status = dev(torch, np.arange(-(-x // T), dtype=np.int32)[None]), dev(torch, np.array([x], np.int32)), core.new_status()
+    kv.store(cache, k, v, table, torch.zeros_like(lens), status)
+    q = dev(torch, rng.standard_normal((n, H * G, D)), torch.float32).to(torch.bfloat16)
+    c = ref.unpack(cache.pages.cpu().numpy(), T, H, D)
+    r = ref.attend(c, q.cpu().double().numpy(), table.cpu().numpy(), [x], [0, n], 1 / np.sqrt(D))
+    q[n - 1, 1, 3] = -np.inf
+    lse, w = torch.zeros(n, H * G, device="cuda"), torch.zeros(1, H, x, device="cuda")
+    out = kv.attend(cache, q, table, lens, status, lse=lse, weights=w)
+    assert int(status) == 0 and int(out[n - 1, 1].abs().sum()) == 0 and float(lse[n - 1, 1]) == -np.inf
+    others = np.arange(n * H * G) != (n - 1) * H * G + 1
+    e = np.abs(out.cpu().double().numpy() - r["out"]) <= ref.out_tolerance(r, torch.finfo(out.dtype).eps, x)
+    assert e.reshape(n * H * G, D)[others].all()
+    assert not w.isnan().any() and abs(float(w.double().sum()) - (n * G - 1)) <= 1e-3 * n * G   # (each row's sum is 1 within the 2^-11 of its log-sum)
+
+
 def test_views_that_overlap(fl):
     """What a call writes may lie between what it reads, but not on it."""
     core, kv, torch = fl
