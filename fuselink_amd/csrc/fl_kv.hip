@@ -1195,7 +1195,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void fl_kv_attend_rows(cons
 
 // The splits' results of every row, weighted by what their shares of the keys add up to.  Rows are numbered as in
 // fl_kv_attend, so those of no sequence are not touched.  A wavefront joins one row: with DL = D / 4 lanes to a split it
-// reads 64 / DL splits at a time, none of the loads waiting for another.
+// reads 64 / DL splits at a time, eight such loads under way.  What it takes is the start of a launch and one or two trips to
+// memory (4 us for few splits).
+constexpr uint32_t kMostSplits = 256;
 template <class E, bool SEL>
 __global__ __launch_bounds__(256) void fl_kv_join(const AttendArgs a, uint32_t TR) {
   warm_kernel_args(a);
@@ -1221,24 +1223,47 @@ __global__ __launch_bounds__(256) void fl_kv_join(const AttendArgs a, uint32_t T
   const uint64_t tok = first + i, hq = h * G + (r - i * G), at = tok * H * G + hq;
   const uint32_t DL = D <= 64 ? 16 : D <= 128 ? 32 : 64, SP = 64 / DL, d = (lane & (DL - 1)) * 4, sub = lane / DL;
 
-  float top = -kInf;
-  for (uint32_t s = lane; s < a.splits; s += 64) top = fmaxf(top, a.part_l[s * row_out + at]);
+  float part[kMostSplits / 64], top = -kInf;
+#pragma unroll
+  for (uint32_t k = 0; k < kMostSplits / 64; ++k) {
+    const uint32_t s = 64 * k + lane;
+    part[k] = -kInf;
+    if (64 * k < a.splits) part[k] = s < a.splits ? a.part_l[s * row_out + at] : -kInf;
+    top = fmaxf(top, part[k]);
+  }
 #pragma unroll
   for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
   const float base = top == -kInf ? 0.f : top;
   float sum = 0.f;
   f4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (uint32_t s0 = 0; s0 < a.splits; s0 += 64) {
-    const float part = s0 + lane < a.splits ? a.part_l[(s0 + lane) * row_out + at] : -kInf;
-    const float w = part == -kInf ? 0.f : exp2_fast(part - base);
+  const float* mine = a.part_o + at * D + (d < D ? d : 0);
+  const uint64_t step = row_out * D;
+#pragma unroll
+  for (uint32_t k = 0; k < kMostSplits / 64; ++k) {
+    if (64 * k >= a.splits) break;
+    const float w = part[k] == -kInf ? 0.f : exp2_fast(part[k] - base);
     sum += w;
-    const uint32_t cnt = a.splits - s0 < 64 ? a.splits - s0 : 64;
-#pragma unroll 4
-    for (uint32_t s = 0; s < cnt; s += SP) {
-      const uint32_t mine = s + sub;
-      const float ws = __shfl(w, (int)(mine & 63));
-      if (mine < cnt && ws != 0.f && d < D) acc += *reinterpret_cast<const f4*>(a.part_o + ((s0 + mine) * row_out + at) * D + d) * ws;
-    }
+    const uint32_t cnt = a.splits - 64 * k < 64 ? a.splits - 64 * k : 64;
+    // A share of no keys has a weight of 0 and may have written no row: what is read for it is not used.
+    const auto add = [&](auto many, uint32_t s) {
+      constexpr uint32_t U = decltype(many)::value;
+      f4 o[U];
+      float ws[U];
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u) {
+        const uint32_t m = s + u * SP + sub;
+        ws[u] = __shfl(w, (int)(m < cnt ? m : cnt - 1));
+        ws[u] = m < cnt ? ws[u] : 0.f;
+        o[u] = *reinterpret_cast<const f4*>(mine + (64 * k + (m < cnt ? m : cnt - 1)) * step);
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += ws[u] == 0.f ? 0.f : o[u][e] * ws[u];
+    };
+    if (cnt <= 2 * SP) add(std::integral_constant<uint32_t, 2>{}, 0);
+    else
+      for (uint32_t s = 0; s < cnt; s += 8 * SP) add(std::integral_constant<uint32_t, 8>{}, s);
   }
 #pragma unroll
   for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
@@ -1829,7 +1854,11 @@ int make_plan(const flh_kv_attend_params* p, Plan* pl) {
   pl->dp = D <= 64 ? 64 : D <= 128 ? 128 : 256;
   const bool sel = p->d_selected != nullptr;
   const uint64_t rows = sel ? G : ((uint64_t)n * G + B - 1) / B;   // of a sequence, on average
-  pl->kvw = rows <= 32 || sel ? 4 : 1;
+  // Few rows: the four wavefronts of a workgroup share its keys; many: its rows, and a code is converted once for 128 of
+  // them.  (8 sequences of 8192 tokens and 8 heads of 128 channels, 64, 128, 256, 512 rows to a head: keys shared 49, 76, 122,
+  // 228 us, rows shared 65, 90, 132, 221; 32 such sequences, 128 and 256 rows: 244, 449 and 257, 434.  256 channels, 16
+  // sequences of 4096, 32 and 128 rows: 72, 233 and 176, 197.)
+  pl->kvw = rows <= (pl->dp == 256 ? 64 : 128) || sel ? 4 : 1;
   pl->nq = pl->kvw == 4 && (pl->dp == 256 || rows <= 16) ? 1 : 2;
   pl->tr = 16 * pl->nq * (4 / pl->kvw);
   // workgroups that stay resident together: what their registers allow, on 256 compute units
@@ -1842,16 +1871,34 @@ int make_plan(const flh_kv_attend_params* p, Plan* pl) {
     est = (uint64_t)n * G / pl->tr > B ? (uint64_t)n * G / pl->tr : B;
   }
   const uint64_t space = sel ? (uint64_t)p->n_selected * p->cache.tokens : (uint64_t)p->seqs.table_width * p->cache.tokens;
-  // Splits: rounds of workgroups times the longest share (in whole rounds of their wavefronts), a start and an end worth
-  // some 384 keys each time, and the join, worth as much again.
-  const uint32_t round = pl->kvw == 4 ? 128 : 64;
-  uint64_t best = ~0ull;
   pl->splits = 1;
-  const uint64_t top = pl->kvw == 4 ? 256 : est * H < seats ? seats / (est * H ? est * H : 1) : 1;   // (many rows: until the seats are taken)
-  for (uint32_t sp = 1; sp <= top && (sp == 1 || (uint64_t)(sp - 1) * round < space); ++sp) {
-    const uint64_t rounds = (est * H * sp + seats - 1) / seats, share = (space + (uint64_t)sp * round - 1) / ((uint64_t)sp * round) * round;
-    const uint64_t cost = rounds * (share + 384) + (sp > 1 ? 384 : 0);
-    if (cost < best) { best = cost; pl->splits = sp; }
+  const uint64_t pairs = est * H, launched = tiles * H;
+  if (pl->kvw == 4 && pl->nq == 1) {
+    // Up to 16 rows to a head, or 256 channels: memory bounds it, and 256 workgroups of one sequence and head each draw
+    // most of what there is to be drawn.  Fewer are split until 512 run, if 1024 keys are left to each (16 sequences of
+    // 131072 tokens, 8 heads: one share 1167 us, two 923, four 726), else until 256 do (one of 32768: 24 us in 32 shares,
+    // 47 in 8, 29 in 96) or until no share is below 128 keys; more only if shares stay long (32 sequences of 8192: 97 us,
+    // 106 in two; up to 65536: 616, 566; 48 of 16384: 300, 281).  Up to 1024 keys a join costs more than it saves (16
+    // times 1024: 46 us, 47 in two).
+    if (space > 1024 && pairs && pairs < 512) {
+      uint64_t sp = (512 + pairs - 1) / pairs;
+      if (seats < 512 || space < sp * (pairs < 256 ? 1024 : 8192)) sp = (256 + pairs - 1) / pairs;
+      if (sp > seats / launched) sp = seats / launched;
+      if (sp > space / 128) sp = space / 128;
+      pl->splits = sp < 1 ? 1 : sp > kMostSplits ? kMostSplits : (uint32_t)sp;
+    }
+  } else {
+    // More rows: rounds of workgroups times the longest share (in whole rounds of their wavefronts), a start and an end
+    // worth some 384 keys each time, and the join, worth as much again.  (20 sequences of 8192, 64 rows: 120 us in one share, 109
+    // in three, as this has it, 126 in eight; 8 of 2048: 28, 24 in four, 32 in eight.)
+    const uint32_t round = pl->kvw == 4 ? 128 : 64;
+    uint64_t best = ~0ull;
+    const uint64_t top = pl->kvw == 4 ? kMostSplits : pairs < seats ? seats / (pairs ? pairs : 1) : 1;   // (rows shared: until the seats are taken)
+    for (uint32_t sp = 1; sp <= top && (sp == 1 || (uint64_t)(sp - 1) * round < space); ++sp) {
+      const uint64_t rounds = (pairs * sp + seats - 1) / seats, share = (space + (uint64_t)sp * round - 1) / ((uint64_t)sp * round) * round;
+      const uint64_t cost = rounds * (share + 384) + (sp > 1 ? 384 : 0);
+      if (cost < best) { best = cost; pl->splits = sp; }
+    }
   }
   if (tiles * H * pl->splits > kMaxGroups) return fl_set_error(FLH_E_ARG, "flh_kv_attend: too much for one launch");
   pl->tiles_x = (uint32_t)tiles;

@@ -108,9 +108,10 @@ int64_t flh_constant(int which) {
     case 4: return sizeof(flh_chunk_desc);
     case 5: return sizeof(flh_sched_state);
     case 6: return sizeof(flh_sched_hdr);
-    case 7: return 4;   // ABI version: 2 added flh_sched_params.d_table_by_lane, the batch entry points, the DMA-BUF export;
+    case 7: return 5;   // ABI version: 2 added flh_sched_params.d_table_by_lane, the batch entry points, the DMA-BUF export;
                         // 3 the per-tile descriptors (flh_sched_params.d_tiles, flh_stripe_tiles / flh_reassemble_tiles) and the fused paged pair;
-                        // 4 batches of up to 32 requests in segments, the completion word / event in flh_uniform_params, flh_schedule_static
+                        // 4 batches of up to 32 requests in segments, the completion word / event in flh_uniform_params, flh_schedule_static;
+                        // 5 the operators on KV pages (flh_kv_*)
     case 8: return sizeof(flh_windows);
     case 9: return sizeof(flh_sched_params);
     case 10: return sizeof(flh_batch_params);

@@ -252,7 +252,8 @@ ATTEND = [  # T, H, G, D, lens, query tokens
     (32, 1, 4, 128, [90, 33], [33, 16]), (16, 1, 3, 64, [150, 40], [70, 40]), (16, 1, 1, 112, [200], [130]), (64, 1, 2, 256, [100, 64], [50, 64]),
     (128, 2, 1, 144, [129], [100]), (16, 1, 4, 128, [3, 10], [9, 10]), (16, 1, 1, 128, [2100], [1]),
     (16, 1, 2, 64, [9000], [1]), (16, 1, 2, 128, list(range(0, 70)), [1] * 70), (16, 1, 4, 64, [(37 * i) % 90 for i in range(70)], [(5 * i) % 11 for i in range(70)]),
-    (32, 1, 2, 80, [700, 40], [90, 40]), (16, 1, 8, 128, [1100], [40]),
+    (32, 1, 2, 80, [700, 40], [90, 40]), (16, 1, 8, 128, [1100], [40]), (16, 2, 4, 128, [1500, 700], [20, 9]), (16, 1, 2, 256, [1200], [20]),
+    (16, 1, 4, 64, [2000, 30], [31, 30]), (48, 1, 6, 256, [1000], [50]),
 ]
 
 
@@ -270,7 +271,7 @@ def test_attend_weights(fl, case):
     run_attend(fl, T, H, G, D, lens, news, "bf16", weights=True)
 
 
-@pytest.mark.parametrize("n", [3, 5, 20])
+@pytest.mark.parametrize("n", [3, 5, 20, 40])
 def test_attend_nan_is_seen_by_those_who_may(fl, n):
     """A NaN among the values reaches exactly the queries that see its token; one among the keys likewise, whole rows."""
     core, kv, torch = fl
@@ -350,7 +351,7 @@ def test_attend_strided_and_uniform(fl):
         assert (res[:, :, :shift] == 7).all() and (res[:, :, shift + D:] == 7).all()
 
 
-@pytest.mark.parametrize("n,x", [(1, 50), (1, 5000), (3, 50), (40, 90), (40, 1500)])
+@pytest.mark.parametrize("n,x", [(1, 50), (1, 5000), (3, 50), (20, 1500), (40, 90), (40, 1500)])
 @pytest.mark.parametrize("kind", ["bf16", "fp16"])
 def test_attend_queries_that_are_not_finite(fl, n, x, kind):
     """A NaN or an infinity in a query makes its own row NaN -- with keys of both signs an infinite channel gives an
@@ -853,14 +854,15 @@ def test_results_do_not_depend_on_the_run_or_the_stream(fl):
         got = []
         for s, st in zip((5, 6), streams):
             x = decode_state(fl, np.random.default_rng(s))
+            q = [x["q"].clone() for _ in range(3)]                 # dropped one by one; made before the streams meet
             st.wait_stream(torch.cuda.current_stream())
             kw = dict(stream=st)
             kv.store(x["cache"], x["k"], x["v"], x["table"], x["lens"], x["status"], **kw)
             with torch.cuda.stream(st):
                 x["lens"] += 1
-            out = kv.attend(x["cache"], x["q"].clone(), x["table"], x["lens"], x["status"], weights=x["w"], **kw)
-            sel = kv.select_pages(x["cache"], x["q"].clone(), x["table"], x["lens"], 5, x["status"], **kw)
-            sparse = kv.attend(x["cache"], x["q"].clone(), x["table"], x["lens"], x["status"], selected=sel, **kw)
+            out = kv.attend(x["cache"], q.pop(), x["table"], x["lens"], x["status"], weights=x["w"], **kw)
+            sel = kv.select_pages(x["cache"], q.pop(), x["table"], x["lens"], 5, x["status"], **kw)
+            sparse = kv.attend(x["cache"], q.pop(), x["table"], x["lens"], x["status"], selected=sel, **kw)
             kept, nw, nl = kv.evict(x["cache"], x["table"], x["lens"], x["w"], 40, x["to"], x["to_table"], x["status"], first=1, recent=4, **kw)
             got.append([out, sel, sparse, kept, nw, nl, x["w"], x["cache"].pages, x["to"].pages])
             del x
