@@ -310,6 +310,8 @@ __device__ __forceinline__ h2 column_pair(h2 v, F f) {
 // largest magnitude of the new tokens fixes the scale, then the same rows become codes: every row is read once and stays
 // in registers between the two, as it was loaded, ROWS of them a lane.  More than one wavefront exchange their largest
 // magnitude and their bounds through shared memory.  In evict the rows are codes of other records under their own scales.
+// Memory bounds it: 16 prompts of up to 4096 tokens, 8 heads of 128 channels in bf16, 267 MB in 53 us, 5.0 TB/s (a copy of 4 GiB: 4.5);
+// 16 sequences cut back to 2048 tokens, 134 MB in 34 us, 3.9 TB/s, every row of 128 bytes from a place of its own.
 template <class E, bool EVICT, int ROWS, int W>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fl_kv_pack(const PackArgs a) {
   warm_kernel_args(a);
@@ -702,7 +704,9 @@ __device__ __forceinline__ void emit8(const AttendArgs& a, uint32_t split, uint3
 // come as rows of codes straight into registers; V's bytes are interleaved token against token on the way to pairs.
 // P is rounded to 16-bit floats (11 bits of mantissa) at 2^8 times its value relative to the row's reference and up to 2^15,
 // normal down to 2^-22 of it (for the tile with the larger value scale of a step).  Sums, references and accumulators
-// are 32 bits wide and rarely rescaled.
+// are 32 bits wide and rarely rescaled.  Memory bounds it for up to 16 rows: 16 sequences of 131072 tokens, 8 heads of 128 channels,
+// 4.3 GB in 713 us, 6.0 TB/s (a sum over 4 GiB: 6.1); 32 of up to 4096, 172 MB in 40 us, 4.3 TB/s, where the launch's
+// start and the longest sequence show; 201 tokens 8 us, 4 of them the launch's.
 template <class E, int DP, int NQ, bool SEL>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) void fl_kv_attend(const AttendArgs a) {
   warm_kernel_args(a);
@@ -983,7 +987,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) 
 // four wavefronts owns 32 rows and all walk over the keys together, 64 at a time.  Every wavefront looks up, fetches and
 // converts one tile of 16 and leaves it in shared memory as the operands of the matrix instructions, with its scales, so
 // that a code is converted once for 128 rows instead of once for 32 and the registers hold a quarter of the codes on
-// their way.  Two barriers to 64 keys; the three workgroups of a compute unit fill each other's waits.
+// their way.  Two barriers to 64 keys; the three workgroups of a compute unit fill each other's waits.  4 sequences of up
+// to 16384 tokens, 1024 of them new, 32 query heads of 128: 632 GFLOP in 815 us, 776 TFLOP/s (a library product of 8192^3
+// in bf16: 1271).  The vector instructions bound it -- exponentials, conversions and packing keep the pipes busy for 63 % of the time,
+// the matrix instructions for 37 %.
 template <class E, int DP>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void fl_kv_attend_rows(const AttendArgs a) {
   warm_kernel_args(a);
@@ -1285,6 +1292,7 @@ __global__ __launch_bounds__(256) void fl_kv_join(const AttendArgs a, uint32_t T
 // What every key of a sequence was worth to the call's queries: the probabilities exp2(s - lse) summed over the rows of
 // its key-value head, on top of w_in.  A wavefront owns NT tiles of 16 keys at a time and walks over all rows, so the
 // sums need no atomics; the next tiles' codes are on their way meanwhile.  Rows that fit one tile are loaded once.
+// Memory bounds it: 16 sequences of up to 8192 tokens, 8 heads of 128 channels, 88 MB of keys in 26 us, 3.4 TB/s.
 template <class E, int DP>
 __global__ __launch_bounds__(256) void fl_kv_weights(const AttendArgs a) {
   warm_kernel_args(a);
@@ -1423,7 +1431,8 @@ __device__ __forceinline__ uint32_t token_limit(const SelectArgs& a, uint32_t le
 // largest product that a key of the page can have with the query, in whole numbers (8-bit queries against the page's
 // 8-bit bounds), so equal scores are equal and the choice does not depend on the order of a sum.  The sum splits into
 // max(q8, 0) . high - max(-q8, 0) . low, two runs of 16 x 16 x 64 integer matrix instructions whose operands are the
-// bytes of the record as they lie.
+// bytes of the record as they lie.  Memory bounds it: bounds of 2 KiB in records of 34 KiB, 65536 pages of 8 heads of 128
+// channels, 139 MB in 29 us, 4.8 TB/s.
 template <class E, int DP>
 __global__ __launch_bounds__(512) void fl_kv_score(const SelectArgs a) {
   warm_kernel_args(a);
@@ -1613,7 +1622,8 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 
 // The k-th largest of n keys (k < n), and how many of its equals belong to the k.  2048 equal bins over the range that
 // the keys span, so that keys of like size do not all count into a few; the bin that holds the k-th is taken for the
-// next range until all of it belongs to the k (then the key returned is the one below it) or it is one value.  Keys of all
+// next range until all of it belongs to the k (then the key returned is the one below it), it is one value or it holds
+// no more than 64.  Keys of all
 // ones (what has to be among the k) are counted apart and do not stretch the range.  The loops are short and rolled:
 // with a few rows to a call, fetching straight-line code for keys in registers took longer than all else here.
 template <int NT, bool ONE, class Key>
@@ -1673,7 +1683,7 @@ __device__ Pick kth_largest(uint32_t n, uint32_t k, Key key, PickShared<NT, ONE>
     uint32_t before = (wave ? bcast_lane_u32(waves, (int)wave - 1) : 0) + incl - own;
 #pragma unroll
     for (int e = 0; e < OWN; ++e) {
-      if (before < k && k <= before + cnt[e]) { sh.word[0] = 2047 - OWN * tid - e; sh.word[1] = k - before; sh.word[3] = cnt[e]; }
+      if (before < k && k <= before + cnt[e]) { sh.word[0] = 2047 - OWN * tid - e; sh.word[1] = k - before; sh.word[2] = 0; sh.word[3] = cnt[e]; }
       before += cnt[e];
     }
     __syncthreads();
@@ -1683,6 +1693,26 @@ __device__ Pick kth_largest(uint32_t n, uint32_t k, Key key, PickShared<NT, ONE>
     k = sh.word[1];
     if (lo == hi) return {lo, k};
     if (k == left) return lo ? Pick{lo - 1, 0} : Pick{0, 0xffffffffu};   // all of the bin
+    if (left <= 64) {              // collected, in any order, and compared each with each
+      for (uint32_t base = tid; base < n; base += 4 * NT) {
+        uint32_t u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[e] = held(base + e * NT < n ? base + e * NT : n - 1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (base + e * NT < n && u[e] >= lo && u[e] <= hi) sh.hist[atomicAdd(&sh.word[2], 1u)] = u[e];
+      }
+      __syncthreads();
+      const uint32_t u = lane < left ? sh.hist[lane] : 0;
+      uint32_t larger = 0, same = 0;
+      for (uint32_t j = 0; j < left; ++j) {
+        const uint32_t v = bcast_lane_u32(u, (int)j);
+        larger += v > u ? 1 : 0;
+        same += v == u ? 1 : 0;
+      }
+      const int l = __builtin_ctzll(__ballot(lane < left && larger < k && k <= larger + same));
+      return {bcast_lane_u32(u, l), k - bcast_lane_u32(larger, l)};
+    }
     __syncthreads();
   }
 }
@@ -1731,6 +1761,8 @@ __device__ void put_picked(uint32_t n, Pick pick, Key key, Along along, Put put,
   }
 }
 
+// A workgroup chooses one row's pages.  Its passes over the keys, one behind the other, bound it: 32 rows of 16384 pages
+// 19 us, 128 of 2048 12 us.
 template <int NT, bool ONE>
 __global__ __launch_bounds__(NT) void fl_kv_pick_pages(const SelectArgs a) {
   warm_kernel_args(a);
@@ -1762,6 +1794,7 @@ struct KeepArgs {
   int32_t* new_lens;
 };
 
+// The same over the weights of a sequence and head: 128 rows of up to 8192 weights 15 us.
 template <int NT, bool ONE>
 __global__ __launch_bounds__(NT) void fl_kv_keep(const KeepArgs a) {
   warm_kernel_args(a);
@@ -1839,6 +1872,8 @@ int finish(const char* what) {
 }
 
 constexpr uint64_t kMaxGroups = (1ull << 24) - 1;   // of 256 threads: a launch counts its threads in 32 bits
+
+bool many_threads(uint32_t rows, uint32_t keys) { return keys > 256 * kHeld || (rows <= 256 && keys > 1024); }
 
 struct Plan {
   int dp, nq, kvw;
@@ -2117,7 +2152,9 @@ int flh_kv_select(const flh_kv_select_params* p, void* stream) {
   if (a.c.D <= 64) { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 64>), grid, block, 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 64>), grid, block, 0, st, a); }
   else if (a.c.D <= 128) { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 128>), grid, block, 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 128>), grid, block, 0, st, a); }
   else { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 256>), grid, block, 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 256>), grid, block, 0, st, a); }
-  if (a.s.width <= 256 * kHeld) FL_LAUNCH((fl_kv_pick_pages<256, true>), dim3(a.s.n_tokens * a.c.H), dim3(256), 0, st, a);
+  // 1024 threads to a row if there are no more rows than compute units and more than 4 keys a thread, or if 256 would hold too few
+  // (evictions of 32 rows of 4000 weights: 26 us with 256, 20 with 1024; 1024 rows of 512 pages: 52 and 59).
+  if (!many_threads(a.s.n_tokens * a.c.H, a.s.width)) FL_LAUNCH((fl_kv_pick_pages<256, true>), dim3(a.s.n_tokens * a.c.H), dim3(256), 0, st, a);
   else if (a.s.width <= 1024 * kHeld) FL_LAUNCH((fl_kv_pick_pages<1024, true>), dim3(a.s.n_tokens * a.c.H), dim3(1024), 0, st, a);
   else FL_LAUNCH((fl_kv_pick_pages<1024, false>), dim3(a.s.n_tokens * a.c.H), dim3(1024), 0, st, a);
   return finish("flh_kv_select");
@@ -2168,7 +2205,7 @@ int flh_kv_evict(const flh_kv_evict_params* p, void* stream) {
   a.per_seq = per;
   fl_prof().kid = 11;
   const hipStream_t st = (hipStream_t)stream;
-  if (k.w_width <= 256 * kHeld) FL_LAUNCH((fl_kv_keep<256, true>), dim3(a.s.n_seqs * a.c.H), dim3(256), 0, st, k);
+  if (!many_threads(a.s.n_seqs * a.c.H, k.w_width)) FL_LAUNCH((fl_kv_keep<256, true>), dim3(a.s.n_seqs * a.c.H), dim3(256), 0, st, k);
   else if (k.w_width <= 1024 * kHeld) FL_LAUNCH((fl_kv_keep<1024, true>), dim3(a.s.n_seqs * a.c.H), dim3(1024), 0, st, k);
   else FL_LAUNCH((fl_kv_keep<1024, false>), dim3(a.s.n_seqs * a.c.H), dim3(1024), 0, st, k);
   launch_pack<__bf16, true>(a, per * a.s.n_seqs, st);
