@@ -1762,7 +1762,7 @@ __device__ void put_picked(uint32_t n, Pick pick, Key key, Along along, Put put,
 }
 
 // A workgroup chooses one row's pages.  Its passes over the keys, one behind the other, bound it: 32 rows of 16384 pages
-// 19 us, 128 of 2048 12 us.
+// 19 us, 128 of 2048 7 us.
 template <int NT, bool ONE>
 __global__ __launch_bounds__(NT) void fl_kv_pick_pages(const SelectArgs a) {
   warm_kernel_args(a);
@@ -1873,7 +1873,7 @@ int finish(const char* what) {
 
 constexpr uint64_t kMaxGroups = (1ull << 24) - 1;   // of 256 threads: a launch counts its threads in 32 bits
 
-bool many_threads(uint32_t rows, uint32_t keys) { return keys > 256 * kHeld || (rows <= 256 && keys > 1024); }
+bool many_threads(uint32_t rows, uint32_t keys) { return keys > 256 * kHeld || (rows <= 256 && keys > 1536); }
 
 struct Plan {
   int dp, nq, kvw;
@@ -2152,7 +2152,8 @@ int flh_kv_select(const flh_kv_select_params* p, void* stream) {
   if (a.c.D <= 64) { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 64>), grid, block, 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 64>), grid, block, 0, st, a); }
   else if (a.c.D <= 128) { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 128>), grid, block, 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 128>), grid, block, 0, st, a); }
   else { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 256>), grid, block, 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 256>), grid, block, 0, st, a); }
-  // 1024 threads to a row if there are no more rows than compute units and more than 4 keys a thread, or if 256 would hold too few
+  // 1024 threads to a row if there are no more rows than compute units and more than 6 keys
+  // a thread, or if 256 would hold too few
   // (evictions of 32 rows of 4000 weights: 26 us with 256, 20 with 1024; 1024 rows of 512 pages: 52 and 59).
   if (!many_threads(a.s.n_tokens * a.c.H, a.s.width)) FL_LAUNCH((fl_kv_pick_pages<256, true>), dim3(a.s.n_tokens * a.c.H), dim3(256), 0, st, a);
   else if (a.s.width <= 1024 * kHeld) FL_LAUNCH((fl_kv_pick_pages<1024, true>), dim3(a.s.n_tokens * a.c.H), dim3(1024), 0, st, a);

@@ -97,7 +97,12 @@ CALLS = [("flh_kv_store", dict(type=3)), ("flh_kv_store", dict(d_k=None)), ("flh
          ("flh_kv_evict", dict(d_new_weights=None)), ("flh_kv_evict", dict(d_new_lens=None)), ("flh_kv_evict", dict(d_to_table=None))]
 
 
-@pytest.mark.parametrize("call", CALLS, ids=str)
+def call_id(call):
+    op, fields = call
+    return op + " " + ", ".join(f"{k}={v if isinstance(v, (int, float)) else type(v).__name__}" for k, v in fields.items())
+
+
+@pytest.mark.parametrize("call", CALLS, ids=call_id)
 def test_calls(lib, call):
     op, bad = call
     assert getattr(lib, op)(C.byref(OPS[op](**bad)), None) == E_ARG
