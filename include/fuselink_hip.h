@@ -563,10 +563,12 @@ int flh_kv_store(const flh_kv_store_params* p, void* stream);
  * gets zeros and a log-sum of -inf, and adds nothing to the weights.  d_lse (optional):
  * natural logarithm of each row's sum, [n_tokens][q_heads].
  * d_selected (optional): [n_tokens][heads][n_selected] indices into the sequence's row of the table, each at most once, -1
- * for none; only these pages are read (flh_kv_select writes it).
+ * for none; only these pages are read, and of a list no more entries than the query sees pages of the sequence, so what is
+ * chosen stands in front (flh_kv_select writes it so).
  * d_weights (optional; not with d_selected): [n_seqs][heads][weights_width], = d_weights_in (the same memory, other memory, or
  * NULL for 0) plus, for each key, the probabilities that all the call's queries of its head gave it.
- * P is rounded to 11 bits of mantissa for the second product; sums, maxima and accumulators hold 32 bits. */
+ * P is rounded to 11 bits of mantissa for the second product; scores, sums, maxima and accumulators hold 32 bits.  The
+ * sequences of a call are cut alike, by their average number of new tokens: single tokens and long prompts are faster in a call each. */
 typedef struct flh_kv_attend_params {
   flh_kv_cache cache;
   flh_kv_seqs  seqs;

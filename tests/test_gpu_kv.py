@@ -457,7 +457,7 @@ def test_pool_past_four_gigabytes(fl):
 # ---- selected pages -------------------------------------------------------------------------------------------------
 SELECT = [  # T, H, G, D, lens, query tokens, count, first, last
     (16, 2, 4, 128, [500], [1], 4, 1, 1), (16, 2, 4, 128, [16, 17, 900], [1, 1, 1], 8, 0, 1), (32, 3, 1, 64, [700, 33], [3, 5], 5, 2, 2),
-    (48, 1, 7, 80, [2000, 0], [1, 0], 9, 0, 0), (16, 1, 20, 96, [1500], [2], 6, 1, 2), (64, 1, 16, 256, [3000], [1], 10, 1, 1),
+    (48, 1, 7, 80, [2000, 0], [1, 0], 9, 0, 0), (48, 2, 4, 128, [3, 200, 1900], [1, 1, 1], 45, 1, 1), (16, 1, 2, 96, [40, 3000], [30, 6], 200, 0, 1), (16, 1, 20, 96, [1500], [2], 6, 1, 2), (64, 1, 16, 256, [3000], [1], 10, 1, 1),
     (16, 2, 2, 16, [300, 40], [40, 40], 3, 0, 1), (16, 1, 1, 128, [20000], [1], 64, 1, 1), (256, 1, 2, 48, [5000], [1], 7, 0, 3),
 ]
 
