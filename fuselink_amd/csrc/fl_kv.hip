@@ -1890,11 +1890,13 @@ int make_plan(const flh_kv_attend_params* p, Plan* pl) {
   pl->dp = D <= 64 ? 64 : D <= 128 ? 128 : 256;
   const bool sel = p->d_selected != nullptr;
   const uint64_t rows = sel ? G : ((uint64_t)n * G + B - 1) / B;   // of a sequence, on average
-  // Few rows: the four wavefronts of a workgroup share its keys; many: its rows, and a code is converted once for 128 of
-  // them.  (8 sequences of 8192 tokens and 8 heads of 128 channels, 64, 128, 256, 512 rows to a head: keys shared 49, 76, 122,
-  // 228 us, rows shared 65, 90, 132, 221; 32 such sequences, 128 and 256 rows: 244, 449 and 257, 434.  256 channels, 16
-  // sequences of 4096, 32 and 128 rows: 72, 233 and 176, 197.)
-  pl->kvw = rows <= (pl->dp == 256 ? 64 : 128) || sel ? 4 : 1;
+  // Few rows, or few tiles of 128 rows: the four wavefronts of a workgroup share its keys; many: its rows, and a code is
+  // converted once for 128 of them.  (8 sequences of 8192 tokens and 8 heads of 128 channels, 64, 128, 256, 512 rows to a head:
+  // keys shared 49, 76, 122, 228 us, rows shared 65, 90, 132, 221; 32 such sequences, 128 and 256 rows: 244, 449 and 257,
+  // 434; two, 256, 512 and 1024 rows: 43, 69, 111 and 57, 79, 122.  256 channels, 16 sequences of 4096, 32 and 128 rows: 72,
+  // 233 and 176, 197.)
+  const bool wide = pl->dp == 256;
+  pl->kvw = sel || rows <= (wide ? 64 : 128) || (!wide && (rows + 127) / 128 * B * H <= 128) ? 4 : 1;
   pl->nq = pl->kvw == 4 && (pl->dp == 256 || rows <= 16) ? 1 : 2;
   pl->tr = 16 * pl->nq * (4 / pl->kvw);
   // workgroups that stay resident together: what their registers allow, on 256 compute units
@@ -2141,12 +2143,13 @@ int flh_kv_select(const flh_kv_select_params* p, void* stream) {
   const hipStream_t st = (hipStream_t)stream;
   // The wavefronts of a workgroup take up to eight heads of the same pages: the pages' translations and the line that
   // holds their scales are then fetched by one compute unit (65536 pages of 8 heads: a head to a workgroup 41 us, four
-  // 31, eight 29).  As many workgroups as stay resident, or 32 pages to a wavefront.
+  // 31, eight 29).  2048 wavefronts over all rows (1024: 10 tokens over 7518 pages of 5 heads of 64 channels 53 us, 46 so;
+  // 4096: 16 over 2048 pages of 8 heads of 128 44 us, 42 so), or 32 pages to each.
   const uint32_t waves = a.c.H >= 8 ? 8 : 4;
   a.heads_wg = a.c.H >= 8 ? 8 : a.c.H >= 4 ? 4 : a.c.H >= 2 ? 2 : 1;
   const uint32_t groups = (a.c.H + a.heads_wg - 1) / a.heads_wg;
   const uint64_t rows = (uint64_t)a.s.n_tokens * groups;
-  const uint32_t per = 32 * (waves / a.heads_wg), want = (uint32_t)((256 + rows - 1) / rows), most = (a.s.width + per - 1) / per;
+  const uint32_t per = 32 * (waves / a.heads_wg), want = (uint32_t)((2048 / waves + rows - 1) / rows), most = (a.s.width + per - 1) / per;
   a.parts = want < most ? want : most;
   const dim3 grid(a.parts * groups, a.s.n_tokens), block(64 * waves);
   const bool bf = p->type == FLH_KV_BF16;

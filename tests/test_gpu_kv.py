@@ -254,6 +254,9 @@ ATTEND = [  # T, H, G, D, lens, query tokens
     (16, 1, 2, 64, [9000], [1]), (16, 1, 2, 128, list(range(0, 70)), [1] * 70), (16, 1, 4, 64, [(37 * i) % 90 for i in range(70)], [(5 * i) % 11 for i in range(70)]),
     (32, 1, 2, 80, [700, 40], [90, 40]), (16, 1, 8, 128, [1100], [40]), (16, 2, 4, 128, [1500, 700], [20, 9]), (16, 1, 2, 256, [1200], [20]),
     (16, 1, 4, 64, [2000, 30], [31, 30]), (48, 1, 6, 256, [1000], [50]),
+    # more than 128 tiles of 128 rows
+    (16, 65, 1, 112, [200], [130]), (16, 65, 3, 64, [150, 40], [70, 40]), (32, 43, 2, 80, [700, 40], [90, 40]), (16, 65, 4, 128, [600], [40]),
+    (16, 1, 4, 64, [33 + (7 * i) % 60 for i in range(70)], [33] * 70), (48, 66, 1, 128, [150, 0, 260], [150, 0, 250]),
 ]
 
 
@@ -271,11 +274,11 @@ def test_attend_weights(fl, case):
     run_attend(fl, T, H, G, D, lens, news, "bf16", weights=True)
 
 
-@pytest.mark.parametrize("n", [3, 5, 20, 40])
-def test_attend_nan_is_seen_by_those_who_may(fl, n):
+@pytest.mark.parametrize("n,H", [(3, 2), (5, 2), (20, 2), (40, 2), (40, 65)])
+def test_attend_nan_is_seen_by_those_who_may(fl, n, H):
     """A NaN among the values reaches exactly the queries that see its token; one among the keys likewise, whole rows."""
     core, kv, torch = fl
-    T, H, G, D, x = 16, 2, 4, 64, 40
+    T, G, D, x = 16, 4, 64, 40
     rng = np.random.default_rng(3)
     for side in (1, 0):
         cache, c, table = make(fl, rng, [x], T, H, D)
@@ -294,9 +297,9 @@ def test_attend_nan_is_seen_by_those_who_may(fl, n):
         o = out.cpu().double().numpy()
         nan = np.zeros(o.shape, bool)
         if side:
-            nan[n - late:, G:, 5] = True
+            nan[n - late:, G:2 * G, 5] = True
         else:
-            nan[n - late:, G:, :] = True
+            nan[n - late:, G:2 * G, :] = True
         np.testing.assert_array_equal(np.isnan(o), nan)
         tol = ref.out_tolerance(r, torch.finfo(torch.bfloat16).eps, x)
         assert (np.abs(o - r["out"])[~nan] <= tol[~nan]).all()
@@ -329,10 +332,12 @@ def test_attend_scale(fl, scale):
     run_attend(fl, 16, 2, 4, 64, [77, 20], [1, 20], "bf16", scale=scale, weights=True)
 
 
-def test_attend_strided_and_uniform(fl):
+@pytest.mark.parametrize("H,lens,n", [(2, [50, 21, 33], 2), (22, [150, 121, 133], 70)], ids=str)
+def test_attend_strided_and_uniform(fl, H, lens, n):
     """Queries and outputs inside wider tensors, at odd offsets; no starts: every sequence has equally many tokens."""
     core, kv, torch = fl
-    T, H, G, D, lens, n = 16, 2, 2, 64, [50, 21, 33], 2
+    T, G, D = 16, 2, 64
+    starts = [0, n, 2 * n, 3 * n]
     rng = np.random.default_rng(9)
     cache, c, table = make(fl, rng, lens, T, H, D)
     for shift in (0, 1, 4):
@@ -346,18 +351,18 @@ def test_attend_strided_and_uniform(fl):
         kv.attend(cache, q, wide_table[:, :table.shape[1]], dev(torch, np.array(lens, np.int32)), status, out=out)
         torch.cuda.synchronize()
         assert int(status) == 0
-        r = ref.attend(c, q.cpu().double().numpy(), table, lens, [0, 2, 4, 6], 1 / np.sqrt(D))
-        check_out(torch, out, None, r, torch.float16, lens, [0, 2, 4, 6])
+        r = ref.attend(c, q.cpu().double().numpy(), table, lens, starts, 1 / np.sqrt(D))
+        check_out(torch, out, None, r, torch.float16, lens, starts)
         assert (res[:, :, :shift] == 7).all() and (res[:, :, shift + D:] == 7).all()
 
 
-@pytest.mark.parametrize("n,x", [(1, 50), (1, 5000), (3, 50), (20, 1500), (40, 90), (40, 1500)])
+@pytest.mark.parametrize("n,x,H", [(1, 50, 2), (1, 5000, 2), (3, 50, 2), (20, 1500, 2), (40, 90, 2), (40, 90, 65), (40, 400, 65)])
 @pytest.mark.parametrize("kind", ["bf16", "fp16"])
-def test_attend_queries_that_are_not_finite(fl, n, x, kind):
+def test_attend_queries_that_are_not_finite(fl, n, x, H, kind):
     """A NaN or an infinity in a query makes its own row NaN -- with keys of both signs an infinite channel gives an
     infinite largest score -- and touches no other row."""
     core, kv, torch = fl
-    T, H, G, D = 16, 2, 4, 128
+    T, G, D = 16, 4, 128
     rng = np.random.default_rng(n + x)
     cache, c, table = make(fl, rng, [x], T, H, D)
     q = dev(torch, rng.standard_normal((n, H * G, D)), torch.float32).to({"bf16": torch.bfloat16, "fp16": torch.float16}[kind])
@@ -373,11 +378,11 @@ def test_attend_queries_that_are_not_finite(fl, n, x, kind):
     assert (np.abs(o - r["out"]) <= ref.out_tolerance(r, torch.finfo(out.dtype).eps, x))[~bad].all()
 
 
-@pytest.mark.parametrize("n,x", [(1, 50), (1, 5000), (3, 50), (20, 90), (40, 1500)])
-def test_attend_scores_that_are_all_minus_infinity(fl, n, x):
+@pytest.mark.parametrize("n,x,H", [(1, 50, 1), (1, 5000, 1), (3, 50, 1), (20, 90, 1), (40, 1500, 1), (40, 300, 65)])
+def test_attend_scores_that_are_all_minus_infinity(fl, n, x, H):
     """Such a row draws nothing from any key: zeros, a log-sum of -inf, and the others' weights as without it."""
     core, kv, torch = fl
-    T, H, G, D = 16, 1, 4, 64
+    T, G, D = 16, 4, 64
     rng = np.random.default_rng(n + x)
     cache = kv.PageCache(torch.zeros(-(-x // T), kv.page_bytes(T, H, D), dtype=torch.uint8, device="cuda"), T, H, D)
     k, v = (dev(torch, rng.uniform(0.5, 1, (x, H, D)), torch.float32) for _ in range(2))
@@ -393,7 +398,7 @@ def test_attend_scores_that_are_all_minus_infinity(fl, n, x):
     others = np.arange(n * H * G) != (n - 1) * H * G + 1
     e = np.abs(out.cpu().double().numpy() - r["out"]) <= ref.out_tolerance(r, torch.finfo(out.dtype).eps, x)
     assert e.reshape(n * H * G, D)[others].all()
-    assert not w.isnan().any() and abs(float(w.double().sum()) - (n * G - 1)) <= 1e-3 * n * G   # (each row's sum is 1 within the 2^-11 of its log-sum)
+    assert not w.isnan().any() and abs(float(w.double().sum()) - (n * H * G - 1)) <= 1e-3 * n * H * G   # (each row's sum is 1 within the 2^-11 of its log-sum)
 
 
 def test_views_that_overlap(fl):
