@@ -104,30 +104,36 @@ def attend(c, q, table, lens, starts, scale, causal=True, selected=None, q_bits=
         n = starts[b + 1] - starts[b]
         for h in range(H):
             k, v = values(c, table[b], h, x)
-            for i in range(n):
-                t = starts[b] + i
-                seen = max(0, x - n + i + 1) if causal else x
-                use = np.arange(seen)
-                if selected is not None:
-                    pick = set(int(j) for j in selected[t, h] if j >= 0)
-                    use = np.array([j for j in range(seen) if j // T in pick], int)
-                if not len(use):
+            heads = slice(h * G, (h + 1) * G)
+            seen = np.clip(x - n + 1 + np.arange(n), 0, None) if causal else np.full(n, x)
+            if selected is None:             # all tokens of the sequence together
+                blocks = [(np.arange(n), np.arange(x), np.arange(x)[None] < seen[:, None])]
+            else:
+                pick = [set(int(j) for j in selected[starts[b] + i, h] if j >= 0) for i in range(n)]
+                use = [np.array([j for j in range(seen[i]) if j // T in pick[i]], int) for i in range(n)]
+                blocks = [(np.array([i]), u, np.ones((1, len(u)), bool)) for i, u in enumerate(use)]
+            for tok, use, vis in blocks:
+                tok, vis = tok[vis.any(1)], vis[vis.any(1)]
+                if not len(tok):
                     continue
-                kk, vv = k[use], v[use]
-                for g in range(G):
-                    row = q[t, h * G + g]
-                    s = kk @ row * scale
-                    m = s.max()
-                    p = np.exp(s - m)
-                    tot = p.sum()
-                    p /= tot
-                    out[t, h * G + g], lse[t, h * G + g] = p @ vv, m + np.log(tot)
-                    # 32-bit sums of D products, the scaling, and the exponential's argument
-                    err = (np.abs(kk) @ np.abs(row) * abs(scale) * (D + 4) + np.abs(s) * 4 + abs(m) * 4 + 32) * 2.0 ** -24
-                    slack[t, h * G + g] = err.max()
-                    spread[t, h * G + g] = p @ np.abs(vv)
-                    weights[b][h, use] += p
-                    wslack[b][h, use] += p * (err + err.max())
+                at, vis, kk, vv = starts[b] + tok, np.repeat(vis, G, 0), k[use], v[use]
+                rows, shape = q[at, heads].reshape(-1, D), (len(tok), G)
+                s = np.where(vis, rows @ kk.T * scale, -np.inf)
+                m = s.max(1, keepdims=True)
+                p = np.where(vis, np.exp(s - m), 0)
+                tot = p.sum(1, keepdims=True)
+                p /= tot
+                nan = np.isnan(vv)
+                o = p @ np.where(nan, 0, vv)
+                o[vis.astype(float) @ nan > 0] = np.nan
+                out[at, heads], lse[at, heads] = o.reshape(*shape, D), (m + np.log(tot)).reshape(shape)
+                # 32-bit sums of D products, the scaling, and the exponential's argument
+                err = (np.abs(rows) @ np.abs(kk).T * abs(scale) * (D + 4) + np.abs(np.where(vis, s, 0)) * 4 + np.abs(m) * 4 + 32) * 2.0 ** -24
+                err = np.where(vis, err, 0)
+                slack[at, heads] = err.max(1).reshape(shape)
+                spread[at, heads] = (p @ np.abs(np.where(nan, 0, vv))).reshape(*shape, D)
+                weights[b][h, use] += p.sum(0)
+                wslack[b][h, use] += (p * (err + err.max(1, keepdims=True))).sum(0)
     return dict(out=out, lse=lse, weights=weights, spread=spread, slack=slack, wslack=wslack)
 
 

@@ -254,9 +254,6 @@ ATTEND = [  # T, H, G, D, lens, query tokens
     (16, 1, 2, 64, [9000], [1]), (16, 1, 2, 128, list(range(0, 70)), [1] * 70), (16, 1, 4, 64, [(37 * i) % 90 for i in range(70)], [(5 * i) % 11 for i in range(70)]),
     (32, 1, 2, 80, [700, 40], [90, 40]), (16, 1, 8, 128, [1100], [40]), (16, 2, 4, 128, [1500, 700], [20, 9]), (16, 1, 2, 256, [1200], [20]),
     (16, 1, 4, 64, [2000, 30], [31, 30]), (48, 1, 6, 256, [1000], [50]),
-    # more than 128 tiles of 128 rows
-    (16, 65, 1, 112, [200], [130]), (16, 65, 3, 64, [150, 40], [70, 40]), (32, 43, 2, 80, [700, 40], [90, 40]), (16, 65, 4, 128, [600], [40]),
-    (16, 1, 4, 64, [33 + (7 * i) % 60 for i in range(70)], [33] * 70), (48, 66, 1, 128, [150, 0, 260], [150, 0, 250]),
 ]
 
 
@@ -272,6 +269,19 @@ def test_attend(fl, case, kind, causal):
 def test_attend_weights(fl, case):
     T, H, G, D, lens, news = case
     run_attend(fl, T, H, G, D, lens, news, "bf16", weights=True)
+
+
+MANY = [  # more than 128 tiles of 128 rows
+    (16, 65, 1, 112, [200], [130]), (16, 65, 3, 64, [150, 40], [70, 40]), (32, 43, 2, 80, [700, 40], [90, 40]), (16, 65, 4, 128, [600], [40]),
+    (16, 1, 4, 64, [33 + (7 * i) % 60 for i in range(70)], [33] * 70), (48, 66, 1, 128, [150, 0, 260], [150, 0, 250]),
+]
+
+
+@pytest.mark.parametrize("case", MANY, ids=str)
+@pytest.mark.parametrize("kind,causal,weights", [("bf16", True, True), ("fp16", False, False)])
+def test_attend_many_tiles(fl, case, kind, causal, weights):
+    T, H, G, D, lens, news = case
+    run_attend(fl, T, H, G, D, lens, news, kind, causal, weights=weights)
 
 
 @pytest.mark.parametrize("n,H", [(3, 2), (5, 2), (20, 2), (40, 2), (40, 65)])
