@@ -989,7 +989,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) 
 // converts one tile of 16 and leaves it in shared memory as the operands of the matrix instructions, with its scales, so
 // that a code is converted once for 128 rows instead of once for 32 and the registers hold a quarter of the codes on
 // their way.  Two barriers to 64 keys; the three workgroups of a compute unit fill each other's waits.  4 sequences of up
-// to 16384 tokens, 1024 of them new, 32 query heads of 128: 632 GFLOP in 815 us, 776 TFLOP/s (a library product of 8192^3
+// to 16384 tokens, 1024 of them new, 32 query heads of 128: 632 GFLOP in 830 us, 760 TFLOP/s (a library product of 8192^3
 // in bf16: 1271).  The vector instructions bound it -- exponentials, conversions and packing keep the pipes busy for 63 % of the time,
 // the matrix instructions for 37 %.
 template <class E, int DP>
