@@ -878,10 +878,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) 
       if (__ballot(seen_nan != 0)) nan_steps = 1;
     }
 
-    // the floor keeps -inf what it is under a block of zeros; what it multiplies otherwise is zero all the same
-    const float kc0 = fmaxf(x.ks[0] * a.scale2, 1e-37f), kc1 = fmaxf(x.ks[1] * a.scale2, 1e-37f);
+    // The floor keeps -inf what it is under a block of zeros; what it multiplies otherwise is zero all the same.  The scales
+    // that came with a tile that is not there are anyone's: none, so that O's scale does not follow them.
+    const float kc0 = fmaxf(x.ok[0] ? x.ks[0] * a.scale2 : 0.f, 1e-37f), kc1 = fmaxf(x.ok[1] ? x.ks[1] * a.scale2 : 0.f, 1e-37f);
     h8 pf[NQ];
-    soften(st, s, kc0, kc1, x.vs[0], x.vs[1], pf);
+    soften(st, s, kc0, kc1, x.ok[0] ? x.vs[0] : 0.f, x.ok[1] ? x.vs[1] : 0.f, pf);
 
 #pragma unroll
     for (int e = 0; e < VW; ++e) {
@@ -1112,7 +1113,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void fl_kv_attend_rows(cons
         *at = u2{__builtin_bit_cast(uint32_t, v[0][j]), __builtin_bit_cast(uint32_t, v[1][j])};
       }
     }
-    if (lane == 0) sm_tile[wave] = f4{fmaxf(s.ks * a.scale2, 1e-37f), s.ok ? s.vs : 0.f, s.ok ? 1.f : 0.f, 0.f};
+    if (lane == 0) sm_tile[wave] = f4{fmaxf(s.ok ? s.ks * a.scale2 : 0.f, 1e-37f), s.ok ? s.vs : 0.f, s.ok ? 1.f : 0.f, 0.f};
   };
 
   if (threadIdx.x == 0) sm_nan = 0;

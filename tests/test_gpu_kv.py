@@ -906,3 +906,64 @@ def test_empty_calls(fl):
     assert kv.attend(cache, q, d_table, lens, status, selected=torch.empty(0, H, 2, dtype=torch.int32, device="cuda")).shape == q.shape
     torch.cuda.synchronize()
     assert torch.equal(w, w_in) and torch.equal(before, cache.pages) and int(status) == 0
+
+
+# ---- pages that are not there ---------------------------------------------------------------------------------------
+WORDS = [-0x55555556, 0x5D800000, 0x7F800000, 0x7FC00000]        # scale words of pages that hold nothing: 0xAAAAAAAA, 2^60, infinity, NaN
+
+
+def strewn(fl, cache, table, word):
+    """The same pool behind a page that no table names, every scale word of a page that holds nothing being `word`: (cache, table, an idle page)."""
+    core, kv, torch = fl
+    c = kv.PageCache(torch.cat([torch.full_like(cache.pages[:1], 0xAA), cache.pages]), cache.tokens, cache.heads, cache.dim)
+    used = set((table[table >= 0] + 1).tolist())
+    idle = [p for p in range(c.pages.shape[0]) if p not in used]
+    c.scales().view(torch.int32)[idle] = word
+    return c, np.where(table < 0, table, table + 1).astype(np.int32), idle[-1]
+
+
+@pytest.mark.parametrize("T", [16, 48])
+@pytest.mark.parametrize("n,H,G", [(1, 2, 4), (5, 2, 4), (20, 2, 4), (40, 65, 4)])
+@pytest.mark.parametrize("word", WORDS, ids=hex)
+def test_absent_page_is_not_seen(fl, T, n, H, G, word):
+    """Whatever lies in the pool's first page, a page number outside the pool only takes its own keys away."""
+    core, kv, torch = fl
+    D, lens = 64, [7 * T - 5, 4 * T]
+    rng = np.random.default_rng(T + n)
+    cache, c, table = make(fl, rng, lens, T, H, D)
+    cache, moved, _ = strewn(fl, cache, table, word)
+    moved[0, 2] = -1
+    q = dev(torch, rng.standard_normal((2 * n, H * G, D)), torch.float32).to(torch.bfloat16)
+    status, w = core.new_status(), torch.zeros(2, H, 7 * T, device="cuda")
+    lse = torch.zeros(2 * n, H * G, device="cuda")
+    out = kv.attend(cache, q, dev(torch, moved), dev(torch, np.array(lens, np.int32)), status, weights=w, lse=lse)
+    assert int(status) == E_RANGE
+    pick = np.full((2 * n, H, 7), -1)
+    pick[:n, :, :6], pick[n:, :, :4] = [0, 1, 3, 4, 5, 6], range(4)
+    starts = [0, n, 2 * n]
+    r = ref.attend(c, q.cpu().double().numpy(), table, lens, starts, 1 / np.sqrt(D), selected=pick)
+    check_out(torch, out, lse, r, torch.bfloat16, lens, starts)
+    for b, x in enumerate(lens):
+        tol = r["wslack"][b] * 1.1 + r["weights"][b] * (n * G + 64) * 2.0 ** -23
+        assert (np.abs(w[b, :, :x].cpu().double().numpy() - r["weights"][b]) <= tol).all()
+
+
+@pytest.mark.parametrize("T", [16, 48])
+@pytest.mark.parametrize("G", [2, 20])
+@pytest.mark.parametrize("word", WORDS, ids=hex)
+def test_selected_index_behind_the_sequence_is_not_seen(fl, T, G, word):
+    """Indices behind the sequence's pages, where the table names no page or one that nothing was stored in: no error, no keys."""
+    core, kv, torch = fl
+    H, D, lens = 2, 64, [7 * T - 5]
+    rng = np.random.default_rng(T + G)
+    cache, c, table = make(fl, rng, lens, T, H, D)
+    cache, moved, idle = strewn(fl, cache, table, word)
+    moved = np.concatenate([moved, np.array([[-1, idle, -1]], np.int32)], 1)
+    q = dev(torch, rng.standard_normal((1, H * G, D)), torch.float32).to(torch.bfloat16)
+    for sel, seen in (([3, 7, 6, 1], [1, 3, 6]), ([3, 8, 6, 0, 9], [0, 3, 6]), ([8, 5], [5]), ([9, 8, 7, 2], [2])):
+        d_sel = dev(torch, np.broadcast_to(np.array(sel, np.int32), (1, H, len(sel))))
+        status = core.new_status()
+        out = kv.attend(cache, q, dev(torch, moved), dev(torch, np.array(lens, np.int32)), status, selected=d_sel)
+        assert int(status) == 0
+        r = ref.attend(c, q.cpu().double().numpy(), table, lens, [0, 1], 1 / np.sqrt(D), selected=np.broadcast_to(np.array(seen), (1, H, len(seen))))
+        check_out(torch, out, None, r, torch.bfloat16, lens, [0, 1])
