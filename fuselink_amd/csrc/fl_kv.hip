@@ -1826,6 +1826,7 @@ __global__ __launch_bounds__(NT) void fl_kv_keep(const KeepArgs a) {
 constexpr uint32_t kMaxPages = (1u << 23) - 1;   // of a sequence: positions fit 31 bits
 
 bool aligned(const void* p, uint64_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+bool overlap(const void* a, const void* b, uint64_t bytes) { return (uintptr_t)a < (uintptr_t)b + bytes && (uintptr_t)b < (uintptr_t)a + bytes; }
 
 int check_cache(const flh_kv_cache* k, Cache* c, const char* what) {
   if (!k->d_pages || !aligned(k->d_pages, 16)) return fl_set_error(FLH_E_ARG, "%s: the pool must be a 16-byte aligned device pointer", what);
@@ -2182,6 +2183,8 @@ int flh_kv_evict(const flh_kv_evict_params* p, void* stream) {
   if (p->to_table_width < per || p->to_table_stride < p->to_table_width)
     return fl_set_error(FLH_E_ARG, "flh_kv_evict: %u tokens need %u pages, the new table has %u", p->budget, per, p->to_table_width);
   if (p->weights_width == 0 || p->new_weights_width < p->budget) return fl_set_error(FLH_E_ARG, "flh_kv_evict: weights of %u positions, new ones of %u", p->weights_width, p->new_weights_width);
+  // (the workgroups of the other heads still read a length when the first one's writes the new one)
+  if (overlap(p->d_new_lens, p->seqs.d_lens, 4ull * a.s.n_seqs)) return fl_set_error(FLH_E_ARG, "flh_kv_evict: the new lengths overlap the lengths");
   if ((uint64_t)per * a.s.n_seqs > kMaxGroups / 4 || (uint64_t)a.s.n_seqs * a.c.H > kMaxGroups / 4) return fl_set_error(FLH_E_ARG, "flh_kv_evict: too much for one launch");
   if ((rc = fl_need_init())) return rc;
   KeepArgs k;

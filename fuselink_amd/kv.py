@@ -303,7 +303,7 @@ def evict(cache: PageCache, page_table: torch.Tensor, lens: torch.Tensor, weight
     """flh_kv_evict: cuts every sequence back to `budget` tokens a head -- the first `first`, the last `recent` and those of the largest
     `weights` [n_seqs, heads, positions] -- packed into the pages of `to` that `to_table` [n_seqs, pages] names, none of which may be
     among those that are read.  Returns (kept, new_weights, new_lens): positions [n_seqs, heads, budget] with -1 behind
-    them, the weights kept with zeros behind them ([n_seqs, heads, >= budget]), and the new lengths."""
+    them, the weights kept with zeros behind them ([n_seqs, heads, >= budget]), and the new lengths (`new_lens` is other memory than `lens`)."""
     seqs, word = _seqs(cache, page_table, lens, status, None, 0)
     b, h = seqs[5], cache.heads
     _need(to.index == cache.index and to.heads == h and to.dim == cache.dim, "the new cache differs in device, heads or head dim")
@@ -334,6 +334,7 @@ def evict(cache: PageCache, page_table: torch.Tensor, lens: torch.Tensor, weight
             (nl,), _ = _check(cache, "new_lens", new_lens, _I32, 1)
             _check_written("new_lens", new_lens)
             _need(nl == b, f"new_lens: [{b}]")
+            _need(_apart(new_lens, lens), "new_lens overlaps lens")
         check(_lib.load().flh_kv_evict(_EVICT.pack(*cache.c, *to.c, *seqs, to_table.data_ptr(), stride, weights.data_ptr(), ws_s, ws_h,
                                                    new_weights.data_ptr(), ns, nh, kept.data_ptr(), new_lens.data_ptr(), to_width, width, nw,
                                                    budget, first, recent, word), sp))

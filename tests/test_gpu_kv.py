@@ -967,3 +967,17 @@ def test_selected_index_behind_the_sequence_is_not_seen(fl, T, G, word):
         assert int(status) == 0
         r = ref.attend(c, q.cpu().double().numpy(), table, lens, [0, 1], 1 / np.sqrt(D), selected=np.broadcast_to(np.array(seen), (1, H, len(seen))))
         check_out(torch, out, None, r, torch.bfloat16, lens, [0, 1])
+
+
+def test_evict_does_not_write_the_lengths_it_reads(fl):
+    core, kv, torch = fl
+    T, H, D, x = 16, 2, 64, 40
+    cache, c, table = make(fl, np.random.default_rng(2), [x, x], T, H, D)
+    words = dev(torch, np.array([x, x, 0, 0], np.int32))
+    to = kv.PageCache(torch.zeros(4, kv.page_bytes(T, H, D), dtype=torch.uint8, device="cuda"), T, H, D)
+    args = torch.ones(2, H, x, device="cuda"), 20, to, dev(torch, np.arange(4, dtype=np.int32).reshape(2, 2)), core.new_status()
+    for new_lens in (words[:2], words[1:3]):
+        with pytest.raises(ValueError, match="new_lens overlaps lens"):
+            kv.evict(cache, dev(torch, table), words[:2], *args, new_lens=new_lens)
+    kv.evict(cache, dev(torch, table), words[:2], *args, new_lens=words[2:])
+    assert words.tolist() == [x, x, 20, 20] and int(args[-1]) == 0

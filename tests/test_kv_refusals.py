@@ -153,3 +153,22 @@ def test_wrapper_refusals():
     for call in bad:
         with pytest.raises(ValueError):
             call()
+
+
+def apart(**kw):
+    """An eviction whose arrays are all memory of their own: a sound call but for `kw`."""
+    at = {n: (i + 2) << 32 for i, n in enumerate(("d_to_table", "d_weights", "d_new_weights", "d_kept", "d_new_lens", "d_status"))}
+    return evict(**{"to": cache(d_pages=1 << 40), "s": seqs(d_lens=1 << 41, d_table=1 << 42), **at, **kw})
+
+
+@pytest.mark.parametrize("bad", [fields for op, fields in CALLS if op == "flh_kv_evict"], ids=lambda f: call_id(("flh_kv_evict", f)))
+def test_evictions_apart(lib, bad):
+    assert lib.flh_kv_evict(C.byref(apart(**bad)), None) == E_ARG
+    assert b"overlap" not in lib.flh_last_error()
+
+
+@pytest.mark.parametrize("shift", [-4, 0, 4])
+def test_evict_lengths_in_place(lib, shift):
+    """The new lengths of 2 sequences written over what the call's other workgroups may still read."""
+    assert lib.flh_kv_evict(C.byref(apart(d_new_lens=(1 << 41) + shift)), None) == E_ARG
+    assert b"overlap" in lib.flh_last_error()
