@@ -2183,6 +2183,7 @@ int flh_kv_evict(const flh_kv_evict_params* p, void* stream) {
   if (p->to_table_width < per || p->to_table_stride < p->to_table_width)
     return fl_set_error(FLH_E_ARG, "flh_kv_evict: %u tokens need %u pages, the new table has %u", p->budget, per, p->to_table_width);
   if (p->weights_width == 0 || p->new_weights_width < p->budget) return fl_set_error(FLH_E_ARG, "flh_kv_evict: weights of %u positions, new ones of %u", p->weights_width, p->new_weights_width);
+  if (p->d_to_table == p->seqs.d_table && a.c.pages == a.from.pages) return fl_set_error(FLH_E_ARG, "flh_kv_evict: the new pages are those that are read");
   // (the workgroups of the other heads still read a length when the first one's writes the new one)
   if (overlap(p->d_new_lens, p->seqs.d_lens, 4ull * a.s.n_seqs)) return fl_set_error(FLH_E_ARG, "flh_kv_evict: the new lengths overlap the lengths");
   if ((uint64_t)per * a.s.n_seqs > kMaxGroups / 4 || (uint64_t)a.s.n_seqs * a.c.H > kMaxGroups / 4) return fl_set_error(FLH_E_ARG, "flh_kv_evict: too much for one launch");

@@ -314,6 +314,7 @@ def evict(cache: PageCache, page_table: torch.Tensor, lens: torch.Tensor, weight
     if b == 1:
         stride = to_width
     _need(tb == b and to_width >= (budget + to.tokens - 1) // to.tokens and stride >= to_width, f"to_table: [{b}, >= {(budget + to.tokens - 1) // to.tokens}]")
+    _need(to_table.data_ptr() != page_table.data_ptr() or to.c[0] != cache.c[0], "to_table is page_table: the new pages must not be among those that are read")
     with _on(cache, stream, cache.pages, to.pages, page_table, lens, weights, to_table, status, kept, new_weights, new_lens) as sp:
         if kept is None:
             kept = torch.empty((b, h, budget), dtype=_I32, device=cache.device)

@@ -618,7 +618,7 @@ int flh_kv_select(const flh_kv_select_params* p, void* stream);
 /* Cuts every sequence back to `budget` tokens a head (those that hold no more are copied whole): the `first` first, the `recent`
  * last and, between them, those of the largest weights (NaN the least; of equal weights the earlier token), in their
  * order.  The tokens kept are packed into the pages that d_to_table names, under scales and bounds of their own;
- * `to` may be the same pool, but the new pages must not be among those the call reads.  d_kept [n_seqs][heads][budget] receives
+ * `to` may be the same pool, but the new pages must not be among those the call reads (the same table over the same pool: FLH_E_ARG).  d_kept [n_seqs][heads][budget] receives
  * the positions (-1 behind them), d_new_weights the weights kept and zeros up to new_weights_width, d_new_lens the new
  * lengths: other memory than d_lens and d_weights (FLH_E_ARG where the two arrays of lengths overlap).  seqs.d_starts and
  * n_tokens are not used. */

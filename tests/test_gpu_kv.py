@@ -981,3 +981,16 @@ def test_evict_does_not_write_the_lengths_it_reads(fl):
             kv.evict(cache, dev(torch, table), words[:2], *args, new_lens=new_lens)
     kv.evict(cache, dev(torch, table), words[:2], *args, new_lens=words[2:])
     assert words.tolist() == [x, x, 20, 20] and int(args[-1]) == 0
+
+
+def test_evict_does_not_pack_into_the_pages_it_reads(fl):
+    core, kv, torch = fl
+    T, H, D, x = 16, 2, 64, 40
+    cache, c, table = make(fl, np.random.default_rng(2), [x, x], T, H, D)
+    d_table, lens, status = dev(torch, table), dev(torch, np.array([x, x], np.int32)), core.new_status()
+    w, before = torch.ones(2, H, x, device="cuda"), cache.pages.clone()
+    with pytest.raises(ValueError, match="new pages"):
+        kv.evict(cache, d_table, lens, w, 20, cache, d_table, status)
+    other = kv.PageCache(torch.zeros_like(cache.pages), T, H, D)
+    kv.evict(cache, d_table, lens, w, 20, other, d_table, status)            # the same numbers in another pool are other pages
+    assert int(status) == 0 and torch.equal(before, cache.pages) and int(other.pages[int(table[0, 0])].sum()) > 0

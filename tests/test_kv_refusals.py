@@ -172,3 +172,8 @@ def test_evict_lengths_in_place(lib, shift):
     """The new lengths of 2 sequences written over what the call's other workgroups may still read."""
     assert lib.flh_kv_evict(C.byref(apart(d_new_lens=(1 << 41) + shift)), None) == E_ARG
     assert b"overlap" in lib.flh_last_error()
+
+
+def test_evict_onto_the_pages_that_are_read(lib):
+    assert lib.flh_kv_evict(C.byref(apart(d_to_table=1 << 42, to=cache())), None) == E_ARG
+    assert b"new pages are those" in lib.flh_last_error()
