@@ -1824,6 +1824,7 @@ __global__ __launch_bounds__(NT) void fl_kv_keep(const KeepArgs a) {
 // host side
 // ------------------------------------------------------------------------------------------------
 constexpr uint32_t kMaxPages = (1u << 23) - 1;   // of a sequence: positions fit 31 bits
+constexpr uint32_t kMaxWidth = 0x7fffffffu;      // of a row that is written to its end: an index that strides past it must not wrap
 
 bool aligned(const void* p, uint64_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 bool overlap(const void* a, const void* b, uint64_t bytes) { return (uintptr_t)a < (uintptr_t)b + bytes && (uintptr_t)b < (uintptr_t)a + bytes; }
@@ -2065,7 +2066,7 @@ int flh_kv_attend(const flh_kv_attend_params* p, void* stream) {
   if (p->d_selected && (p->n_selected == 0 || p->n_selected > kMaxPages)) return fl_set_error(FLH_E_ARG, "flh_kv_attend: %u selected pages", p->n_selected);
   if (p->d_selected && p->d_weights) return fl_set_error(FLH_E_ARG, "flh_kv_attend: weights are kept over all pages, not over selected ones");
   if (!p->d_weights && p->d_weights_in) return fl_set_error(FLH_E_ARG, "flh_kv_attend: weights to start from, but none to write");
-  if (p->d_weights && p->weights_width == 0) return fl_set_error(FLH_E_ARG, "flh_kv_attend: weights of no positions");
+  if (p->d_weights && (p->weights_width == 0 || p->weights_width > kMaxWidth)) return fl_set_error(FLH_E_ARG, "flh_kv_attend: weights of %u positions (1..2^31 - 1)", p->weights_width);
   Plan pl;
   if ((rc = make_plan(p, &pl))) return rc;
   if (pl.bytes && (!p->d_workspace || !aligned(p->d_workspace, 16) || p->workspace_bytes < pl.bytes))
@@ -2121,7 +2122,7 @@ int flh_kv_select(const flh_kv_select_params* p, void* stream) {
   if (rc) return rc;
   if (p->type != FLH_KV_BF16 && p->type != FLH_KV_FP16) return fl_set_error(FLH_E_ARG, "flh_kv_select: type %u (bf16 or fp16)", p->type);
   if (p->q_heads == 0 || p->q_heads % p->cache.heads) return fl_set_error(FLH_E_ARG, "flh_kv_select: %u query heads over %u key-value heads", p->q_heads, p->cache.heads);
-  if (p->count == 0 || (uint64_t)p->first + p->last > p->count) return fl_set_error(FLH_E_ARG, "flh_kv_select: %u pages with %u first and %u last ones", p->count, p->first, p->last);
+  if (p->count == 0 || p->count > kMaxWidth || (uint64_t)p->first + p->last > p->count) return fl_set_error(FLH_E_ARG, "flh_kv_select: %u pages with %u first and %u last ones", p->count, p->first, p->last);
   if (p->seqs.n_tokens > 65535 || (uint64_t)p->seqs.n_tokens * p->cache.heads > kMaxGroups / 4)
     return fl_set_error(FLH_E_ARG, "flh_kv_select: %u tokens of %u heads in one call (up to 65535, and 2^22 - 1 rows)", p->seqs.n_tokens, p->cache.heads);
   if (p->seqs.n_tokens == 0) return FLH_OK;
@@ -2182,7 +2183,8 @@ int flh_kv_evict(const flh_kv_evict_params* p, void* stream) {
   const uint32_t per = (p->budget + a.c.T - 1) / a.c.T;
   if (p->to_table_width < per || p->to_table_stride < p->to_table_width)
     return fl_set_error(FLH_E_ARG, "flh_kv_evict: %u tokens need %u pages, the new table has %u", p->budget, per, p->to_table_width);
-  if (p->weights_width == 0 || p->new_weights_width < p->budget) return fl_set_error(FLH_E_ARG, "flh_kv_evict: weights of %u positions, new ones of %u", p->weights_width, p->new_weights_width);
+  if (p->weights_width == 0 || p->weights_width > kMaxWidth || p->new_weights_width < p->budget || p->new_weights_width > kMaxWidth)
+    return fl_set_error(FLH_E_ARG, "flh_kv_evict: weights of %u positions, new ones of %u", p->weights_width, p->new_weights_width);
   if (p->d_to_table == p->seqs.d_table && a.c.pages == a.from.pages) return fl_set_error(FLH_E_ARG, "flh_kv_evict: the new pages are those that are read");
   // (the workgroups of the other heads still read a length when the first one's writes the new one)
   if (overlap(p->d_new_lens, p->seqs.d_lens, 4ull * a.s.n_seqs)) return fl_set_error(FLH_E_ARG, "flh_kv_evict: the new lengths overlap the lengths");

@@ -512,8 +512,9 @@ void* flh_region_translate(const flh_region* r, uint32_t lane, const void* data)
  * with them is found there: FLH_E_RANGE is stored to *d_status for a page number outside the pool (the page is not
  * written; its keys are not seen), a length the table (or the weights) cannot hold (cut off), or starts that leave the call's
  * tokens or descend (the sequence is skipped).  Nothing is read or written out of bounds.  All entry points only launch: they
- * neither allocate nor wait and can be captured into a graph.  What a call writes overlaps nothing that it reads but where it
- * says so, and a workspace belongs to one call at a time: calls on two streams, or graphs that may run at once, need one each. */
+ * neither allocate nor wait and can be captured into a graph.  Positions, budgets and counts of pages are below 2^31.  What a
+ * call writes overlaps nothing that it reads but where it says so, and a workspace belongs to one call at a time: calls on
+ * two streams, or graphs that may run at once, need one each. */
 #define FLH_KV_BF16 0u
 #define FLH_KV_FP16 1u
 #define FLH_KV_FP32 2u

@@ -177,3 +177,11 @@ def test_evict_lengths_in_place(lib, shift):
 def test_evict_onto_the_pages_that_are_read(lib):
     assert lib.flh_kv_evict(C.byref(apart(d_to_table=1 << 42, to=cache())), None) == E_ARG
     assert b"new pages are those" in lib.flh_last_error()
+
+
+@pytest.mark.parametrize("width", [1 << 31, (1 << 32) - 1024, (1 << 32) - 1])
+def test_widths_past_31_bits(lib, width):
+    """Rows that a workgroup walks to their end, by strides that would wrap around."""
+    for op, p in (("flh_kv_select", select(count=width)), ("flh_kv_attend", attend(d_weights=P, weights_width=width)),
+                  ("flh_kv_evict", apart(weights_width=width)), ("flh_kv_evict", apart(new_weights_width=width))):
+        assert getattr(lib, op)(C.byref(p), None) == E_ARG
