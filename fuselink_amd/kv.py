@@ -144,24 +144,24 @@ def _queries(cache: PageCache, q: torch.Tensor):
 
 class _On:
     """Device and stream of a call that names a stream, or whose tensors are not on the current device: allocations inside belong
-    to the stream, and the tensors given are marked as used on it."""
+    to the stream, and the tensors given (all found sound by then) are marked as used on it."""
 
     def __init__(self, cache: PageCache, stream: Optional[torch.cuda.Stream], *tensors):
-        self.stack = contextlib.ExitStack()
-        if stream is None:
-            self.stack.enter_context(torch.cuda.device(cache.device))
-            self.ptr = torch.cuda.current_stream(cache.device).cuda_stream
-            return
-        _need(stream.device == cache.device, f"stream of {stream.device}, tensors of {cache.device}")
-        self.stack.enter_context(torch.cuda.stream(stream))
-        self.ptr = stream.cuda_stream
-        if not torch.cuda.is_current_stream_capturing():
-            for t in tensors:
-                if t is not None:
-                    t.record_stream(stream)
+        _need(stream is None or stream.device == cache.device, f"stream of {stream and stream.device}, tensors of {cache.device}")
+        self.cache, self.stream, self.tensors, self.stack = cache, stream, tensors, contextlib.ExitStack()
 
     def __enter__(self):
-        return self.ptr
+        if self.stream is None:
+            self.stack.enter_context(torch.cuda.device(self.cache.device))
+            return torch.cuda.current_stream(self.cache.device).cuda_stream
+        with contextlib.ExitStack() as stack:      # (undone if anything below raises)
+            stack.enter_context(torch.cuda.stream(self.stream))
+            if not torch.cuda.is_current_stream_capturing():
+                for t in self.tensors:
+                    if t is not None:
+                        t.record_stream(self.stream)
+            self.stack = stack.pop_all()
+        return self.stream.cuda_stream
 
     def __exit__(self, *exc):
         self.stack.close()
@@ -186,17 +186,22 @@ def _on(cache: PageCache, stream, *tensors):
     return _On(cache, stream, *tensors)
 
 
+def _check_workspace(cache: PageCache, given: Optional[torch.Tensor], need: int) -> Optional[torch.Tensor]:
+    """The workspace that the caller gives, if the call needs one."""
+    if given is None or need == 0:
+        return None
+    _need(given.get_device() == cache.index and given.is_contiguous() and given.numel() * given.element_size() >= need and given.data_ptr() % 16 == 0,
+          f"workspace: {need} contiguous bytes on {cache.device}, 16-byte aligned")
+    return given
+
+
 def _workspace(cache: PageCache, given: Optional[torch.Tensor], need: int):
     """Address and bytes of a workspace, and what owns it."""
     if need == 0:
         return 0, 0, None
     if given is None:
         given = torch.empty(need, dtype=torch.uint8, device=cache.device)
-        return given.data_ptr(), need, given
-    nbytes = given.numel() * given.element_size()
-    _need(given.get_device() == cache.index and given.is_contiguous() and nbytes >= need and given.data_ptr() % 16 == 0,
-          f"workspace: {need} contiguous bytes on {cache.device}, 16-byte aligned")
-    return given.data_ptr(), nbytes, given
+    return given.data_ptr(), given.numel() * given.element_size(), given
 
 
 def store(cache: PageCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor, status: torch.Tensor, *,
@@ -251,26 +256,30 @@ def attend(cache: PageCache, q: torch.Tensor, page_table: torch.Tensor, lens: to
             _need((win_p == w_p and (wis, wih) == (ws, wh)) or _apart(weights, weights_in), "weights and weights_in overlap without being the same")
     else:
         _need(weights_in is None, "weights_in without weights")
+    if out is not None:
+        _check(cache, "out", out, q.dtype, 3)
+        _check_written("out", out)
+        _need(out.shape == q.shape, f"out {tuple(out.shape)} for q {tuple(q.shape)}")
+        _need(_apart(out, q), "out overlaps q")
     lib = _lib.load()
+
+    def block(out_p, ot, oh, wp, wb):
+        return _ATTEND.pack(*cache.c, *seqs, q.data_ptr(), out_p, qt, qh, ot, oh, lse_p, kind, hq, 1.0 / math.sqrt(cache.dim) if scale is None else scale,
+                            1 if causal else 0, sel_p, win_p, w_p, wis, wih, ws, wh, count, width, wp, wb, word)
+
+    sizes = (cache.c[3:], seqs[4:7], seqs[0] != 0, hq, count, w_p != 0)
+    need = _needs.get(sizes)
+    if need is None:
+        if len(_needs) >= 4096:
+            _needs.clear()
+        need = _needs[sizes] = check(lib.flh_kv_attend_workspace_bytes(block(0, 0, 0, 0, 0)))
+    workspace = _check_workspace(cache, workspace, need)
     with _on(cache, stream, cache.pages, q, page_table, lens, status, starts, lse, selected, weights, weights_in, out, workspace) as sp:
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        else:
-            _check(cache, "out", out, q.dtype, 3)
-            _check_written("out", out)
-            _need(out.shape == q.shape, f"out {tuple(out.shape)} for q {tuple(q.shape)}")
-            _need(_apart(out, q), "out overlaps q")
         ot, oh, _ = out.stride()
-        head = (*cache.c, *seqs, q.data_ptr(), out.data_ptr(), qt, qh, ot, oh, lse_p, kind, hq,
-                1.0 / math.sqrt(cache.dim) if scale is None else scale, 1 if causal else 0, sel_p, win_p, w_p, wis, wih, ws, wh, count, width)
-        sizes = (cache.c[3:], seqs[4:7], seqs[0] != 0, hq, count, w_p != 0)
-        need = _needs.get(sizes)
-        if need is None:
-            if len(_needs) >= 4096:
-                _needs.clear()
-            need = _needs[sizes] = check(lib.flh_kv_attend_workspace_bytes(_ATTEND.pack(*head, 0, 0, word)))
         wp, wb, owner = _workspace(cache, workspace, need)
-        check(lib.flh_kv_attend(_ATTEND.pack(*head, wp, wb, word), sp))
+        check(lib.flh_kv_attend(block(out.data_ptr(), ot, oh, wp, wb), sp))
     return out
 
 
@@ -285,13 +294,15 @@ def select_pages(cache: PageCache, q: torch.Tensor, page_table: torch.Tensor, le
     n, hq, qt, qh, kind = _queries(cache, q)
     _need(0 < count < 2 ** 31 and first >= 0 and last >= 0 and first + last <= count, f"{count} pages with {first} first and {last} last ones")
     seqs, word = _seqs(cache, page_table, lens, status, starts, n)
+    if out is not None:
+        shape, _ = _check(cache, "out", out, _I32, 3)
+        _need(out.is_contiguous() and tuple(shape) == (n, cache.heads, count), f"out: contiguous [{n}, {cache.heads}, {count}]")
+    need = 4 * n * cache.heads * seqs[4]         # flh_kv_select_workspace_bytes
+    workspace = _check_workspace(cache, workspace, need)
     with _on(cache, stream, cache.pages, q, page_table, lens, status, starts, out, workspace) as sp:
         if out is None:
             out = torch.empty((n, cache.heads, count), dtype=_I32, device=cache.device)
-        else:
-            shape, _ = _check(cache, "out", out, _I32, 3)
-            _need(out.is_contiguous() and tuple(shape) == (n, cache.heads, count), f"out: contiguous [{n}, {cache.heads}, {count}]")
-        wp, wb, owner = _workspace(cache, workspace, 4 * n * cache.heads * seqs[4])     # flh_kv_select_workspace_bytes
+        wp, wb, owner = _workspace(cache, workspace, need)
         check(_lib.load().flh_kv_select(_SELECT.pack(*cache.c, *seqs, q.data_ptr(), qt, qh, kind, hq, count, first, last, 1 if causal else 0,
                                                      out.data_ptr(), wp, wb, word), sp))
     return out
@@ -315,27 +326,28 @@ def evict(cache: PageCache, page_table: torch.Tensor, lens: torch.Tensor, weight
         stride = to_width
     _need(tb == b and to_width >= (budget + to.tokens - 1) // to.tokens and stride >= to_width, f"to_table: [{b}, >= {(budget + to.tokens - 1) // to.tokens}]")
     _need(to_table.data_ptr() != page_table.data_ptr() or to.c[0] != cache.c[0], "to_table is page_table: the new pages must not be among those that are read")
+    if kept is not None:
+        shape, _ = _check(cache, "kept", kept, _I32, 3)
+        _need(kept.is_contiguous() and tuple(shape) == (b, h, budget), f"kept: contiguous [{b}, {h}, {budget}]")
+    if new_weights is not None:
+        (nb, nhh, nw), (ns, nh, _) = _check(cache, "new_weights", new_weights, _F32, 3)
+        _check_written("new_weights", new_weights)
+        _need(nb == b and nhh == h and nw >= budget, f"new_weights: [{b}, {h}, >= {budget}]")
+        _need(_apart(new_weights, weights), "new_weights overlaps weights")
+    else:
+        ns, nh, nw = h * budget, budget, budget
+    if new_lens is not None:
+        (nl,), _ = _check(cache, "new_lens", new_lens, _I32, 1)
+        _check_written("new_lens", new_lens)
+        _need(nl == b, f"new_lens: [{b}]")
+        _need(_apart(new_lens, lens), "new_lens overlaps lens")
     with _on(cache, stream, cache.pages, to.pages, page_table, lens, weights, to_table, status, kept, new_weights, new_lens) as sp:
         if kept is None:
             kept = torch.empty((b, h, budget), dtype=_I32, device=cache.device)
-        else:
-            shape, _ = _check(cache, "kept", kept, _I32, 3)
-            _need(kept.is_contiguous() and tuple(shape) == (b, h, budget), f"kept: contiguous [{b}, {h}, {budget}]")
         if new_weights is None:
             new_weights = torch.empty((b, h, budget), dtype=_F32, device=cache.device)
-            ns, nh, nw = h * budget, budget, budget
-        else:
-            (nb, nhh, nw), (ns, nh, _) = _check(cache, "new_weights", new_weights, _F32, 3)
-            _check_written("new_weights", new_weights)
-            _need(nb == b and nhh == h and nw >= budget, f"new_weights: [{b}, {h}, >= {budget}]")
-            _need(_apart(new_weights, weights), "new_weights overlaps weights")
         if new_lens is None:
             new_lens = torch.empty(b, dtype=_I32, device=cache.device)
-        else:
-            (nl,), _ = _check(cache, "new_lens", new_lens, _I32, 1)
-            _check_written("new_lens", new_lens)
-            _need(nl == b, f"new_lens: [{b}]")
-            _need(_apart(new_lens, lens), "new_lens overlaps lens")
         check(_lib.load().flh_kv_evict(_EVICT.pack(*cache.c, *to.c, *seqs, to_table.data_ptr(), stride, weights.data_ptr(), ws_s, ws_h,
                                                    new_weights.data_ptr(), ns, nh, kept.data_ptr(), new_lens.data_ptr(), to_width, width, nw,
                                                    budget, first, recent, word), sp))

@@ -994,3 +994,31 @@ def test_evict_does_not_pack_into_the_pages_it_reads(fl):
     other = kv.PageCache(torch.zeros_like(cache.pages), T, H, D)
     kv.evict(cache, d_table, lens, w, 20, other, d_table, status)            # the same numbers in another pool are other pages
     assert int(status) == 0 and torch.equal(before, cache.pages) and int(other.pages[int(table[0, 0])].sum()) > 0
+
+
+def test_refused_calls_leave_the_stream_alone(fl):
+    """What is refused on a named stream is refused as elsewhere, and the caller's stream stays the current one."""
+    core, kv, torch = fl
+    T, H, G, D, x = 16, 2, 4, 64, 40
+    rng = np.random.default_rng(2)
+    cache, c, table = make(fl, rng, [x, x], T, H, D)
+    q = dev(torch, rng.standard_normal((2, H * G, D)), torch.float32).to(torch.bfloat16)
+    d_table, lens, status = dev(torch, table), dev(torch, np.array([x, x], np.int32)), core.new_status()
+    w = torch.ones(2, H, 64, device="cuda")
+    to = kv.PageCache(torch.zeros(4, kv.page_bytes(T, H, D), dtype=torch.uint8, device="cuda"), T, H, D)
+    to_table = dev(torch, np.arange(4, dtype=np.int32).reshape(2, 2))
+    side, here = torch.cuda.Stream(), torch.cuda.current_stream()
+    host = lambda dtype, *shape: torch.zeros(*shape, dtype=dtype)
+    evict = lambda **kw: kv.evict(cache, d_table, lens, w, 20, to, to_table, status, **kw)
+    calls = [lambda **kw: kv.attend(cache, q, d_table, lens, status, out=q.cpu(), **kw),
+             lambda **kw: kv.attend(cache, q, d_table, lens, status, weights=w, workspace=host(torch.uint8, 1 << 20), **kw),
+             lambda **kw: kv.select_pages(cache, q, d_table, lens, 2, status, out=host(torch.int32, 2, H, 2), **kw),
+             lambda **kw: kv.select_pages(cache, q, d_table, lens, 2, status, workspace=host(torch.uint8, 1 << 20), **kw),
+             lambda **kw: evict(kept=host(torch.int32, 2, H, 20), **kw), lambda **kw: evict(new_weights=host(torch.float32, 2, H, 20), **kw),
+             lambda **kw: evict(new_lens=host(torch.int32, 2), **kw)]
+    for call in calls:
+        for kw in ({}, dict(stream=side)):
+            with pytest.raises(ValueError):
+                call(**kw)
+            assert torch.cuda.current_stream() == here
+    assert int(status) == 0
