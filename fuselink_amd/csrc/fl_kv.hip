@@ -82,9 +82,9 @@ __device__ __forceinline__ uint32_t uniform_len(const Seqs& s, uint32_t T, uint3
 // Item x of the sequences' items laid end to end: its sequence, which of that one's items it is, and the sequence's
 // tokens.  A wavefront looks at 64 sequences at a time, all it needs to know of them loaded at once.  False if there
 // are fewer items.  LONGEST: the sequences of 64 are laid out by length, the longest first, so that what is handed out
-// last is short.
+// last is short.  APPEND: tokens go behind the length, so a negative one (empty otherwise) leaves them no place.
 struct Item { uint32_t b, local, first, n, len; };
-template <bool LONGEST = false, class Count>
+template <bool LONGEST = false, bool APPEND = false, class Count>
 __device__ __forceinline__ bool find_item(const Seqs& s, uint32_t T, uint32_t x, Count count, Item& it) {
   const int lane = threadIdx.x & 63;
   for (uint32_t base = 0; base < s.n_seqs; base += 64) {
@@ -95,6 +95,7 @@ __device__ __forceinline__ bool find_item(const Seqs& s, uint32_t T, uint32_t x,
       const uint32_t most = s.width * T;   // (the host keeps it within 31 bits)
       len = held < 0 ? 0u : (uint32_t)held > most ? most : (uint32_t)held;
       if ((uint32_t)held != len) report(s.status);
+      if (APPEND && held < 0) n = 0;
       c = count(n, len);
     }
     uint32_t incl = wave_incl_sum_u32(c, lane);
@@ -337,7 +338,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fl_kv_pack(const PackAr
     page = scalar_load(a.to_table + b * a.to_stride + j);
   } else {
     Item it;
-    if (!find_item(a.s, T, blockIdx.x, [&](uint32_t m, uint32_t l) { return m ? (l + m + T - 1) / T - l / T : 0; }, it)) return;
+    if (!find_item<false, true>(a.s, T, blockIdx.x, [&](uint32_t m, uint32_t l) { return m ? (l + m + T - 1) / T - l / T : 0; }, it)) return;
     b = it.b;
     first = it.first;
     n = it.n;

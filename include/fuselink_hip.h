@@ -510,11 +510,12 @@ void* flh_region_translate(const flh_region* r, uint32_t lane, const void* data)
  * tokens it holds, d_starts (n_seqs + 1 ascending, or NULL for n_tokens / n_seqs each) which of the call's n_tokens tokens are its
  * own; tokens before the first and behind the last start are left alone.  These live on the device, so what is wrong
  * with them is found there: FLH_E_RANGE is stored to *d_status for a page number outside the pool (the page is not
- * written; its keys are not seen), a length the table (or the weights) cannot hold (cut off), or starts that leave the call's
- * tokens or descend (the sequence is skipped).  Nothing is read or written out of bounds.  All entry points only launch: they
- * neither allocate nor wait and can be captured into a graph.  Positions, budgets and counts of pages are below 2^31.  What a
- * call writes overlaps nothing that it reads but where it says so, and a workspace belongs to one call at a time: calls on
- * two streams, or graphs that may run at once, need one each. */
+ * written; its keys are not seen), a length the table (or the weights) cannot hold (cut off; a negative one
+ * counts as 0), or starts that leave the call's tokens or descend (the sequence is skipped; tokens that starts behind a descent
+ * give to a second sequence are not defined in either).  Nothing is read or written out of bounds.  All entry points only
+ * launch: they neither allocate nor wait and can be captured into a graph.  Positions, budgets and counts of pages are below
+ * 2^31.  What a call writes overlaps nothing that it reads but where it says so, and a workspace belongs to one call at a
+ * time: calls on two streams, or graphs that may run at once, need one each. */
 #define FLH_KV_BF16 0u
 #define FLH_KV_FP16 1u
 #define FLH_KV_FP32 2u
@@ -544,7 +545,8 @@ uint64_t flh_kv_page_bytes(uint32_t tokens, uint32_t heads, uint32_t dim);
 /* Appends the call's keys and values [n_tokens][heads][dim] (strides in elements, channels contiguous) to their
  * sequences, which hold d_lens tokens before it.  A page that holds tokens already keeps its scale unless the new ones
  * need a larger one; its codes are then rounded once more.  The slots behind the last token are zero in a page that the
- * call opens.  A page may be written by one sequence of a call only. */
+ * call opens.  A page may be written by one sequence of a call only.  Tokens that the table has no page for, and all of a
+ * sequence of a negative length, are not stored. */
 typedef struct flh_kv_store_params {
   flh_kv_cache cache;
   flh_kv_seqs  seqs;

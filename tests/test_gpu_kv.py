@@ -1022,3 +1022,19 @@ def test_refused_calls_leave_the_stream_alone(fl):
                 call(**kw)
             assert torch.cuda.current_stream() == here
     assert int(status) == 0
+
+
+@pytest.mark.parametrize("n0", [-1, -2 ** 31])
+def test_store_skips_a_sequence_of_negative_length(fl, n0):
+    """Nothing of such a sequence is written, above all not its first tokens; the others' tokens are stored."""
+    core, kv, torch = fl
+    T, H, D = 16, 2, 64
+    rng = np.random.default_rng(4)
+    cache, c, table = make(fl, rng, [48, 30, 17], T, H, D)
+    exp = held(cache, T, H, D)
+    k, v = (dev(torch, rng.standard_normal((6, H, D)), torch.float32) for _ in range(2))
+    status = core.new_status()
+    kv.store(cache, k, v, dev(torch, table), dev(torch, np.array([n0, 30, 17], np.int32)), status)
+    assert int(status) == E_RANGE
+    ref.store(exp, k.cpu().double().numpy(), v.cpu().double().numpy(), table, [48, 30, 17], [2, 2, 4, 6])
+    same_cache(held(cache, T, H, D), exp)
