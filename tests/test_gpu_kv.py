@@ -1038,3 +1038,63 @@ def test_store_skips_a_sequence_of_negative_length(fl, n0):
     assert int(status) == E_RANGE
     ref.store(exp, k.cpu().double().numpy(), v.cpu().double().numpy(), table, [48, 30, 17], [2, 2, 4, 6])
     same_cache(held(cache, T, H, D), exp)
+
+
+STARTS = [[0, 3, 2], [-1, 1, 2], [0, 1, 5], [0, 2 ** 31 - 1, 2], [0, -2 ** 31, 2], [0, 2, 9, 3], [1, 3, -1, 4], [5, 5, 6, 4]]
+
+
+@pytest.mark.parametrize("starts", STARTS, ids=str)
+@pytest.mark.parametrize("H,G", [(1, 2), (33, 210)])
+def test_bad_starts(fl, starts, H, G):
+    """Each entry point reports starts that leave the call's tokens or descend, skips those sequences and serves the others."""
+    core, kv, torch = fl
+    T, D = 16, 32
+    B, lens = len(starts) - 1, [48, 30, 20][:len(starts) - 1]
+    n = 2 if B == 2 else 4
+    rng = np.random.default_rng(4)
+    cache, c, table = make(fl, rng, lens, T, H, D)
+    ok = [0 <= a <= b <= n for a, b in zip(starts, starts[1:])]
+    news = [b - a if o else 0 for a, b, o in zip(starts, starts[1:], ok)]
+    tok = [range(a, b) if o else range(0) for a, b, o in zip(starts, starts[1:], ok)]
+    order = [i for t in tok for i in t]                       # the tokens that are somebody's, sequence by sequence
+    packed = np.concatenate([[0], np.cumsum(news)])
+    d_table, d_lens, d_starts = dev(torch, table), dev(torch, np.array(lens, np.int32)), dev(torch, np.array(starts, np.int32))
+    q = dev(torch, rng.standard_normal((n, H * G, D)), torch.float32).to(torch.bfloat16)
+    qn = q.cpu().double().numpy()[order]
+    nobody = [i for i in range(n) if i not in order]
+
+    status, w_in = core.new_status(), torch.rand(B, H, 50, device="cuda")
+    out, lse, w = torch.full_like(q, 7.0), torch.full((n, H * G), 7.0, device="cuda"), torch.full_like(w_in, -1.0)
+    kv.attend(cache, q, d_table, d_lens, status, starts=d_starts, out=out, lse=lse, weights=w, weights_in=w_in)
+    assert int(status) == E_RANGE and (out[nobody] == 7).all() and (lse[nobody] == 7).all()
+    r = ref.attend(c, qn, table, lens, packed, 1 / np.sqrt(D))
+    check_out(torch, out[order], lse[order], r, torch.bfloat16, lens, packed)
+    got, base = (x.cpu().double().numpy() for x in (w, w_in))
+    for b, x in enumerate(lens):
+        tol = r["wslack"][b] * 1.1 + (r["weights"][b] + base[b, :, :x]) * (n * G + 64) * 2.0 ** -23
+        assert (np.abs(got[b, :, :x] - base[b, :, :x] - r["weights"][b]) <= tol).all()
+        np.testing.assert_array_equal(got[b, :, x:], base[b, :, x:])
+
+    status.zero_()
+    sel = torch.full((n, H, 2), -7, dtype=torch.int32, device="cuda")
+    kv.select_pages(cache, q, d_table, d_lens, 2, status, starts=d_starts, out=sel)
+    assert int(status) == E_RANGE and (sel[nobody] == -7).all()
+    exp = ref.select(c, qn, table, lens, packed, 2, 1, 1)
+    np.testing.assert_array_equal(sel.cpu().numpy()[order], exp)
+
+    status.zero_()
+    out.fill_(7.0)
+    kv.attend(cache, q, d_table, d_lens, status, starts=d_starts, out=out, selected=sel)
+    assert int(status) == E_RANGE and (out[nobody] == 7).all()
+    check_out(torch, out[order], None, ref.attend(c, qn, table, lens, packed, 1 / np.sqrt(D), selected=exp), torch.bfloat16, lens, packed)
+
+    status.zero_()
+    before, c2 = cache.pages.clone(), held(cache, T, H, D)
+    k, v = (dev(torch, rng.standard_normal((n, H, D)), torch.float32) for _ in range(2))
+    had = [x - 4 for x in lens]
+    kv.store(cache, k, v, d_table, dev(torch, np.array(had, np.int32)), status, starts=d_starts)
+    assert int(status) == E_RANGE
+    ref.store(c2, k.cpu().double().numpy()[order], v.cpu().double().numpy()[order], table, had, packed)
+    same_cache(held(cache, T, H, D), c2)
+    mine = {int(table[b, p // T]) for b in range(B) for p in range(had[b], had[b] + news[b])}
+    assert set((before != cache.pages).any(1).nonzero().flatten().tolist()) <= mine
