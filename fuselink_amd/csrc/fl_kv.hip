@@ -581,7 +581,6 @@ __device__ __forceinline__ void clear(Rows<NQ, VJ>& r, const uint32_t (&lim)[NQ]
   r.ev = r.elow = 0;
   r.fresh = true;
 }
-__device__ __forceinline__ float scale_of(int ev) { return ev > 0 ? __uint_as_float((uint32_t)ev << 23) : 0.f; }
 
 // One step of the softmax: scores of 32 keys (two tiles under K scales kc0 and kc1, base 2, and value scales v0 and v1) to
 // probabilities and their sums.
@@ -955,14 +954,16 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) 
   if (bad && lane == 0) report(a.s.status);
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
-    const float l = column_sum(st.l[q]), vref = scale_of(st.ev);
-    const int w = (int)wave * 16 * NQ + q * 16 + c;
+    // O is the sum l times an average of values, in units of their scale, and may pass an end of the range that the average
+    // keeps within: the scale goes on together with the power of two of l, which the factors below give back.
+    const float l = column_sum(st.l[q]);
+    const int w = (int)wave * 16 * NQ + q * 16 + c, e = st.ev - 127 - __builtin_amdgcn_frexp_expf(l);
     if (g == 0) { sm_m[w] = l == 0.f ? -kInf : st.ref[q]; sm_l[w] = l; }
     float* p = sm_o + w * (DP + 4) + g * 4 * VJ;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < VJ; ++j) p[i * VJ + j] = st.o[q][j][i] * vref;
+      for (int j = 0; j < VJ; ++j) p[i * VJ + j] = __builtin_amdgcn_ldexpf(st.o[q][j][i], e);
   }
   __syncthreads();
   for (uint32_t u = threadIdx.x; u < 16 * NQ * (DP / 8); u += 256) {
@@ -972,16 +973,20 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) 
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = 0.f;
     for (uint32_t w = 0; w < KVW; ++w) mm = fmaxf(mm, sm_m[w * 16 * NQ + rr]);
-    for (uint32_t w = 0; w < KVW; ++w) {
-      const float f = mm == -kInf ? 1.f : exp2_fast(sm_m[w * 16 * NQ + rr] - mm);
-      ll += sm_l[w * 16 * NQ + rr] * f;
-      const float* p = sm_o + (w * 16 * NQ + rr) * (DP + 4) + d;
+    float share[KVW];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += p[e] * f;
+    for (uint32_t w = 0; w < KVW; ++w) {
+      const float l = sm_l[w * 16 * NQ + rr], f = mm == -kInf ? 1.f : exp2_fast(sm_m[w * 16 * NQ + rr] - mm);
+      ll += l * f;
+      share[w] = __builtin_amdgcn_ldexpf(f, __builtin_amdgcn_frexp_expf(l));
     }
     const float f = ll == 0.f ? 0.f : 1.f / ll;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] *= f;
+    for (uint32_t w = 0; w < KVW; ++w) {
+      const float* p = sm_o + (w * 16 * NQ + rr) * (DP + 4) + d;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += p[e] * (share[w] * f);
+    }
     emit8<E>(a, split, first, h, r, mm, ll, v, d, d == 0);
   }
 }
@@ -1191,13 +1196,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void fl_kv_attend_rows(cons
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
     const uint32_t r = wr0 + q * 16 + c;
-    const float l = column_sum(st.l[q]), f = l == 0.f ? 0.f : scale_of(st.ev) / l;
+    const float l = column_sum(st.l[q]), f = l == 0.f ? 0.f : 1.f / l;   // (then the scale: together they may leave the range)
     if (r >= rows) continue;
     float v[4 * VJ];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < VJ; ++j) v[i * VJ + j] = st.o[q][j][i] * f;
+      for (int j = 0; j < VJ; ++j) v[i * VJ + j] = __builtin_amdgcn_ldexpf(st.o[q][j][i] * f, st.ev - 127);
 #pragma unroll
     for (int u = 0; u < 4 * VJ; u += 8) emit8<E>(a, split, first, h, r, l == 0.f ? -kInf : st.ref[q], l, v + u, g * 4 * VJ + u, g == 0 && u == 0);
   }
@@ -1251,7 +1256,7 @@ __global__ __launch_bounds__(256) void fl_kv_join(const AttendArgs a, uint32_t T
 #pragma unroll
   for (uint32_t k = 0; k < kMostSplits / 64; ++k) {
     if (64 * k >= a.splits) break;
-    const float w = part[k] == -kInf ? 0.f : exp2_fast(part[k] - base);
+    const float w = part[k] == -kInf ? 0.f : exp2_fast(part[k] - base) * (1.f / kMostSplits);   // (no sum of them passes what it averages)
     sum += w;
     const uint32_t cnt = a.splits - 64 * k < 64 ? a.splits - 64 * k : 64;
     // A share of no keys has a weight of 0 and may have written no row: what is read for it is not used.
@@ -1280,7 +1285,7 @@ __global__ __launch_bounds__(256) void fl_kv_join(const AttendArgs a, uint32_t T
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     for (uint32_t o = DL; o < 64; o <<= 1) acc[e] += __shfl_xor(acc[e], (int)o);
-  const float f = sum == 0.f ? 0.f : 1.f / sum, lg = sum == 0.f ? -kInf : base + __builtin_amdgcn_logf(sum);
+  const float f = sum == 0.f ? 0.f : 1.f / sum, lg = sum == 0.f ? -kInf : base + __builtin_amdgcn_logf(sum * kMostSplits);
   if (lane == 0) {
     if (a.lse) a.lse[at] = lg * 0.6931471805599453f;
     if (a.lse2) a.lse2[at] = lg;

@@ -1098,3 +1098,25 @@ def test_bad_starts(fl, starts, H, G):
     same_cache(held(cache, T, H, D), c2)
     mine = {int(table[b, p // T]) for b in range(B) for p in range(had[b], had[b] + news[b])}
     assert set((before != cache.pages).any(1).nonzero().flatten().tolist()) <= mine
+
+
+@pytest.mark.parametrize("size", [1e38, 1e-35, 1e-36])
+@pytest.mark.parametrize("n,x,H,G,D", [(1, 50, 2, 4, 64), (1, 9000, 1, 2, 64), (20, 200, 2, 4, 128), (20, 1500, 2, 4, 128), (3, 300, 1, 2, 256), (40, 90, 65, 4, 128), (40, 600, 65, 4, 128),
+                                       (100, 400, 1, 4, 256)])
+def test_attend_values_near_the_ends_of_the_range(fl, size, n, x, H, G, D):
+    """Outputs are averages of the values: where those are representable, so are these, whatever the sums pass on the way."""
+    core, kv, torch = fl
+    T = 16
+    rng = np.random.default_rng(n + x)
+    k, v = rng.standard_normal((x, H, D)), rng.uniform(0.5, 2, (x, H, D)) * size
+    table, pages = tables(rng, [x], T)
+    c = ref.empty(pages, T, H, D)
+    ref.store(c, k, v, table, [0], [0, x])
+    cache = records(fl, c, T, H, D, [x], table)
+    q = dev(torch, rng.standard_normal((n, H * G, D)), torch.float32).to(torch.bfloat16)
+    status = core.new_status()
+    out = kv.attend(cache, q, dev(torch, table), dev(torch, np.array([x], np.int32)), status).cpu().double().numpy()
+    r = ref.attend(c, q.cpu().double().numpy(), table, [x], [0, n], 1 / np.sqrt(D))
+    # all values are within a factor of 4 of each other: no probability is lost beside another; 2^-140: 256 parts of 2^-149 and less
+    tol = ref.out_tolerance(r, torch.finfo(torch.bfloat16).eps, x) - 1e-30 + 2.0 ** -140
+    assert int(status) == 0 and (np.abs(out - r["out"]) <= tol).all()
