@@ -187,7 +187,7 @@ struct PackArgs {
   uint64_t to_stride;
   const int32_t* kept;
   uint64_t kept_stride;
-  uint32_t budget, per_seq;
+  uint32_t per_seq, most;                     // most: tokens of a sequence that can be kept, by the budget and by the weights
 };
 
 // Eight neighbouring channels of a token as they lie in memory, and as numbers.
@@ -332,7 +332,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fl_kv_pack(const PackAr
     b = blockIdx.x / a.per_seq;
     j = blockIdx.x - b * a.per_seq;
     n = uniform_len(a.s, a.from.T, b);
-    if (n > a.budget) n = a.budget;
+    if (n > a.most) n = a.most;
     held = 0;
     if (j * T >= n) return;
     page = scalar_load(a.to_table + b * a.to_stride + j);
@@ -2222,7 +2222,7 @@ int flh_kv_evict(const flh_kv_evict_params* p, void* stream) {
   a.to_stride = p->to_table_stride;
   a.kept = p->d_kept;
   a.kept_stride = p->budget;
-  a.budget = p->budget;
+  a.most = p->budget < p->weights_width ? p->budget : p->weights_width;
   a.per_seq = per;
   fl_prof().kid = 11;
   const hipStream_t st = (hipStream_t)stream;

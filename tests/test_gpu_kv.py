@@ -1120,3 +1120,26 @@ def test_attend_values_near_the_ends_of_the_range(fl, size, n, x, H, G, D):
     # all values are within a factor of 4 of each other: no probability is lost beside another; 2^-140: 256 parts of 2^-149 and less
     tol = ref.out_tolerance(r, torch.finfo(torch.bfloat16).eps, x) - 1e-30 + 2.0 ** -140
     assert int(status) == 0 and (np.abs(out - r["out"]) <= tol).all()
+
+
+@pytest.mark.parametrize("T2", [16, 32])
+def test_evict_by_weights_of_fewer_positions(fl, T2):
+    """Sequences longer than their weights are cut off there: what is packed, counted and bounded is what the weights know."""
+    core, kv, torch = fl
+    T, H, D, lens, width, budget = 16, 2, 64, [100, 60, 20], 41, 50
+    rng = np.random.default_rng(6)
+    cache, c, table = make(fl, rng, lens, T, H, D)
+    w = rng.random((3, H, width)).astype(np.float32)
+    per = -(-budget // T2)
+    table2 = np.arange(3 * per, dtype=np.int32).reshape(3, per)
+    to = kv.PageCache(torch.full((3 * per, kv.page_bytes(T2, H, D)), 0xA5, dtype=torch.uint8, device="cuda"), T2, H, D)
+    exp = held(to, T2, H, D)
+    status = core.new_status()
+    kept, nw, nl = kv.evict(cache, dev(torch, table), dev(torch, np.array(lens, np.int32)), dev(torch, w), budget, to, dev(torch, table2), status)
+    assert int(status) == E_RANGE
+    cut = [min(x, width) for x in lens]
+    k, x = ref.evict(c, table, cut, w, budget, 0, 0, exp, table2)
+    np.testing.assert_array_equal(nl.cpu().numpy(), cut)
+    np.testing.assert_array_equal(kept.cpu().numpy(), k)
+    same_numbers(nw.cpu().double().numpy(), x, "weights")
+    same_cache(held(to, T2, H, D), exp)
