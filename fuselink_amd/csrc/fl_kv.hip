@@ -2072,6 +2072,7 @@ int flh_kv_attend(const flh_kv_attend_params* p, void* stream) {
   if (rc) return rc;
   if (p->type != FLH_KV_BF16 && p->type != FLH_KV_FP16) return fl_set_error(FLH_E_ARG, "flh_kv_attend: type %u (bf16 or fp16)", p->type);
   if (p->seqs.n_tokens && (!p->d_q || !p->d_out || !aligned(p->d_q, 2) || !aligned(p->d_out, 2))) return fl_set_error(FLH_E_ARG, "flh_kv_attend: queries and output are required");
+  if (!(fabsf(p->scale) * 1.4426950408889634f < kInf)) return fl_set_error(FLH_E_ARG, "flh_kv_attend: a scale of %g", (double)p->scale);
   if (p->d_selected && (p->n_selected == 0 || p->n_selected > kMaxPages)) return fl_set_error(FLH_E_ARG, "flh_kv_attend: %u selected pages", p->n_selected);
   if (p->d_selected && p->d_weights) return fl_set_error(FLH_E_ARG, "flh_kv_attend: weights are kept over all pages, not over selected ones");
   if (!p->d_weights && p->d_weights_in) return fl_set_error(FLH_E_ARG, "flh_kv_attend: weights to start from, but none to write");

@@ -561,7 +561,7 @@ int flh_kv_store(const flh_kv_store_params* p, void* stream);
 
 /* Attention of queries [n_tokens][q_heads][dim] (bf16 or fp16; query head h reads key-value head h / (q_heads / heads))
  * over the d_lens tokens of their sequences:  out = sum_j p_j v_j, p = softmax over the keys j a query sees of
- * scale * q . k_j.  causal: the call's n tokens of a sequence are the last n of its d_lens, and token i sees the keys before and
+ * scale * q . k_j (scale: any sign, and finite, also times log2(e)).  causal: the call's n tokens of a sequence are the last n of its d_lens, and token i sees the keys before and
  * at its own position; else all see all.  A query that sees no key, or only ones of a score of -inf,
  * gets zeros and a log-sum of -inf, and adds nothing to the weights.  d_lse (optional):
  * natural logarithm of each row's sum, [n_tokens][q_heads].

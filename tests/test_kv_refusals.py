@@ -185,3 +185,9 @@ def test_widths_past_31_bits(lib, width):
     for op, p in (("flh_kv_select", select(count=width)), ("flh_kv_attend", attend(d_weights=P, weights_width=width)),
                   ("flh_kv_evict", apart(weights_width=width)), ("flh_kv_evict", apart(new_weights_width=width))):
         assert getattr(lib, op)(C.byref(p), None) == E_ARG
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 3e38])
+def test_scales_that_are_not_finite(lib, scale):
+    assert lib.flh_kv_attend(C.byref(attend(scale=scale)), None) == E_ARG
+    assert b"scale" in lib.flh_last_error()
