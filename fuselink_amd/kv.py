@@ -6,7 +6,10 @@ Every call launches on `stream` (default: the current stream of the tensors' dev
 allocates -- results that were not given, workspaces -- comes from that stream's pool.  A call that names a stream marks the
 tensors given as used on it.  A workspace that is given belongs to one call at a time: calls on two streams, or two
 graphs that may run at once, need one each.  What is wrong with device-resident page numbers, lengths and starts shows as
-FLH_E_RANGE in `status` (core.new_status())."""
+FLH_E_RANGE in `status` (core.new_status()).
+
+No operator has a gradient: where gradients are recorded, tensors that require one are refused.  What a call writes (pages, outputs
+and weights given, status) is written behind autograd's back, without a new version of the tensor."""
 from __future__ import annotations
 
 import contextlib
@@ -88,6 +91,12 @@ def _check(cache: PageCache, name: str, t: torch.Tensor, dtype, dims: int):
     if t.dtype is not dtype or len(shape) != dims or (stride[-1] != 1 and shape[-1] > 1) or t.get_device() != cache.index:
         _wrong(cache, name, t, f"{dims} dimensions of {dtype}")
     return shape, stride
+
+
+def _no_gradient(*tensors) -> None:
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("the operators on KV pages have no gradient: detach what requires one, or call them under torch.no_grad()")
 
 
 def _check_written(name: str, t: torch.Tensor) -> None:
@@ -208,6 +217,7 @@ def store(cache: PageCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.
           starts: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> None:
     """flh_kv_store: appends k and v [n_tokens, heads, dim] (bf16, fp16 or fp32) to sequences that hold `lens` tokens
     before the call.  `starts` [n_seqs + 1] says whose tokens are whose; without it every sequence has equally many."""
+    _no_gradient(k, v)
     kind = TYPES.get(k.dtype)
     if kind is None:
         _wrong(cache, "k", k, "bf16, fp16 or fp32")
@@ -231,6 +241,7 @@ def attend(cache: PageCache, q: torch.Tensor, page_table: torch.Tensor, lens: to
     contiguous) receives the logarithms of the rows' sums.  `selected` (from select_pages) restricts every query token and head to
     those pages.  `weights` (float32 [n_seqs, heads, positions]) gains what attention every key drew: it is added to in
     place, or written as `weights_in` plus the gain when that is given."""
+    _no_gradient(q, out, lse, weights, weights_in)
     n, hq, qt, qh, kind = _queries(cache, q)
     seqs, word = _seqs(cache, page_table, lens, status, starts, n)
     n_seqs, heads = seqs[5], cache.heads
@@ -315,6 +326,7 @@ def evict(cache: PageCache, page_table: torch.Tensor, lens: torch.Tensor, weight
     `weights` [n_seqs, heads, positions] -- packed into the pages of `to` that `to_table` [n_seqs, pages] names, none of which may be
     among those that are read.  Returns (kept, new_weights, new_lens): positions [n_seqs, heads, budget] with -1 behind
     them, the weights kept with zeros behind them ([n_seqs, heads, >= budget]), and the new lengths (`new_lens` is other memory than `lens`)."""
+    _no_gradient(weights, new_weights)
     seqs, word = _seqs(cache, page_table, lens, status, None, 0)
     b, h = seqs[5], cache.heads
     _need(to.index == cache.index and to.heads == h and to.dim == cache.dim, "the new cache differs in device, heads or head dim")

@@ -1143,3 +1143,19 @@ def test_evict_by_weights_of_fewer_positions(fl, T2):
     np.testing.assert_array_equal(kept.cpu().numpy(), k)
     same_numbers(nw.cpu().double().numpy(), x, "weights")
     same_cache(held(to, T2, H, D), exp)
+
+
+def test_parameters_without_recording(fl):
+    """Keys, values and queries made of parameters: served where no gradient is recorded, as detached ones are."""
+    core, kv, torch = fl
+    T, H, G, D, x = 16, 2, 4, 64, 40
+    cache, c, table = make(fl, np.random.default_rng(2), [x], T, H, D)
+    args = dev(torch, table), dev(torch, np.array([x], np.int32)), core.new_status()
+    w = torch.randn(D, H * G * D, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    q = (torch.randn(1, D, device="cuda", dtype=torch.bfloat16) @ w).view(1, H * G, D)
+    with pytest.raises(ValueError, match="no gradient"):
+        kv.attend(cache, q, *args)
+    exp = kv.attend(cache, q.detach(), *args)
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            assert torch.equal(kv.attend(cache, q, *args), exp)

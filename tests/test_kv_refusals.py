@@ -191,3 +191,20 @@ def test_widths_past_31_bits(lib, width):
 def test_scales_that_are_not_finite(lib, scale):
     assert lib.flh_kv_attend(C.byref(attend(scale=scale)), None) == E_ARG
     assert b"scale" in lib.flh_last_error()
+
+
+def test_tensors_that_require_a_gradient():
+    need = kv.page_bytes(16, 2, 32)
+    c = kv.PageCache(torch.zeros(2, need, dtype=torch.uint8), 16, 2, 32)
+    i = torch.zeros(2, dtype=torch.int32)
+    t = i.view(2, 1)
+    k, q, w = torch.zeros(2, 2, 32), torch.zeros(2, 4, 32, dtype=torch.float16), torch.zeros(2, 2, 32)
+    g = lambda x: x.clone().requires_grad_()
+    calls = [lambda: kv.store(c, g(k), k, t, i, i), lambda: kv.store(c, k, g(k), t, i, i), lambda: kv.attend(c, g(q), t, i, i), lambda: kv.attend(c, g(q) * 2, t, i, i),
+             lambda: kv.attend(c, q, t, i, i, out=g(q)), lambda: kv.attend(c, q, t, i, i, weights=g(w)), lambda: kv.attend(c, q, t, i, i, weights=w, weights_in=g(w)),
+             lambda: kv.attend(c, q, t, i, i, lse=g(w[:, :, 0])), lambda: kv.evict(c, t, i, g(w), 16, c, t, i), lambda: kv.evict(c, t, i, w, 16, c, t, i, new_weights=g(w))]
+    for call in calls:
+        with pytest.raises(ValueError, match="no gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="no CPU path"):     # what comes next here
+            call()
