@@ -582,6 +582,12 @@ __device__ __forceinline__ void clear(Rows<NQ, VJ>& r, const uint32_t (&lim)[NQ]
   r.fresh = true;
 }
 
+// the exponent field of a value scale, 0 for none
+__device__ __forceinline__ int scale_bits(float v) { return (int)(uniform(__float_as_uint(v)) >> 23); }
+// Value scales of a step's two tiles more than 2^6 apart: the smaller one's probabilities would lose their bits to the larger
+// one's unit, for rows, too, that do not see the larger.  The smaller tile is then left out, and taken alone behind all others.
+__device__ __forceinline__ bool apart(int x0, int x1) { return x0 && x1 && (uint32_t)(x0 - x1 + 6) > 12; }
+
 // One step of the softmax: scores of 32 keys (two tiles under K scales kc0 and kc1, base 2, and value scales v0 and v1) to
 // probabilities and their sums.
 //
@@ -589,11 +595,12 @@ __device__ __forceinline__ void clear(Rows<NQ, VJ>& r, const uint32_t (&lim)[NQ]
 // which is seen from the rounded ones themselves, two to a word; the maximum proper is taken in that case only.  The
 // tiles' value scales go into the probabilities as powers of two of the scale that O counts in (exact, and free in the
 // exponent), so that V's codes meet them as they are.  That scale is the larger of the two blocks', kept while it stays
-// within 2^6 below; it never falls more than 2^60 below the largest so far, or what O holds would overflow.  The sums
+// within 2^6 below; it never falls more than 2^60 below the largest so far, or what O holds would overflow (the other tile of
+// a step is at most 2^6 smaller, see apart()).  The sums
 // take the probabilities before they are rounded: logarithms and weights are 32 bits wide and come from them.
 template <int NQ, int VJ>
 __device__ __forceinline__ void soften(Rows<NQ, VJ>& r, const f4 (&s)[NQ][2], float kc0, float kc1, float v0, float v1, h8 (&pf)[NQ]) {
-  const int x0 = (int)(uniform(__float_as_uint(v0)) >> 23), x1 = (int)(uniform(__float_as_uint(v1)) >> 23), xm = x0 > x1 ? x0 : x1, xt = xm > r.elow ? xm : r.elow;
+  const int x0 = scale_bits(v0), x1 = scale_bits(v1), xm = x0 > x1 ? x0 : x1, xt = xm > r.elow ? xm : r.elow;
   const int enew = xm > 0 && !(xt <= r.ev && xt + 6 >= r.ev) ? xt : r.ev;
   const int d0 = x0 - enew < -64 ? -64 : x0 - enew, d1 = x1 - enew < -64 ? -64 : x1 - enew;   // (a block of zeros: the least)
   const float e0 = (float)d0, e1 = (float)d1;
@@ -702,8 +709,8 @@ __device__ __forceinline__ void emit8(const AttendArgs& a, uint32_t split, uint3
 // other rows, and S^T leaves the first product in the very lanes and order in which the second one wants P^T if the
 // 32 keys of a step are numbered (two tiles of 16) x (four lane groups) x 4 -- an order that sums do not see.  K and V
 // come as rows of codes straight into registers; V's bytes are interleaved token against token on the way to pairs.
-// P is rounded to 16-bit floats (11 bits of mantissa) at 2^8 times its value relative to the row's reference and up to 2^15,
-// normal down to 2^-22 of it (for the tile with the larger value scale of a step).  Sums, references and accumulators
+// P is rounded to 16-bit floats (11 bits of mantissa) at 2^8 to 2^15 times its value relative to the row's largest and, for
+// value scales below the one O counts in, at up to 2^-12 of that: normal down to 2^-22 of the largest, and to 2^-10 at worst.  Sums, references and accumulators
 // are 32 bits wide and rarely rescaled.  Memory bounds it for up to 16 rows: 16 sequences of 131072 tokens, 8 heads of 128 channels,
 // 4.3 GB in 713 us, 6.0 TB/s (a sum over 4 GiB: 6.1); 32 of up to 4096, 172 MB in 40 us, 4.3 TB/s, where the launch's
 // start and the longest sequence show; 201 tokens 8 us, 4 of them the launch's.
@@ -773,7 +780,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) 
   for (int i = 0; i < KW / 4; ++i) k_lane[i] = c * D + (g * (DP / 4) + 16 * i < D ? g * (DP / 4) + 16 * i : 0);
 #pragma unroll
   for (int i = 0; i < 4; ++i) v_lane[i] = (4 * g + i) * D + ((uint32_t)(c * VJ) < D ? c * VJ : 0);
-  uint32_t bad = 0, nan_steps = 0;
+  uint32_t bad = 0, nan_steps = 0, left_out = 0;
 
   // Four steps are under way at a time: the choice of a page (a load if pages were selected), its number, the codes and
   // scales, the sums.  Nothing in the first three branches: past the end they look at the last tile again.
@@ -843,6 +850,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) 
   };
   const auto work = [&](Stage& x) {
     if (!x.ok[0] && !x.ok[1]) return;
+    if (const int x0 = scale_bits(x.vs[0]), x1 = scale_bits(x.vs[1]); x.ok[0] && x.ok[1] && apart(x0, x1)) {
+      asm volatile("");
+      x.ok[x0 < x1 ? 0 : 1] = false;
+      left_out = 1;
+    }
     const bool masked = !x.ok[0] || !x.ok[1] || x.pos[0] + 16 > l_min || x.pos[1] + 16 > l_min;
 
     f4 s[NQ][2];
@@ -930,12 +942,22 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) 
         if (k >= k1) break;
       }
     }
+    if (left_out) {   // the smaller tiles of steps whose value scales lie apart
+      for (k = k0 + (wave * 32); k < k1; k += kStep) {
+        Stage s;
+        fetch(s, look_up(choose(k)));
+        const int x0 = scale_bits(s.vs[0]), x1 = scale_bits(s.vs[1]);
+        if (!s.ok[0] || !s.ok[1] || !apart(x0, x1)) continue;
+        s.ok[x0 < x1 ? 1 : 0] = false;
+        work(s);
+      }
+    }
     if (nan_steps) {   // a NaN value that not every row of the tile sees: into the sums of those that do
       for (k = k0 + (wave * 32); k < k1; k += kStep) {
         Where w = look_up(choose(k));
 #pragma unroll
         for (int t = 0; t < 2; ++t) w.ok[t] = w.ok[t] && w.page[t] < a.c.n_pages;
-        if (w.ok[0] && w.ok[1] && w.pos[0] + 16 <= l_min && w.pos[1] + 16 <= l_min) continue;
+        if (!left_out && w.ok[0] && w.ok[1] && w.pos[0] + 16 <= l_min && w.pos[1] + 16 <= l_min) continue;
         for (int t = 0; t < 2; ++t) {
           if (!w.ok[t]) continue;
           const uint8_t* base = a.c.pages + (uint64_t)w.page[t] * a.c.stride + a.c.side + w.off[t];
@@ -1011,7 +1033,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void fl_kv_attend_rows(cons
   __shared__ v8 sm_k[4 * KK * 64];                     // [tile][kk][lane]
   __shared__ h8 sm_v[2 * VJ * 64];                     // [pair of tiles][j][lane]
   __shared__ f4 sm_tile[4];                            // K scale * scale2, V scale, there is such a tile
-  __shared__ uint32_t sm_nan;
+  __shared__ float sm_scale[4];                        // V scales of the next 64 keys' tiles, 0 for none
+  __shared__ uint32_t sm_nan, sm_left_out;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const uint32_t wave = uniform(threadIdx.x >> 6), H = a.c.H, G = a.G, T = a.c.T, D = a.c.D;
   const uint32_t h = blockIdx.x % H, rest = blockIdx.x / H, split = rest / a.tiles_x, x = rest - split * a.tiles_x;
@@ -1053,7 +1076,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void fl_kv_attend_rows(cons
   for (int i = 0; i < KW / 4; ++i) k_lane[i] = c * D + (g * (DP / 4) + 16 * i < D ? g * (DP / 4) + 16 * i : 0);
 #pragma unroll
   for (int i = 0; i < 4; ++i) v_lane[i] = (4 * g + i) * D + ((uint32_t)(c * VJ) < D ? c * VJ : 0);
-  uint32_t bad = 0, nan_steps = 0;
+  uint32_t bad = 0, nan_steps = 0, left_out = 0;
 
   // this wavefront's tile of the 64 keys from k on: where it lies, its codes, its operands
   struct Where { uint32_t pos, page, off; bool ok; };
@@ -1097,7 +1120,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void fl_kv_attend_rows(cons
       }
     }
   };
-  const auto stage = [&](Stage& s) {
+  const auto stage = [&](Stage& s, bool second) {
+    const int x = scale_bits(s.vs), y = scale_bits(sm_scale[wave ^ 1]);   // and of the tile that shares the step
+    const bool small = s.ok && x < y && apart(x, y), take = s.ok && small == second;
+    if (small) left_out = 1;
     if (!s.ok || s.pos + 16 > l_min) {   // as in fl_kv_attend: values nobody sees, and NaN, are left out
       asm volatile("");
       uint32_t seen = 0;
@@ -1122,18 +1148,19 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void fl_kv_attend_rows(cons
         *at = u2{__builtin_bit_cast(uint32_t, v[0][j]), __builtin_bit_cast(uint32_t, v[1][j])};
       }
     }
-    if (lane == 0) sm_tile[wave] = f4{fmaxf(s.ok ? s.ks * a.scale2 : 0.f, 1e-37f), s.ok ? s.vs : 0.f, s.ok ? 1.f : 0.f, 0.f};
+    if (lane == 0) sm_tile[wave] = f4{fmaxf(s.ok ? s.ks * a.scale2 : 0.f, 1e-37f), take ? s.vs : 0.f, take ? 1.f : 0.f, 0.f};
   };
 
-  if (threadIdx.x == 0) sm_nan = 0;
-  if (k0 < k1) {
+  if (threadIdx.x == 0) sm_nan = sm_left_out = 0;
+  for (bool second = false; k0 < k1; second = true) {   // all tiles but the small ones beside large ones; then those, if there are any
     Stage s;
     Where w = look_up((k0 >> 4) + wave);
     fetch(s, w);
     w = look_up((k0 >> 4) + 4 + wave);
     for (uint32_t k = k0; k < k1; k += 64) {
+      if (lane == 0) sm_scale[wave] = s.ok ? s.vs : 0.f;
       __syncthreads();                                 // the last 64 keys have been used
-      stage(s);
+      stage(s, second);
       fetch(s, w);
       w = look_up((k >> 4) + 8 + wave);
       __syncthreads();
@@ -1174,6 +1201,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void fl_kv_attend_rows(cons
         }
       }
     }
+    if (left_out) sm_left_out = 1;
+    __syncthreads();
+    if (second || !sm_left_out) break;
   }
   if (nan_steps) sm_nan = 1;
   __syncthreads();

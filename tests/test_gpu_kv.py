@@ -1159,3 +1159,57 @@ def test_parameters_without_recording(fl):
     for mode in (torch.no_grad, torch.inference_mode):
         with mode():
             assert torch.equal(kv.attend(cache, q, *args), exp)
+
+
+@pytest.mark.parametrize("gap", [6, 7, 12, 24, 40, 60])
+@pytest.mark.parametrize("n,H,G,D", [(20, 1, 1, 64), (40, 2, 1, 128), (64, 1, 4, 64), (64, 66, 4, 128), (64, 1, 4, 256), (64, 2, 1, 256)])
+def test_attend_value_scales_apart_from_page_to_page(fl, gap, n, H, G, D):
+    """Neighbouring pages whose value scales are 2^gap apart: queries that see only the smaller ones, and queries to whom the larger ones'
+    keys are worth nothing, get their averages as exactly as without such neighbours."""
+    core, kv, torch = fl
+    T, x = 16, 64
+    rng = np.random.default_rng(gap + n)
+    k, v = rng.standard_normal((x, H, D)), rng.uniform(0.5, 1, (x, H, D)) * 2.0 ** -(gap // 2)
+    for j in (1, 2):
+        v[j * T:(j + 1) * T] *= 2.0 ** gap
+        k[j * T:(j + 1) * T, :, 0] = -150.0                      # times a query of 8 or 0 there, over sqrt(D): worth nothing, or as much as others
+    k[:T, :, 0] = k[3 * T:, :, 0] = 0
+    table, pages = tables(rng, [x], T)
+    c = ref.empty(pages, T, H, D)
+    ref.store(c, k, v, table, [0], [0, x])
+    cache = records(fl, c, T, H, D, [x], table)
+    qn = rng.standard_normal((n, H * G, D))
+    qn[:, :, 0] = np.where(np.arange(n)[:, None] % 3 == 0, 12.0, 0.0)
+    q = dev(torch, qn, torch.float32).to(torch.bfloat16)
+    status = core.new_status()
+    for causal in (True, False):
+        out = kv.attend(cache, q, dev(torch, table), dev(torch, np.array([x], np.int32)), status, causal=causal).cpu().double().numpy()
+        r = ref.attend(c, q.cpu().double().numpy(), table, [x], [0, n], 1 / np.sqrt(D), causal)
+        tol = ref.out_tolerance(r, torch.finfo(torch.bfloat16).eps, x) - 1e-30 + 2.0 ** -140
+        assert int(status) == 0 and (np.abs(out - r["out"]) <= tol).all()
+
+
+@pytest.mark.parametrize("at", [3, 21, 50])
+@pytest.mark.parametrize("n,H,G,D", [(1, 2, 4, 64), (20, 1, 4, 128), (64, 1, 4, 64), (64, 66, 4, 128), (64, 1, 4, 256)])
+def test_attend_nan_beside_value_scales_apart(fl, at, n, H, G, D):
+    """A NaN among the values of a page that is taken apart from its neighbour reaches those that see it, and no other."""
+    core, kv, torch = fl
+    T, x = 16, 64
+    rng = np.random.default_rng(n)
+    k, v = rng.standard_normal((x, H, D)), rng.uniform(0.5, 1, (x, H, D))
+    v[T:3 * T] *= 2.0 ** 24
+    table, pages = tables(rng, [x], T)
+    c = ref.empty(pages, T, H, D)
+    ref.store(c, k, v, table, [0], [0, x])
+    c["v"][table[0, at // T], H - 1, at % T, 5] = np.nan
+    cache = records(fl, c, T, H, D, [x], table)
+    q = dev(torch, rng.standard_normal((n, H * G, D)), torch.float32).to(torch.bfloat16)
+    for causal in (True, False):
+        out = kv.attend(cache, q, dev(torch, table), dev(torch, np.array([x], np.int32)), core.new_status(), causal=causal).cpu().double().numpy()
+        with np.errstate(invalid="ignore"):
+            r = ref.attend(c, q.cpu().double().numpy(), table, [x], [0, n], 1 / np.sqrt(D), causal)
+        nan = np.isnan(r["out"])
+        seen = (x - n + 1 + np.arange(n) > at) if causal else np.ones(n, bool)
+        assert (nan[:, (H - 1) * G:, 5].all(1) == seen).all() and nan.sum() == seen.sum() * G
+        np.testing.assert_array_equal(np.isnan(out), nan)
+        assert (np.abs(out - r["out"]) <= ref.out_tolerance(r, torch.finfo(torch.bfloat16).eps, x))[~nan].all()
