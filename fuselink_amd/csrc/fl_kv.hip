@@ -24,6 +24,7 @@ typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 
 constexpr float kInf = __builtin_inff();
 constexpr float kNan = __builtin_nanf("");
+constexpr float kLeast = 0x1p-149f;      // stands for 0 as a factor of scores: what it multiplies is zero then, or -inf and stays so
 
 // ------------------------------------------------------------------------------------------------
 // records and sequences
@@ -893,8 +894,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) 
         if (!x.ok[t]) x.ks[t] = x.vs[t] = 0.f;   // anyone's: O's scale must not follow them
     }
 
-    // the floor keeps -inf what it is under a block of zeros; what it multiplies otherwise is zero all the same
-    const float kc0 = fmaxf(x.ks[0] * a.scale2, 1e-37f), kc1 = fmaxf(x.ks[1] * a.scale2, 1e-37f);
+    const float kc0 = fmaxf(x.ks[0] * a.scale2, kLeast), kc1 = fmaxf(x.ks[1] * a.scale2, kLeast);
     h8 pf[NQ];
     soften(st, s, kc0, kc1, x.vs[0], x.vs[1], pf);
 
@@ -1148,7 +1148,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void fl_kv_attend_rows(cons
         *at = u2{__builtin_bit_cast(uint32_t, v[0][j]), __builtin_bit_cast(uint32_t, v[1][j])};
       }
     }
-    if (lane == 0) sm_tile[wave] = f4{fmaxf(s.ok ? s.ks * a.scale2 : 0.f, 1e-37f), take ? s.vs : 0.f, take ? 1.f : 0.f, 0.f};
+    if (lane == 0) sm_tile[wave] = f4{fmaxf(s.ok ? s.ks * a.scale2 : 0.f, kLeast), take ? s.vs : 0.f, take ? 1.f : 0.f, 0.f};
   };
 
   if (threadIdx.x == 0) sm_nan = sm_left_out = 0;
@@ -1368,7 +1368,7 @@ __global__ __launch_bounds__(256) void fl_kv_weights(const AttendArgs a) {
       s.ok[t] = t0 + t < tiles && there;
       bad |= there ? 0 : 1;
       const uint8_t* rec = a.c.pages + (uint64_t)(there ? page[t] : 0) * a.c.stride;
-      s.kc[t] = scalar_load(reinterpret_cast<const float*>(rec + a.c.scales) + 2 * h) * a.scale2;
+      s.kc[t] = fmaxf(scalar_load(reinterpret_cast<const float*>(rec + a.c.scales) + 2 * h) * a.scale2, kLeast);
       const uint8_t* base = rec + (uint64_t)(h * T + slot[t]) * D;
       asm("" : "+s"(base));
 #pragma unroll

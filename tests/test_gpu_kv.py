@@ -1213,3 +1213,27 @@ def test_attend_nan_beside_value_scales_apart(fl, at, n, H, G, D):
         assert (nan[:, (H - 1) * G:, 5].all(1) == seen).all() and nan.sum() == seen.sum() * G
         np.testing.assert_array_equal(np.isnan(out), nan)
         assert (np.abs(out - r["out"]) <= ref.out_tolerance(r, torch.finfo(torch.bfloat16).eps, x))[~nan].all()
+
+
+@pytest.mark.parametrize("n,x,H,G", [(1, 50, 2, 4), (20, 200, 2, 4), (40, 90, 65, 4)])
+def test_attend_least_keys_under_huge_queries(fl, n, x, H, G):
+    """Keys at the least scale there is, under queries as large as their products with the codes allow: the scores are what they are."""
+    core, kv, torch = fl
+    T, D = 16, 64
+    rng = np.random.default_rng(n + x)
+    k, v = rng.standard_normal((x, H, D)) * 1e-37, rng.standard_normal((x, H, D))
+    table, pages = tables(rng, [x], T)
+    c = ref.empty(pages, T, H, D)
+    ref.store(c, k, v, table, [0], [0, x])
+    assert (c["s"][table[0], :, 0] == 2.0 ** -126).all()
+    cache = records(fl, c, T, H, D, [x], table)
+    q = dev(torch, rng.standard_normal((n, H * G, D)) * 1e35, torch.float32).to(torch.bfloat16)
+    # no order of a sum of |q| |code| passes the range
+    assert (np.abs(q.cpu().double().numpy()).max(2) * np.nansum(np.abs(c["k"]), 3).max() < 2.0 ** 128).all()
+    status, w, lse = core.new_status(), torch.zeros(1, H, x, device="cuda"), torch.zeros(n, H * G, device="cuda")
+    out = kv.attend(cache, q, dev(torch, table), dev(torch, np.array([x], np.int32)), status, scale=1.0, weights=w, lse=lse)
+    assert int(status) == 0
+    r = ref.attend(c, q.cpu().double().numpy(), table, [x], [0, n], 1.0)
+    check_out(torch, out, lse, r, torch.bfloat16, [x], [0, n])
+    tol = r["wslack"][0] * 1.1 + r["weights"][0] * (n * G + 64) * 2.0 ** -23
+    assert (np.abs(w[0].cpu().double().numpy() - r["weights"][0]) <= tol).all()
