@@ -312,8 +312,9 @@ __device__ __forceinline__ h2 column_pair(h2 v, F f) {
 // largest magnitude of the new tokens fixes the scale, then the same rows become codes: every row is read once and stays
 // in registers between the two, as it was loaded, ROWS of them a lane.  More than one wavefront exchange their largest
 // magnitude and their bounds through shared memory.  In evict the rows are codes of other records under their own scales.
-// Memory bounds it: 16 prompts of up to 4096 tokens, 8 heads of 128 channels in bf16, 267 MB in 53 us, 5.0 TB/s (a copy of 4 GiB: 4.5);
-// 16 sequences cut back to 2048 tokens, 134 MB in 34 us, 3.9 TB/s, every row of 128 bytes from a place of its own.
+// Memory bounds it: 16 prompts of up to 4096 tokens, 8 heads of 128 channels in bf16, 267 MB in 62 us, 4.3 TB/s (a copy of 4 GiB: 4.5);
+// 16 sequences cut back to 2048 tokens, 134 MB in 44 us, 3.0 TB/s, every row of 128 bytes from a place of its own, behind three
+// loads that tell where.  (Here and at the kernels below inputs change from call to call and do not fit the caches together.)
 template <class E, bool EVICT, int ROWS, int W>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fl_kv_pack(const PackArgs a) {
   warm_kernel_args(a);
@@ -713,8 +714,8 @@ __device__ __forceinline__ void emit8(const AttendArgs& a, uint32_t split, uint3
 // P is rounded to 16-bit floats (11 bits of mantissa) at 2^8 to 2^15 times its value relative to the row's largest and, for
 // value scales below the one O counts in, at up to 2^-12 of that: normal down to 2^-22 of the largest, and to 2^-10 at worst.  Sums, references and accumulators
 // are 32 bits wide and rarely rescaled.  Memory bounds it for up to 16 rows: 16 sequences of 131072 tokens, 8 heads of 128 channels,
-// 4.3 GB in 713 us, 6.0 TB/s (a sum over 4 GiB: 6.1); 32 of up to 4096, 172 MB in 40 us, 4.3 TB/s, where the launch's
-// start and the longest sequence show; 201 tokens 8 us, 4 of them the launch's.
+// 4.3 GB in 720 us, 6.0 TB/s (a sum over 4 GiB: 6.1); 32 of up to 4096, 172 MB in 47 us, 3.7 TB/s, where the launch's
+// start and the longest sequence show; 201 tokens 9 us, 4 of them the launch's.
 template <class E, int DP, int NQ, bool SEL>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) void fl_kv_attend(const AttendArgs a) {
   warm_kernel_args(a);
@@ -1021,9 +1022,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NQ == 1 && DP == 128 ? 3 : 2) 
 // converts one tile of 16 and leaves it in shared memory as the operands of the matrix instructions, with its scales, so
 // that a code is converted once for 128 rows instead of once for 32 and the registers hold a quarter of the codes on
 // their way.  Two barriers to 64 keys; the three workgroups of a compute unit fill each other's waits.  4 sequences of up
-// to 16384 tokens, 1024 of them new, 32 query heads of 128: 632 GFLOP in 830 us, 760 TFLOP/s (a library product of 8192^3
-// in bf16: 1271).  The vector instructions bound it -- exponentials, conversions and packing keep the pipes busy for 63 % of the time,
-// the matrix instructions for 37 %.
+// to 16384 tokens, 1024 of them new, 32 query heads of 128: 632 GFLOP in 812 us, 780 TFLOP/s (a library product of 8192^3
+// in bf16: 1271).  Neither kind of instruction bounds it: matrix instructions keep their pipes busy for 36 % of a SIMD's cycles,
+// vector instructions (exponentials, conversions, packing) theirs for 53 %, and they take turns more than they overlap -- in
+// a wavefront the softmax stands between the two products, and the barriers keep the four in step.
 template <class E, int DP>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void fl_kv_attend_rows(const AttendArgs a) {
   warm_kernel_args(a);
@@ -1244,7 +1246,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void fl_kv_attend_rows(cons
 // The splits' results of every row, weighted by what their shares of the keys add up to.  Rows are numbered as in
 // fl_kv_attend, so those of no sequence are not touched.  A wavefront joins one row: with DL = D / 4 lanes to a split it
 // reads 64 / DL splits at a time, eight such loads under way.  What it takes is the start of a launch and one or two trips to
-// memory (4 us for few splits).
+// memory (5 us for few splits).
 constexpr uint32_t kMostSplits = 256;
 template <class E, bool SEL>
 __global__ __launch_bounds__(256) void fl_kv_join(const AttendArgs a, uint32_t TR) {
@@ -1473,7 +1475,7 @@ __device__ __forceinline__ uint32_t token_limit(const SelectArgs& a, uint32_t le
 // 8-bit bounds), so equal scores are equal and the choice does not depend on the order of a sum.  The sum splits into
 // max(q8, 0) . high - max(-q8, 0) . low, two runs of 16 x 16 x 64 integer matrix instructions whose operands are the
 // bytes of the record as they lie.  Memory bounds it: bounds of 2 KiB in records of 34 KiB, 65536 pages of 8 heads of 128
-// channels, 139 MB in 29 us, 4.8 TB/s.
+// channels, 139 MB in 36 us, 3.8 TB/s; up to 2048 pages for each of 16 tokens, 42 MB, take 18.
 template <class E, int DP>
 __global__ __launch_bounds__(512) void fl_kv_score(const SelectArgs a) {
   warm_kernel_args(a);
@@ -1803,7 +1805,7 @@ __device__ void put_picked(uint32_t n, Pick pick, Key key, Along along, Put put,
 }
 
 // A workgroup chooses one row's pages.  Its passes over the keys, one behind the other, bound it: 32 rows of 16384 pages
-// 19 us, 128 of 2048 7 us.
+// 19 us, 128 of 2048 8 us.
 template <int NT, bool ONE>
 __global__ __launch_bounds__(NT) void fl_kv_pick_pages(const SelectArgs a) {
   warm_kernel_args(a);
@@ -1835,7 +1837,7 @@ struct KeepArgs {
   int32_t* new_lens;
 };
 
-// The same over the weights of a sequence and head: 128 rows of up to 8192 weights 15 us.
+// The same over the weights of a sequence and head: 128 rows of up to 8192 weights 17 us.
 template <int NT, bool ONE>
 __global__ __launch_bounds__(NT) void fl_kv_keep(const KeepArgs a) {
   warm_kernel_args(a);
@@ -2185,8 +2187,8 @@ int flh_kv_select(const flh_kv_select_params* p, void* stream) {
   fl_prof().kid = 10;
   const hipStream_t st = (hipStream_t)stream;
   // The wavefronts of a workgroup take up to eight heads of the same pages: the pages' translations and the line that
-  // holds their scales are then fetched by one compute unit (65536 pages of 8 heads: a head to a workgroup 41 us, four
-  // 31, eight 29).  2048 wavefronts over all rows (1024: 10 tokens over 7518 pages of 5 heads of 64 channels 53 us, 46 so;
+  // holds their scales are then fetched by one compute unit (65536 pages of 8 heads, the same ones each time: a head to a
+  // workgroup 41 us, four 31, eight 29).  2048 wavefronts over all rows (1024: 10 tokens over 7518 pages of 5 heads of 64 channels 53 us, 46 so;
   // 4096: 16 over 2048 pages of 8 heads of 128 44 us, 42 so), or 32 pages to each.
   const uint32_t waves = a.c.H >= 8 ? 8 : 4;
   a.heads_wg = a.c.H >= 8 ? 8 : a.c.H >= 4 ? 4 : a.c.H >= 2 ? 2 : 1;
@@ -2199,9 +2201,9 @@ int flh_kv_select(const flh_kv_select_params* p, void* stream) {
   if (a.c.D <= 64) { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 64>), grid, block, 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 64>), grid, block, 0, st, a); }
   else if (a.c.D <= 128) { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 128>), grid, block, 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 128>), grid, block, 0, st, a); }
   else { if (bf) FL_LAUNCH((fl_kv_score<__bf16, 256>), grid, block, 0, st, a); else FL_LAUNCH((fl_kv_score<_Float16, 256>), grid, block, 0, st, a); }
-  // 1024 threads to a row if there are no more rows than compute units and more than 6 keys
-  // a thread, or if 256 would hold too few
-  // (evictions of 32 rows of 4000 weights: 26 us with 256, 20 with 1024; 1024 rows of 512 pages: 52 and 59).
+  // 1024 threads to a row if there are no more rows than compute units and more than 6 keys to a thread of 256, or if 256 would
+  // hold too few.  (The choice of 32 rows of 1024, 1536, 2048 and 4000 keys: 6.0, 7.4, 8.0, 11.9 us with 256 threads, 6.5, 6.8,
+  // 6.8, 7.6 with 1024; 256 rows: 6.3, 7.8, 8.3, 13.4 and 7.0, 7.2, 7.2, 8.4; 512 rows: 7.0, 8.9, 9.4, 15.7 and 9.6, 9.7, 10.0, 11.3.)
   if (!many_threads(a.s.n_tokens * a.c.H, a.s.width)) FL_LAUNCH((fl_kv_pick_pages<256, true>), dim3(a.s.n_tokens * a.c.H), dim3(256), 0, st, a);
   else if (a.s.width <= 1024 * kHeld) FL_LAUNCH((fl_kv_pick_pages<1024, true>), dim3(a.s.n_tokens * a.c.H), dim3(1024), 0, st, a);
   else FL_LAUNCH((fl_kv_pick_pages<1024, false>), dim3(a.s.n_tokens * a.c.H), dim3(1024), 0, st, a);

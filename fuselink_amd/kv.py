@@ -8,6 +8,8 @@ tensors given as used on it.  A workspace that is given belongs to one call at a
 graphs that may run at once, need one each.  What is wrong with device-resident page numbers, lengths and starts shows as
 FLH_E_RANGE in `status` (core.new_status()).
 
+Results that were not given hold nothing defined in the rows of tokens that are no sequence's.
+
 No operator has a gradient: where gradients are recorded, tensors that require one are refused.  What a call writes (pages, outputs
 and weights given, status) is written behind autograd's back, without a new version of the tensor."""
 from __future__ import annotations

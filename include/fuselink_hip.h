@@ -569,7 +569,8 @@ int flh_kv_store(const flh_kv_store_params* p, void* stream);
  * for none; only these pages are read, and of a list no more entries than the query sees pages of the sequence, so what is
  * chosen stands in front (flh_kv_select writes it so).
  * d_weights (optional; not with d_selected): [n_seqs][heads][weights_width], = d_weights_in (the same memory, other memory, or
- * NULL for 0) plus, for each key, the probabilities that all the call's queries of its head gave it.
+ * NULL for 0) plus, for each key, the probabilities that all the call's queries of its head gave it; keys behind weights_width
+ * are attended to all the same (FLH_E_RANGE).
  * P is rounded to 16-bit floats for the second product: 11 bits of mantissa down to 2^-22 of the row's largest P (2^-10 where
  * value scales of neighbouring pages differ by up to 2^12), steps of 2^-32 (2^-20) of it below.  Blocks of values more than 2^60
  * smaller than one before them in the sequence count with fewer bits.  Scores, sums, log-sums, weights and accumulators hold 32
@@ -603,7 +604,8 @@ int flh_kv_attend(const flh_kv_attend_params* p, void* stream);
  * sequence has fewer: [n_tokens][heads][count].  score(page) = max over the head's query heads of
  * sum_d q8_d (q8_d > 0 ? high_d : low_d) * step * K scale, with q8 = round(q / step) and step the smallest power of two with
  * |q| <= 127 step (what is not finite counts as 0).  The first `first` and last `last` pages that the query sees are always
- * among them; of equal scores the lower index is taken.  Only what causal lets a query see is counted as a page. */
+ * among them; of equal scores the lower index is taken.  (Scores are 32-bit floats, exact while they stay in range.)  Only
+ * what causal lets a query see is counted as a page. */
 typedef struct flh_kv_select_params {
   flh_kv_cache cache;
   flh_kv_seqs  seqs;
