@@ -573,9 +573,10 @@ int flh_kv_store(const flh_kv_store_params* p, void* stream);
  * are attended to all the same (FLH_E_RANGE).
  * P is rounded to 16-bit floats for the second product: 11 bits of mantissa down to 2^-22 of the row's largest P (2^-10 where
  * value scales of neighbouring pages differ by up to 2^12), steps of 2^-32 (2^-20) of it below.  Blocks of values more than 2^60
- * smaller than one before them in the sequence count with fewer bits.  Scores, sums, log-sums, weights and accumulators hold 32
- * bits; a query's products with the codes and their sums (up to |q| * 448 * dim) have to stay in that range.  The sequences of a
- * call are cut alike, by their average number of new tokens: single tokens and long prompts are faster in a call each. */
+ * smaller than another one of the sequence may count with fewer bits, or none.  Scores, sums, log-sums, weights and accumulators
+ * hold 32 bits; a query's products with the codes and their sums (up to |q| * 448 * dim) have to stay in that range.  The
+ * sequences of a call are cut alike, by their average number of new tokens: single tokens and long prompts are faster in a
+ * call each. */
 typedef struct flh_kv_attend_params {
   flh_kv_cache cache;
   flh_kv_seqs  seqs;
